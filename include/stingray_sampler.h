@@ -422,6 +422,143 @@ STG_API int stg_history_append(StgHandle handle, const int32_t *tokens, int32_t 
 /* Tokens slot holds now, or a negative STG_ERR_* code. */
 STG_API int stg_history_length(StgHandle handle, int32_t slot);
 
+/* ---- beam search (no counterpart in the reference, which samples; the rows, masks and soft caps are those of
+ *      stg_sample_rows) ---------------------------------------------------------------------------------
+ * A sequence that is decoded with beams has n_beams rows of logits: beam k of sequence b is row
+ * b * n_beams + k everywhere.  Per token: stg_beam_select finds the best continuations of every sequence,
+ * stg_beam_advance makes them the beams of the next token and collects what has ended, stg_beam_reorder lets
+ * per-beam state follow; stg_beam_start opens a sequence and stg_beam_backtrace reads the hypotheses' tokens.
+ * Every array is device memory unless it says otherwise, int32, float and double arrays aligned to their
+ * elements, and no output may overlap an input.  n_seq * n_beams <= max_rows.
+ *
+ * Streams and captured graphs: the calls are enqueued on `stream` and wait for nothing.  Only
+ * stg_beam_select uses workspace of the handle; it is ordered behind the handle's other calls as they are.  A
+ * call on a stream that is being captured gets workspace of its own, held until stg_destroy, so graphs
+ * captured from one handle may be replayed beside one another and beside direct calls. */
+#define STG_BEAM_MAX_BEAMS 32
+#define STG_BEAM_MAX_CANDIDATES 128 /* per sequence; also the hypotheses of stg_beam_backtrace */
+#define STG_BEAM_MAX_EOS 8
+
+/* per-sequence flags of stg_beam_select */
+enum {
+    STG_BEAM_SHORT = 1u << 0,   /* fewer than n_candidates candidates: the rest is token -1, parent -1, -infinity */
+    STG_BEAM_BAD_ROW = 1u << 1  /* an allowed logit of a beam was NaN or +infinity: the beam had no candidates */
+                                /* STG_ROW_FULLY_MASKED: a beam had no finite logit and no candidates */
+};
+
+/* The n_candidates best continuations of every sequence over its beams and the vocabulary.  With x the logits of
+ * beam k as stg_sample_rows reads them (bf16 widened, soft cap applied, masked tokens -infinity), the candidate
+ * (k, v) scores scores[k] + x[v] - log(sum(exp(x))), compared in 64 bits.  Order: larger score; of equal ones the lower
+ * beam, then the larger logit, then the lower token.  Logits of -infinity are no candidates.  A beam whose score
+ * is not finite is dead: it has no candidates and its row is not read. */
+typedef struct StgBeamBatch {
+    int32_t struct_size;            /* = sizeof(StgBeamBatch) */
+    int32_t n_seq;
+    int32_t n_beams;                /* 1 .. STG_BEAM_MAX_BEAMS */
+    int32_t vocab;
+    int32_t logits_dtype;           /* STG_DTYPE_* */
+    int32_t n_candidates;           /* 1 .. STG_BEAM_MAX_CANDIDATES; n_beams * (1 + end tokens) leaves n_beams that go on */
+    const void *logits;             /* [n_seq * n_beams, row_stride] */
+    int64_t row_stride;             /* elements between rows (>= vocab) */
+    const float *scores;            /* [n_seq, n_beams] running log-probabilities */
+    const uint32_t *mask;           /* allowed-token bitmask [n_seq * n_beams, mask_row_stride] or NULL, as StgSampleBatch.mask */
+    int64_t mask_row_stride;        /* 32-bit words between mask rows */
+    const uint8_t *row_uses_mask;   /* DEVICE [n_seq * n_beams] or NULL (every row), as stg_mask_compose writes it */
+    float logit_softcap;            /* as StgSampleBatch.logit_softcap */
+    int32_t *tokens;                /* out [n_seq, n_candidates], best first */
+    int32_t *parents;               /* out, same shape: the beam (0 .. n_beams - 1) that the candidate continues */
+    float *candidate_scores;        /* out, same shape, rounded once from 64 bits */
+    float *log_norms;               /* out [n_seq, n_beams] or NULL: log(sum(exp(x))) of each beam, -infinity where the
+                                       beam is dead or has no finite logit */
+    uint32_t *seq_flags;            /* out [n_seq] or NULL */
+} StgBeamBatch;
+STG_API int stg_beam_select(StgHandle handle, const StgBeamBatch *batch, void *stream);
+
+/* The search itself, in caller-owned device memory. */
+typedef struct StgBeamSearch {
+    int32_t struct_size;            /* = sizeof(StgBeamSearch) */
+    int32_t n_seq;
+    int32_t n_beams;
+    int32_t max_steps;              /* tokens there is room for in the trail */
+    int32_t n_eos;                  /* 0 .. STG_BEAM_MAX_EOS */
+    int32_t pad_token;              /* token of beams that do not go on */
+    int32_t early_stopping;         /* != 0: a sequence is done as soon as its pool is full */
+    const int32_t *eos_tokens;      /* HOST [n_eos] */
+    const double *norms;            /* [max_steps]: a hypothesis that ends with token t (from 0) competes with score / norms[t] */
+    int32_t *tokens;                /* [n_seq, n_beams]: the token each beam was continued with */
+    int32_t *parents;               /* [n_seq, n_beams]: the beam it continues (itself where it does not go on) */
+    float *scores;                  /* [n_seq, n_beams]: running log-probabilities, -infinity: dead */
+    int32_t *steps;                 /* [n_seq]: tokens taken so far */
+    int32_t *done;                  /* [n_seq]: != 0: the sequence takes no more tokens */
+    float *pool_scores;             /* [n_seq, n_beams]: its best ended hypotheses, best first, -infinity: none */
+    int32_t *pool_steps;            /* [n_seq, n_beams]: the step of the last token, -1: none */
+    int32_t *pool_parents;          /* [n_seq, n_beams]: the beam that token continues */
+    int32_t *pool_tokens;           /* [n_seq, n_beams]: that token */
+    int32_t *trail_tokens;          /* [max_steps, n_seq, n_beams]: tokens and parents of every step taken */
+    int32_t *trail_parents;
+} StgBeamSearch;
+
+/* Opens sequences [first_seq, first_seq + count): beam 0 alive with score 0, the others dead, nothing taken,
+ * the pool empty.  The trail is left as it is. */
+STG_API int stg_beam_start(StgHandle handle, const StgBeamSearch *search, int32_t first_seq, int32_t count, void *stream);
+
+/* Takes one token of every sequence that is not done.  Of its candidates (n_candidates per sequence, best first, as
+ * stg_beam_select writes them; a token below 0, a parent outside the beams or a score of -infinity or NaN is none) the
+ * first n_beams that are no end token become the beams, in order; end tokens among the first n_beams candidates go
+ * into the pool of the n_beams best hypotheses by score / norms[step] in 64 bits, rounded once (an equal one stands
+ * behind the older).  The step is written into the trail and counted.  A sequence is done when no beam goes on,
+ * when the pool is full and its worst is no worse than the best beam would be if it ended now (or
+ * early_stopping is set), when `finish` is set, or when the trail is full; in the last two cases the beams that go on are
+ * offered to the pool as well.  The beams of a sequence that is done, now or before, come out dead: pad_token, itself as
+ * parent, -infinity; its trail and pool are left as they are from then on. */
+STG_API int stg_beam_advance(StgHandle handle, const StgBeamSearch *search, int32_t n_candidates,
+                             const int32_t *cand_tokens, const int32_t *cand_parents, const float *cand_scores,
+                             int32_t finish, void *stream);
+
+/* One tensor of per-beam state: row r lies at data + r * row_stride and is a set of runs of inner_bytes, one for
+ * each combination of up to three outer dimensions (size 1: unused).  A state that grows along the sequence names the
+ * dimension that does: only the positions in use are moved. */
+typedef struct StgBeamState {
+    void *data;
+    int64_t row_stride;             /* bytes between beams */
+    int64_t inner_bytes;            /* contiguous bytes of a run, all positions */
+    int64_t position_bytes;         /* position_dim 3: bytes of one position of a run */
+    int64_t stride[3];              /* bytes */
+    int32_t size[3];
+    int32_t position_dim;           /* 0 .. 2: that outer dimension; 3: the runs themselves; -1: none, rows are moved whole */
+} StgBeamState;
+
+typedef struct StgBeamReorder {
+    int32_t struct_size;            /* = sizeof(StgBeamReorder) */
+    int32_t n_seq;
+    int32_t n_beams;
+    int32_t n_states;
+    const StgBeamState *states;     /* HOST [n_states] */
+    const int32_t *parents;         /* [n_seq, n_beams] */
+    const int32_t *positions;       /* [n_seq]: positions in use of each sequence, or NULL: n_positions */
+    int32_t n_positions;            /* < 0: all */
+    uint32_t mem_flags;             /* STG_MEM_HISTORY_RING: the handle's histories of slots 0 .. n_seq * n_beams - 1 too */
+} StgBeamReorder;
+
+/* Row k of every sequence becomes what its row parents[k] was, in place.  Rows whose parent is themselves, or
+ * outside the beams, stay as they are, and so do positions beyond those in use and rows behind the last sequence.  The
+ * rows and runs of a state must not overlap one another (STG_ERR_INVALID_ARGUMENT where the strides say that they do);
+ * two states must not share memory.  With STG_MEM_HISTORY_RING the histories of one sequence's beams must be of one
+ * length, as they are when every beam appends a token a step. */
+STG_API int stg_beam_reorder(StgHandle handle, const StgBeamReorder *reorder, void *stream);
+
+/* The tokens of n_hyps hypotheses per sequence (<= STG_BEAM_MAX_CANDIDATES) out of a trail of n_steps steps.
+ * Hypothesis (step, parent, token) - the pool's arrays - ends with `token` at `step`, before it stand the trail's tokens
+ * along the parents, from beam `parent` of step - 1 on.  sequences [n_seq, n_hyps, out_stride]: tokens 0 .. step, then
+ * pad_token up to n_steps (out_stride >= n_steps; what lies behind is not written).  lengths [n_seq, n_hyps] or NULL:
+ * step + 1.  A step outside [0, n_steps) is no hypothesis: all padding, length 0; a parent outside the beams ends the
+ * walk and leaves padding in front. */
+STG_API int stg_beam_backtrace(StgHandle handle, const int32_t *trail_tokens, const int32_t *trail_parents,
+                               int32_t n_steps, int32_t n_seq, int32_t n_beams, int32_t n_hyps,
+                               const int32_t *hyp_steps, const int32_t *hyp_parents, const int32_t *hyp_tokens,
+                               int32_t pad_token, int32_t *sequences, int64_t out_stride, int32_t *lengths,
+                               void *stream);
+
 /* ---- vocabulary-sharded mode (no counterpart in the reference, which is single-device:
  *      src/OpenTail.Stingray.Cli/RunCommand.cs:100) ------------------------------------------------
  * Each rank holds the column slice [vocab_offset, vocab_offset + batch->vocab) of every row, the

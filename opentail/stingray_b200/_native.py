@@ -18,6 +18,8 @@ MEM_HOST_UNIFORMS, MEM_HOST_OUTPUTS, MEM_HOST_DRAFT = 16, 32, 64
 MEM_HISTORY_RING = 128
 MASK_AND, MASK_OR = 0, 1
 CFG_HOST_LOGITS = 1
+BEAM_SHORT, BEAM_BAD_ROW = 1 << 0, 1 << 1
+BEAM_MAX_BEAMS, BEAM_MAX_CANDIDATES, BEAM_MAX_EOS = 32, 128, 8
 SEQ_EMPTY_RESIDUAL, SEQ_BAD_DRAFT = 1 << 8, 1 << 9
 
 EXPORTS = [
@@ -29,6 +31,7 @@ EXPORTS = [
     "stg_shard_select", "stg_shard_allgather", "stg_shard_exchange_bytes", "stg_shard_finish", "stg_shard_gather_local",
     "stg_mask_cache_put", "stg_mask_cache_contains", "stg_mask_compose",
     "stg_history_reset", "stg_history_load", "stg_history_append", "stg_history_length",
+    "stg_beam_select", "stg_beam_start", "stg_beam_advance", "stg_beam_reorder", "stg_beam_backtrace",
 ]
 
 
@@ -72,6 +75,41 @@ class StgSpecBatch(C.Structure):
         ("accepted", C.c_void_p), ("correction", C.c_void_p), ("accept_probs", C.c_void_p),
         ("seq_flags", C.c_void_p), ("mem_flags", C.c_uint32),
         ("target_softcap", C.c_float), ("draft_softcap", C.c_float),
+    ]
+
+
+class StgBeamBatch(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32), ("n_seq", C.c_int32), ("n_beams", C.c_int32), ("vocab", C.c_int32),
+        ("logits_dtype", C.c_int32), ("n_candidates", C.c_int32), ("logits", C.c_void_p), ("row_stride", C.c_int64),
+        ("scores", C.c_void_p), ("mask", C.c_void_p), ("mask_row_stride", C.c_int64), ("row_uses_mask", C.c_void_p),
+        ("logit_softcap", C.c_float), ("tokens", C.c_void_p), ("parents", C.c_void_p), ("candidate_scores", C.c_void_p),
+        ("log_norms", C.c_void_p), ("seq_flags", C.c_void_p),
+    ]
+
+
+class StgBeamSearch(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32), ("n_seq", C.c_int32), ("n_beams", C.c_int32), ("max_steps", C.c_int32),
+        ("n_eos", C.c_int32), ("pad_token", C.c_int32), ("early_stopping", C.c_int32), ("eos_tokens", C.c_void_p),
+        ("norms", C.c_void_p), ("tokens", C.c_void_p), ("parents", C.c_void_p), ("scores", C.c_void_p),
+        ("steps", C.c_void_p), ("done", C.c_void_p), ("pool_scores", C.c_void_p), ("pool_steps", C.c_void_p),
+        ("pool_parents", C.c_void_p), ("pool_tokens", C.c_void_p), ("trail_tokens", C.c_void_p), ("trail_parents", C.c_void_p),
+    ]
+
+
+class StgBeamState(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p), ("row_stride", C.c_int64), ("inner_bytes", C.c_int64), ("position_bytes", C.c_int64),
+        ("stride", C.c_int64 * 3), ("size", C.c_int32 * 3), ("position_dim", C.c_int32),
+    ]
+
+
+class StgBeamReorder(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32), ("n_seq", C.c_int32), ("n_beams", C.c_int32), ("n_states", C.c_int32),
+        ("states", C.c_void_p), ("parents", C.c_void_p), ("positions", C.c_void_p), ("n_positions", C.c_int32),
+        ("mem_flags", C.c_uint32),
     ]
 
 
@@ -130,6 +168,11 @@ def load() -> C.CDLL:
     lib.stg_shard_exchange_bytes.argtypes = [vp, C.POINTER(C.c_uint64)]
     lib.stg_shard_finish.argtypes = [vp, C.POINTER(StgSampleBatch), i32, vp]
     lib.stg_shard_gather_local.argtypes = [vp, C.POINTER(vp), i32, vp]
+    lib.stg_beam_select.argtypes = [vp, C.POINTER(StgBeamBatch), vp]
+    lib.stg_beam_start.argtypes = [vp, C.POINTER(StgBeamSearch), i32, i32, vp]
+    lib.stg_beam_advance.argtypes = [vp, C.POINTER(StgBeamSearch), i32, vp, vp, vp, i32, vp]
+    lib.stg_beam_reorder.argtypes = [vp, C.POINTER(StgBeamReorder), vp]
+    lib.stg_beam_backtrace.argtypes = [vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, i32, vp, i64, vp, vp]
     for name in EXPORTS:
         fn = getattr(lib, name)
         if name != "stg_last_error":

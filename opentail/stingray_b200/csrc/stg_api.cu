@@ -10,6 +10,7 @@
 #include <string>
 #include <vector>
 
+#include "stg_beam.h"
 #include "stg_emul2.cuh"
 #include "stg_flat.cuh"
 #include "stg_handle.h"
@@ -762,11 +763,13 @@ int run_batch(StgHandle h, const StgSampleBatch *b, const BatchExtra &x, void *s
 // every device buffer a handle owns
 std::vector<DevBuf *> all_buffers(StgHandle h)
 {
-    return {&h->plans[0].dev, &h->plans[1].dev, &h->flat_rows, &h->fw_redo, &h->fw_e, &h->fw_ids, &h->dr_redo,
+    std::vector<DevBuf *> all = {&h->plans[0].dev, &h->plans[1].dev, &h->flat_rows, &h->fw_redo, &h->fw_e, &h->fw_ids, &h->dr_redo,
             &h->cand, &h->cand_count, &h->tickets, &h->work_counter, &h->escratch, &h->keyscratch, &h->listscratch, &h->dists, &h->st_hist, &h->st_bias_ids, &h->st_bias_vals, &h->st_uniforms,
             &h->st_mask, &h->st_logits, &h->o_tokens, &h->o_probs, &h->o_flags, &h->o_topk_ids, &h->o_topk_vals, &h->o_topk_probs,
             &h->o_pairs, &h->ticks, &h->ring_ids, &h->ring_len_dev, &h->mc_words, &h->mc_slots, &h->sp_draft, &h->sp_uniforms,
-            &h->sp_accepted, &h->sp_correction, &h->sp_aprobs, &h->sp_flags, &h->sp_rowstats, &h->xchg_local, &h->xchg_gather};
+            &h->sp_accepted, &h->sp_correction, &h->sp_aprobs, &h->sp_flags, &h->sp_rowstats, &h->xchg_local, &h->xchg_gather, &h->bm_ws};
+    for (DevBuf &b : h->bm_captured) all.push_back(&b);
+    return all;
 }
 
 }  // namespace stg
@@ -855,6 +858,7 @@ int stg_create(const StgConfig *cfg, StgHandle *out)
         A(h->st_mask, 256);
         A(h->st_logits, 256);
     }
+    A(h->bm_ws, beam_ws_bytes(h));
     A(h->o_tokens, R * 4); A(h->o_probs, R * 4); A(h->o_flags, R * 4);
     const size_t tk = R * std::max<size_t>(cfg->max_top_k, 1) * 4;
     A(h->o_topk_ids, tk); A(h->o_topk_vals, tk); A(h->o_topk_probs, tk);

@@ -1,0 +1,36 @@
+// Beam search (stg_beam_*.cu): limits and the workspace of the selection.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../../include/stingray_sampler.h"
+#include "stg_handle.h"
+
+namespace stg {
+
+// What one CTA leaves of its piece of a row: the maximum of the logits it read, the sum of exp(x - max) over
+// them, and how many of the row's best it found (BeamWs::keys, descending).
+struct BeamPart {
+    double s;
+    float m;
+    int32_t count;
+};
+
+struct BeamWs {
+    BeamPart *parts;           // [rows, pieces]
+    unsigned long long *keys;  // [rows, pieces, n_candidates]: make_key (stg_select.cuh)
+};
+
+// Pieces that all rows of a call together may be cut into beyond one each.
+constexpr int kBeamExtraPieces = 4096;
+inline size_t beam_ws_bytes(StgHandle h)
+{
+    return ((size_t)h->cfg.max_rows + kBeamExtraPieces) * (sizeof(BeamPart) + STG_BEAM_MAX_CANDIDATES * 8) + 256;
+}
+
+// device arrays are checked for their elements' alignment, which the host can see
+inline bool misaligned(const void *p, size_t to) { return ((uintptr_t)p % to) != 0; }
+
+int beam_check_rows(StgHandle h, const char *who, int32_t n_seq, int32_t n_beams);
+
+}  // namespace stg

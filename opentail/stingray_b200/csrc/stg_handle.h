@@ -125,6 +125,9 @@ struct StgSampler_ {
     uint64_t mc_tick = 0;
     std::unordered_map<uint64_t, int> mc_index;  // key -> entry
     std::vector<int32_t> mc_slot_scratch;
+    // beam search (stg_beam_select.cu): the selection's workspace, and those of calls that were captured into graphs
+    stg::DevBuf bm_ws;
+    std::vector<stg::DevBuf> bm_captured;
 };
 
 namespace stg {

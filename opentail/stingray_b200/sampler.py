@@ -29,6 +29,9 @@ PARAMS_DTYPE = np.dtype([
 ])
 
 
+_BEAM_DTYPES = {"torch.float32": N.DTYPE_F32, "torch.bfloat16": N.DTYPE_BF16}
+
+
 class StingrayError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"{N.ERR_NAMES.get(code, code)}: {message}")
@@ -480,6 +483,138 @@ class BatchSampler:
         if n < 0:
             raise StingrayError(-n, self._error(self._h))
         return n
+
+    # -- beam search ----------------------------------------------------------------------------------
+    def _stream_here(self, stream) -> Optional[int]:
+        if stream is not None:
+            return getattr(stream, "cuda_stream", stream)
+        import torch
+
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _beam_array(self, name: str, x, dtype, shape):
+        """The address of a contiguous CUDA tensor of this type and shape on the handle's device."""
+        if x.dtype != dtype or x.shape != shape or x.get_device() != self.device or not x.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{self.device}, "
+                             f"got {x.dtype} {tuple(x.shape)} on {x.device}")
+        return x.data_ptr()
+
+    def beam_select(self, logits, scores, n_candidates: Optional[int] = None, *, mask=None, row_uses_mask=None,
+                    softcap: float = 0.0, want_norms: bool = False, want_flags: bool = False, stream=None,
+                    out: Optional[dict] = None):
+        """The best continuations of every sequence over its beams and the vocabulary (``stg_beam_select``).
+        ``scores`` ``[n_seq, n_beams]`` float32 are the beams' running log-probabilities (not finite: a dead
+        beam), ``logits`` ``[n_seq * n_beams, vocab]`` fp32 or bf16 their rows; ``mask`` int32 bitmask words per row
+        and ``row_uses_mask`` uint8 per row, both on the device, as ``mask_compose`` returns them.  Returns a dict with
+        ``tokens``, ``parents`` and ``scores`` ``[n_seq, n_candidates]`` (default 2 per beam), best first, and
+        ``log_norms`` ``[n_seq, n_beams]`` / ``flags`` ``[n_seq]`` where asked for.  ``out``: the dict of a
+        previous call with the same shapes and options, whose tensors are written again."""
+        import torch
+
+        n_seq, beams = scores.shape
+        rows, vocab = logits.shape
+        n = 2 * beams if n_candidates is None else n_candidates
+        dtype = _BEAM_DTYPES.get(str(logits.dtype))
+        if dtype is None or rows != n_seq * beams or logits.get_device() != self.device or (vocab > 1 and logits.stride(1) != 1):
+            raise ValueError(f"logits must be float32 or bfloat16 [n_seq * n_beams = {n_seq * beams}, vocab] on cuda:{self.device} with "
+                             f"contiguous rows, got {logits.dtype} {tuple(logits.shape)} on {logits.device}")
+        sp = self._beam_array("scores", scores, torch.float32, (n_seq, beams))
+        mp = up = None
+        mstride = 0
+        if mask is not None:
+            if mask.dtype != torch.int32 or mask.dim() != 2 or mask.shape[0] != rows or mask.shape[1] < (vocab + 31) // 32 or \
+                    mask.get_device() != self.device or mask.stride(1) != 1:
+                raise ValueError(f"mask must be int32 [{rows}, {(vocab + 31) // 32}] on cuda:{self.device} with contiguous rows")
+            mp, mstride = mask.data_ptr(), mask.stride(0) if rows > 1 else mask.shape[1]
+            if row_uses_mask is not None:
+                up = self._beam_array("row_uses_mask", row_uses_mask, torch.uint8, (rows,))
+        elif row_uses_mask is not None:
+            raise ValueError("row_uses_mask without a mask")
+        if out is None:
+            dev = logits.device
+            out = {"tokens": torch.empty((n_seq, n), dtype=torch.int32, device=dev),
+                   "parents": torch.empty((n_seq, n), dtype=torch.int32, device=dev),
+                   "scores": torch.empty((n_seq, n), dtype=torch.float32, device=dev)}
+            if want_norms:
+                out["log_norms"] = torch.empty((n_seq, beams), dtype=torch.float32, device=dev)
+            if want_flags:
+                out["flags"] = torch.empty(n_seq, dtype=torch.int32, device=dev)
+        b = N.StgBeamBatch(
+            C.sizeof(N.StgBeamBatch), n_seq, beams, vocab, dtype, n, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, sp, mp, mstride, up,
+            softcap, self._beam_array("out['tokens']", out["tokens"], torch.int32, (n_seq, n)),
+            self._beam_array("out['parents']", out["parents"], torch.int32, (n_seq, n)),
+            self._beam_array("out['scores']", out["scores"], torch.float32, (n_seq, n)),
+            self._beam_array("out['log_norms']", out["log_norms"], torch.float32, (n_seq, beams)) if want_norms else None,
+            self._beam_array("out['flags']", out["flags"], torch.int32, (n_seq,)) if want_flags else None)
+        self._check(self._lib.stg_beam_select(self._h, C.byref(b), self._stream_here(stream)))
+        return out
+
+    def _beam_search(self, search):
+        if search.device_index != self.device:
+            raise ValueError(f"the search lies on cuda:{search.device_index}, the handle on cuda:{self.device}")
+        return C.byref(search.struct)
+
+    def beam_start(self, search, first_seq: int = 0, count: Optional[int] = None, stream=None):
+        """Opens sequences ``[first_seq, first_seq + count)`` of a ``BeamSearch`` (all of them): beam 0 alive with
+        score 0, nothing taken, no hypotheses (``stg_beam_start``)."""
+        n = search.n_seq - first_seq if count is None else count
+        self._check(self._lib.stg_beam_start(self._h, self._beam_search(search), first_seq, n, self._stream_here(stream)))
+
+    def beam_advance(self, search, candidates: dict, finish: bool = False, stream=None):
+        """Takes one token of every sequence of ``search`` out of its ``candidates`` - the dict that ``beam_select``
+        returns - into the continuing beams (``search.tokens``, ``.parents``, ``.scores``), the pool of ended hypotheses and the
+        trail (``stg_beam_advance``).  ``finish``: nothing follows, the beams that go on are hypotheses too."""
+        import torch
+
+        tok, par, sc = candidates["tokens"], candidates["parents"], candidates["scores"]
+        shape = (search.n_seq, tok.shape[1])
+        self._check(self._lib.stg_beam_advance(
+            self._h, self._beam_search(search), shape[1], self._beam_array("candidates['tokens']", tok, torch.int32, shape),
+            self._beam_array("candidates['parents']", par, torch.int32, shape),
+            self._beam_array("candidates['scores']", sc, torch.float32, shape), 1 if finish else 0, self._stream_here(stream)))
+
+    def beam_reorder(self, states, parents, *, positions=None, history: bool = False, stream=None):
+        """Row k of every sequence becomes what its row ``parents[seq, k]`` was, in place, in every tensor of ``states`` (a
+        ``BeamStates``, or None) and, with ``history``, in the handle's own histories (``stg_beam_reorder``).
+        ``positions``: how many positions are in use - a number, or a device int32 tensor ``[n_seq]`` -
+        in tensors that name a position dimension; None: all."""
+        import torch
+
+        n_seq, beams = parents.shape
+        if states is not None and (states.rows != n_seq * beams or states.device_index != self.device):
+            raise ValueError(f"states of {states.rows} rows on cuda:{states.device_index}, parents of {n_seq * beams} rows on cuda:{self.device}")
+        pp, n_pos = None, -1
+        if positions is not None:
+            if _is_torch(positions):
+                pp = self._beam_array("positions", positions, torch.int32, (n_seq,))
+            else:
+                n_pos = int(positions)
+                if n_pos < 0:
+                    raise ValueError("positions must be >= 0")
+        r = N.StgBeamReorder(C.sizeof(N.StgBeamReorder), n_seq, beams, 0 if states is None else states.count,
+                             None if states is None else states.address, self._beam_array("parents", parents, torch.int32, (n_seq, beams)), pp, n_pos,
+                             N.MEM_HISTORY_RING if history else 0)
+        self._check(self._lib.stg_beam_reorder(self._h, C.byref(r), self._stream_here(stream)))
+
+    def beam_backtrace(self, trail_tokens, trail_parents, steps, parents, tokens, *, pad: int = 0, stream=None, out: Optional[dict] = None):
+        """The tokens of hypotheses (``stg_beam_backtrace``): a trail ``[n_steps, n_seq, n_beams]`` of tokens and parents and,
+        per sequence, the hypotheses' last step, the beam it continues and its token ``[n_seq, n_hyps]`` (a
+        ``BeamSearch``'s ``trail_*`` and ``pool_*``).  Returns ``sequences`` ``[n_seq, n_hyps, n_steps]``, padded with ``pad``,
+        and ``lengths`` ``[n_seq, n_hyps]``, 0 where there is no hypothesis."""
+        import torch
+
+        n_steps, n_seq, beams = trail_tokens.shape
+        hyps = steps.shape[1]
+        if out is None:
+            out = {"sequences": torch.empty((n_seq, hyps, n_steps), dtype=torch.int32, device=trail_tokens.device),
+                   "lengths": torch.empty((n_seq, hyps), dtype=torch.int32, device=trail_tokens.device)}
+        i32, shape, trail = torch.int32, (n_seq, hyps), (n_steps, n_seq, beams)
+        self._check(self._lib.stg_beam_backtrace(
+            self._h, self._beam_array("trail_tokens", trail_tokens, i32, trail), self._beam_array("trail_parents", trail_parents, i32, trail),
+            n_steps, n_seq, beams, hyps, self._beam_array("steps", steps, i32, shape), self._beam_array("parents", parents, i32, shape),
+            self._beam_array("tokens", tokens, i32, shape), pad, self._beam_array("out['sequences']", out["sequences"], i32, (n_seq, hyps, n_steps)),
+            n_steps, self._beam_array("out['lengths']", out["lengths"], i32, shape), self._stream_here(stream)))
+        return out
 
     # -- vocabulary-sharded mode ---------------------------------------------------------------------
     @staticmethod
