@@ -767,7 +767,7 @@ std::vector<DevBuf *> all_buffers(StgHandle h)
             &h->cand, &h->cand_count, &h->tickets, &h->work_counter, &h->escratch, &h->keyscratch, &h->listscratch, &h->dists, &h->st_hist, &h->st_bias_ids, &h->st_bias_vals, &h->st_uniforms,
             &h->st_mask, &h->st_logits, &h->o_tokens, &h->o_probs, &h->o_flags, &h->o_topk_ids, &h->o_topk_vals, &h->o_topk_probs,
             &h->o_pairs, &h->ticks, &h->ring_ids, &h->ring_len_dev, &h->mc_words, &h->mc_slots, &h->sp_draft, &h->sp_uniforms,
-            &h->sp_accepted, &h->sp_correction, &h->sp_aprobs, &h->sp_flags, &h->sp_rowstats, &h->xchg_local, &h->xchg_gather, &h->bm_ws};
+            &h->sp_accepted, &h->sp_correction, &h->sp_aprobs, &h->sp_flags, &h->sp_rowstats, &h->xchg_local, &h->xchg_gather, &h->bm_ws, &h->bm_tickets};
     for (DevBuf &b : h->bm_captured) all.push_back(&b);
     return all;
 }
@@ -859,6 +859,7 @@ int stg_create(const StgConfig *cfg, StgHandle *out)
         A(h->st_logits, 256);
     }
     A(h->bm_ws, beam_ws_bytes(h));
+    A(h->bm_tickets, R * 4);
     A(h->o_tokens, R * 4); A(h->o_probs, R * 4); A(h->o_flags, R * 4);
     const size_t tk = R * std::max<size_t>(cfg->max_top_k, 1) * 4;
     A(h->o_topk_ids, tk); A(h->o_topk_vals, tk); A(h->o_topk_probs, tk);
@@ -895,6 +896,7 @@ int stg_create(const StgConfig *cfg, StgHandle *out)
         e = cudaMemset(h->work_counter.p, 0, 256);
         if (e == cudaSuccess) e = cudaMemset(h->tickets.p, 0, h->tickets.bytes);
         if (e == cudaSuccess) e = cudaMemset(h->ring_len_dev.p, 0, h->ring_len_dev.bytes);
+        if (e == cudaSuccess) e = cudaMemset(h->bm_tickets.p, 0, h->bm_tickets.bytes);
         if (e == cudaSuccess) e = cudaMemset(h->flat_rows.p, 0, h->flat_rows.bytes);  // keys and tickets are zero between steps
         if (e != cudaSuccess) rc = cuda_fail(nullptr, e, "cudaMemset");
     }

@@ -8,24 +8,23 @@
 
 namespace stg {
 
-// What one CTA leaves of its piece of a row: the maximum of the logits it read, the sum of exp(x - max) over
-// them, and how many of the row's best it found (BeamWs::keys, descending).
+// What one CTA leaves of its piece of a row: the sum of exp(x - ref) over its logits, and their maximum.
 struct BeamPart {
     double s;
-    float m;
-    int32_t count;
+    float ref, top;
 };
 
 struct BeamWs {
     BeamPart *parts;           // [rows, pieces]
-    unsigned long long *keys;  // [rows, pieces, n_candidates]: make_key (stg_select.cuh)
+    unsigned long long *keys;  // [rows, pieces, n_candidates]: the best of each as make_key (stg_select.cuh), descending, 0: none
+    uint32_t *tickets;         // [n_seq]: CTAs of a sequence that have ended; zero between calls
 };
 
 // Pieces that all rows of a call together may be cut into beyond one each.
 constexpr int kBeamExtraPieces = 4096;
 inline size_t beam_ws_bytes(StgHandle h)
 {
-    return ((size_t)h->cfg.max_rows + kBeamExtraPieces) * (sizeof(BeamPart) + STG_BEAM_MAX_CANDIDATES * 8) + 256;
+    return ((size_t)h->cfg.max_rows + kBeamExtraPieces) * (sizeof(BeamPart) + STG_BEAM_MAX_CANDIDATES * 8) + 512;
 }
 
 // device arrays are checked for their elements' alignment, which the host can see

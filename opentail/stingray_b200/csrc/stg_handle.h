@@ -126,7 +126,7 @@ struct StgSampler_ {
     std::unordered_map<uint64_t, int> mc_index;  // key -> entry
     std::vector<int32_t> mc_slot_scratch;
     // beam search (stg_beam_select.cu): the selection's workspace, and those of calls that were captured into graphs
-    stg::DevBuf bm_ws;
+    stg::DevBuf bm_ws, bm_tickets;
     std::vector<stg::DevBuf> bm_captured;
 };
 
