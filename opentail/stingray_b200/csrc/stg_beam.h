@@ -8,23 +8,22 @@
 
 namespace stg {
 
-// What one CTA leaves of its piece of a row: the sum of exp(x - ref) over its logits, and their maximum.
+// What one CTA leaves of its piece of a row: the sum of exp(x - ref) over its logits.
 struct BeamPart {
-    double s;
-    float ref, top;
+    double s, ref;
 };
 
 struct BeamWs {
-    BeamPart *parts;           // [rows, pieces]
-    unsigned long long *keys;  // [rows, pieces, n_candidates]: the best of each as make_key (stg_select.cuh), descending, 0: none
-    uint32_t *tickets;         // [n_seq]: CTAs of a sequence that have ended; zero between calls
+    BeamPart *parts;    // [rows, pieces]
+    float *tops;        // [rows, groups]: the largest logit of each group of neighbours
+    uint32_t *tickets;  // [n_seq]: CTAs of a sequence that have ended; zero between calls
 };
 
 // Pieces that all rows of a call together may be cut into beyond one each.
-constexpr int kBeamExtraPieces = 4096;
+constexpr int kBeamExtraPieces = 8192;
 inline size_t beam_ws_bytes(StgHandle h)
 {
-    return ((size_t)h->cfg.max_rows + kBeamExtraPieces) * (sizeof(BeamPart) + STG_BEAM_MAX_CANDIDATES * 8) + 512;
+    return ((size_t)h->cfg.max_rows + kBeamExtraPieces) * sizeof(BeamPart) + (size_t)h->cfg.max_rows * ((size_t)h->cfg.max_vocab / 512 + 1) * 4 + 1024;
 }
 
 // device arrays are checked for their elements' alignment, which the host can see

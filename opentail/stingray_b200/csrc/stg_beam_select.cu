@@ -1,14 +1,17 @@
 // stg_beam_select: the best continuations of every sequence over its beams and the vocabulary.
 //
-// With x the logits of beam k, m their maximum and S = sum exp(x - m), candidate (k, v) scores
-//     score[k] + ((x[v] - m) - log S)
-// in 64 bits.  Within a beam the order is that of the logits alone, so a row is read once: a running maximum, a
-// running sum, and the list of its best logits as 64-bit keys (stg_select.cuh); the scores are made for the few
-// that are left when a sequence's rows come together.  The terms of S are computed and added up in 32 bits over the 16 or
-// 32 elements that a thread holds, in 64 beyond: their roundings (1e-7 each, either way) leave about 1e-8 of S, so two
-// beams' candidates change places only if they lie closer than that.
+// With x the logits of beam k, S = sum exp(x - r) for any r near their maximum, candidate (k, v) scores
+//     score[k] + ((x[v] - r) - log S)
+// in 64 bits.  Within a beam the order is that of the logits alone, and S is not known before the row has been read, so
+// the pass over the logits selects nothing: it adds up S and keeps the maximum of every group of 512 (fp32) or 1024 (bf16)
+// neighbouring logits.  Order the groups of all beams of a sequence by the score of their best candidate, equal ones as
+// candidates are: n groups have n candidates that are ahead of everything in the groups behind them, so the n best
+// candidates lie in the n best groups, whatever ties.  The CTA that ends last with a sequence finds those groups and
+// reads them once more.  One launch, no barrier and no list in the pass.
 //
-// A row is cut into pieces, one CTA each, and the CTA that ends last joins a sequence's pieces: one launch.
+// The terms of S are computed and added up in 32 bits over the 16 or 32 elements that a thread holds, in 64 beyond: their
+// roundings (1e-7 each, either way) leave about 1e-8 of S, so two beams' candidates change places only if they lie
+// closer than that.
 #include <cuda_runtime.h>
 #include <math_constants.h>
 #include <stdint.h>
@@ -22,13 +25,10 @@
 
 namespace stg {
 
-constexpr int kBeamThreads = 256;
+constexpr int kBeamThreads = 512;
 constexpr int kBeamWarps = kBeamThreads / 32;
-constexpr int kBeamList = 1024;    // a piece's list in shared memory, a power of two
-constexpr int kMergeList = 512;    // a sequence's
-constexpr int kMergeParts = 2048;  // pieces of a sequence's rows together
-// What is no candidate - -infinity - lies at or below this key.
-constexpr u64 kNoKey = ((u64)0x007FFFFFu << 32) | 0xFFFFFFFFu;
+constexpr int kBeamList = 512;  // candidates in shared memory
+constexpr int kBeamRoom = 256;  // so many are offered between two looks at the list, where it may overflow
 
 struct BeamSelect {
     const void *logits;
@@ -39,7 +39,7 @@ struct BeamSelect {
     const uint8_t *uses_mask;
     float softcap;
     int32_t n_seq, beams, vocab, n;
-    int32_t pieces, piece_len;
+    int32_t pieces, piece_len, groups;  // CTAs of a row, their elements, and the row's groups
     BeamWs ws;
     int32_t *tokens, *parents;
     float *out_scores, *log_norms;
@@ -47,20 +47,22 @@ struct BeamSelect {
 };
 
 // A thread's share of a tile, U loads of E elements, kept as it was read: bf16 stays packed, two to a word, unless a soft
-// cap makes other numbers of it.  VEC: loads of 16 bytes, element e of load u is (u * 256 + thread) * E + e of the tile; else
-// single elements, (u * E + e) * 256 + thread: the same for every row, so that equal rows have equal sums.
+// cap makes other numbers of it.  A warp's share is a group, kGroup neighbouring elements.  VEC: loads of 16 bytes, element e of
+// load u is (u * 32 + lane) * E + e of the group; else single elements, (u * E + e) * 32 + lane.  The same for every row of a
+// call, so that equal rows have equal sums.
 template <bool BF16, bool VEC, bool CAP>
 struct BeamTile {
     static constexpr int E = BF16 ? 8 : 4;
     static constexpr int U = 4;
-    static constexpr int kLen = kBeamThreads * U * E;
+    static constexpr int kGroup = 32 * U * E;
+    static constexpr int kLen = kBeamWarps * kGroup;
     static constexpr bool kPacked = BF16 && !CAP;
-    static constexpr uint32_t kLow = kPacked ? 0xFF80FF80u : 0xFF800000u;  // -infinity
     uint32_t w[U][kPacked ? E / 2 : E];
 
     static __device__ __forceinline__ int at(int u, int e)
     {
-        return VEC ? (u * kBeamThreads + (int)threadIdx.x) * E + e : (u * E + e) * kBeamThreads + (int)threadIdx.x;
+        const int lane = threadIdx.x & 31;
+        return VEC ? (u * 32 + lane) * E + e : (u * E + e) * 32 + lane;
     }
     __device__ __forceinline__ float get(int u, int e) const
     {
@@ -81,278 +83,230 @@ struct BeamTile {
             w[u][e] = __float_as_uint(load_one<BF16>(row, j));
         }
     }
-
-    // The tile that starts at `base`; masked elements and those at or beyond `end` read as -infinity.  A vector without an
-    // allowed element is not read.
-    __device__ __forceinline__ void load(const LogitRow row, const uint32_t *mrow, int base, int end)
+    __device__ __forceinline__ void whole(const LogitRow row, int i, int u)
     {
-        uint32_t allowed[U];
+        const uint4 t = BF16 ? __ldcs((const uint4 *)((const uint16_t *)row.p + i)) : __ldcs((const uint4 *)((const float *)row.p + i));
+        if constexpr (kPacked || !BF16) {
+            w[u][0] = t.x; w[u][1] = t.y; w[u][2] = t.z; w[u][3] = t.w;
+        } else {
+            const uint32_t p[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            allowed[u] = 0xFFu;
-            if (mrow == nullptr) continue;
-            const int i = base + at(u, 0);
-            if constexpr (VEC) {
-                allowed[u] = i < end ? (uint32_t)__ldg((const uint8_t *)mrow + (i >> 3)) >> (i & 7) : 0u;
-                if (!BF16) allowed[u] &= 0xFu;
-            } else {
-                allowed[u] = 0u;
-#pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (base + at(u, e) < end && mask_bit(mrow, base + at(u, e))) allowed[u] |= 1u << e;
-            }
+            for (int e = 0; e < E; e++) w[u][e] = (e & 1) ? p[e / 2] & 0xFFFF0000u : p[e / 2] << 16;
         }
+        if constexpr (CAP)
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int i = base + at(u, 0);
-#pragma unroll
-            for (int x = 0; x < (kPacked ? E / 2 : E); x++) w[u][x] = kLow;
-            if (VEC && i + E <= end) {
-                if (allowed[u] == 0u) continue;
-                if constexpr (BF16) {
-                    const uint4 t = __ldcs((const uint4 *)((const uint16_t *)row.p + i));
-                    if constexpr (kPacked) {
-                        w[u][0] = t.x; w[u][1] = t.y; w[u][2] = t.z; w[u][3] = t.w;
-                    } else {
-                        const uint32_t p[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-                        for (int e = 0; e < E; e++) w[u][e] = (e & 1) ? p[e / 2] & 0xFFFF0000u : p[e / 2] << 16;
-                    }
-                } else {
-                    const uint4 t = __ldcs((const uint4 *)((const float *)row.p + i));
-                    w[u][0] = t.x; w[u][1] = t.y; w[u][2] = t.z; w[u][3] = t.w;
-                }
-                if constexpr (CAP)
-#pragma unroll
-                    for (int e = 0; e < E; e++) w[u][e] = __float_as_uint(soft_cap(get(u, e), row.cap));
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (base + at(u, e) < end && (allowed[u] >> e & 1u)) one(row, u, e, base + at(u, e));
-            }
-        }
-        if (VEC && mrow != nullptr)
+            for (int e = 0; e < E; e++) w[u][e] = __float_as_uint(soft_cap(get(u, e), row.cap));
+    }
+
+    __device__ __forceinline__ float top() const
+    {
+        if constexpr (kPacked) {
+            uint32_t m = w[0][0];
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
+                for (int x = 0; x < E / 2; x++) asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[u][x]));
+            return fmaxf(fmaxf(-CUDART_INF_F, bf16_lo(m)), bf16_hi(m));
+        } else {
+            float m = -CUDART_INF_F;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int e = 0; e < E; e += 2) asm("max.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(get(u, e)), "f"(get(u, e + 1)));
+            return m;
+        }
+    }
+
+    // Which elements of the thread's share of the group at `base` are allowed, bit u * E + e
+    static __device__ __forceinline__ uint32_t allowed(const uint32_t *mrow, int base, int end)
+    {
+        if (mrow == nullptr) return 0xFFFFFFFFu;
+        uint32_t ok = 0u;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = base + at(u, 0);
+            if constexpr (VEC) {
+                const uint32_t b = i < end ? (uint32_t)__ldg((const uint8_t *)mrow + (i >> 3)) >> (i & 7) : 0u;
+                ok |= (b & (BF16 ? 0xFFu : 0xFu)) << (u * E);
+            } else {
+#pragma unroll
                 for (int e = 0; e < E; e++)
-                    if (!(allowed[u] >> e & 1u)) set_low(u, e);
-    }
-};
-
-// exp(d), d <= 0 or little above it: 2 to the power of d * log2(e), whose low bits log2(e) needs two floats for
-static __device__ __forceinline__ float beam_exp(float d)
-{
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(d, 1.9259629e-8f, d * 1.44269502f)));
-    return e;
-}
-
-struct RowShared {
-    u64 list[kBeamList];
-    uint32_t tops[kBeamThreads];  // largest logits of the first tile
-    float ref[kBeamWarps], top[kBeamWarps];
-    double sum[kBeamWarps];
-    u64 thr;                      // later elements are among the n best only above this key
-    int cnt;
-};
-
-struct MergeShared {
-    u64 score[kMergeList], key[kMergeList];  // candidates: score, and logit and token
-    uint8_t beam[kMergeList];
-    float top[kMergeParts];                  // largest logit of a piece
-    uint16_t open[kMergeParts];              // pieces that hold a candidate
-    uint32_t tops[kBeamThreads];
-    double base[STG_BEAM_MAX_BEAMS];         // a beam's candidates score base + (logit - ref); -infinity: it has none
-    float ref[STG_BEAM_MAX_BEAMS];
-    u64 bound;                               // candidates with a lower score are not among the n best
-    uint32_t head;                           // ... the same, as a float rounded down
-    uint32_t flags;
-    int cnt, n_open;
-};
-
-// Sorts the first `cnt` entries of `list` descending (bitonic, padded with zeros: no key is 0).  All threads.
-static __device__ void sort_list(u64 *list, int cnt)
-{
-    int len = 32;
-    while (len < cnt) len <<= 1;
-    for (int i = cnt + threadIdx.x; i < len; i += kBeamThreads) list[i] = 0ull;
-    __syncthreads();
-    for (int k = 2; k <= len; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int t = threadIdx.x; t < len / 2; t += kBeamThreads) {
-                const int a = 2 * j * (t / j) + t % j, b = a + j;
-                const u64 x = list[a], y = list[b];
-                if ((x < y) == ((a & k) == 0)) { list[a] = y; list[b] = x; }
+                    if (base + at(u, e) < end && mask_bit(mrow, base + at(u, e))) ok |= 1u << (u * E + e);
             }
-            __syncthreads();
         }
-}
-
-// Leaves the n best of the list, sorted, and the n-th as the bound.  All threads; the list has settled.
-static __device__ void keep_best(RowShared &sh, int n)
-{
-    const int c = sh.cnt, tid = threadIdx.x;
-    if (c > kBeamThreads) {
-        sort_list(sh.list, c);
-    } else {  // every entry counts those ahead of it: the keys are distinct
-        const u64 mine = tid < c ? sh.list[tid] : 0ull;
-        int ahead = kBeamThreads;
-        if (tid < c) {
-            ahead = 0;
-            for (int i = 0; i < c; i++) ahead += sh.list[i] > mine;
+        return ok;
+    }
+    // The group that starts at `base`; elements that are not `ok` and those at or beyond `end` read as -infinity.  A vector
+    // without an allowed element is not read.
+    __device__ __forceinline__ void load(const LogitRow row, bool masked, uint32_t ok, int base, int end)
+    {
+        if (!masked && base + kGroup <= end) {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if constexpr (VEC) whole(row, base + at(u, 0), u);
+                else
+#pragma unroll
+                    for (int e = 0; e < E; e++) one(row, u, e, base + at(u, e));
+            }
+            return;
         }
-        __syncthreads();
-        if (ahead < n) sh.list[ahead] = mine;
-        __syncthreads();
+        constexpr uint32_t kAll = BF16 ? 0xFFu : 0xFu;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+#pragma unroll
+            for (int x = 0; x < (kPacked ? E / 2 : E); x++) w[u][x] = kPacked ? 0xFF80FF80u : 0xFF800000u;
+            if (VEC && base + at(u, 0) + E <= end) {
+                if (ok >> (u * E) & kAll) whole(row, base + at(u, 0), u);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (base + at(u, e) < end && (ok >> (u * E + e) & 1u)) one(row, u, e, base + at(u, e));
+            }
+        }
     }
-    if (tid == 0) {
-        sh.cnt = min(c, n);
-        if (c >= n) sh.thr = sh.list[n - 1];
+    // ... once the loads are back
+    __device__ __forceinline__ void mask(uint32_t ok)
+    {
+        if (ok == (uint32_t)((1ull << (U * E)) - 1ull) || ok == 0xFFFFFFFFu) return;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (!(ok >> (u * E + e) & 1u)) set_low(u, e);
     }
-    __syncthreads();
-}
+};
 
-// The n-th largest of `tops` (`len` entries, a multiple of 32), found by counting; published by the thread that holds it.
-static __device__ __forceinline__ bool is_nth(const uint32_t *tops, int len, int n)
+typedef unsigned long long f32x2;
+static __device__ __forceinline__ f32x2 pair(float a, float b)
 {
-    const int tid = threadIdx.x;
-    if (tid >= len) return false;
-    const uint32_t mine = tops[tid];
-    int ahead = 0;
-    for (int i = 0; i < len; i += 4) {
-        const uint4 t = *(const uint4 *)(tops + i);
-        ahead += (t.x > mine || (t.x == mine && i < tid)) + (t.y > mine || (t.y == mine && i + 1 < tid)) +
-                 (t.z > mine || (t.z == mine && i + 2 < tid)) + (t.w > mine || (t.w == mine && i + 3 < tid));
-    }
-    return ahead == n - 1;
+    f32x2 p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+static __device__ __forceinline__ void unpair(f32x2 p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+static __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b)
+{
+    f32x2 c;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(c) : "l"(a), "l"(b));
+    return c;
+}
+static __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c)
+{
+    f32x2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
 }
 
-// One piece of a row: its sum and its n best logits, into the workspace.
+// exp(x) / 2^c of two numbers, as 2^(x log2(e) - c), for which log2(e) takes two floats: one alone is off by 1.3e-8, which a
+// row's sum would be off by times its logits' distance from zero.  The product with the first is not rounded before
+// c is taken off.
+static __device__ __forceinline__ f32x2 exp_pair(f32x2 x, f32x2 minus_c)
+{
+    float a, b;
+    unpair(fma2(x, pair(1.9259629e-8f, 1.9259629e-8f), fma2(x, pair(1.44269502f, 1.44269502f), minus_c)), a, b);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+    return pair(a, b);
+}
+
+static __device__ __forceinline__ float warp_max(float v)
+{
+    asm("redux.sync.max.f32 %0, %0, 0xFFFFFFFF;" : "+f"(v));
+    return v;
+}
+
+// What a sum with reference `from` is multiplied by to have reference `to`
+static __device__ __noinline__ double scale(double from, double to) { return exp(from - to); }
+
+constexpr double kLn2 = 0.69314718055994530942;
+constexpr float kHuge = 1e6f;  // logits beyond take the slow way: c could not tell them apart
+
+// The largest reference of a warp, or one that 32 bits do not tell from it
+static __device__ __forceinline__ double warp_ref(double r)
+{
+    const float f = (float)r;
+    return __shfl_sync(0xFFFFFFFFu, r, __ffs(__ballot_sync(0xFFFFFFFFu, f == warp_max(f))) - 1);
+}
+
+// The sum of exp(x - top) over a group with logits beyond kHuge, element by element.
 template <bool BF16, bool VEC, bool CAP>
-static __device__ __forceinline__ void beam_piece(const BeamSelect &a, RowShared &sh, int row, int piece)
+static __device__ __noinline__ float huge_group(const LogitRow lr, const uint32_t *mrow, int base, int end, float top)
+{
+    float part = 0.f;
+#pragma unroll 1
+    for (int i = base + (int)(threadIdx.x & 31); i < min(end, base + BeamTile<BF16, VEC, CAP>::kGroup); i += 32)
+        if (mrow == nullptr || mask_bit(mrow, i)) part += expf(load_one<BF16>(lr, i) - top);
+    return part;
+}
+
+// One piece of a row: its part of the sum and the maxima of its groups.
+template <bool BF16, bool VEC, bool CAP>
+static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, int piece)
 {
     typedef BeamTile<BF16, VEC, CAP> T;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n;
+    __shared__ double refs[kBeamWarps], sums[kBeamWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const LogitRow lr{(const char *)a.logits + (int64_t)row * a.row_stride * (BF16 ? 2 : 4), CAP ? a.softcap : 0.f};
     const uint32_t *mrow = a.mask != nullptr && (a.uses_mask == nullptr || a.uses_mask[row]) ? a.mask + (int64_t)row * a.mask_stride : nullptr;
-    const int begin = piece * a.piece_len, end = min(a.vocab, begin + a.piece_len);
-    if (tid == 0) { sh.cnt = 0; sh.thr = kNoKey; }
-    __syncthreads();
-    float ref = -CUDART_INF_F;  // the sum's terms are exp(x - ref); the same for a warp
-    float best = -CUDART_INF_F;
-    double s = 0.0;
-
+    const int begin = piece * a.piece_len + warp * T::kGroup, end = min(a.vocab, (piece + 1) * a.piece_len);
+    float *tops = a.ws.tops + (int64_t)row * a.groups;
+    // The sum's terms are exp(x) / 2^c; the same for a warp.  2^c need only be near the largest: c is a multiple of 16, so
+    // that most warps of a row have the same and their sums need no scaling, and follows the maximum `limit` at a time.
+    float c = 0.f, limit = -CUDART_INF_F;
+    double ref = -CUDART_INF, s = 0.0;  // c ln 2, what the terms are relative to
+    // A group's loads are in flight while the one ahead of it is added up, its mask's a group earlier still.
+    uint32_t ok = T::allowed(mrow, begin, end), next_ok = T::allowed(mrow, begin + T::kLen, end);
+    T next;
+    if (begin < end) next.load(lr, mrow != nullptr, ok, begin, end);
+#pragma unroll 1
     for (int base = begin; base < end; base += T::kLen) {
-        T t;
-        t.load(lr, mrow, base, end);
-        float top = -CUDART_INF_F;
-#pragma unroll
-        for (int u = 0; u < T::U; u++)
-#pragma unroll
-            for (int e = 0; e < T::E; e++) top = fmaxf(top, t.get(u, e));
-        best = fmaxf(best, top);
-        // The reference need not be the maximum: it follows when a logit is so far above it that terms grow large.
-        if (__any_sync(0xFFFFFFFFu, top > ref + 16.f)) {
-            const float now = unord32(__reduce_max_sync(0xFFFFFFFFu, ord32(fmaxf(top, ref))));
-            s *= exp((double)ref - (double)now);
+        T t = next;
+        t.mask(ok);
+        ok = next_ok;
+        if (base + T::kLen < end) {
+            next.load(lr, mrow != nullptr, ok, base + T::kLen, end);
+            next_ok = T::allowed(mrow, base + 2 * T::kLen, end);
+        }
+        const float top = warp_max(t.top());
+        if (lane == 0) tops[base / T::kGroup] = top;
+        if ((fabsf(top) > kHuge || ref > (double)kHuge) && top > -CUDART_INF_F) {
+            const double now = fmax(ref, (double)top);
+            if (now != ref) {
+                s *= scale(ref, now);
+                ref = now;
+                limit = -CUDART_INF_F;  // no c any more
+            }
+            s += (double)huge_group<BF16, VEC, CAP>(lr, mrow, base, end, top) * scale((double)top, now);
+            continue;
+        }
+        if (top > limit) {
+            c = floorf(top * (1.44269502f / 16.f)) * 16.f;
+            limit = (c + 48.f) * 0.693147181f;
+            const double now = (double)c * kLn2;
+            if (now != ref) s *= scale(ref, now);
             ref = now;
         }
-        const float r = ref == -CUDART_INF_F ? 0.f : ref;  // nothing yet but -infinity, and NaN, which the sum has to show
-        float part = 0.f;
+        f32x2 part = pair(0.f, 0.f);
+        const f32x2 minus_c = pair(-c, -c);
 #pragma unroll
         for (int u = 0; u < T::U; u++)
 #pragma unroll
-            for (int e = 0; e < T::E; e++) part += beam_exp(t.get(u, e) - r);
-        s += (double)part;
-
-        if (base == begin) {
-            // At least n elements are as large as the n-th largest of the maxima of disjoint groups of them: 64 groups
-            // bound it well for up to 32, and are counted through in a quarter of the time of 256.
-            const int groups = n <= 32 ? 64 : kBeamThreads;
-            float g = top;
-            if (n <= 32) {
-                g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, 1));
-                g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, 2));
-                if ((tid & 3) == 0) sh.tops[tid >> 2] = ord32(g);
-            } else {
-                sh.tops[tid] = ord32(g);
-            }
-            __syncthreads();
-            if (is_nth(sh.tops, groups, n) && sh.tops[tid] > (uint32_t)(kNoKey >> 32)) sh.thr = (u64)sh.tops[tid] << 32;
-            __syncthreads();
-        }
-        u64 bound = sh.thr;
-        const float low = key_val(bound);
-        const int before = sh.cnt;
-        if (!__syncthreads_or(top >= low && top > -CUDART_INF_F)) continue;
-        if (top >= low) {
-#pragma unroll
-            for (int u = 0; u < T::U; u++)
-#pragma unroll
-                for (int e = 0; e < T::E; e++) {
-                    const float x = t.get(u, e);
-                    if (x >= low) {
-                        const u64 key = make_key(x, base + T::at(u, e));
-                        if (key > bound) {
-                            const int slot = atomicAdd(&sh.cnt, 1);
-                            if (slot < kBeamList) sh.list[slot] = key;
-                        }
-                    }
-                }
-        }
-        __syncthreads();
-        const int c = sh.cnt;
-        if (c > kBeamList) {
-            // More than there is room for (a row that ascends, or one of equal logits): once more, one element of every
-            // thread at a time.
-            __syncthreads();
-            if (tid == 0) sh.cnt = before;
-#pragma unroll
-            for (int u = 0; u < T::U; u++)
-#pragma unroll
-                for (int e = 0; e < T::E; e++) {
-                    __syncthreads();
-                    const int now = sh.cnt;
-                    __syncthreads();  // read by all before anyone appends
-                    if (now > kBeamList - kBeamThreads) {
-                        keep_best(sh, n);
-                        bound = sh.thr;
-                    }
-                    const float x = t.get(u, e);
-                    const u64 key = make_key(x, base + T::at(u, e));
-                    if (x >= key_val(bound) && key > bound) sh.list[atomicAdd(&sh.cnt, 1)] = key;
-                }
-            __syncthreads();
-            keep_best(sh, n);
-        } else if (c >= 2 * n) {
-            keep_best(sh, n);
-        }
+            for (int e = 0; e < T::E; e += 2) part = add2(part, exp_pair(pair(t.get(u, e), t.get(u, e + 1)), minus_c));
+        float p0, p1;
+        unpair(part, p0, p1);
+        s += (double)(p0 + p1);
     }
-
-    keep_best(sh, n);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-        best = fmaxf(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
-    }
-    if (lane == 0) { sh.sum[warp] = s; sh.ref[warp] = ref; sh.top[warp] = best; }
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    if (lane == 0) { sums[warp] = s; refs[warp] = ref; }
     __syncthreads();
-    const int64_t at = (int64_t)row * a.pieces + piece;
-    for (int i = tid; i < n; i += kBeamThreads) a.ws.keys[at * n + i] = i < sh.cnt ? sh.list[i] : 0ull;
     if (warp == 0) {
-        const float wr = sh.ref[lane & 7];
-        float r = wr, b = sh.top[lane & 7];
-        double ws = sh.sum[lane & 7];
+        const double wr = refs[lane % kBeamWarps], r = warp_ref(wr);
+        double ws = sums[lane % kBeamWarps];
+        if (wr != r) ws *= scale(wr, r);  // 0 for a warp that has read -infinity alone
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
-            r = fmaxf(r, __shfl_xor_sync(0xFFFFFFFFu, r, o));
-            b = fmaxf(b, __shfl_xor_sync(0xFFFFFFFFu, b, o));
-        }
-        if (wr != r) ws *= exp((double)wr - (double)r);  // 0 for a warp that has read -infinity alone
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) ws += __shfl_xor_sync(0xFFFFFFFFu, ws, o);
-        if (lane == 0) a.ws.parts[at] = BeamPart{ws, r, b};
+        for (int o = kBeamWarps / 2; o > 0; o >>= 1) ws += __shfl_xor_sync(0xFFFFFFFFu, ws, o);
+        if (lane == 0) a.ws.parts[(int64_t)row * a.pieces + piece] = BeamPart{ws, r};
     }
 }
 
@@ -366,161 +320,394 @@ static __device__ __forceinline__ double unord64(u64 k)
     return __longlong_as_double((long long)((k >> 63) ? (k & 0x7FFFFFFFFFFFFFFFull) : ~k));
 }
 
-static __device__ __forceinline__ double beam_score(const MergeShared &sh, int k, float x)
-{
-    return ((double)x - (double)sh.ref[k]) + sh.base[k];
-}
+// What is ordered: groups, by their best candidate, and candidates.  Larger score (ord64), then lower beam, then larger key
+// (make_key: the logit, then the lower group or token).
+constexpr int kStage = 8;  // loads of a thread in flight, 8 of 4 bytes or 4 of 16
+struct MergeShared {
+    union {
+        float head[kStage][kBeamThreads];
+        uint4 vec[kStage / 2][kBeamThreads];
+    } stage;
+    u64 score[kBeamList], key[kBeamList];
+    uint32_t tops[256];
+    uint8_t beam[kBeamList];
+    u64 kept_score[STG_BEAM_MAX_CANDIDATES], kept_key[STG_BEAM_MAX_CANDIDATES];
+    uint8_t kept_beam[STG_BEAM_MAX_CANDIDATES];
+    double base[STG_BEAM_MAX_BEAMS];   // a beam's candidates score base + (logit - ref); -infinity: it has none
+    double ref[STG_BEAM_MAX_BEAMS];
+    float about[STG_BEAM_MAX_BEAMS];   // ... about that + logit
+    float least[STG_BEAM_MAX_BEAMS];   // no smaller logit reaches `low`; NaN: the beam has no candidates
+    int group[STG_BEAM_MAX_CANDIDATES];          // the groups that are read again
+    uint8_t group_beam[STG_BEAM_MAX_CANDIDATES];
+    u64 bound_score, bound_key;        // the n-th best so far
+    int bound_beam;
+    uint32_t low;                      // a float, as ord32, that n scores reach; 0: none
+    uint32_t flags;
+    int cnt;
 
-// Leaves the n best candidates of the list, in order.  All threads; the list has settled.
-static __device__ void keep_candidates(MergeShared &sh, int n)
-{
-    constexpr int kOwn = kMergeList / kBeamThreads;
-    const int c = sh.cnt, tid = threadIdx.x;
-    u64 s[kOwn], w[kOwn];
-    uint8_t k[kOwn];
-    int rank[kOwn];
-#pragma unroll
-    for (int r = 0; r < kOwn; r++) {
-        const int e = r * kBeamThreads + tid;
-        rank[r] = kMergeList;
-        if (e >= c) continue;
-        s[r] = sh.score[e]; w[r] = sh.key[e]; k[r] = sh.beam[e];
-        int ahead = 0;
-        for (int o = 0; o < c; o++) {
-            const u64 x = sh.score[o];
-            if (x < s[r]) continue;
-            ahead += x > s[r] || sh.beam[o] < k[r] || (sh.beam[o] == k[r] && sh.key[o] > w[r]);
+    __device__ __forceinline__ u64 score_of(int k, float x) const { return ord64(((double)x - ref[k]) + base[k]); }
+    __device__ __forceinline__ static uint32_t round_down(u64 score) { return ord32(__double2float_rd(unord64(score))); }
+    __device__ __forceinline__ void clear()
+    {
+        cnt = 0;
+        bound_score = bound_key = 0ull;
+        bound_beam = STG_BEAM_MAX_BEAMS;
+    }
+    // `least` of beam k: the sum that makes a score is off by a few 2^-53 of its terms
+    __device__ __forceinline__ void set_least(int k)
+    {
+        const double b = base[k], r = ref[k];
+        float x = b > -CUDART_INF ? -CUDART_INF_F : CUDART_NAN_F;
+        if (low != 0u && b > -CUDART_INF) {
+            const double l = (double)unord32(low);
+            x = __double2float_rd(((l - b) + r) - 1e-14 * (fabs(l) + fabs(b) + fabs(r)));
         }
-        rank[r] = ahead;
+        least[k] = x;
     }
-    __syncthreads();
+    // x has reached `least`: it may be one of the n best.  Its score is made when all have come.
+    __device__ __forceinline__ void offer(float x, int k, int pos)
+    {
+        const int at = atomicAdd(&cnt, 1);
+        if (at < kBeamList) { key[at] = make_key(x, pos); beam[at] = (uint8_t)k; }
+    }
+    // The same with its score at once, which the n-th best so far is held against
+    __device__ __noinline__ void offer_if_ahead(float x, int k, int pos)
+    {
+        const u64 s = score_of(k, x), w = make_key(x, pos);
+        if (s < bound_score || (s == bound_score && (k > bound_beam || (k == bound_beam && w <= bound_key)))) return;
+        const int at = atomicAdd(&cnt, 1);
+        if (at < kBeamList) { score[at] = s; key[at] = w; beam[at] = (uint8_t)k; }
+    }
+};
+
+// The code below runs once per call and sequence, so what it takes is latency, that of fetching its instructions
+// included: loops are left rolled and what is used twice is a function, while loads are issued several at a time.
+
+// `low` out of every thread's best item (x of beam k; -infinity: none), such that n scores reach it.  Up to 32: the n-th
+// largest of 64 groups of threads, each of which counts those above its own.  Beyond: the upper 20 bits of the n-th
+// largest of 256, found two by two (0.9 us against 0.3).  0 where there are no n.  All threads.
+static __device__ __noinline__ void find_low(MergeShared &sh, int K, int n, float x, int k)
+{
+    const int tid = threadIdx.x;
+    uint32_t mine = x > -CUDART_INF_F ? MergeShared::round_down(sh.score_of(k, x)) : 0u;
+    const int per = n <= 32 ? kBeamThreads / 64 : kBeamThreads / 256;
 #pragma unroll
-    for (int r = 0; r < kOwn; r++)
-        if (rank[r] < n) { sh.score[rank[r]] = s[r]; sh.key[rank[r]] = w[r]; sh.beam[rank[r]] = k[r]; }
+    for (int o = 1; o < kBeamThreads / 64; o *= 2)
+        if (o < per) mine = max(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, o));
+    if (tid % per == 0) sh.tops[tid / per] = mine;
     __syncthreads();
-    if (tid == 0) {
-        sh.cnt = min(c, n);
-        if (c >= n) sh.bound = sh.score[n - 1];
+    if (n <= 32) {
+        if (tid < 64) {
+            mine = sh.tops[tid];
+            int ahead = 0;
+#pragma unroll 4
+            for (int i = 0; i < 64; i += 4) {
+                const uint4 v = *(const uint4 *)(sh.tops + i);
+                ahead += (v.x > mine || (v.x == mine && i < tid)) + (v.y > mine || (v.y == mine && i + 1 < tid)) +
+                         (v.z > mine || (v.z == mine && i + 2 < tid)) + (v.w > mine || (v.w == mine && i + 3 < tid));
+            }
+            if (ahead == n - 1) sh.low = max(sh.low, mine);
+        }
+    } else if (tid < 32) {
+        uint32_t v[8], found = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = sh.tops[tid + 32 * i];
+#pragma unroll 1
+        for (int shift = 30; shift >= 12; shift -= 2) {
+            const uint32_t t1 = found | (1u << shift), t2 = found | (2u << shift), t3 = found | (3u << shift);
+            uint32_t reach = 0u;  // three counts of up to 256
+#pragma unroll
+            for (int i = 0; i < 8; i++) reach += (v[i] >= t1 ? 1u : 0u) + (v[i] >= t2 ? 1u << 10 : 0u) + (v[i] >= t3 ? 1u << 20 : 0u);
+            reach = __reduce_add_sync(0xFFFFFFFFu, reach);
+            if ((reach >> 20) >= (uint32_t)n) found = t3;
+            else if ((reach >> 10 & 1023u) >= (uint32_t)n) found = t2;
+            else if ((reach & 1023u) >= (uint32_t)n) found = t1;
+        }
+        if (tid == 0) sh.low = max(sh.low, found);
     }
+    __syncthreads();
+    if (tid < K) sh.set_least(tid);
     __syncthreads();
 }
 
-// The candidates of one sequence out of its rows' pieces, which other CTAs have written: read past the first-level cache.
+// Hands the n best of a list of c entries to emit(place, score, key, beam), in whatever order.  Eight threads per entry count
+// those ahead of it: no two are the same.  All threads; the list has settled.
+template <class Emit>
+static __device__ __forceinline__ void rank_list(MergeShared &sh, int c, int n, Emit emit)
+{
+    constexpr int kPer = 8;
+    const int tid = threadIdx.x, sub = tid % kPer;
+#pragma unroll 1
+    for (int first = 0; first < c; first += kBeamThreads / kPer) {
+        const int e = first + tid / kPer;
+        u64 s = 0ull, w = 0ull;
+        int k = 0, ahead = 0;
+        if (e < c) {
+            s = sh.score[e]; w = sh.key[e]; k = sh.beam[e];
+#pragma unroll 2
+            for (int o = sub; o < c; o += kPer) {
+                const u64 x = sh.score[o];
+                if (x >= s) ahead += x > s || sh.beam[o] < k || (sh.beam[o] == k && sh.key[o] > w);
+            }
+        }
+#pragma unroll
+        for (int o = kPer / 2; o > 0; o >>= 1) ahead += __shfl_xor_sync(0xFFFFFFFFu, ahead, o);
+        if (e < c && sub == 0 && ahead < n) emit(ahead, s, w, k);
+    }
+}
+
+// Leaves the n best of the list and the n-th as the bound.  All threads; the list has settled, and settles again.
+static __device__ __noinline__ void keep_best(MergeShared &sh, int c, int n)
+{
+    rank_list(sh, c, n, [&](int to, u64 s, u64 w, int k) {
+        sh.kept_score[to] = s; sh.kept_key[to] = w; sh.kept_beam[to] = (uint8_t)k;
+        if (to == n - 1) { sh.bound_score = s; sh.bound_key = w; sh.bound_beam = k; }
+    });
+    __syncthreads();
+    const int left = min(c, n), tid = threadIdx.x;
+    if (tid < left) { sh.score[tid] = sh.kept_score[tid]; sh.key[tid] = sh.kept_key[tid]; sh.beam[tid] = sh.kept_beam[tid]; }
+    if (tid == 0) sh.cnt = left;
+    __syncthreads();
+}
+
+// After items have been offered: the list holds the n best of them and perhaps more; how many.  Where more were offered than
+// it takes - many equal ones - all of them are offered again, get(i, x, k, pos) for i below `total`, some at a time, with a
+// bound that tells them apart.
+template <class Get>
+static __device__ __forceinline__ int settle(MergeShared &sh, int total, int n, Get get)
+{
+    __syncthreads();
+    int c = sh.cnt;
+    if (c <= kBeamList) {
+#pragma unroll 1
+        for (int i = threadIdx.x; i < c; i += kBeamThreads) sh.score[i] = sh.score_of(sh.beam[i], key_val(sh.key[i]));
+        __syncthreads();
+        return c;
+    }
+    __syncthreads();  // read by all before it changes
+    if (threadIdx.x == 0) sh.cnt = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int first = 0; first < total; first += kBeamRoom) {
+        float x;
+        int k, pos;
+        const int i = first + (int)threadIdx.x;
+        if (threadIdx.x < kBeamRoom && i < total && get(i, x, k, pos) && x >= sh.least[k] && x > -CUDART_INF_F) sh.offer_if_ahead(x, k, pos);
+        __syncthreads();
+        c = sh.cnt;
+        __syncthreads();
+        if (c > kBeamList - kBeamRoom) keep_best(sh, c, n);
+    }
+    c = sh.cnt;
+    __syncthreads();
+    return c;
+}
+
+// The candidates of one sequence out of its rows' sums and group maxima, which other CTAs have written: read past the
+// first-level cache.
+template <bool BF16, bool VEC, bool CAP>
 static __device__ __forceinline__ void beam_merge(const BeamSelect &a, MergeShared &sh, int seq)
 {
+    typedef BeamTile<BF16, VEC, CAP> T;
     const int tid = threadIdx.x, lane = tid & 31;
-    const int K = a.beams, n = a.n, C = a.pieces, P = K * C;
-    const BeamPart *parts = a.ws.parts + (int64_t)seq * P;
-    const u64 *keys = a.ws.keys + (int64_t)seq * P * n;
-    if (tid == 0) { sh.cnt = 0; sh.n_open = 0; sh.bound = 0ull; sh.head = 0u; sh.flags = 0u; }
+    const int K = a.beams, n = a.n, C = a.pieces, G = a.groups, heads = K * G;
+    const float *tops = a.ws.tops + (int64_t)seq * heads;
+    float head[kStage];
+    auto load_heads = [&](int from) {
+#pragma unroll
+        for (int j = 0; j < kStage; j++) head[j] = from + j * kBeamThreads + tid < heads ? __ldcg(tops + from + j * kBeamThreads + tid) : -CUDART_INF_F;
+    };
+    auto stage_heads = [&]() {
+#pragma unroll
+        for (int j = 0; j < kStage; j++) sh.stage.head[j][tid] = head[j];  // a thread reads what it wrote
+    };
+    load_heads(0);
+    if (tid == 0) { sh.clear(); sh.low = 0u; sh.flags = 0u; }
     __syncthreads();
+#pragma unroll 1
     for (int k = tid >> 5; k < K; k += kBeamWarps) {
         const int row = seq * K + k;
         const float score = a.scores[row];
         const bool alive = score > -CUDART_INF_F && score < CUDART_INF_F;
-        float r = -CUDART_INF_F;
-        double s = 0.0;
+        double r = -CUDART_INF, s = 0.0;
+#pragma unroll 1
         for (int c = lane; c < C; c += 32) {
-            BeamPart p{0.0, -CUDART_INF_F, -CUDART_INF_F};
-            if (alive) {
-                const uint4 raw = __ldcg((const uint4 *)(parts + k * C + c));
-                p.s = __hiloint2double((int)raw.y, (int)raw.x);
-                p.ref = __uint_as_float(raw.z);
-                p.top = __uint_as_float(raw.w);
-            }
-            sh.top[k * C + c] = p.top;
-            const float now = fmaxf(r, p.ref);
-            if (now != r) s *= exp((double)r - (double)now);
-            s += p.ref == now ? p.s : p.s * exp((double)p.ref - (double)now);
+            const double2 p = __ldcg((const double2 *)(a.ws.parts + (int64_t)row * C + c));  // of a dead beam: not written, not used
+            const double now = fmax(r, p.y);
+            if (now != r) s *= scale(r, now);
+            s += p.y != now ? p.x * scale(p.y, now) : p.x;
             r = now;
         }
-        float m = r;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        if (r != m) s *= exp((double)r - (double)m);
+        if (!alive) { r = -CUDART_INF; s = 0.0; }
+        const double m = warp_ref(r);
+        if (r != m) s *= scale(r, m);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
         if (lane == 0) {
-            const bool none = m == -CUDART_INF_F && s == 0.0;        // dead, or nothing in the row
+            const bool none = m == -CUDART_INF && s == 0.0;         // dead, or nothing in the row
             const bool bad = !none && !(s > 0.0 && s < CUDART_INF);  // NaN or +infinity among the logits
             const double logs = log(s);
             sh.base[k] = none || bad ? -CUDART_INF : (double)score - logs;
             sh.ref[k] = m;
+            sh.about[k] = (float)(((double)score - logs) - m);
+            sh.least[k] = none || bad ? CUDART_NAN_F : -CUDART_INF_F;
             if (bad) atomicOr(&sh.flags, STG_BEAM_BAD_ROW);
             if (alive && none) atomicOr(&sh.flags, STG_ROW_FULLY_MASKED);
-            if (a.log_norms) a.log_norms[row] = none ? -CUDART_INF_F : (float)((double)m + logs);
+            if (a.log_norms) a.log_norms[row] = none ? -CUDART_INF_F : (float)(m + logs);
         }
     }
+    stage_heads();
     __syncthreads();
-    // The n-th largest of the pieces' best candidates (of groups of pieces, one per thread) bounds all others from below.
-    // Rounded down to 32 bits, which keeps their order.
-    uint32_t mine = 0u;
-    for (int p = tid; p < P; p += kBeamThreads) {
-        const int k = p / C;
-        if (sh.base[k] > -CUDART_INF && sh.top[p] > -CUDART_INF_F) mine = max(mine, ord32(__double2float_rd(beam_score(sh, k, sh.top[p]))));
-    }
-    sh.tops[tid] = mine;
-    __syncthreads();
-    const int groups = min(kBeamThreads, (P + 31) & ~31);
-    if (n <= groups && is_nth(sh.tops, groups, n)) sh.head = mine;
-    __syncthreads();
-    const uint32_t head = sh.head;
-    for (int p = tid; p < P; p += kBeamThreads) {
-        const int k = p / C;
-        if (sh.base[k] > -CUDART_INF && sh.top[p] > -CUDART_INF_F && ord32(__double2float_rd(beam_score(sh, k, sh.top[p]))) >= head)
-            sh.open[atomicAdd(&sh.n_open, 1)] = (uint16_t)p;
-    }
-    __syncthreads();
-    const int total = sh.n_open * n;
-    for (int first = 0; first < total; first += kBeamThreads) {
-        const int i = first + tid;
-        if (i < total) {
-            const int p = sh.open[i / n], k = p / C;
-            const u64 key = __ldcg(keys + (int64_t)p * n + i % n);
-            if (key != 0ull) {
-                const double v = beam_score(sh, k, key_val(key));
-                const u64 s = ord64(v);
-                if (ord32(__double2float_rd(v)) >= head && s >= sh.bound) {
-                    const int at = atomicAdd(&sh.cnt, 1);
-                    sh.score[at] = s; sh.key[at] = key; sh.beam[at] = (uint8_t)k;
+
+    // ---- the n best groups.  First a bound: the n-th of the threads' best, in a float that is never too high. ----
+    float best = -CUDART_INF_F, best_about = -CUDART_INF_F;
+    int best_beam = 0;
+    auto watch = [&](float x, int k) {
+        const float e = x + sh.about[k];
+        if (best == -CUDART_INF_F || e > best_about) { best = x; best_beam = k; best_about = e; }
+    };
+#pragma unroll 1
+    for (int pass = 0; pass < 2; pass++) {
+        int k = (int)((unsigned)tid / (unsigned)G), g = tid - k * G;  // of head i, which goes up by kBeamThreads
+#pragma unroll 1
+        for (int from = 0; from < heads; from += kStage * kBeamThreads) {
+            if (heads > kStage * kBeamThreads) {
+                load_heads(from);
+                stage_heads();
+            }
+#pragma unroll 2
+            for (int j = 0; j < kStage; j++) {
+                const int i = from + j * kBeamThreads + tid;
+                if (i >= heads) break;
+                const float x = sh.stage.head[j][tid];
+                if (x >= sh.least[k] && x > -CUDART_INF_F) {
+                    if (pass == 0) watch(x, k); else sh.offer(x, k, g);
                 }
+                if (i + kBeamThreads >= heads) break;
+                for (g += kBeamThreads; g >= G; g -= G) k++;
             }
         }
-        __syncthreads();
-        const bool full = sh.cnt > kMergeList - kBeamThreads;
-        __syncthreads();  // read by all before anyone appends
-        if (full) keep_candidates(sh, n);
+        if (pass == 0) find_low(sh, K, n, best, best_beam);
     }
-    keep_candidates(sh, n);
-    const int c = sh.cnt;
-    for (int i = tid; i < n; i += kBeamThreads) {
-        const int64_t o = (int64_t)seq * n + i;
-        a.tokens[o] = i < c ? key_idx(sh.key[i]) : -1;
-        a.parents[o] = i < c ? (int)sh.beam[i] : -1;
-        a.out_scores[o] = i < c ? (float)unord64(sh.score[i]) : -CUDART_INF_F;
+    int c = settle(sh, heads, n, [&](int i, float &x, int &k, int &g) {
+        k = (int)((unsigned)i / (unsigned)G);
+        g = i - k * G;
+        x = __ldcg(tops + i);
+        return true;
+    });
+    rank_list(sh, c, n, [&](int to, u64, u64 w, int k) { sh.group[to] = key_idx(w); sh.group_beam[to] = (uint8_t)k; });
+    __syncthreads();
+
+    // ---- the n best candidates, which lie in them ----
+    const int open = min(c, n);
+    if (tid == 0) sh.clear();
+    __syncthreads();
+    constexpr int E = T::E, kVecs = T::kGroup / E, kBatch = kStage / 2;
+    const int vecs = open * kVecs;
+    auto row_of = [&](int k) { return LogitRow{(const char *)a.logits + (int64_t)(seq * K + k) * a.row_stride * (BF16 ? 2 : 4), CAP ? a.softcap : 0.f}; };
+    auto allowed = [&](int k, int v) {
+        const int row = seq * K + k;
+        return v < a.vocab && (a.mask == nullptr || (a.uses_mask != nullptr && !a.uses_mask[row]) || mask_bit(a.mask + (int64_t)row * a.mask_stride, v));
+    };
+    auto first_of = [&](int i) { return sh.group[i / kVecs] * T::kGroup + i % kVecs * E; };
+    // Few groups: what bounds them is no close bound, so the threads' best elements give one first.
+    best = best_about = -CUDART_INF_F;
+#pragma unroll 1
+    for (int pass = heads < 8 * n ? 0 : 1; pass < 2; pass++) {
+#pragma unroll 1
+        for (int from = tid; from < vecs; from += kBatch * kBeamThreads) {
+            uint4 raw[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; j++) {
+                const int i = from + j * kBeamThreads;
+                raw[j] = make_uint4(0u, 0u, 0u, 0u);
+                if (i >= vecs) continue;
+                const int v = first_of(i);
+                const void *p = row_of(sh.group_beam[i / kVecs]).p;
+                if (VEC && v + E <= a.vocab) {
+                    raw[j] = BF16 ? __ldg((const uint4 *)((const uint16_t *)p + v)) : __ldg((const uint4 *)((const float *)p + v));
+                } else {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        if constexpr (BF16) {
+                            w[q] = v + 2 * q < a.vocab ? __ldg((const uint16_t *)p + v + 2 * q) : 0u;
+                            if (v + 2 * q + 1 < a.vocab) w[q] |= (uint32_t)__ldg((const uint16_t *)p + v + 2 * q + 1) << 16;
+                        } else {
+                            w[q] = v + q < a.vocab ? __ldg((const uint32_t *)p + v + q) : 0u;
+                        }
+                    }
+                    raw[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            uint32_t passed = 0u;  // bit j * E + e: that element reaches `least`
+#pragma unroll
+            for (int j = 0; j < kBatch; j++) {
+                sh.stage.vec[j][tid] = raw[j];  // a thread reads what it wrote
+                const int i = from + j * kBeamThreads;
+                if (i >= vecs) continue;
+                const float least = CAP ? -CUDART_INF_F : sh.least[sh.group_beam[i / kVecs]];
+                const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const float x = BF16 ? ((e & 1) ? bf16_hi(w[e / 2]) : bf16_lo(w[e / 2])) : __uint_as_float(w[e]);
+                    passed |= x >= least ? 1u << (j * E + e) : 0u;
+                }
+            }
+#pragma unroll 1
+            for (; passed != 0u; passed &= passed - 1u) {
+                const int b = __ffs(passed) - 1, j = b / E, e = b % E, i = from + j * kBeamThreads;
+                const int k = sh.group_beam[i / kVecs], v = first_of(i) + e;
+                float x = BF16 ? __uint_as_float((uint32_t)((const uint16_t *)&sh.stage.vec[j][tid])[e] << 16) : ((const float *)&sh.stage.vec[j][tid])[e];
+                if constexpr (CAP) x = soft_cap(x, a.softcap);
+                if (!(x >= sh.least[k]) || x == -CUDART_INF_F || !allowed(k, v)) continue;
+                if (pass == 0) watch(x, k); else sh.offer(x, k, v);
+            }
+        }
+        if (pass == 0) find_low(sh, K, n, best, best_beam);
+    }
+    c = settle(sh, open * T::kGroup, n, [&](int i, float &x, int &k, int &v) {
+        const int g = i / T::kGroup;
+        k = sh.group_beam[g];
+        v = sh.group[g] * T::kGroup + i % T::kGroup;
+        if (!allowed(k, v)) return false;
+        x = load_one<BF16>(row_of(k), v);
+        return true;
+    });
+    rank_list(sh, c, n, [&](int to, u64 s, u64 w, int k) {
+        const int64_t o = (int64_t)seq * n + to;
+        a.tokens[o] = key_idx(w);
+        a.parents[o] = k;
+        a.out_scores[o] = (float)unord64(s);
+    });
+    if (tid >= c && tid < n) {
+        const int64_t o = (int64_t)seq * n + tid;
+        a.tokens[o] = a.parents[o] = -1;
+        a.out_scores[o] = -CUDART_INF_F;
     }
     if (tid == 0 && a.flags) a.flags[seq] = sh.flags | (c < n ? (uint32_t)STG_BEAM_SHORT : 0u);
 }
+static_assert(STG_BEAM_MAX_CANDIDATES <= kBeamThreads && STG_BEAM_MAX_CANDIDATES + kBeamRoom <= kBeamList && kBeamRoom <= kBeamThreads, "room in the list");
 
-// grid (pieces, rows).  The CTA that arrives last at its sequence's ticket joins the sequence's pieces and leaves the ticket
+// grid (pieces, rows).  The CTA that arrives last at its sequence's ticket joins the sequence's rows and leaves the ticket
 // at zero, as it was found.
 template <bool BF16, bool VEC, bool CAP>
-__global__ void __launch_bounds__(kBeamThreads, BF16 && CAP ? 3 : 5) k_beam_select(const __grid_constant__ BeamSelect a)
+__global__ void __launch_bounds__(kBeamThreads, BF16 && CAP ? 1 : 2) k_beam_select(const __grid_constant__ BeamSelect a)
 {
-    __shared__ union { RowShared row; MergeShared merge; } sh;
+    __shared__ MergeShared sh;
     __shared__ bool last;
     const int row = blockIdx.y, seq = row / a.beams;
     const float score = a.scores[row];
-    if (score > -CUDART_INF_F && score < CUDART_INF_F) beam_piece<BF16, VEC, CAP>(a, sh.row, row, blockIdx.x);  // else a dead beam
-    __threadfence();
+    if (score > -CUDART_INF_F && score < CUDART_INF_F) beam_piece<BF16, VEC, CAP>(a, row, blockIdx.x);  // else a dead beam
     __syncthreads();
     if (threadIdx.x == 0) {
-        last = atomicAdd(a.ws.tickets + seq, 1u) == (uint32_t)(a.beams * a.pieces - 1);
+        uint32_t before;  // behind the barrier: for what the whole CTA has written, and what the others have
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.ws.tickets + seq) : "memory");
+        last = before == (uint32_t)(a.beams * a.pieces - 1);
         if (last) a.ws.tickets[seq] = 0u;
-        __threadfence();
     }
     __syncthreads();
-    if (last) beam_merge(a, sh.merge, seq);
+    if (last) beam_merge<BF16, VEC, CAP>(a, sh, seq);
 }
 
 int beam_check_rows(StgHandle h, const char *who, int32_t n_seq, int32_t n_beams)
@@ -546,22 +733,23 @@ static int captured_workspace(StgHandle h, size_t bytes, void **out)
     return STG_OK;
 }
 
-// How many CTAs share a row: the cut that gives the busiest SM the least, where a CTA's first tile costs about half a tile more
-// than the others.  A tile of a CTA by itself takes about three times as long as one of a full SM, so few rows are
-// cut into single tiles.
-static void beam_pieces(int rows, int beams, int vocab, int tile, int sms, int &pieces, int &len)
+// How many CTAs share a row.  Two fit an SM; of the cuts into whole tiles the one with the least time, waves of CTAs
+// times tiles of each and about two tiles' worth for the rest of a CTA.  (256 rows of 151,936 fp32: one piece 35.2 us, two
+// 37.2, ten 51.2; 64 rows of 262,144 bf16 behind masks: four pieces 27, three 35, eight 29; 4 rows of 151,936: nineteen
+// pieces 11.7, ten 12.5.)
+static void beam_pieces(int rows, int vocab, int tile, int sms, int &pieces, int &len)
 {
     const int tiles = (vocab + tile - 1) / tile;
-    const int most = std::max(1, std::min({tiles, kMergeParts / beams, kBeamExtraPieces / rows + 1}));
-    double least = 0.0;
-    pieces = 1;
+    const int most = std::max(1, std::min(tiles, kBeamExtraPieces / rows + 1));
+    int64_t least = INT64_MAX;
+    int each = tiles;
     for (int c = 1; c <= most; c++) {
         const int per = (tiles + c - 1) / c, got = (tiles + per - 1) / per;
-        if (got != c) continue;
-        const double cost = std::max((double)(((int64_t)rows * c + sms - 1) / sms) * (per + 0.5) * 0.3, per + 1.0);
-        if (c == 1 || cost < least) { least = cost; pieces = c; }
+        const int64_t cost = (((int64_t)rows * got + 2 * sms - 1) / (2 * sms)) * (per + 2);
+        if (cost < least) { least = cost; each = per; }
     }
-    len = (tiles + pieces - 1) / pieces * tile;
+    pieces = (tiles + each - 1) / each;
+    len = each * tile;
 }
 
 static int beam_select(StgHandle h, const StgBeamBatch *b, cudaStream_t stream)
@@ -594,10 +782,12 @@ static int beam_select(StgHandle h, const StgBeamBatch *b, cudaStream_t stream)
     a.n_seq = b->n_seq; a.beams = b->n_beams; a.vocab = b->vocab; a.n = b->n_candidates;
     a.tokens = b->tokens; a.parents = b->parents; a.out_scores = b->candidate_scores; a.log_norms = b->log_norms; a.flags = b->seq_flags;
     const int rows = b->n_seq * b->n_beams;
-    const int tile = 4096 * (b->logits_dtype == STG_DTYPE_BF16 ? 2 : 1);
-    beam_pieces(rows, b->n_beams, b->vocab, tile, h->sm_count, a.pieces, a.piece_len);
+    const int group = b->logits_dtype == STG_DTYPE_BF16 ? 1024 : 512, tile = group * kBeamWarps;
+    a.groups = (b->vocab + group - 1) / group;
+    beam_pieces(rows, b->vocab, tile, h->sm_count, a.pieces, a.piece_len);
 
-    const size_t b_parts = round_up((size_t)rows * a.pieces * sizeof(BeamPart), 256), b_keys = round_up((size_t)rows * a.pieces * a.n * 8, 256);
+    const size_t b_parts = round_up((size_t)rows * a.pieces * sizeof(BeamPart), 256), b_tops = round_up((size_t)rows * a.groups * 4, 256),
+                 bytes = b_parts + b_tops;
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     CK(cudaStreamIsCapturing(stream, &cap));
     const bool captured = cap != cudaStreamCaptureStatusNone;
@@ -605,16 +795,16 @@ static int beam_select(StgHandle h, const StgBeamBatch *b, cudaStream_t stream)
     a.ws.tickets = (uint32_t *)h->bm_tickets.p;
     if (captured) {
         void *own = nullptr;
-        rc = captured_workspace(h, b_parts + b_keys + (size_t)b->n_seq * 4, &own);
+        rc = captured_workspace(h, bytes + (size_t)b->n_seq * 4, &own);
         ws = (char *)own;
-        a.ws.tickets = (uint32_t *)(ws + b_parts + b_keys);
+        a.ws.tickets = (uint32_t *)(ws + bytes);
     } else {
-        if (b_parts + b_keys > h->bm_ws.bytes) return fail(h, STG_ERR_CAPACITY, "stg_beam_select: workspace too small");
+        if (bytes > h->bm_ws.bytes) return fail(h, STG_ERR_CAPACITY, "stg_beam_select: workspace too small");
         rc = order_behind_last(h, stream);
     }
     if (rc) return rc;
     a.ws.parts = (BeamPart *)ws;
-    a.ws.keys = (u64 *)(ws + b_parts);
+    a.ws.tops = (float *)(ws + b_parts);
     if (captured) CK(cudaMemsetAsync(a.ws.tickets, 0, (size_t)b->n_seq * 4, stream));  // part of the graph
     const bool vec = !misaligned(b->logits, 16) && (rows == 1 || (size_t)b->row_stride * esz % 16 == 0);
     const bool capped = b->logit_softcap != 0.f;

@@ -137,6 +137,27 @@ def test_equal_logits_go_to_the_lower_token(bs, V, dtype):
     _check(bs, x, _scores(6, 1, V), 128)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_logits_of_any_size(bs, dtype):
+    """Rows far from zero, rows that grow along the vocabulary, logits next to and beyond 1e6, and mixtures of all of them."""
+    import torch
+
+    V = 40000
+    x = _normal(16, V, 21)
+    for r, shift in enumerate((300.0, -300.0, 5000.0, -5000.0, 999990.0, -999990.0, 1e6, -1e6, 1.5e6, -1.5e6, 3e7, -3e7)):
+        x[r] = x[r] * (0.01 if abs(shift) > 1e5 else 1.0) + shift
+    x[12] += torch.arange(V) * 0.02                      # 800 from one end to the other
+    x[13] -= torch.arange(V) * 0.02
+    x[14, ::5000] = torch.tensor([1e6, -1e6, 2e6, 999999.0, -3e6, 1000001.0, 5.0, 2000003.0])
+    x[15, 700:20000] = torch.finfo(torch.float32).min
+    x[15, 20000:] -= 1e6
+    x = x.to(torch.bfloat16) if dtype == "bf16" else x
+    _check(bs, x, _scores(16, 1, 5), 20)
+    _check(bs, x, _scores(4, 4, 5), 20)
+    _check(bs, x.flip(1), _scores(8, 2, 5), 9)
+    _check(bs, x[:, :39990], _scores(16, 1, 5), 20, stride=40001)
+
+
 @pytest.mark.parametrize("V", [4096, 20011, 100000])
 def test_rows_that_ascend_and_descend(bs, V):
     import torch
