@@ -24,9 +24,10 @@ struct MoveState {
     int32_t size[3];
     int32_t pos_dim;
     int32_t vec;          // bytes a thread moves at a time: 16, 8, 4, 2 or 1
-    int32_t cols;         // vectors of a run, the last one possibly cut off
-    int64_t first_tile;   // of this state; a tile is kMoveThreads columns of one sequence
-    int64_t seq_tiles;    // tiles of one sequence
+    int32_t cols;         // vectors that a run can touch; the first and the last may be in part another run's
+    int32_t run_tiles;    // tiles of a run; 0: a tile's columns go on from run to run
+    int32_t seq_tiles;    // tiles of one sequence
+    int32_t first_tile;   // of this state
 };
 
 struct MoveArgs {
@@ -35,79 +36,160 @@ struct MoveArgs {
     const int32_t *parents, *positions;
 };
 
+// What the beams of a sequence move: rows that others continue, and where to
+struct Moves {
+    int64_t src[STG_BEAM_MAX_BEAMS], dst[STG_BEAM_MAX_BEAMS];  // offsets of rows
+    int first[STG_BEAM_MAX_BEAMS + 1];                          // row src[i] goes to dst[first[i] .. first[i + 1])
+    int n;
+};
+
 template <int MOVES, class V>
-__device__ __forceinline__ void move_column(char *col, int64_t row_stride, const int *src, const uint32_t *dst, int n)
+static __device__ __forceinline__ void load_rows(V (&v)[MOVES], const char *at, const Moves &m, int n)
 {
-    V v[MOVES];
 #pragma unroll
     for (int i = 0; i < MOVES; i++)
-        if (i < n) v[i] = *(const V *)(col + src[i] * row_stride);
+        if (i < n) v[i] = *(const V *)(at + m.src[i]);
+}
+template <int MOVES, class V>
+static __device__ __forceinline__ void store_rows(const V (&v)[MOVES], char *at, const Moves &m, int n)
+{
 #pragma unroll
     for (int i = 0; i < MOVES; i++)
         if (i < n)
-            for (uint32_t d = dst[i]; d != 0u; d &= d - 1u) *(V *)(col + (__ffs(d) - 1) * row_stride) = v[i];
+            for (int d = m.first[i]; d < m.first[i + 1]; d++) *(V *)(at + m.dst[d]) = v[i];
+}
+template <int MOVES, class V>
+static __device__ __forceinline__ void move_column(char *at, const Moves &m, int n)
+{
+    V v[MOVES];
+    load_rows(v, at, m, n);
+    store_rows(v, at, m, n);
 }
 
+// Fewer bytes than a vector, in pieces as large as they are aligned.  Where one end is a vector's, a size occurs once at most,
+// and few rows' pieces are all loaded before any is stored.
 template <int MOVES>
-__global__ void __launch_bounds__(kMoveThreads) k_beam_move(const __grid_constant__ MoveArgs a)
+static __device__ __noinline__ void move_part(char *at, int bytes, int vec, const Moves &m, int n)
 {
-    __shared__ int src[STG_BEAM_MAX_BEAMS];        // rows that others continue
-    __shared__ uint32_t dst[STG_BEAM_MAX_BEAMS];   // ... and which those are, one bit each
-    __shared__ int n_src;
+    const bool tail = ((uintptr_t)at & (unsigned)(vec - 1)) == 0, head = (((uintptr_t)at + bytes) & (unsigned)(vec - 1)) == 0;
+    if (MOVES <= 8 && (tail || head)) {
+        // where the pieces of 8, 4, 2 and 1 begin: large ones first behind an aligned beginning, last ahead of an aligned end
+        char *const p8 = at + (tail ? 0 : bytes & 7), *const p4 = at + (tail ? bytes & 8 : bytes & 3), *const p2 = at + (tail ? bytes & 12 : bytes & 1),
+             *const p1 = at + (tail ? bytes & 14 : 0);
+        uint2 v8[MOVES];
+        uint32_t v4[MOVES];
+        uint16_t v2[MOVES];
+        uint8_t v1[MOVES];
+        if (bytes & 8) load_rows(v8, p8, m, n);
+        if (bytes & 4) load_rows(v4, p4, m, n);
+        if (bytes & 2) load_rows(v2, p2, m, n);
+        if (bytes & 1) load_rows(v1, p1, m, n);
+        if (bytes & 8) store_rows(v8, p8, m, n);
+        if (bytes & 4) store_rows(v4, p4, m, n);
+        if (bytes & 2) store_rows(v2, p2, m, n);
+        if (bytes & 1) store_rows(v1, p1, m, n);
+        return;
+    }
+#pragma unroll 1
+    while (bytes > 0) {
+        int by = 8;
+        while (by > bytes || ((uintptr_t)at & (unsigned)(by - 1)) != 0) by >>= 1;
+        switch (by) {
+            case 8: move_column<MOVES, uint2>(at, m, n); break;
+            case 4: move_column<MOVES, uint32_t>(at, m, n); break;
+            case 2: move_column<MOVES, uint16_t>(at, m, n); break;
+            default: move_column<MOVES, uint8_t>(at, m, n); break;
+        }
+        at += by;
+        bytes -= by;
+    }
+}
+
+// A tile is kMoveThreads columns of one sequence, one to a thread: occupancy is worth more than several columns' loads in flight
+// (four beams, eight layers' caches of 1000 positions: 35.5 us with eight CTAs an SM, 40.9 with five, 43.2 with four columns
+// a thread and three CTAs; 32 sequences of eight beams, 3.2 GB moved: 511 us with five CTAs, 568 with four).  More than 16
+// beams move 8 bytes a thread: 199 us against 263 with 16 and one CTA an SM.  Where runs are shorter than four
+// tiles a tile's columns go on from run to run, at a division each.
+constexpr int move_blocks(int moves) { return moves <= 4 ? 8 : moves <= 8 ? 5 : 3; }
+__host__ __device__ constexpr int move_bytes(int beams) { return beams <= 16 ? 16 : 8; }
+
+template <int MOVES>
+__global__ void __launch_bounds__(kMoveThreads, move_blocks(MOVES)) k_beam_move(const __grid_constant__ MoveArgs a)
+{
+    __shared__ Moves moves;
     const int tid = threadIdx.x, K = a.beams;
     int lo = 0, hi = a.n_states - 1;  // the last state whose first tile is not behind this one
     while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
-        if ((int64_t)blockIdx.x >= a.st[mid].first_tile) lo = mid; else hi = mid - 1;
+        if ((int)blockIdx.x >= a.st[mid].first_tile) lo = mid; else hi = mid - 1;
     }
     const MoveState &st = a.st[lo];
-    const int64_t tile = (int64_t)blockIdx.x - st.first_tile;
-    const int seq = (int)(tile / st.seq_tiles);
-    const int64_t col0 = (tile - seq * st.seq_tiles) * kMoveThreads;
+    const unsigned tile = blockIdx.x - (unsigned)st.first_tile, seq = tile / (unsigned)st.seq_tiles, in_seq = tile - seq * (unsigned)st.seq_tiles;
+    const int64_t pos = a.positions ? (int64_t)max(a.positions[seq], 0) : 0;
     if (tid < 32) {
         const int p = tid < K ? a.parents[(int64_t)seq * K + tid] : -1;
-        const bool moves = p >= 0 && p < K && p != tid;
+        const int parent = p >= 0 && p < K && p != tid ? p : -1;
         uint32_t followers = 0u;
+        for (int k = 0; k < K; k++)
+            if (__shfl_sync(0xFFFFFFFFu, parent, k) == tid) followers |= 1u << k;
+        const unsigned on = __ballot_sync(0xFFFFFFFFu, followers != 0u), before = (1u << tid) - 1u;
+        int first = 0;  // followers of the rows ahead
         for (int k = 0; k < K; k++) {
-            const int pk = __shfl_sync(0xFFFFFFFFu, moves ? p : -1, k);
-            if (pk == tid) followers |= 1u << k;
+            const int f = __popc(__shfl_sync(0xFFFFFFFFu, followers, k));
+            first += k < tid ? f : 0;
         }
-        const unsigned on = __ballot_sync(0xFFFFFFFFu, followers != 0u);
-        const int at = __popc(on & ((1u << tid) - 1u));
-        if (followers != 0u) { src[at] = tid; dst[at] = followers; }
-        if (tid == 0) n_src = __popc(on);
+        if (followers != 0u) {
+            const int at = __popc(on & before);
+            moves.src[at] = tid * st.row_stride;
+            moves.first[at] = first;
+            for (uint32_t f = followers; f != 0u; f &= f - 1u) moves.dst[first++] = (__ffs(f) - 1) * st.row_stride;
+            if ((on & ~before & ~(1u << tid)) == 0u) moves.first[at + 1] = first;  // the last one
+        }
+        if (tid == 0) moves.n = __popc(on);
     }
     __syncthreads();
-    const int n = n_src;
-    if (n == 0) return;
-    const int64_t pos = a.positions ? (int64_t)max(a.positions[seq], 0) : 0;
-    const int64_t o0 = col0 / st.cols;
-    const int rest = (int)(col0 - o0 * st.cols) + tid;
-    const int64_t outer = o0 + rest / st.cols;
-    const int col = rest % st.cols;
-    const int64_t i0 = outer % st.size[0], o1 = outer / st.size[0], i1 = o1 % st.size[1], i2 = o1 / st.size[1];
-    if (i2 >= st.size[2]) return;
-    int64_t limit = st.inner;
-    if (a.positions) {
-        if (st.pos_dim == 0 && i0 >= pos) return;
-        if (st.pos_dim == 1 && i1 >= pos) return;
-        if (st.pos_dim == 2 && i2 >= pos) return;
-        if (st.pos_dim == 3) limit = min(limit, pos * st.pos_bytes);
-    }
-    const int64_t off = (int64_t)col * st.vec;
-    const int64_t left = limit - off;
-    if (left <= 0) return;
-    char *p = st.data + (int64_t)seq * K * st.row_stride + i0 * st.stride[0] + i1 * st.stride[1] + i2 * st.stride[2] + off;
-    if (left >= st.vec) {
-        switch (st.vec) {
-            case 16: move_column<MOVES, uint4>(p, st.row_stride, src, dst, n); break;
-            case 8: move_column<MOVES, uint2>(p, st.row_stride, src, dst, n); break;
-            case 4: move_column<MOVES, uint32_t>(p, st.row_stride, src, dst, n); break;
-            case 2: move_column<MOVES, uint16_t>(p, st.row_stride, src, dst, n); break;
-            default: move_column<MOVES, uint8_t>(p, st.row_stride, src, dst, n); break;
+    if (moves.n == 0) return;
+    char *const row = st.data + (int64_t)(seq * (unsigned)K) * st.row_stride;
+    const int64_t limit = a.positions && st.pos_dim == 3 ? min(st.inner, pos * st.pos_bytes) : st.inner;
+    // the run `outer`, or null where it is not to be moved
+    auto run = [&](unsigned outer) -> char * {
+        unsigned i0 = outer, i1 = 0u, i2 = 0u;
+        if (st.size[1] > 1 || st.size[2] > 1) {
+            i1 = outer / (unsigned)st.size[0]; i0 = outer - i1 * (unsigned)st.size[0];
+            i2 = i1 / (unsigned)st.size[1]; i1 -= i2 * (unsigned)st.size[1];
         }
+        if (i2 >= (unsigned)st.size[2] || i1 >= (unsigned)st.size[1] || i0 >= (unsigned)st.size[0]) return nullptr;
+        if (a.positions && st.pos_dim >= 0 && st.pos_dim < 3 && (int64_t)(st.pos_dim == 0 ? i0 : st.pos_dim == 1 ? i1 : i2) >= pos) return nullptr;
+        return row + i0 * st.stride[0] + i1 * st.stride[1] + i2 * st.stride[2];
+    };
+    char *r;
+    unsigned c = tid;
+    if (st.run_tiles > 0) {
+        const unsigned outer = in_seq / (unsigned)st.run_tiles;
+        r = run(outer);
+        c += (in_seq - outer * (unsigned)st.run_tiles) * kMoveThreads;
     } else {
-        for (int b = 0; b < (int)left; b++) move_column<MOVES, uint8_t>(p + b, st.row_stride, src, dst, n);
+        const unsigned g = in_seq * kMoveThreads + tid, outer = g / (unsigned)st.cols;
+        r = run(outer);
+        c = g - outer * (unsigned)st.cols;
+    }
+    if (r == nullptr) return;
+    // Columns begin at multiples of `vec` in memory, which are the same for all rows: a run's first may begin ahead of it.
+    const int64_t begin = (int64_t)c * st.vec - (int64_t)((uintptr_t)r & (unsigned)(st.vec - 1)), end = begin + st.vec;
+    const int n = moves.n;
+    if (begin >= limit) return;
+    if (begin < 0 || end > limit) {
+        move_part<MOVES>(r + max(begin, (int64_t)0), (int)(min(end, limit) - max(begin, (int64_t)0)), st.vec, moves, n);
+        return;
+    }
+    switch (st.vec) {
+        case 16:
+            if constexpr (move_bytes(MOVES) == 16) move_column<MOVES, uint4>(r + begin, moves, n);
+            break;
+        case 8: move_column<MOVES, uint2>(r + begin, moves, n); break;
+        case 4: move_column<MOVES, uint32_t>(r + begin, moves, n); break;
+        case 2: move_column<MOVES, uint16_t>(r + begin, moves, n); break;
+        default: move_column<MOVES, uint8_t>(r + begin, moves, n); break;
     }
 }
 
@@ -126,7 +208,7 @@ static bool nested(const StgBeamState &s, int64_t rows)
 }
 
 // `b` split into what the kernel works on; false: nothing of it is to be moved
-static bool move_state(const StgBeamState &b, int n_positions, MoveState &m)
+static bool move_state(const StgBeamState &b, int beams, int n_positions, MoveState &m)
 {
     memset(&m, 0, sizeof(m));
     m.data = (char *)b.data;
@@ -138,11 +220,8 @@ static bool move_state(const StgBeamState &b, int n_positions, MoveState &m)
     if (n_positions >= 0 && b.position_dim == 3) m.inner = std::min(m.inner, (int64_t)n_positions * b.position_bytes);
     if (n_positions >= 0 && b.position_dim >= 0 && b.position_dim < 3) m.size[b.position_dim] = std::min(m.size[b.position_dim], n_positions);
     if (m.inner <= 0 || m.size[0] <= 0 || m.size[1] <= 0 || m.size[2] <= 0) return false;
-    uint64_t bits = (uint64_t)(uintptr_t)m.data | (uint64_t)m.row_stride;
-    for (int i = 0; i < 3; i++)
-        if (m.size[i] > 1) bits |= (uint64_t)m.stride[i];
-    m.vec = 16;
-    while (bits % (uint64_t)m.vec != 0) m.vec >>= 1;
+    m.vec = move_bytes(beams);  // as rows are apart: a run's bytes then lie alike in all of them
+    while (m.row_stride % m.vec != 0) m.vec >>= 1;
     while (m.vec > 1 && m.vec > m.inner) m.vec >>= 1;
     return true;
 }
@@ -190,14 +269,21 @@ static int reorder(StgHandle h, const StgBeamReorder *r, cudaStream_t stream)
     std::vector<MoveState> moves;  // all of it is checked before any of it is moved
     for (int i = 0; i < total; i++) {
         MoveState m;
-        if (!move_state(i < r->n_states ? r->states[i] : ring[0], r->positions ? -1 : r->n_positions, m)) continue;
-        const int64_t cols = (m.inner + m.vec - 1) / m.vec;
-        const int64_t runs = (int64_t)m.size[0] * m.size[1];
-        if (cols > INT32_MAX / 2 || runs > INT64_MAX / 8 / cols / m.size[2])
-            return fail(h, STG_ERR_UNSUPPORTED, "stg_beam_reorder: state " + std::to_string(i) + " is too large");
-        m.cols = (int32_t)cols;
-        m.seq_tiles = (cols * runs * m.size[2] + kMoveThreads - 1) / kMoveThreads;
-        if (m.seq_tiles > INT32_MAX / r->n_seq) return fail(h, STG_ERR_UNSUPPORTED, "stg_beam_reorder: state " + std::to_string(i) + " is too large");
+        if (!move_state(i < r->n_states ? r->states[i] : ring[0], r->n_beams, r->positions ? -1 : r->n_positions, m)) continue;
+        uint64_t where = (uint64_t)(uintptr_t)m.data;
+        for (int j = 0; j < 3; j++)
+            if (m.size[j] > 1) where |= (uint64_t)m.stride[j];
+        const int64_t cols = (m.inner + m.vec - 1) / m.vec + (where % (uint64_t)m.vec != 0 ? 1 : 0), runs = (int64_t)m.size[0] * m.size[1];
+        const bool too_many = cols > INT32_MAX / 2 || runs > INT32_MAX / m.size[2];
+        int64_t per_seq = INT64_MAX;
+        if (!too_many) {
+            const bool joined = cols < 4 * kMoveThreads && cols * (runs * m.size[2]) < INT32_MAX - kMoveThreads;
+            m.cols = (int32_t)cols;
+            m.run_tiles = joined ? 0 : (int32_t)((cols + kMoveThreads - 1) / kMoveThreads);
+            per_seq = joined ? (cols * (runs * m.size[2]) + kMoveThreads - 1) / kMoveThreads : m.run_tiles * (runs * m.size[2]);
+        }
+        if (per_seq > INT32_MAX / r->n_seq) return fail(h, STG_ERR_UNSUPPORTED, "stg_beam_reorder: state " + std::to_string(i) + " is too large");
+        m.seq_tiles = (int32_t)per_seq;
         moves.push_back(m);
     }
     MoveArgs a;
@@ -220,12 +306,12 @@ static int reorder(StgHandle h, const StgBeamReorder *r, cudaStream_t stream)
         return STG_OK;
     };
     for (MoveState &m : moves) {
-        if (a.n_states == kMoveStates || tiles + m.seq_tiles * r->n_seq > INT32_MAX) {
+        if (a.n_states == kMoveStates || tiles + (int64_t)m.seq_tiles * r->n_seq > INT32_MAX) {
             rc = launch();
             if (rc) return rc;
         }
-        m.first_tile = tiles;
-        tiles += m.seq_tiles * r->n_seq;
+        m.first_tile = (int32_t)tiles;
+        tiles += (int64_t)m.seq_tiles * r->n_seq;
         a.st[a.n_states++] = m;
     }
     return launch();
