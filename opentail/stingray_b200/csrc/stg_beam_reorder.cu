@@ -10,6 +10,7 @@
 #include <algorithm>
 
 #include "stg_beam.h"
+#include "stg_pdl.cuh"
 #include "stg_types.h"
 
 namespace stg {
@@ -125,6 +126,8 @@ __global__ void __launch_bounds__(kMoveThreads, move_blocks(MOVES)) k_beam_move(
     }
     const MoveState &st = a.st[lo];
     const unsigned tile = blockIdx.x - (unsigned)st.first_tile, seq = tile / (unsigned)st.seq_tiles, in_seq = tile - seq * (unsigned)st.seq_tiles;
+    pdl_release();
+    pdl_wait();
     const int64_t pos = a.positions ? (int64_t)max(a.positions[seq], 0) : 0;
     if (tid < 32) {
         const int p = tid < K ? a.parents[(int64_t)seq * K + tid] : -1;
@@ -295,11 +298,8 @@ static int reorder(StgHandle h, const StgBeamReorder *r, cudaStream_t stream)
     auto launch = [&]() -> int {
         if (a.n_states == 0) return STG_OK;
         const unsigned grid = (unsigned)tiles;
-        if (r->n_beams <= 4) k_beam_move<4><<<grid, kMoveThreads, 0, stream>>>(a);
-        else if (r->n_beams <= 8) k_beam_move<8><<<grid, kMoveThreads, 0, stream>>>(a);
-        else if (r->n_beams <= 16) k_beam_move<16><<<grid, kMoveThreads, 0, stream>>>(a);
-        else k_beam_move<32><<<grid, kMoveThreads, 0, stream>>>(a);
-        CK(cudaGetLastError());
+        const auto fn = r->n_beams <= 4 ? k_beam_move<4> : r->n_beams <= 8 ? k_beam_move<8> : r->n_beams <= 16 ? k_beam_move<16> : k_beam_move<32>;
+        CK(launch_behind(fn, dim3(grid), kMoveThreads, 0, stream, a));
         h->stats.kernel_launches++;
         a.n_states = 0;
         tiles = 0;

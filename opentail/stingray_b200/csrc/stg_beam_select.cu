@@ -20,6 +20,7 @@
 #include <new>
 
 #include "stg_beam.h"
+#include "stg_pdl.cuh"
 #include "stg_select.cuh"
 #include "stg_types.h"
 
@@ -333,36 +334,33 @@ struct MergeShared {
     uint8_t beam[kBeamList];
     u64 kept_score[STG_BEAM_MAX_CANDIDATES], kept_key[STG_BEAM_MAX_CANDIDATES];
     uint8_t kept_beam[STG_BEAM_MAX_CANDIDATES];
-    double base[STG_BEAM_MAX_BEAMS];   // a beam's candidates score base + (logit - ref); -infinity: it has none
+    double sum[STG_BEAM_MAX_BEAMS];    // S of a beam, relative to ref
     double ref[STG_BEAM_MAX_BEAMS];
+    double base[STG_BEAM_MAX_BEAMS];   // a beam's candidates score base + (logit - ref)
     float about[STG_BEAM_MAX_BEAMS];   // ... about that + logit
     float least[STG_BEAM_MAX_BEAMS];   // no smaller logit reaches `low`; NaN: the beam has no candidates
     int group[STG_BEAM_MAX_CANDIDATES];          // the groups that are read again
     uint8_t group_beam[STG_BEAM_MAX_CANDIDATES];
     u64 bound_score, bound_key;        // the n-th best so far
     int bound_beam;
-    uint32_t low;                      // a float, as ord32, that n scores reach; 0: none
+    uint32_t low;                      // a float, as ord32, that n candidates reach in `about`; 0: none
     uint32_t flags;
     int cnt;
 
     __device__ __forceinline__ u64 score_of(int k, float x) const { return ord64(((double)x - ref[k]) + base[k]); }
-    __device__ __forceinline__ static uint32_t round_down(u64 score) { return ord32(__double2float_rd(unord64(score))); }
     __device__ __forceinline__ void clear()
     {
         cnt = 0;
         bound_score = bound_key = 0ull;
         bound_beam = STG_BEAM_MAX_BEAMS;
     }
-    // `least` of beam k: the sum that makes a score is off by a few 2^-53 of its terms
-    __device__ __forceinline__ void set_least(int k)
+    // x + about is off by a few roundings (2^-24) of x, of what `about` was made of - the normaliser's logarithm, at most 46
+    // beside `ref`, among it - and of the sum; `size` is the largest |about| + |ref| of the beams.
+    __device__ __forceinline__ void set_least(int k, float size)
     {
-        const double b = base[k], r = ref[k];
-        float x = b > -CUDART_INF ? -CUDART_INF_F : CUDART_NAN_F;
-        if (low != 0u && b > -CUDART_INF) {
-            const double l = (double)unord32(low);
-            x = __double2float_rd(((l - b) + r) - 1e-14 * (fabs(l) + fabs(b) + fabs(r)));
-        }
-        least[k] = x;
+        if (low == 0u || !(about[k] > -CUDART_INF_F)) return;  // no bound, or a beam without candidates
+        const float l = unord32(low), x = l - about[k];
+        least[k] = x - (1e-6f * (fabsf(x) + fabsf(l)) + 2e-6f * size + 2e-5f);
     }
     // x has reached `least`: it may be one of the n best.  Its score is made when all have come.
     __device__ __forceinline__ void offer(float x, int k, int pos)
@@ -383,31 +381,33 @@ struct MergeShared {
 // The code below runs once per call and sequence, so what it takes is latency, that of fetching its instructions
 // included: loops are left rolled and what is used twice is a function, while loads are issued several at a time.
 
-// `low` out of every thread's best item (x of beam k; -infinity: none), such that n scores reach it.  Up to 32: the n-th
+// `low` out of every thread's best item (its x + about; -infinity: none), such that n of them reach it.  Up to 32: the n-th
 // largest of 64 groups of threads, each of which counts those above its own.  Beyond: the upper 20 bits of the n-th
-// largest of 256, found two by two (0.9 us against 0.3).  0 where there are no n.  All threads.
-static __device__ __noinline__ void find_low(MergeShared &sh, int K, int n, float x, int k)
+// largest of 256, found two by two (0.9 us against 0.3).  0 where there are no n.  Meanwhile `aside` is called by a warp
+// that has nothing to do with it.  All threads.
+template <class Aside>
+static __device__ __forceinline__ void find_low(MergeShared &sh, int K, int n, float best, Aside aside)
 {
     const int tid = threadIdx.x;
-    uint32_t mine = x > -CUDART_INF_F ? MergeShared::round_down(sh.score_of(k, x)) : 0u;
+    uint32_t mine = best > -CUDART_INF_F ? ord32(best) : 0u;
     const int per = n <= 32 ? kBeamThreads / 64 : kBeamThreads / 256;
 #pragma unroll
     for (int o = 1; o < kBeamThreads / 64; o *= 2)
         if (o < per) mine = max(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, o));
     if (tid % per == 0) sh.tops[tid / per] = mine;
     __syncthreads();
-    if (n <= 32) {
-        if (tid < 64) {
-            mine = sh.tops[tid];
-            int ahead = 0;
+    if (tid >= 64) {
+        if (tid < 96) aside(tid - 64);
+    } else if (n <= 32) {
+        mine = sh.tops[tid];
+        int ahead = 0;
 #pragma unroll 4
-            for (int i = 0; i < 64; i += 4) {
-                const uint4 v = *(const uint4 *)(sh.tops + i);
-                ahead += (v.x > mine || (v.x == mine && i < tid)) + (v.y > mine || (v.y == mine && i + 1 < tid)) +
-                         (v.z > mine || (v.z == mine && i + 2 < tid)) + (v.w > mine || (v.w == mine && i + 3 < tid));
-            }
-            if (ahead == n - 1) sh.low = max(sh.low, mine);
+        for (int i = 0; i < 64; i += 4) {
+            const uint4 v = *(const uint4 *)(sh.tops + i);
+            ahead += (v.x > mine || (v.x == mine && i < tid)) + (v.y > mine || (v.y == mine && i + 1 < tid)) +
+                     (v.z > mine || (v.z == mine && i + 2 < tid)) + (v.w > mine || (v.w == mine && i + 3 < tid));
         }
+        if (ahead == n - 1) sh.low = max(sh.low, mine);
     } else if (tid < 32) {
         uint32_t v[8], found = 0u;
 #pragma unroll
@@ -426,7 +426,10 @@ static __device__ __noinline__ void find_low(MergeShared &sh, int K, int n, floa
         if (tid == 0) sh.low = max(sh.low, found);
     }
     __syncthreads();
-    if (tid < K) sh.set_least(tid);
+    if (tid < 32) {
+        const float size = warp_max(tid < K && sh.about[tid] > -CUDART_INF_F ? fabsf(sh.about[tid]) + fabsf((float)sh.ref[tid]) : 0.f);
+        if (tid < K) sh.set_least(tid, size);
+    }
     __syncthreads();
 }
 
@@ -544,27 +547,26 @@ static __device__ __forceinline__ void beam_merge(const BeamSelect &a, MergeShar
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
         if (lane == 0) {
-            const bool none = m == -CUDART_INF && s == 0.0;         // dead, or nothing in the row
+            const bool none = m == -CUDART_INF && s == 0.0;          // dead, or nothing in the row
             const bool bad = !none && !(s > 0.0 && s < CUDART_INF);  // NaN or +infinity among the logits
-            const double logs = log(s);
-            sh.base[k] = none || bad ? -CUDART_INF : (double)score - logs;
+            sh.sum[k] = s;
             sh.ref[k] = m;
-            sh.about[k] = (float)(((double)score - logs) - m);
+            sh.about[k] = none || bad ? -CUDART_INF_F : (score - logf((float)s)) - (float)m;
             sh.least[k] = none || bad ? CUDART_NAN_F : -CUDART_INF_F;
             if (bad) atomicOr(&sh.flags, STG_BEAM_BAD_ROW);
             if (alive && none) atomicOr(&sh.flags, STG_ROW_FULLY_MASKED);
-            if (a.log_norms) a.log_norms[row] = none ? -CUDART_INF_F : (float)(m + logs);
         }
     }
     stage_heads();
     __syncthreads();
 
-    // ---- the n best groups.  First a bound: the n-th of the threads' best, in a float that is never too high. ----
-    float best = -CUDART_INF_F, best_about = -CUDART_INF_F;
-    int best_beam = 0;
-    auto watch = [&](float x, int k) {
-        const float e = x + sh.about[k];
-        if (best == -CUDART_INF_F || e > best_about) { best = x; best_beam = k; best_about = e; }
+    // ---- the n best groups.  First a bound: the n-th of the threads' best, of which 32 bits are enough. ----
+    float best = -CUDART_INF_F;
+    auto norms = [&](int k) {  // what takes 64
+        if (k >= K) return;
+        const double logs = log(sh.sum[k]);
+        sh.base[k] = (double)a.scores[seq * K + k] - logs;
+        if (a.log_norms) a.log_norms[seq * K + k] = sh.sum[k] == 0.0 ? -CUDART_INF_F : (float)(sh.ref[k] + logs);
     };
 #pragma unroll 1
     for (int pass = 0; pass < 2; pass++) {
@@ -581,13 +583,13 @@ static __device__ __forceinline__ void beam_merge(const BeamSelect &a, MergeShar
                 if (i >= heads) break;
                 const float x = sh.stage.head[j][tid];
                 if (x >= sh.least[k] && x > -CUDART_INF_F) {
-                    if (pass == 0) watch(x, k); else sh.offer(x, k, g);
+                    if (pass == 0) best = fmaxf(best, x + sh.about[k]); else sh.offer(x, k, g);
                 }
                 if (i + kBeamThreads >= heads) break;
                 for (g += kBeamThreads; g >= G; g -= G) k++;
             }
         }
-        if (pass == 0) find_low(sh, K, n, best, best_beam);
+        if (pass == 0) find_low(sh, K, n, best, norms);
     }
     int c = settle(sh, heads, n, [&](int i, float &x, int &k, int &g) {
         k = (int)((unsigned)i / (unsigned)G);
@@ -611,7 +613,7 @@ static __device__ __forceinline__ void beam_merge(const BeamSelect &a, MergeShar
     };
     auto first_of = [&](int i) { return sh.group[i / kVecs] * T::kGroup + i % kVecs * E; };
     // Few groups: what bounds them is no close bound, so the threads' best elements give one first.
-    best = best_about = -CUDART_INF_F;
+    best = -CUDART_INF_F;
 #pragma unroll 1
     for (int pass = heads < 8 * n ? 0 : 1; pass < 2; pass++) {
 #pragma unroll 1
@@ -661,10 +663,10 @@ static __device__ __forceinline__ void beam_merge(const BeamSelect &a, MergeShar
                 float x = BF16 ? __uint_as_float((uint32_t)((const uint16_t *)&sh.stage.vec[j][tid])[e] << 16) : ((const float *)&sh.stage.vec[j][tid])[e];
                 if constexpr (CAP) x = soft_cap(x, a.softcap);
                 if (!(x >= sh.least[k]) || x == -CUDART_INF_F || !allowed(k, v)) continue;
-                if (pass == 0) watch(x, k); else sh.offer(x, k, v);
+                if (pass == 0) best = fmaxf(best, x + sh.about[k]); else sh.offer(x, k, v);
             }
         }
-        if (pass == 0) find_low(sh, K, n, best, best_beam);
+        if (pass == 0) find_low(sh, K, n, best, [](int) {});
     }
     c = settle(sh, open * T::kGroup, n, [&](int i, float &x, int &k, int &v) {
         const int g = i / T::kGroup;
@@ -689,7 +691,7 @@ static __device__ __forceinline__ void beam_merge(const BeamSelect &a, MergeShar
 }
 static_assert(STG_BEAM_MAX_CANDIDATES <= kBeamThreads && STG_BEAM_MAX_CANDIDATES + kBeamRoom <= kBeamList && kBeamRoom <= kBeamThreads, "room in the list");
 
-// grid (pieces, rows).  The CTA that arrives last at its sequence's ticket joins the sequence's rows and leaves the ticket
+// grid (pieces, rows); like all kernels of a search launched while the one ahead of it ends.  The CTA that arrives last at its sequence's ticket joins the sequence's rows and leaves the ticket
 // at zero, as it was found.
 template <bool BF16, bool VEC, bool CAP>
 __global__ void __launch_bounds__(kBeamThreads, BF16 && CAP ? 1 : 2) k_beam_select(const __grid_constant__ BeamSelect a)
@@ -697,6 +699,8 @@ __global__ void __launch_bounds__(kBeamThreads, BF16 && CAP ? 1 : 2) k_beam_sele
     __shared__ MergeShared sh;
     __shared__ bool last;
     const int row = blockIdx.y, seq = row / a.beams;
+    pdl_release();
+    pdl_wait();
     const float score = a.scores[row];
     if (score > -CUDART_INF_F && score < CUDART_INF_F) beam_piece<BF16, VEC, CAP>(a, row, blockIdx.x);  // else a dead beam
     __syncthreads();
@@ -813,8 +817,7 @@ static int beam_select(StgHandle h, const StgBeamBatch *b, cudaStream_t stream)
                                                     : (capped ? k_beam_select<true, false, true> : k_beam_select<true, false, false>);
     else fn = vec ? (capped ? k_beam_select<false, true, true> : k_beam_select<false, true, false>)
                   : (capped ? k_beam_select<false, false, true> : k_beam_select<false, false, false>);
-    fn<<<dim3((unsigned)a.pieces, (unsigned)rows), kBeamThreads, 0, stream>>>(a);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_behind(fn, dim3((unsigned)a.pieces, (unsigned)rows), kBeamThreads, 0, stream, a);
     if (e != cudaSuccess) return cuda_fail(h, e, "k_beam_select launch");
     h->stats.calls++;
     h->stats.kernel_launches++;

@@ -10,6 +10,7 @@
 #include <string.h>
 
 #include "stg_beam.h"
+#include "stg_pdl.cuh"
 #include "stg_types.h"
 
 namespace stg {
@@ -24,6 +25,8 @@ struct EosSet {
 __global__ void __launch_bounds__(kStepWarps * 32) k_beam_start(const __grid_constant__ StgBeamSearch s, int first, int count)
 {
     const int lane = threadIdx.x & 31, i = blockIdx.x * kStepWarps + (threadIdx.x >> 5);
+    pdl_release();
+    pdl_wait();
     if (i >= count) return;
     const int seq = first + i, K = s.n_beams;
     if (lane < K) {
@@ -61,6 +64,8 @@ __global__ void __launch_bounds__(kStepWarps * 32) k_beam_advance(const __grid_c
     __shared__ int32_t next_tok[kStepWarps][32], next_par[kStepWarps][32];
     __shared__ float next_sc[kStepWarps][32];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, seq = blockIdx.x * kStepWarps + w;
+    pdl_release();
+    pdl_wait();
     if (seq >= s.n_seq) return;  // whole warps
     const int K = s.n_beams, o = seq * K + lane;
     const int t = s.steps[seq];
@@ -162,6 +167,8 @@ __global__ void __launch_bounds__(kTraceThreads) k_beam_backtrace(const __grid_c
     const int seq = blockIdx.x / C, tid = threadIdx.x, K = a.beams, N = a.hyps, W = K + 1;
     const int64_t row = (int64_t)a.n_seq * K;  // of the trail
     const int span = C * segment;
+    pdl_release();
+    pdl_wait();
     const uint32_t over_k = 0xFFFFFFFFu / (uint32_t)K + 1u;  // i / K is the upper half of i * over_k, for the i below and K > 1
     for (int n = tid; n < N; n += kTraceThreads) {
         const int64_t hyp = (int64_t)seq * N + n;
@@ -326,8 +333,7 @@ try {
         return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_beam_start: sequences outside [0, n_seq)");
     if (count == 0) return STG_OK;
     CK(cudaSetDevice(h->cfg.device));
-    k_beam_start<<<(count + kStepWarps - 1) / kStepWarps, kStepWarps * 32, 0, (cudaStream_t)stream>>>(*search, first_seq, count);
-    CK(cudaGetLastError());
+    CK(launch_behind(k_beam_start, dim3((unsigned)(count + kStepWarps - 1) / kStepWarps), kStepWarps * 32, 0, (cudaStream_t)stream, *search, first_seq, count));
     h->stats.kernel_launches++;
     return STG_OK;
 } catch (const std::bad_alloc &) {
@@ -350,9 +356,8 @@ try {
     eos.n = search->n_eos;
     for (int i = 0; i < eos.n; i++) eos.id[i] = search->eos_tokens[i];
     CK(cudaSetDevice(h->cfg.device));
-    k_beam_advance<<<(search->n_seq + kStepWarps - 1) / kStepWarps, kStepWarps * 32, 0, (cudaStream_t)stream>>>(
-        *search, eos, n_candidates, cand_tokens, cand_parents, cand_scores, finish);
-    CK(cudaGetLastError());
+    CK(launch_behind(k_beam_advance, dim3((unsigned)(search->n_seq + kStepWarps - 1) / kStepWarps), kStepWarps * 32, 0, (cudaStream_t)stream, *search, eos,
+                     n_candidates, cand_tokens, cand_parents, cand_scores, finish));
     h->stats.kernel_launches++;
     return STG_OK;
 } catch (const std::bad_alloc &) {
@@ -389,17 +394,19 @@ try {
     while (cluster < 8 && cluster * segment < n_steps) cluster *= 2;
     const size_t smem = trace_smem(n_beams);
     if (smem > 24 * 1024) CK(cudaFuncSetAttribute(k_beam_backtrace, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)cluster;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)n_seq * (unsigned)cluster);
     cfg.blockDim = dim3(kTraceThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t)stream;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
     CK(cudaLaunchKernelEx(&cfg, k_beam_backtrace, a, segment));
     h->stats.kernel_launches++;
     return STG_OK;

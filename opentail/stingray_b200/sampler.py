@@ -490,7 +490,7 @@ class BatchSampler:
             return getattr(stream, "cuda_stream", stream)
         import torch
 
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.device)  # current_stream builds an object around it: 1.3 us
 
     def _beam_array(self, name: str, x, dtype, shape):
         """The address of a contiguous CUDA tensor of this type and shape on the handle's device."""
