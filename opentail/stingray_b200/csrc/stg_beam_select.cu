@@ -70,11 +70,6 @@ struct BeamTile {
         if constexpr (kPacked) return (e & 1) ? bf16_hi(w[u][e / 2]) : bf16_lo(w[u][e / 2]);
         else return __uint_as_float(w[u][e]);
     }
-    __device__ __forceinline__ void set_low(int u, int e)
-    {
-        if constexpr (kPacked) w[u][e / 2] = (e & 1) ? (w[u][e / 2] & 0xFFFFu) | 0xFF800000u : (w[u][e / 2] & 0xFFFF0000u) | 0xFF80u;
-        else w[u][e] = 0xFF800000u;
-    }
     __device__ __forceinline__ void one(const LogitRow row, int u, int e, int j)
     {
         if constexpr (kPacked) {
@@ -168,12 +163,20 @@ struct BeamTile {
     // ... once the loads are back
     __device__ __forceinline__ void mask(uint32_t ok)
     {
-        if (ok == (uint32_t)((1ull << (U * E)) - 1ull) || ok == 0xFFFFFFFFu) return;
+        if (ok == 0xFFFFFFFFu) return;
 #pragma unroll
         for (int u = 0; u < U; u++)
+            if constexpr (kPacked) {
 #pragma unroll
-            for (int e = 0; e < E; e++)
-                if (!(ok >> (u * E + e) & 1u)) set_low(u, e);
+                for (int x = 0; x < E / 2; x++) {  // a byte permutation takes each half from the word or from -infinity
+                    const uint32_t two = ok >> (u * E + 2 * x) & 3u;
+                    w[u][x] = __byte_perm(0xFF80FF80u, w[u][x], 0x3210u + ((two | two << 7) & 0x101u) * 0x44u);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (!(ok >> (u * E + e) & 1u)) w[u][e] = 0xFF800000u;
+            }
     }
 };
 
@@ -447,7 +450,7 @@ static __device__ __forceinline__ void rank_list(MergeShared &sh, int c, int n, 
         int k = 0, ahead = 0;
         if (e < c) {
             s = sh.score[e]; w = sh.key[e]; k = sh.beam[e];
-#pragma unroll 2
+#pragma unroll 4
             for (int o = sub; o < c; o += kPer) {
                 const u64 x = sh.score[o];
                 if (x >= s) ahead += x > s || sh.beam[o] < k || (sh.beam[o] == k && sh.key[o] > w);
