@@ -108,6 +108,36 @@ public:
         check(stg_mtp_accept(h_, logits, dtype, rows, vocab, row_stride, draft, p_min, accept, argmax, prob, stream),
               "stg_mtp_accept");
     }
+    // Beam search: the best continuations of every sequence, their bookkeeping, per-beam state that follows, the hypotheses
+    void beam_select(StgBeamBatch batch, void *stream = nullptr)
+    {
+        batch.struct_size = (int32_t)sizeof(StgBeamBatch);
+        check(stg_beam_select(h_, &batch, stream), "stg_beam_select");
+    }
+    void beam_start(StgBeamSearch search, int first_seq, int count, void *stream = nullptr)
+    {
+        search.struct_size = (int32_t)sizeof(StgBeamSearch);
+        check(stg_beam_start(h_, &search, first_seq, count, stream), "stg_beam_start");
+    }
+    void beam_advance(StgBeamSearch search, int n_candidates, const int32_t *tokens, const int32_t *parents,
+                      const float *scores, bool finish = false, void *stream = nullptr)
+    {
+        search.struct_size = (int32_t)sizeof(StgBeamSearch);
+        check(stg_beam_advance(h_, &search, n_candidates, tokens, parents, scores, finish ? 1 : 0, stream), "stg_beam_advance");
+    }
+    void beam_reorder(StgBeamReorder reorder, void *stream = nullptr)
+    {
+        reorder.struct_size = (int32_t)sizeof(StgBeamReorder);
+        check(stg_beam_reorder(h_, &reorder, stream), "stg_beam_reorder");
+    }
+    // sequences: device int32 [n_seq, n_hyps, max_steps], out of the search's own trail
+    void beam_backtrace(const StgBeamSearch &search, int n_hyps, const int32_t *steps, const int32_t *parents,
+                        const int32_t *tokens, int32_t *sequences, int32_t *lengths = nullptr, void *stream = nullptr)
+    {
+        check(stg_beam_backtrace(h_, search.trail_tokens, search.trail_parents, search.max_steps, search.n_seq, search.n_beams,
+                                 n_hyps, steps, parents, tokens, search.pad_token, sequences, search.max_steps, lengths, stream),
+              "stg_beam_backtrace");
+    }
     StgStats stats() const
     {
         StgStats s{};

@@ -8,9 +8,10 @@
 
 namespace stg {
 
-// What one CTA leaves of its piece of a row: the sum of exp(x - ref) over its logits.
+// What one CTA leaves of its piece of a row: the sum of exp(x) over its logits, relative to a BeamRef (stg_beam_select.cu).
 struct BeamPart {
-    double s, ref;
+    double s;
+    float c, logit;
 };
 
 struct BeamWs {
@@ -28,6 +29,21 @@ inline size_t beam_ws_bytes(StgHandle h)
 
 // device arrays are checked for their elements' alignment, which the host can see
 inline bool misaligned(const void *p, size_t to) { return ((uintptr_t)p % to) != 0; }
+
+// The handle's device for the time of a call; the caller's is current again behind it.
+struct OnDevice {
+    int before = -1;
+    cudaError_t error;
+    explicit OnDevice(int device)
+    {
+        error = cudaGetDevice(&before);
+        if (error == cudaSuccess && before != device) error = cudaSetDevice(device);
+        if (before == device) before = -1;
+    }
+    ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
+    OnDevice(const OnDevice &) = delete;
+    OnDevice &operator=(const OnDevice &) = delete;
+};
 
 int beam_check_rows(StgHandle h, const char *who, int32_t n_seq, int32_t n_beams);
 

@@ -267,7 +267,8 @@ static int reorder(StgHandle h, const StgBeamReorder *r, cudaStream_t stream)
     if (rows == 0 || r->n_beams == 1) return STG_OK;
     if (!r->parents || misaligned(r->parents, 4) || misaligned(r->positions, 4))
         return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_beam_reorder: parents are missing, or an array is not aligned to its elements");
-    CK(cudaSetDevice(h->cfg.device));
+    const OnDevice on(h->cfg.device);
+    CK(on.error);
     const int total = r->n_states + (int)ring.size();
     std::vector<MoveState> moves;  // all of it is checked before any of it is moved
     for (int i = 0; i < total; i++) {

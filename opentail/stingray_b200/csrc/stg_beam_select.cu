@@ -9,9 +9,13 @@
 // candidates lie in the n best groups, whatever ties.  The CTA that ends last with a sequence finds those groups and
 // reads them once more.  One launch, no barrier and no list in the pass.
 //
-// The terms of S are computed and added up in 32 bits over the 16 or 32 elements that a thread holds, in 64 beyond: their
-// roundings (1e-7 each, either way) leave about 1e-8 of S, so two beams' candidates change places only if they lie
-// closer than that.
+// The terms of S are computed and added up in 32 bits over the 16 or 32 elements that a thread holds, in 64 beyond, and
+// every warp's largest is put right in 64: the others' roundings (1e-7 each, either way) leave 1e-8 of S (measured on rows of
+// 151,936, N(0, 2.5^2) and peaked: 1.0e-8 and 1.5e-8 in the mean square, 1.2e-7 at most), so two beams' candidates change
+// places only if they lie closer than that.
+//
+// What bounds it: the pass by HBM, 95 % of the copy rate on 256 rows of 151,936 fp32 (155 MB in 25 us); the join by latency,
+// 7 us for four beams and 13 for sixteen, of which only the last sequences' shows.
 #include <cuda_runtime.h>
 #include <math_constants.h>
 #include <stdint.h>
@@ -219,17 +223,33 @@ static __device__ __forceinline__ float warp_max(float v)
     return v;
 }
 
-// What a sum with reference `from` is multiplied by to have reference `to`
-static __device__ __noinline__ double scale(double from, double to) { return exp(from - to); }
-
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr float kHuge = 1e6f;  // logits beyond take the slow way: c could not tell them apart
 
-// The largest reference of a warp, or one that 32 bits do not tell from it
-static __device__ __forceinline__ double warp_ref(double r)
+// What a sum's terms are relative to: 2^c, c a whole number; or exp(logit) where that is not 0, -infinity as long as there
+// are none.
+struct BeamRef {
+    float c, logit;
+    __device__ __forceinline__ double natural() const { return logit != 0.f ? (double)logit : (double)c * kLn2; }
+};
+static __device__ __noinline__ double exp64(double x) { return exp(x); }
+
+// What a sum relative to `from` is multiplied by to be relative to `to`: without rounding where both are powers of two
+static __device__ __noinline__ double scale(BeamRef from, BeamRef to)
 {
-    const float f = (float)r;
-    return __shfl_sync(0xFFFFFFFFu, r, __ffs(__ballot_sync(0xFFFFFFFFu, f == warp_max(f))) - 1);
+    if (from.logit == 0.f && to.logit == 0.f) {
+        const int by = (int)(from.c - to.c);
+        return by < -1022 ? 0.0 : __hiloint2double((1023 + min(by, 1023)) << 20, 0);
+    }
+    return from.logit == -CUDART_INF_F ? 0.0 : exp(from.natural() - to.natural());
+}
+
+// The largest reference of a warp, or one that 32 bits do not tell from it
+static __device__ __forceinline__ BeamRef warp_ref(BeamRef r)
+{
+    const float f = (float)r.natural();
+    const int lane = __ffs(__ballot_sync(0xFFFFFFFFu, f == warp_max(f))) - 1;
+    return BeamRef{__shfl_sync(0xFFFFFFFFu, r.c, lane), __shfl_sync(0xFFFFFFFFu, r.logit, lane)};
 }
 
 // The sum of exp(x - top) over a group with logits beyond kHuge, element by element.
@@ -248,16 +268,18 @@ template <bool BF16, bool VEC, bool CAP>
 static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, int piece)
 {
     typedef BeamTile<BF16, VEC, CAP> T;
-    __shared__ double refs[kBeamWarps], sums[kBeamWarps];
+    __shared__ double sums[kBeamWarps];
+    __shared__ BeamRef refs[kBeamWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const LogitRow lr{(const char *)a.logits + (int64_t)row * a.row_stride * (BF16 ? 2 : 4), CAP ? a.softcap : 0.f};
     const uint32_t *mrow = a.mask != nullptr && (a.uses_mask == nullptr || a.uses_mask[row]) ? a.mask + (int64_t)row * a.mask_stride : nullptr;
     const int begin = piece * a.piece_len + warp * T::kGroup, end = min(a.vocab, (piece + 1) * a.piece_len);
     float *tops = a.ws.tops + (int64_t)row * a.groups;
-    // The sum's terms are exp(x) / 2^c; the same for a warp.  2^c need only be near the largest: c is a multiple of 16, so
-    // that most warps of a row have the same and their sums need no scaling, and follows the maximum `limit` at a time.
-    float c = 0.f, limit = -CUDART_INF_F;
-    double ref = -CUDART_INF, s = 0.0;  // c ln 2, what the terms are relative to
+    // The sum's terms are exp(x) / 2^c; the same c for a warp.  2^c lies near the largest, as the exponent's rounding goes with
+    // its size, and follows when a logit is `limit` or more.
+    BeamRef ref{0.f, -CUDART_INF_F};
+    float limit = -CUDART_INF_F, best = -CUDART_INF_F;
+    double s = 0.0;
     // A group's loads are in flight while the one ahead of it is added up, its mask's a group earlier still.
     uint32_t ok = T::allowed(mrow, begin, end), next_ok = T::allowed(mrow, begin + T::kLen, end);
     T next;
@@ -273,25 +295,25 @@ static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, 
         }
         const float top = warp_max(t.top());
         if (lane == 0) tops[base / T::kGroup] = top;
-        if ((fabsf(top) > kHuge || ref > (double)kHuge) && top > -CUDART_INF_F) {
-            const double now = fmax(ref, (double)top);
-            if (now != ref) {
+        if ((fabsf(top) > kHuge || ref.logit > kHuge) && top > -CUDART_INF_F) {
+            if ((double)top > ref.natural()) {
+                const BeamRef now{0.f, top};
                 s *= scale(ref, now);
                 ref = now;
                 limit = -CUDART_INF_F;  // no c any more
             }
-            s += (double)huge_group<BF16, VEC, CAP>(lr, mrow, base, end, top) * scale((double)top, now);
+            s += (double)huge_group<BF16, VEC, CAP>(lr, mrow, base, end, top) * exp64((double)top - ref.natural());
             continue;
         }
+        best = fmaxf(best, top);
         if (top > limit) {
-            c = floorf(top * (1.44269502f / 16.f)) * 16.f;
-            limit = (c + 48.f) * 0.693147181f;
-            const double now = (double)c * kLn2;
-            if (now != ref) s *= scale(ref, now);
+            const BeamRef now{floorf(top * 1.44269502f), 0.f};
+            s *= scale(ref, now);
             ref = now;
+            limit = (now.c + 4.f) * 0.693147181f;
         }
         f32x2 part = pair(0.f, 0.f);
-        const f32x2 minus_c = pair(-c, -c);
+        const f32x2 minus_c = pair(-ref.c, -ref.c);
 #pragma unroll
         for (int u = 0; u < T::U; u++)
 #pragma unroll
@@ -300,17 +322,23 @@ static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, 
         unpair(part, p0, p1);
         s += (double)(p0 + p1);
     }
+    // The largest term was made with the c that there is now.  Where a row's sum is little more than its largest term, that one's
+    // error is the sum's, so the warps' largest are put right: 64 bits in place of what was added.
+    if (lane == 0 && ref.logit == 0.f && best > -CUDART_INF_F) {
+        float was, unused;
+        unpair(exp_pair(pair(best, best), pair(-ref.c, -ref.c)), was, unused);
+        s += exp64((double)best - ref.natural()) - (double)was;
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
     if (lane == 0) { sums[warp] = s; refs[warp] = ref; }
     __syncthreads();
     if (warp == 0) {
-        const double wr = refs[lane % kBeamWarps], r = warp_ref(wr);
-        double ws = sums[lane % kBeamWarps];
-        if (wr != r) ws *= scale(wr, r);  // 0 for a warp that has read -infinity alone
+        const BeamRef wr = refs[lane % kBeamWarps], r = warp_ref(wr);
+        double ws = sums[lane % kBeamWarps] * scale(wr, r);  // 0 for a warp that has read -infinity alone
 #pragma unroll
         for (int o = kBeamWarps / 2; o > 0; o >>= 1) ws += __shfl_xor_sync(0xFFFFFFFFu, ws, o);
-        if (lane == 0) a.ws.parts[(int64_t)row * a.pieces + piece] = BeamPart{ws, r};
+        if (lane == 0) a.ws.parts[(int64_t)row * a.pieces + piece] = BeamPart{ws, r.c, r.logit};
     }
 }
 
@@ -386,7 +414,7 @@ struct MergeShared {
 
 // `low` out of every thread's best item (its x + about; -infinity: none), such that n of them reach it.  Up to 32: the n-th
 // largest of 64 groups of threads, each of which counts those above its own.  Beyond: the upper 20 bits of the n-th
-// largest of 256, found two by two (0.9 us against 0.3).  0 where there are no n.  Meanwhile `aside` is called by a warp
+// largest of 256, found two by two, which takes longer.  0 where there are no n.  Meanwhile `aside` is called by a warp
 // that has nothing to do with it.  All threads.
 template <class Aside>
 static __device__ __forceinline__ void find_low(MergeShared &sh, int K, int n, float best, Aside aside)
@@ -535,18 +563,19 @@ static __device__ __forceinline__ void beam_merge(const BeamSelect &a, MergeShar
         const int row = seq * K + k;
         const float score = a.scores[row];
         const bool alive = score > -CUDART_INF_F && score < CUDART_INF_F;
-        double r = -CUDART_INF, s = 0.0;
+        BeamRef r{0.f, -CUDART_INF_F};
+        double s = 0.0;
 #pragma unroll 1
         for (int c = lane; c < C; c += 32) {
-            const double2 p = __ldcg((const double2 *)(a.ws.parts + (int64_t)row * C + c));  // of a dead beam: not written, not used
-            const double now = fmax(r, p.y);
-            if (now != r) s *= scale(r, now);
-            s += p.y != now ? p.x * scale(p.y, now) : p.x;
+            const uint4 raw = __ldcg((const uint4 *)(a.ws.parts + (int64_t)row * C + c));  // of a dead beam: not written, not used
+            const BeamRef p{__uint_as_float(raw.z), __uint_as_float(raw.w)}, now = p.natural() > r.natural() ? p : r;
+            s = s * scale(r, now) + __hiloint2double((int)raw.y, (int)raw.x) * scale(p, now);
             r = now;
         }
-        if (!alive) { r = -CUDART_INF; s = 0.0; }
-        const double m = warp_ref(r);
-        if (r != m) s *= scale(r, m);
+        if (!alive) { r = BeamRef{0.f, -CUDART_INF_F}; s = 0.0; }
+        const BeamRef row_ref = warp_ref(r);
+        const double m = row_ref.natural();
+        s *= scale(r, row_ref);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
         if (lane == 0) {
@@ -694,18 +723,18 @@ static __device__ __forceinline__ void beam_merge(const BeamSelect &a, MergeShar
 }
 static_assert(STG_BEAM_MAX_CANDIDATES <= kBeamThreads && STG_BEAM_MAX_CANDIDATES + kBeamRoom <= kBeamList && kBeamRoom <= kBeamThreads, "room in the list");
 
-// grid (pieces, rows); like all kernels of a search launched while the one ahead of it ends.  The CTA that arrives last at its sequence's ticket joins the sequence's rows and leaves the ticket
-// at zero, as it was found.
+// A CTA per piece of a row; like all kernels of a search launched while the one ahead of it ends.  The CTA that arrives last at
+// its sequence's ticket joins the sequence's rows and leaves the ticket at zero, as it was found.
 template <bool BF16, bool VEC, bool CAP>
 __global__ void __launch_bounds__(kBeamThreads, BF16 && CAP ? 1 : 2) k_beam_select(const __grid_constant__ BeamSelect a)
 {
     __shared__ MergeShared sh;
     __shared__ bool last;
-    const int row = blockIdx.y, seq = row / a.beams;
+    const int row = (int)(blockIdx.x / (unsigned)a.pieces), piece = (int)(blockIdx.x % (unsigned)a.pieces), seq = row / a.beams;
     pdl_release();
     pdl_wait();
     const float score = a.scores[row];
-    if (score > -CUDART_INF_F && score < CUDART_INF_F) beam_piece<BF16, VEC, CAP>(a, row, blockIdx.x);  // else a dead beam
+    if (score > -CUDART_INF_F && score < CUDART_INF_F) beam_piece<BF16, VEC, CAP>(a, row, piece);  // else a dead beam
     __syncthreads();
     if (threadIdx.x == 0) {
         uint32_t before;  // behind the barrier: for what the whole CTA has written, and what the others have
@@ -741,9 +770,9 @@ static int captured_workspace(StgHandle h, size_t bytes, void **out)
 }
 
 // How many CTAs share a row.  Two fit an SM; of the cuts into whole tiles the one with the least time, waves of CTAs
-// times tiles of each and about two tiles' worth for the rest of a CTA.  (256 rows of 151,936 fp32: one piece 35.2 us, two
-// 37.2, ten 51.2; 64 rows of 262,144 bf16 behind masks: four pieces 27, three 35, eight 29; 4 rows of 151,936: nineteen
-// pieces 11.7, ten 12.5.)
+// times tiles of each and about two tiles' worth for the rest of a CTA.  (256 rows of 151,936 fp32: one piece 33.6 us, two
+// 34.7, ten 49.0; 64 rows of 262,144 bf16 behind masks: four pieces 20.3, three 24.4, eight 22.0; 4 rows of 151,936: nineteen
+// pieces 10.3, ten 10.8.)
 static void beam_pieces(int rows, int vocab, int tile, int sms, int &pieces, int &len)
 {
     const int tiles = (vocab + tile - 1) / tile;
@@ -780,7 +809,8 @@ static int beam_select(StgHandle h, const StgBeamBatch *b, cudaStream_t stream)
     if (misaligned(b->logits, esz) || misaligned(b->scores, 4) || misaligned(b->mask, 4) || misaligned(b->tokens, 4) || misaligned(b->parents, 4) ||
         misaligned(b->candidate_scores, 4) || misaligned(b->log_norms, 4) || misaligned(b->seq_flags, 4))
         return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_beam_select: an array is not aligned to its elements");
-    CK(cudaSetDevice(h->cfg.device));
+    const OnDevice on(h->cfg.device);
+    CK(on.error);
     BeamSelect a;
     memset(&a, 0, sizeof(a));
     a.logits = b->logits; a.row_stride = b->row_stride; a.scores = b->scores;
@@ -820,7 +850,7 @@ static int beam_select(StgHandle h, const StgBeamBatch *b, cudaStream_t stream)
                                                     : (capped ? k_beam_select<true, false, true> : k_beam_select<true, false, false>);
     else fn = vec ? (capped ? k_beam_select<false, true, true> : k_beam_select<false, true, false>)
                   : (capped ? k_beam_select<false, false, true> : k_beam_select<false, false, false>);
-    const cudaError_t e = launch_behind(fn, dim3((unsigned)a.pieces, (unsigned)rows), kBeamThreads, 0, stream, a);
+    const cudaError_t e = launch_behind(fn, dim3((unsigned)a.pieces * (unsigned)rows), kBeamThreads, 0, stream, a);
     if (e != cudaSuccess) return cuda_fail(h, e, "k_beam_select launch");
     h->stats.calls++;
     h->stats.kernel_launches++;

@@ -1,8 +1,8 @@
 """stg_beam_select against the definition in 64 bits.
 
-Tolerances.  The sum S of a row's exp(x - m) is made of fp32 terms: expf is off by at most 2 units in the last place (2^-22
-of the term), its argument's rounding moves a term exp(-d) by at most d * 2^-24 of it (d * exp(-d) <= 0.37 of the largest: below 2^-25
-of S per term of size one, and S >= 1), and at most 32 terms are added up in 32 bits before 64 take over, 31 * 2^-24.  Together
+Tolerances.  The sum S of a row's terms 2^(x log2(e) - c) is made of fp32 terms: the exponential is off by at most 2^-22 of a
+term; its argument is rounded twice, by 2^-24 of its size, which is at most 5 for the largest terms and of no account for the small
+ones (d * 2^-d < 0.54): 2 * 5 * 0.7 * 2^-24; and at most 32 terms are added up in 32 bits before 64 take over, 31 * 2^-24.  Together
 below 2.3e-6 of S, which is what log S and every score of the row may be off by (LSE); a score is rounded to 32 bits once more.
 So two candidates of different beams may change places only if their scores lie within 2 * LSE; candidates of one beam never."""
 import numpy as np
@@ -356,6 +356,50 @@ def test_captured_calls_have_workspace_of_their_own(bs):
         torch.cuda.synchronize()
         for o, w in zip(outs, want):
             assert all(torch.equal(o[k], w[k]) for k in w)
+
+
+def test_normalisers_are_closer_than_their_bound(bs):
+    """Rows whose best logit is 0, beams whose score is the row's normaliser as a float: the best candidate's score is what that
+    rounds off, a number so small that 32 bits show how exact the normaliser is.  The terms' errors go either way and their
+    sum's is that of their mean square: with p_i the probabilities, 2^-22 * sqrt(sum p_i^2) from the exponentials and as much from
+    the additions in 32 bits, five times that as a bound for the worst of 64 rows."""
+    import torch
+
+    for V, scale in ((50257, 2.5), (151936, 3.0)):
+        x = _normal(64, V, 5, scale=scale)
+        x[::2, :16] += 8.0  # peaked rows
+        x = (x - x.amax(1, keepdim=True)).cuda()
+        norm = torch.logsumexp(x.double(), 1)
+        p = torch.exp(x.double() - norm[:, None])
+        bound = 5 * 2 * 2.0 ** -22 * p.square().sum(1).sqrt()
+        got = bs.beam_select(x, norm.float().view(64, 1), 1)
+        assert ((got["scores"].view(64).double() - (norm.float().double() - norm)).abs() <= bound).all()
+
+
+def test_more_rows_than_a_grid_has_in_one_dimension():
+    import torch
+
+    b = _sampler(max_rows=66000, max_vocab=64, max_history=1, max_top_k=1)
+    try:
+        x = torch.randn((66000, 40), generator=torch.Generator().manual_seed(2)).cuda()
+        got = b.beam_select(x, torch.zeros((66000, 1), device="cuda"), 2)
+        best = x.topk(2, 1)
+        assert torch.equal(got["tokens"].long(), best.indices)
+        lp = best.values.double() - torch.logsumexp(x.double(), 1, keepdim=True)
+        assert ((got["scores"] - lp).abs() <= 2 * LSE + lp.abs() * 2.0 ** -24).all()
+    finally:
+        b.close()
+
+
+def test_outputs_stay_within_their_tensors(bs):
+    import torch
+
+    x, s = _normal(12, 3001, 2).cuda(), torch.from_numpy(_scores(3, 4, 2)).cuda()
+    wide = {k: torch.full((5, 9), -77, dtype=d, device="cuda") for k, d in (("tokens", torch.int32), ("parents", torch.int32), ("scores", torch.float32))}
+    out = bs.beam_select(x, s, 9, out={k: v[1:4] for k, v in wide.items()})
+    want = bs.beam_select(x, s, 9)
+    for k, v in wide.items():
+        assert torch.equal(out[k], want[k]) and (v[0] == -77).all() and (v[4] == -77).all()
 
 
 def test_refusals(bs):

@@ -518,6 +518,37 @@ def _decode(bs, B, K, V, T, eos, seed, capture):
     return path, search
 
 
+def test_kernels_behind_one_another_wait_for_one_another(bs):
+    """Each kernel starts while the one ahead of it ends: a chain without a pause gives what it gives with one behind every call."""
+    import torch
+    from opentail.stingray_b200 import BeamSearch, BeamStates
+
+    def chain(pause):
+        g = torch.Generator().manual_seed(9)
+        B, K, V, T = 16, 4, 4001, 60
+        logits = torch.randn((T, B * K, V), generator=g).cuda() * 2
+        state = torch.randn((B * K, 3, 37), generator=g).cuda()
+        search = BeamSearch(B, K, T, eos=[1, 2], length_penalty=0.9)
+        states = BeamStates([state], K)
+        bs.beam_start(search)
+        pause()
+        best = None
+        for t in range(T):
+            best = bs.beam_select(logits[t], search.scores, search.n_candidates, out=best)
+            pause()
+            bs.beam_advance(search, best)
+            pause()
+            bs.beam_reorder(states, search.parents)
+            pause()
+        found = bs.beam_backtrace(search.trail_tokens, search.trail_parents, search.pool_steps, search.pool_parents, search.pool_tokens)
+        return [state, search.pool_scores, search.steps, found["sequences"], found["lengths"]]
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(5):
+        for a, b in zip(chain(lambda: None), want):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("capture", [False, True])
 @pytest.mark.parametrize("B,K,V,T,eos", [(1, 4, 97, 12, [2]), (5, 3, 201, 9, [2, 7]), (3, 8, 64, 20, []), (2, 1, 50, 6, [1])])
 def test_a_whole_search(bs, B, K, V, T, eos, capture):
