@@ -481,7 +481,8 @@ static __device__ __forceinline__ void rank_list(MergeShared &sh, int c, int n, 
 #pragma unroll 4
             for (int o = sub; o < c; o += kPer) {
                 const u64 x = sh.score[o];
-                if (x >= s) ahead += x > s || sh.beam[o] < k || (sh.beam[o] == k && sh.key[o] > w);
+                ahead += x > s;
+                if (x == s && o != e) ahead += sh.beam[o] < k || (sh.beam[o] == k && sh.key[o] > w);
             }
         }
 #pragma unroll
