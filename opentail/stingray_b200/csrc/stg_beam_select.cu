@@ -413,9 +413,9 @@ struct MergeShared {
 // included: loops are left rolled and what is used twice is a function, while loads are issued several at a time.
 
 // `low` out of every thread's best item (its x + about; -infinity: none), such that n of them reach it.  Up to 32: the n-th
-// largest of 64 groups of threads, each of which counts those above its own.  Beyond: the upper 20 bits of the n-th
-// largest of 256, found two by two, which takes longer.  0 where there are no n.  Meanwhile `aside` is called by a warp
-// that has nothing to do with it.  All threads.
+// largest of 64 groups of threads, made distinct by their last six bits, for each of which four threads count those above
+// it.  Beyond: the upper 20 bits of the n-th largest of 256, found two by two, which takes longer.  0 where there are no n.
+// Meanwhile `aside` is called by a warp that has nothing to do with it.  All threads.
 template <class Aside>
 static __device__ __forceinline__ void find_low(MergeShared &sh, int K, int n, float best, Aside aside)
 {
@@ -425,20 +425,22 @@ static __device__ __forceinline__ void find_low(MergeShared &sh, int K, int n, f
 #pragma unroll
     for (int o = 1; o < kBeamThreads / 64; o *= 2)
         if (o < per) mine = max(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, o));
+    if (n <= 32) mine = mine >= 64u ? (mine & ~63u) | (63u - (unsigned)(tid / per)) : 0u;
     if (tid % per == 0) sh.tops[tid / per] = mine;
     __syncthreads();
-    if (tid >= 64) {
-        if (tid < 96) aside(tid - 64);
+    if (tid >= 256) {
+        if (tid < 288) aside(tid - 256);
     } else if (n <= 32) {
-        mine = sh.tops[tid];
+        mine = sh.tops[tid / 4];
         int ahead = 0;
-#pragma unroll 4
-        for (int i = 0; i < 64; i += 4) {
-            const uint4 v = *(const uint4 *)(sh.tops + i);
-            ahead += (v.x > mine || (v.x == mine && i < tid)) + (v.y > mine || (v.y == mine && i + 1 < tid)) +
-                     (v.z > mine || (v.z == mine && i + 2 < tid)) + (v.w > mine || (v.w == mine && i + 3 < tid));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint4 v = *(const uint4 *)(sh.tops + (tid % 4 + 4 * i) * 4);
+            ahead += (v.x > mine) + (v.y > mine) + (v.z > mine) + (v.w > mine);
         }
-        if (ahead == n - 1) sh.low = max(sh.low, mine);
+        ahead += __shfl_xor_sync(0xFFFFFFFFu, ahead, 1);
+        ahead += __shfl_xor_sync(0xFFFFFFFFu, ahead, 2);
+        if (ahead == n - 1 && tid % 4 == 0) sh.low = max(sh.low, mine & ~63u);
     } else if (tid < 32) {
         uint32_t v[8], found = 0u;
 #pragma unroll
@@ -569,9 +571,16 @@ static __device__ __forceinline__ void beam_merge(const BeamSelect &a, MergeShar
 #pragma unroll 1
         for (int c = lane; c < C; c += 32) {
             const uint4 raw = __ldcg((const uint4 *)(a.ws.parts + (int64_t)row * C + c));  // of a dead beam: not written, not used
-            const BeamRef p{__uint_as_float(raw.z), __uint_as_float(raw.w)}, now = p.natural() > r.natural() ? p : r;
-            s = s * scale(r, now) + __hiloint2double((int)raw.y, (int)raw.x) * scale(p, now);
-            r = now;
+            const BeamRef p{__uint_as_float(raw.z), __uint_as_float(raw.w)};
+            const double ps = __hiloint2double((int)raw.y, (int)raw.x);
+            if (c < 32) {  // the only one as a rule
+                s = ps;
+                r = p;
+            } else {
+                const BeamRef now = p.natural() > r.natural() ? p : r;
+                s = s * scale(r, now) + ps * scale(p, now);
+                r = now;
+            }
         }
         if (!alive) { r = BeamRef{0.f, -CUDART_INF_F}; s = 0.0; }
         const BeamRef row_ref = warp_ref(r);
