@@ -33,7 +33,6 @@ namespace stg {
 constexpr int kBeamThreads = 512;
 constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kBeamList = 512;  // candidates in shared memory
-constexpr int kBeamRoom = 256;  // so many are offered between two looks at the list, where it may overflow
 
 struct BeamSelect {
     const void *logits;
@@ -352,19 +351,33 @@ static __device__ __forceinline__ double unord64(u64 k)
     return __longlong_as_double((long long)((k >> 63) ? (k & 0x7FFFFFFFFFFFFFFFull) : ~k));
 }
 
-// What is ordered: groups, by their best candidate, and candidates.  Larger score (ord64), then lower beam, then larger key
-// (make_key: the logit, then the lower group or token).
+// What is ordered: groups, by their best candidate, and candidates.  `score` is the score as ord64; `rest` decides between equal
+// ones: the lower beam, then the larger logit, then the lower group or token.
+struct BeamItem {
+    u64 score, rest;
+};
+constexpr int kPosBits = 27;  // 5 bits for the beam, 32 for the logit
+constexpr u64 kPosMask = (1ull << kPosBits) - 1ull;
+static __device__ __forceinline__ u64 item_rest(float x, int k, int pos)
+{
+    return (u64)(STG_BEAM_MAX_BEAMS - 1 - k) << 59 | (u64)ord32(x) << kPosBits | (kPosMask - (u64)pos);
+}
+static __device__ __forceinline__ int item_beam(u64 rest) { return STG_BEAM_MAX_BEAMS - 1 - (int)(rest >> 59); }
+static __device__ __forceinline__ float item_logit(u64 rest) { return unord32((uint32_t)(rest >> kPosBits)); }
+static __device__ __forceinline__ int item_pos(u64 rest) { return (int)(kPosMask - (rest & kPosMask)); }
+static __device__ __forceinline__ bool ahead_of(const BeamItem a, const BeamItem b)
+{
+    return a.score > b.score || (a.score == b.score && a.rest > b.rest);
+}
+
 constexpr int kStage = 8;  // loads of a thread in flight, 8 of 4 bytes or 4 of 16
 struct MergeShared {
     union {
         float head[kStage][kBeamThreads];
         uint4 vec[kStage / 2][kBeamThreads];
     } stage;
-    u64 score[kBeamList], key[kBeamList];
+    BeamItem list[kBeamList];
     uint32_t tops[256];
-    uint8_t beam[kBeamList];
-    u64 kept_score[STG_BEAM_MAX_CANDIDATES], kept_key[STG_BEAM_MAX_CANDIDATES];
-    uint8_t kept_beam[STG_BEAM_MAX_CANDIDATES];
     double sum[STG_BEAM_MAX_BEAMS];    // S of a beam, relative to ref
     double ref[STG_BEAM_MAX_BEAMS];
     double base[STG_BEAM_MAX_BEAMS];   // a beam's candidates score base + (logit - ref)
@@ -372,19 +385,11 @@ struct MergeShared {
     float least[STG_BEAM_MAX_BEAMS];   // no smaller logit reaches `low`; NaN: the beam has no candidates
     int group[STG_BEAM_MAX_CANDIDATES];          // the groups that are read again
     uint8_t group_beam[STG_BEAM_MAX_CANDIDATES];
-    u64 bound_score, bound_key;        // the n-th best so far
-    int bound_beam;
     uint32_t low;                      // a float, as ord32, that n candidates reach in `about`; 0: none
     uint32_t flags;
     int cnt;
 
     __device__ __forceinline__ u64 score_of(int k, float x) const { return ord64(((double)x - ref[k]) + base[k]); }
-    __device__ __forceinline__ void clear()
-    {
-        cnt = 0;
-        bound_score = bound_key = 0ull;
-        bound_beam = STG_BEAM_MAX_BEAMS;
-    }
     // x + about is off by a few roundings (2^-24) of x, of what `about` was made of - the normaliser's logarithm, at most 46
     // beside `ref`, among it - and of the sum; `size` is the largest |about| + |ref| of the beams.
     __device__ __forceinline__ void set_least(int k, float size)
@@ -393,19 +398,22 @@ struct MergeShared {
         const float l = unord32(low), x = l - about[k];
         least[k] = x - (1e-6f * (fabsf(x) + fabsf(l)) + 2e-6f * size + 2e-5f);
     }
+    // More than the list takes have come: nothing of it will be used, so nobody need come any more
+    __device__ __forceinline__ bool full() const { return *(const volatile int *)&cnt > kBeamList; }
     // x has reached `least`: it may be one of the n best.  Its score is made when all have come.
     __device__ __forceinline__ void offer(float x, int k, int pos)
     {
+        if (full()) return;
         const int at = atomicAdd(&cnt, 1);
-        if (at < kBeamList) { key[at] = make_key(x, pos); beam[at] = (uint8_t)k; }
+        if (at < kBeamList) list[at].rest = item_rest(x, k, pos);
     }
-    // The same with its score at once, which the n-th best so far is held against
-    __device__ __noinline__ void offer_if_ahead(float x, int k, int pos)
+    // The same with its score at once, unless it is behind `bound`
+    __device__ __noinline__ void offer_from(float x, int k, int pos, const BeamItem bound)
     {
-        const u64 s = score_of(k, x), w = make_key(x, pos);
-        if (s < bound_score || (s == bound_score && (k > bound_beam || (k == bound_beam && w <= bound_key)))) return;
+        const BeamItem item{score_of(k, x), item_rest(x, k, pos)};
+        if (ahead_of(bound, item)) return;
         const int at = atomicAdd(&cnt, 1);
-        if (at < kBeamList) { score[at] = s; key[at] = w; beam[at] = (uint8_t)k; }
+        if (at < kBeamList) list[at] = item;
     }
 };
 
@@ -466,78 +474,87 @@ static __device__ __forceinline__ void find_low(MergeShared &sh, int K, int n, f
     __syncthreads();
 }
 
-// Hands the n best of a list of c entries to emit(place, score, key, beam), in whatever order.  Eight threads per entry count
-// those ahead of it: no two are the same.  All threads; the list has settled.
+// Sorts the first c entries of the list, best first (bitonic; what it is filled up with is behind everything).  All threads.
+static __device__ __noinline__ void sort_list(MergeShared &sh, int c)
+{
+    int len = 32;
+    while (len < c) len <<= 1;
+    for (int i = c + (int)threadIdx.x; i < len; i += kBeamThreads) sh.list[i] = BeamItem{0ull, 0ull};
+    __syncthreads();
+    for (int k = 2; k <= len; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            for (int t = threadIdx.x; t < len / 2; t += kBeamThreads) {
+                const int a = 2 * j * (t / j) + t % j, b = a + j;
+                const BeamItem x = sh.list[a], y = sh.list[b];
+                if (ahead_of(y, x) == ((a & k) == 0)) { sh.list[a] = y; sh.list[b] = x; }
+            }
+            __syncthreads();
+        }
+}
+
+// Hands the n best of a list of c entries to emit(place, rest, score), in whatever order.  Few: eight threads per entry count
+// those ahead of it, no two being the same.  All threads; the list has settled.
 template <class Emit>
 static __device__ __forceinline__ void rank_list(MergeShared &sh, int c, int n, Emit emit)
 {
     constexpr int kPer = 8;
     const int tid = threadIdx.x, sub = tid % kPer;
+    if (c > 4 * (kBeamThreads / kPer)) {  // 512 entries: 45 steps of the sort against 8 rounds of 64
+        sort_list(sh, c);
+        if (tid < min(c, n)) emit(tid, sh.list[tid].rest, sh.list[tid].score);
+        return;
+    }
 #pragma unroll 1
     for (int first = 0; first < c; first += kBeamThreads / kPer) {
         const int e = first + tid / kPer;
-        u64 s = 0ull, w = 0ull;
-        int k = 0, ahead = 0;
+        BeamItem mine{0ull, 0ull};
+        int ahead = 0;
         if (e < c) {
-            s = sh.score[e]; w = sh.key[e]; k = sh.beam[e];
+            mine = sh.list[e];
 #pragma unroll 4
-            for (int o = sub; o < c; o += kPer) {
-                const u64 x = sh.score[o];
-                ahead += x > s;
-                if (x == s && o != e) ahead += sh.beam[o] < k || (sh.beam[o] == k && sh.key[o] > w);
-            }
+            for (int o = sub; o < c; o += kPer) ahead += ahead_of(sh.list[o], mine);
         }
 #pragma unroll
         for (int o = kPer / 2; o > 0; o >>= 1) ahead += __shfl_xor_sync(0xFFFFFFFFu, ahead, o);
-        if (e < c && sub == 0 && ahead < n) emit(ahead, s, w, k);
+        if (e < c && sub == 0 && ahead < n) emit(ahead, mine.rest, mine.score);
     }
 }
 
-// Leaves the n best of the list and the n-th as the bound.  All threads; the list has settled, and settles again.
-static __device__ __noinline__ void keep_best(MergeShared &sh, int c, int n)
-{
-    rank_list(sh, c, n, [&](int to, u64 s, u64 w, int k) {
-        sh.kept_score[to] = s; sh.kept_key[to] = w; sh.kept_beam[to] = (uint8_t)k;
-        if (to == n - 1) { sh.bound_score = s; sh.bound_key = w; sh.bound_beam = k; }
-    });
-    __syncthreads();
-    const int left = min(c, n), tid = threadIdx.x;
-    if (tid < left) { sh.score[tid] = sh.kept_score[tid]; sh.key[tid] = sh.kept_key[tid]; sh.beam[tid] = sh.kept_beam[tid]; }
-    if (tid == 0) sh.cnt = left;
-    __syncthreads();
-}
-
 // After items have been offered: the list holds the n best of them and perhaps more; how many.  Where more were offered than
-// it takes - many equal ones - all of them are offered again, get(i, x, k, pos) for i below `total`, some at a time, with a
-// bound that tells them apart.
+// it takes - equal ones, a row that ascends - get(i, x, k, pos) for i below `total` is gone through again, every thread a stretch
+// of its own, until the list is full; the n-th best of what it holds then is a bound for the next time.  As the list is
+// an even sample, that leaves about n of kBeamList.
 template <class Get>
 static __device__ __forceinline__ int settle(MergeShared &sh, int total, int n, Get get)
 {
+    const int tid = threadIdx.x;
     __syncthreads();
     int c = sh.cnt;
     if (c <= kBeamList) {
 #pragma unroll 1
-        for (int i = threadIdx.x; i < c; i += kBeamThreads) sh.score[i] = sh.score_of(sh.beam[i], key_val(sh.key[i]));
+        for (int i = tid; i < c; i += kBeamThreads) sh.list[i].score = sh.score_of(item_beam(sh.list[i].rest), item_logit(sh.list[i].rest));
         __syncthreads();
         return c;
     }
-    __syncthreads();  // read by all before it changes
-    if (threadIdx.x == 0) sh.cnt = 0;
-    __syncthreads();
+    const int stretch = (total + kBeamThreads - 1) / kBeamThreads;
+    BeamItem bound{0ull, 0ull};
+    for (;;) {  // ends: of a full list all but n entries are behind the next bound
+        __syncthreads();  // cnt and the list have been read by all
+        if (tid == 0) sh.cnt = 0;
+        __syncthreads();
 #pragma unroll 1
-    for (int first = 0; first < total; first += kBeamRoom) {
-        float x;
-        int k, pos;
-        const int i = first + (int)threadIdx.x;
-        if (threadIdx.x < kBeamRoom && i < total && get(i, x, k, pos) && x >= sh.least[k] && x > -CUDART_INF_F) sh.offer_if_ahead(x, k, pos);
+        for (int i = tid * stretch; i < min(total, (tid + 1) * stretch) && !sh.full(); i++) {
+            float x;
+            int k, pos;
+            if (get(i, x, k, pos) && x >= sh.least[k] && x > -CUDART_INF_F) sh.offer_from(x, k, pos, bound);
+        }
         __syncthreads();
         c = sh.cnt;
+        if (c <= kBeamList) return c;
         __syncthreads();
-        if (c > kBeamList - kBeamRoom) keep_best(sh, c, n);
+        sort_list(sh, kBeamList);
+        bound = sh.list[n - 1];
     }
-    c = sh.cnt;
-    __syncthreads();
-    return c;
 }
 
 // The candidates of one sequence out of its rows' sums and group maxima, which other CTAs have written: read past the
@@ -559,7 +576,7 @@ static __device__ __forceinline__ void beam_merge(const BeamSelect &a, MergeShar
         for (int j = 0; j < kStage; j++) sh.stage.head[j][tid] = head[j];  // a thread reads what it wrote
     };
     load_heads(0);
-    if (tid == 0) { sh.clear(); sh.low = 0u; sh.flags = 0u; }
+    if (tid == 0) { sh.cnt = 0; sh.low = 0u; sh.flags = 0u; }
     __syncthreads();
 #pragma unroll 1
     for (int k = tid >> 5; k < K; k += kBeamWarps) {
@@ -639,12 +656,12 @@ static __device__ __forceinline__ void beam_merge(const BeamSelect &a, MergeShar
         x = __ldcg(tops + i);
         return true;
     });
-    rank_list(sh, c, n, [&](int to, u64, u64 w, int k) { sh.group[to] = key_idx(w); sh.group_beam[to] = (uint8_t)k; });
+    rank_list(sh, c, n, [&](int to, u64 rest, u64) { sh.group[to] = item_pos(rest); sh.group_beam[to] = (uint8_t)item_beam(rest); });
     __syncthreads();
 
     // ---- the n best candidates, which lie in them ----
     const int open = min(c, n);
-    if (tid == 0) sh.clear();
+    if (tid == 0) sh.cnt = 0;
     __syncthreads();
     constexpr int E = T::E, kVecs = T::kGroup / E, kBatch = kStage / 2;
     const int vecs = open * kVecs;
@@ -718,11 +735,11 @@ static __device__ __forceinline__ void beam_merge(const BeamSelect &a, MergeShar
         x = load_one<BF16>(row_of(k), v);
         return true;
     });
-    rank_list(sh, c, n, [&](int to, u64 s, u64 w, int k) {
+    rank_list(sh, c, n, [&](int to, u64 rest, u64 score) {
         const int64_t o = (int64_t)seq * n + to;
-        a.tokens[o] = key_idx(w);
-        a.parents[o] = k;
-        a.out_scores[o] = (float)unord64(s);
+        a.tokens[o] = item_pos(rest);
+        a.parents[o] = item_beam(rest);
+        a.out_scores[o] = (float)unord64(score);
     });
     if (tid >= c && tid < n) {
         const int64_t o = (int64_t)seq * n + tid;
@@ -731,7 +748,7 @@ static __device__ __forceinline__ void beam_merge(const BeamSelect &a, MergeShar
     }
     if (tid == 0 && a.flags) a.flags[seq] = sh.flags | (c < n ? (uint32_t)STG_BEAM_SHORT : 0u);
 }
-static_assert(STG_BEAM_MAX_CANDIDATES <= kBeamThreads && STG_BEAM_MAX_CANDIDATES + kBeamRoom <= kBeamList && kBeamRoom <= kBeamThreads, "room in the list");
+static_assert(STG_BEAM_MAX_BEAMS == 32 && STG_BEAM_MAX_CANDIDATES <= kBeamThreads && 2 * STG_BEAM_MAX_CANDIDATES <= kBeamList, "bits of an item, room in the list");
 
 // A CTA per piece of a row; like all kernels of a search launched while the one ahead of it ends.  The CTA that arrives last at
 // its sequence's ticket joins the sequence's rows and leaves the ticket at zero, as it was found.
@@ -805,6 +822,7 @@ static int beam_select(StgHandle h, const StgBeamBatch *b, cudaStream_t stream)
     if (rc) return rc;
     if (b->vocab <= 0) return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_beam_select: vocab must be > 0");
     if (b->vocab > h->cfg.max_vocab) return fail(h, STG_ERR_CAPACITY, "vocab exceeds max_vocab");
+    if ((int64_t)b->vocab > (int64_t)kPosMask) return fail(h, STG_ERR_UNSUPPORTED, "stg_beam_select: vocab beyond 2^27");
     if (b->n_candidates < 1) return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_beam_select: n_candidates must be >= 1");
     if (b->n_candidates > STG_BEAM_MAX_CANDIDATES) return fail(h, STG_ERR_CAPACITY, "stg_beam_select: at most 128 candidates per sequence");
     if (b->logits_dtype != STG_DTYPE_F32 && b->logits_dtype != STG_DTYPE_BF16) return fail(h, STG_ERR_INVALID_ARGUMENT, "unknown logits_dtype");
