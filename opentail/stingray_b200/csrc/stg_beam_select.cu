@@ -163,6 +163,31 @@ struct BeamTile {
             }
         }
     }
+    // The `kFew` allowed elements at most that a thread has where a mask leaves little, each by a load of its own, as numbers
+    static constexpr int kFew = 8, kWords = kPacked ? E / 2 : E;
+    __device__ __forceinline__ void load_few(const LogitRow row, uint32_t ok, int base)
+    {
+#pragma unroll
+        for (int q = 0; q < kFew; q++) {
+            const int b = __ffs(ok) - 1;
+            ok &= ok - 1u;
+            uint32_t x = 0xFF800000u;
+            if (b >= 0) {
+                const int j = base + (VEC ? ((b / E) * 32 + (int)(threadIdx.x & 31)) * E + b % E : b * 32 + (int)(threadIdx.x & 31));
+                x = BF16 ? (uint32_t)__ldg((const uint16_t *)row.p + j) << 16 : __ldg((const uint32_t *)row.p + j);
+            }
+            w[q / kWords][q % kWords] = x;
+        }
+    }
+    __device__ __forceinline__ void cap_few(uint32_t ok, float cap)
+    {
+        if constexpr (CAP)
+#pragma unroll
+            for (int q = 0; q < kFew; q++)
+                if (q < __popc(ok)) w[q / kWords][q % kWords] = __float_as_uint(soft_cap(few(q), cap));
+    }
+    __device__ __forceinline__ float few(int q) const { return __uint_as_float(w[q / kWords][q % kWords]); }
+
     // ... once the loads are back
     __device__ __forceinline__ void mask(uint32_t ok)
     {
@@ -263,7 +288,7 @@ static __device__ __noinline__ float huge_group(const LogitRow lr, const uint32_
 }
 
 // One piece of a row: its part of the sum and the maxima of its groups.
-template <bool BF16, bool VEC, bool CAP>
+template <bool BF16, bool VEC, bool CAP, bool MASK>
 static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, int piece)
 {
     typedef BeamTile<BF16, VEC, CAP> T;
@@ -271,7 +296,7 @@ static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, 
     __shared__ BeamRef refs[kBeamWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const LogitRow lr{(const char *)a.logits + (int64_t)row * a.row_stride * (BF16 ? 2 : 4), CAP ? a.softcap : 0.f};
-    const uint32_t *mrow = a.mask != nullptr && (a.uses_mask == nullptr || a.uses_mask[row]) ? a.mask + (int64_t)row * a.mask_stride : nullptr;
+    const uint32_t *mrow = MASK && (a.uses_mask == nullptr || a.uses_mask[row]) ? a.mask + (int64_t)row * a.mask_stride : nullptr;
     const int begin = piece * a.piece_len + warp * T::kGroup, end = min(a.vocab, (piece + 1) * a.piece_len);
     float *tops = a.ws.tops + (int64_t)row * a.groups;
     // The sum's terms are exp(x) / 2^c; the same c for a warp.  2^c lies near the largest, as the exponent's rounding goes with
@@ -279,20 +304,38 @@ static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, 
     BeamRef ref{0.f, -CUDART_INF_F};
     float limit = -CUDART_INF_F, best = -CUDART_INF_F;
     double s = 0.0;
-    // A group's loads are in flight while the one ahead of it is added up, its mask's a group earlier still.
+    // A group's loads are in flight while the one ahead of it is added up, its mask's a group earlier still.  Behind a mask that leaves
+    // no thread more than eight elements of its 32 bf16 ones - densities up to about a tenth - these alone are read and added up
+    // (256 rows of 262,144, densities of 0.1, 5 and 20 %: 35, 45 and 50 us, all in the long way 46, 47 and 47).  Of the 16 fp32
+    // ones that a thread has it is no gain (57, 62 and 64 against 53, 57 and 58).
+    const auto is_sparse = [&](uint32_t bits) { return MASK && BF16 && mrow != nullptr && __reduce_max_sync(0xFFFFFFFFu, (unsigned)__popc(bits)) <= (unsigned)T::kFew; };
     uint32_t ok = T::allowed(mrow, begin, end), next_ok = T::allowed(mrow, begin + T::kLen, end);
+    bool sparse = is_sparse(ok);
     T next;
-    if (begin < end) next.load(lr, mrow != nullptr, ok, begin, end);
+    if (begin < end) {
+        if (sparse) next.load_few(lr, ok, begin);
+        else next.load(lr, mrow != nullptr, ok, begin, end);
+    }
 #pragma unroll 1
     for (int base = begin; base < end; base += T::kLen) {
         T t = next;
-        t.mask(ok);
+        const bool few = sparse;
+        if (few) t.cap_few(ok, lr.cap); else t.mask(ok);
         ok = next_ok;
         if (base + T::kLen < end) {
-            next.load(lr, mrow != nullptr, ok, base + T::kLen, end);
+            sparse = is_sparse(ok);
+            if (sparse) next.load_few(lr, ok, base + T::kLen);
+            else next.load(lr, mrow != nullptr, ok, base + T::kLen, end);
             next_ok = T::allowed(mrow, base + 2 * T::kLen, end);
         }
-        const float top = warp_max(t.top());
+        float top = -CUDART_INF_F;
+        if (few) {
+#pragma unroll
+            for (int q = 0; q < T::kFew; q++) top = fmaxf(top, t.few(q));
+        } else {
+            top = t.top();
+        }
+        top = warp_max(top);
         if (lane == 0) tops[base / T::kGroup] = top;
         if ((fabsf(top) > kHuge || ref.logit > kHuge) && top > -CUDART_INF_F) {
             if ((double)top > ref.natural()) {
@@ -313,10 +356,15 @@ static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, 
         }
         f32x2 part = pair(0.f, 0.f);
         const f32x2 minus_c = pair(-ref.c, -ref.c);
+        if (few) {
 #pragma unroll
-        for (int u = 0; u < T::U; u++)
+            for (int q = 0; q < T::kFew; q += 2) part = add2(part, exp_pair(pair(t.few(q), t.few(q + 1)), minus_c));
+        } else {
 #pragma unroll
-            for (int e = 0; e < T::E; e += 2) part = add2(part, exp_pair(pair(t.get(u, e), t.get(u, e + 1)), minus_c));
+            for (int u = 0; u < T::U; u++)
+#pragma unroll
+                for (int e = 0; e < T::E; e += 2) part = add2(part, exp_pair(pair(t.get(u, e), t.get(u, e + 1)), minus_c));
+        }
         float p0, p1;
         unpair(part, p0, p1);
         s += (double)(p0 + p1);
@@ -752,7 +800,7 @@ static_assert(STG_BEAM_MAX_BEAMS == 32 && STG_BEAM_MAX_CANDIDATES <= kBeamThread
 
 // A CTA per piece of a row; like all kernels of a search launched while the one ahead of it ends.  The CTA that arrives last at
 // its sequence's ticket joins the sequence's rows and leaves the ticket at zero, as it was found.
-template <bool BF16, bool VEC, bool CAP>
+template <bool BF16, bool VEC, bool CAP, bool MASK>
 __global__ void __launch_bounds__(kBeamThreads, BF16 && CAP ? 1 : 2) k_beam_select(const __grid_constant__ BeamSelect a)
 {
     __shared__ MergeShared sh;
@@ -761,7 +809,7 @@ __global__ void __launch_bounds__(kBeamThreads, BF16 && CAP ? 1 : 2) k_beam_sele
     pdl_release();
     pdl_wait();
     const float score = a.scores[row];
-    if (score > -CUDART_INF_F && score < CUDART_INF_F) beam_piece<BF16, VEC, CAP>(a, row, piece);  // else a dead beam
+    if (score > -CUDART_INF_F && score < CUDART_INF_F) beam_piece<BF16, VEC, CAP, MASK>(a, row, piece);  // else a dead beam
     __syncthreads();
     if (threadIdx.x == 0) {
         uint32_t before;  // behind the barrier: for what the whole CTA has written, and what the others have
@@ -872,12 +920,14 @@ static int beam_select(StgHandle h, const StgBeamBatch *b, cudaStream_t stream)
     a.ws.tops = (float *)(ws + b_parts);
     if (captured) CK(cudaMemsetAsync(a.ws.tickets, 0, (size_t)b->n_seq * 4, stream));  // part of the graph
     const bool vec = !misaligned(b->logits, 16) && (rows == 1 || (size_t)b->row_stride * esz % 16 == 0);
-    const bool capped = b->logit_softcap != 0.f;
-    void (*fn)(BeamSelect);
-    if (b->logits_dtype == STG_DTYPE_BF16) fn = vec ? (capped ? k_beam_select<true, true, true> : k_beam_select<true, true, false>)
-                                                    : (capped ? k_beam_select<true, false, true> : k_beam_select<true, false, false>);
-    else fn = vec ? (capped ? k_beam_select<false, true, true> : k_beam_select<false, true, false>)
-                  : (capped ? k_beam_select<false, false, true> : k_beam_select<false, false, false>);
+    using Kernel = void (*)(BeamSelect);
+    // [bf16][vec][capped][masked]
+    static const Kernel kernels[2][2][2][2] = {
+        {{{k_beam_select<false, false, false, false>, k_beam_select<false, false, false, true>}, {k_beam_select<false, false, true, false>, k_beam_select<false, false, true, true>}},
+         {{k_beam_select<false, true, false, false>, k_beam_select<false, true, false, true>}, {k_beam_select<false, true, true, false>, k_beam_select<false, true, true, true>}}},
+        {{{k_beam_select<true, false, false, false>, k_beam_select<true, false, false, true>}, {k_beam_select<true, false, true, false>, k_beam_select<true, false, true, true>}},
+         {{k_beam_select<true, true, false, false>, k_beam_select<true, true, false, true>}, {k_beam_select<true, true, true, false>, k_beam_select<true, true, true, true>}}}};
+    const Kernel fn = kernels[b->logits_dtype == STG_DTYPE_BF16][vec][b->logit_softcap != 0.f][b->mask != nullptr];
     const cudaError_t e = launch_behind(fn, dim3((unsigned)a.pieces * (unsigned)rows), kBeamThreads, 0, stream, a);
     if (e != cudaSuccess) return cuda_fail(h, e, "k_beam_select launch");
     h->stats.calls++;

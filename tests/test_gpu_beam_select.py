@@ -263,6 +263,20 @@ def test_softcap_reads_as_the_capped_logits(bs, dtype):
     _check(bs, _normal(6, 4096, 3, dtype, scale=200.0), _scores(2, 3, 4), 7, softcap=5.0)  # most of the row at the cap
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [4097, 65536])
+@pytest.mark.parametrize("garbage", [None, float("nan"), float("-inf")])
+def test_softcap_behind_masks(bs, dtype, V, garbage):
+    """A masked token is no candidate whatever the cap would make of it; an allowed -infinity is one at the cap's lower end."""
+    rng = np.random.default_rng(V)
+    allowed = rng.random((8, V)) < np.array([[0.001], [0.01], [0.05], [0.1], [0.2], [0.5], [1.0], [0.0]])
+    x = _normal(8, V, 3, dtype, scale=12.0)
+    x[2, 5] = x[5, 7] = float("-inf")
+    allowed[2, 5] = allowed[5, 7] = True
+    _check(bs, x, _scores(2, 4, 4), 9, allowed=allowed, garbage=garbage, softcap=20.0)
+    _check(bs, x, _scores(4, 2, 4), 9, allowed=allowed, uses=[1, 1, 0, 1, 0, 1, 1, 0], softcap=20.0)
+
+
 def test_equal_beams_go_to_the_lower_one(bs):
     """Beams that are alike in every bit: their candidates tie exactly."""
     for V, stride in ((5003, 5003), (8192, 8192), (20011, 20012)):
