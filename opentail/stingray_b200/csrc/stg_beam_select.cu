@@ -116,7 +116,7 @@ struct BeamTile {
         }
     }
 
-    // Which elements of the thread's share of the group at `base` are allowed, bit u * E + e
+    // Which elements of the thread's share of the group at `base` are allowed, bit u * E + e.  Behind `end` a mask's bits say nothing.
     static __device__ __forceinline__ uint32_t allowed(const uint32_t *mrow, int base, int end)
     {
         if (mrow == nullptr) return 0xFFFFFFFFu;
@@ -163,7 +163,8 @@ struct BeamTile {
             }
         }
     }
-    // The `kFew` allowed elements at most that a thread has where a mask leaves little, each by a load of its own, as numbers
+    // The `kFew` allowed elements at most that a thread has where a mask leaves little, each by a load of its own, as numbers; of
+    // a group that does not reach beyond the row
     static constexpr int kFew = 8, kWords = kPacked ? E / 2 : E;
     __device__ __forceinline__ void load_few(const LogitRow row, uint32_t ok, int base)
     {
@@ -308,9 +309,11 @@ static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, 
     // no thread more than eight elements of its 32 bf16 ones - densities up to about a tenth - these alone are read and added up
     // (256 rows of 262,144, densities of 0.1, 5 and 20 %: 35, 45 and 50 us, all in the long way 46, 47 and 47).  Of the 16 fp32
     // ones that a thread has it is no gain (57, 62 and 64 against 53, 57 and 58).
-    const auto is_sparse = [&](uint32_t bits) { return MASK && BF16 && mrow != nullptr && __reduce_max_sync(0xFFFFFFFFu, (unsigned)__popc(bits)) <= (unsigned)T::kFew; };
+    const auto is_sparse = [&](uint32_t bits, int at) {
+        return MASK && BF16 && mrow != nullptr && at + T::kGroup <= end && __reduce_max_sync(0xFFFFFFFFu, (unsigned)__popc(bits)) <= (unsigned)T::kFew;
+    };
     uint32_t ok = T::allowed(mrow, begin, end), next_ok = T::allowed(mrow, begin + T::kLen, end);
-    bool sparse = is_sparse(ok);
+    bool sparse = is_sparse(ok, begin);
     T next;
     if (begin < end) {
         if (sparse) next.load_few(lr, ok, begin);
@@ -323,7 +326,7 @@ static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, 
         if (few) t.cap_few(ok, lr.cap); else t.mask(ok);
         ok = next_ok;
         if (base + T::kLen < end) {
-            sparse = is_sparse(ok);
+            sparse = is_sparse(ok, base + T::kLen);
             if (sparse) next.load_few(lr, ok, base + T::kLen);
             else next.load(lr, mrow != nullptr, ok, base + T::kLen, end);
             next_ok = T::allowed(mrow, base + 2 * T::kLen, end);

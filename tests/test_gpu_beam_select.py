@@ -234,6 +234,32 @@ def test_masks(bs, V, dtype, garbage):
     _check(bs, _normal(8, V, 3, dtype), _scores(4, 2, 4), 9, allowed=allowed, uses=[1, 0, 1, 1, 0, 1, 1, 0])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V,stride", [(4097, 4104), (20011, 20016), (8185, 8192), (33, 40), (4097, 4097)])
+def test_bits_behind_the_vocabulary_say_nothing(bs, dtype, V, stride):
+    """Masks whose last word is all ones behind the last token, as compositions come out; what lies there in a row's stride is the
+    largest logit of all."""
+    import torch
+
+    rng = np.random.default_rng(V)
+    for dens in (0.002, 0.5):
+        allowed = rng.random((6, V)) < dens
+        allowed[:, V - 1] = [True, False, True, False, True, False]
+        words = _words(allowed).view(np.uint32)
+        words[:, -1] |= np.uint32(0xFFFFFFFF ^ ((1 << (V % 32)) - 1))
+        x = _normal(6, V, 8, dtype)
+        buf = torch.full((6, stride), 50.0, dtype=x.dtype, device="cuda")
+        buf[:, :V] = x.cuda()
+        s = _scores(2, 3, 8)
+        got = bs.beam_select(buf[:, :V], torch.from_numpy(s).cuda(), 9, mask=torch.from_numpy(words.view(np.int32)).cuda(), want_norms=True)
+        want, norms = beam_oracle.select(np.where(allowed, x.float().numpy(), -np.inf), s, 9)
+        for b in range(2):
+            n = len(want[b])
+            assert [(int(p), int(t)) for p, t in zip(got["parents"][b][:n], got["tokens"][b][:n])] == [(k, v) for _, k, v, _ in want[b]]
+        on = np.isfinite(norms)
+        assert np.allclose(got["log_norms"].cpu().numpy()[on], norms[on], rtol=2.0 ** -24, atol=LSE)
+
+
 def test_mask_compose_feeds_the_selection():
     import torch
 
