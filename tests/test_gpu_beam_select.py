@@ -158,6 +158,24 @@ def test_logits_of_any_size(bs, dtype):
     _check(bs, x[:, :39990], _scores(16, 1, 5), 20, stride=40001)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("K,V,n", [(8, 39168, 24), (8, 39168, 38), (8, 39168, 40), (8, 20011, 20), (8, 20011, 41), (4, 65536, 63), (4, 65536, 65),
+                                   (3, 131072, 128), (2, 8192, 7), (2, 8192, 9)])
+def test_one_beam_far_ahead(bs, K, V, n, dtype):
+    """All candidates come from one beam, which has about as many groups as there are candidates, or fewer: bounds out of
+    the other beams' groups keep nothing away."""
+    for masked in (False, True):
+        scores = _scores(3, K, n) - 60.0
+        scores[0, 0] += 60.0
+        scores[1, K - 1] += 60.0
+        scores[2] += 60.0
+        scores[2, 1:] = -np.inf
+        allowed = np.random.default_rng(n).random((3 * K, V)) < 0.3 if masked else None
+        _check(bs, _normal(3 * K, V, n, dtype), scores, n, allowed=allowed, uses=np.arange(3 * K) % 3 != 1 if masked else None)
+    for cap in (2.0, 30.0):
+        _check(bs, _normal(3 * K, V, n, dtype) - (0.0 if cap > 2.0 else 20.0), scores, n, softcap=cap)
+
+
 @pytest.mark.parametrize("V", [4096, 20011, 100000])
 def test_rows_that_ascend_and_descend(bs, V):
     import torch
