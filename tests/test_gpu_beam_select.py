@@ -252,6 +252,23 @@ def test_masks(bs, V, dtype, garbage):
     _check(bs, _normal(8, V, 3, dtype), _scores(4, 2, 4), 9, allowed=allowed, uses=[1, 0, 1, 1, 0, 1, 1, 0])
 
 
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("V,stride,shift", [(20010, 20010, 0), (20011, 20014, 0), (20010, 20014, 1), (20011, 20011, 1), (4098, 4098, 2), (1023, 1026, 0)])
+def test_masked_rows_of_pairs(bs, V, stride, shift, softcap):
+    """bf16 rows that begin at 4 bytes but not at 16 are read two tokens at a time, allowed or not."""
+    rng = np.random.default_rng(V + shift)
+    for density in (0.001, 0.05, 0.4, 1.0):
+        allowed = rng.random((12, V)) < density
+        allowed[:, -1] = True
+        x = _normal(12, V, V, "bf16")
+        _check(bs, x, _scores(3, 4, V), 8, allowed=allowed, uses=np.arange(12) % 4 != 1, softcap=softcap, stride=stride, shift=shift)
+        same = x[:1].expand(12, V).contiguous()  # rows that begin elsewhere, but are alike: equal sums, so the lower beam goes first
+        got = _check(bs, same, np.zeros((3, 4)), 8, softcap=softcap, stride=stride, shift=shift)
+        assert (got["log_norms"] == got["log_norms"][0, 0]).all()
+        best = int((x[0] == x[0].max()).sum())  # tokens that tie for a beam's first place; a cap of 30 leaves those behind them behind
+        assert (got["parents"] == np.repeat(np.arange(4), best)[:8]).all() if best > 1 else (got["parents"][:, :4] == np.arange(4)).all()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("V,stride", [(4097, 4104), (20011, 20016), (8185, 8192), (33, 40), (4097, 4097)])
 def test_bits_behind_the_vocabulary_say_nothing(bs, dtype, V, stride):
