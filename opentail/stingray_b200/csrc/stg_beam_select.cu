@@ -151,8 +151,11 @@ struct BeamTile {
                 }
             } else {
 #pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (base + at(u, e) < end && mask_bit(mrow, base + at(u, e))) ok |= 1u << (u * E + e);
+                for (int e = 0; e < E; e++) {  // a word for all lanes, of which each has one bit
+                    const int j = base + at(u, e);
+                    const uint32_t b = j < end ? __ldg(mrow + (j >> 5)) >> (j & 31) : 0u;
+                    ok |= (b & 1u) << (u * E + e);
+                }
             }
         }
         return ok;
@@ -194,13 +197,14 @@ struct BeamTile {
             }
         }
     }
-    // The `kFew` allowed elements at most that a thread has where a mask leaves little, each by a load of its own, as numbers; of
+    // The allowed elements where a mask leaves a thread no more than `some`, kLeast or kFew, each by a load of its own, as numbers; of
     // a group that does not reach beyond the row
-    static constexpr int kFew = 8, kWords = kPacked ? E / 2 : E;
-    __device__ __forceinline__ void load_few(const LogitRow row, uint32_t ok, int base)
+    static constexpr int kFew = 8, kLeast = 4, kWords = kPacked ? E / 2 : E;
+    __device__ __forceinline__ void load_few(const LogitRow row, uint32_t ok, int some, int base)
     {
 #pragma unroll
         for (int q = 0; q < kFew; q++) {
+            if (q == kLeast && some == kLeast) break;
             const int b = __ffs(ok) - 1;
             ok &= ok - 1u;
             uint32_t x = 0xFF800000u;
@@ -223,7 +227,7 @@ struct BeamTile {
     // ... once the loads are back
     __device__ __forceinline__ void mask(uint32_t ok)
     {
-        if (ok == 0xFFFFFFFFu) return;
+        if (ok == 0xFFFFFFFFu || (!VEC && !BF16)) return;  // fp32 elements that are read one by one are read if allowed
 #pragma unroll
         for (int u = 0; u < U; u++)
             if constexpr (kPacked) {
@@ -337,35 +341,41 @@ static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, 
     float limit = -CUDART_INF_F, best = -CUDART_INF_F;
     double s = 0.0;
     // A group's loads are in flight while the one ahead of it is added up, its mask's a group earlier still.  Behind a mask that leaves
-    // no thread more than eight elements of its 32 bf16 ones - densities up to about a tenth - these alone are read and added up
-    // (256 rows of 262,144, densities of 0.1, 5 and 20 %: 35, 45 and 50 us, all in the long way 46, 47 and 47).  Of the 16 fp32
-    // ones that a thread has it is no gain (57, 62 and 64 against 53, 57 and 58).
-    const auto is_sparse = [&](uint32_t bits, int at) {
-        return MASK && BF16 && mrow != nullptr && at + T::kGroup <= end && __reduce_max_sync(0xFFFFFFFFu, (unsigned)__popc(bits)) <= (unsigned)T::kFew;
+    // no thread more than four or eight elements of its 32 bf16 ones - densities up to about a tenth - these alone are read and added up
+    // (256 rows of 262,144, densities of 0.1, 1, 5, 10 and 20 %: 29, 32, 41, 45 and 50 us, all in the long way 46, 46, 47, 47 and 47).
+    // Of the 16 fp32 ones that a thread has it is no gain: 41, 49, 57, 62 and 64 against 53, 56, 58, 59 and 59.
+    constexpr int kDense = 32;
+    const auto most = [&](uint32_t bits, int at) {
+        if (!MASK || !BF16 || mrow == nullptr || at + T::kGroup > end) return kDense;
+        const int m = (int)__reduce_max_sync(0xFFFFFFFFu, (unsigned)__popc(bits));
+        return m > T::kFew ? kDense : m > T::kLeast ? T::kFew : T::kLeast;
     };
     uint32_t ok = T::allowed(mrow, begin, end), next_ok = T::allowed(mrow, begin + T::kLen, end);
-    bool sparse = is_sparse(ok, begin);
+    int some = most(ok, begin);
     T next;
     if (begin < end) {
-        if (sparse) next.load_few(lr, ok, begin);
+        if (some < kDense) next.load_few(lr, ok, some, begin);
         else next.load(lr, mrow != nullptr, ok, begin, end);
     }
 #pragma unroll 1
     for (int base = begin; base < end; base += T::kLen) {
         T t = next;
-        const bool few = sparse;
-        if (few) t.cap_few(ok, lr.cap); else t.mask(ok);
+        const int few = some;
+        if (few < kDense) t.cap_few(ok, lr.cap); else t.mask(ok);
         ok = next_ok;
         if (base + T::kLen < end) {
-            sparse = is_sparse(ok, base + T::kLen);
-            if (sparse) next.load_few(lr, ok, base + T::kLen);
+            some = most(ok, base + T::kLen);
+            if (some < kDense) next.load_few(lr, ok, some, base + T::kLen);
             else next.load(lr, mrow != nullptr, ok, base + T::kLen, end);
             next_ok = T::allowed(mrow, base + 2 * T::kLen, end);
         }
         float top = -CUDART_INF_F;
-        if (few) {
+        if (few < kDense) {
 #pragma unroll
-            for (int q = 0; q < T::kFew; q++) top = fmaxf(top, t.few(q));
+            for (int q = 0; q < T::kFew; q += 2) {
+                if (q == T::kLeast && few == T::kLeast) break;
+                top = fmaxf(top, fmaxf(t.few(q), t.few(q + 1)));
+            }
         } else {
             top = t.top();
         }
@@ -390,9 +400,12 @@ static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, 
         }
         f32x2 part = pair(0.f, 0.f);
         const f32x2 minus_c = pair(-ref.c, -ref.c);
-        if (few) {
+        if (few < kDense) {
 #pragma unroll
-            for (int q = 0; q < T::kFew; q += 2) part = add2(part, exp_pair(pair(t.few(q), t.few(q + 1)), minus_c));
+            for (int q = 0; q < T::kFew; q += 2) {
+                if (q == T::kLeast && few == T::kLeast) break;
+                part = add2(part, exp_pair(pair(t.few(q), t.few(q + 1)), minus_c));
+            }
         } else {
 #pragma unroll
             for (int u = 0; u < T::U; u++)
