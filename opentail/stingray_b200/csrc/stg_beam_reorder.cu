@@ -106,13 +106,16 @@ static __device__ __noinline__ void move_part(char *at, int bytes, int vec, cons
     }
 }
 
-// A tile is kMoveThreads columns of one sequence, one to a thread: occupancy is worth more than several columns' loads in flight
+// A tile is kMoveThreads columns of one sequence, one to a thread (two of two beams): occupancy is worth more than several columns' loads in flight
 // (four beams, eight layers' caches of 1000 positions: 35.5 us with eight CTAs an SM, 40.9 with five, 43.2 with four columns
 // a thread and three CTAs; 32 sequences of eight beams, 3.2 GB moved: 511 us with five CTAs, 568 with four).  More than 16
-// beams move 8 bytes a thread: 199 us against 263 with 16 and one CTA an SM.  Where runs are shorter than four
-// tiles a tile's columns go on from run to run, at a division each.
+// beams move 8 bytes a thread: 199 us against 263 with 16 and one CTA an SM.  Two beams move one row or swap: two columns fit
+// where four beams have one, and half the CTAs (63 sequences' caches of 1445 positions, 0.2 GB: 77.7 us, 91.8 with one column).
+// Where runs are shorter than four tiles a tile's columns go on from run to run, at a division each.
 constexpr int move_blocks(int moves) { return moves <= 4 ? 8 : moves <= 8 ? 5 : 3; }
 __host__ __device__ constexpr int move_bytes(int beams) { return beams <= 16 ? 16 : 8; }
+__host__ __device__ constexpr int move_cols(int beams) { return beams <= 2 ? 2 : 1; }  // of a thread
+__host__ __device__ constexpr int tile_cols(int beams) { return move_cols(beams) * kMoveThreads; }
 
 template <int MOVES>
 __global__ void __launch_bounds__(kMoveThreads, move_blocks(MOVES)) k_beam_move(const __grid_constant__ MoveArgs a)
@@ -165,34 +168,58 @@ __global__ void __launch_bounds__(kMoveThreads, move_blocks(MOVES)) k_beam_move(
         if (a.positions && st.pos_dim >= 0 && st.pos_dim < 3 && (int64_t)(st.pos_dim == 0 ? i0 : st.pos_dim == 1 ? i1 : i2) >= pos) return nullptr;
         return row + i0 * st.stride[0] + i1 * st.stride[1] + i2 * st.stride[2];
     };
-    char *r;
-    unsigned c = tid;
-    if (st.run_tiles > 0) {
-        const unsigned outer = in_seq / (unsigned)st.run_tiles;
-        r = run(outer);
-        c += (in_seq - outer * (unsigned)st.run_tiles) * kMoveThreads;
-    } else {
-        const unsigned g = in_seq * kMoveThreads + tid, outer = g / (unsigned)st.cols;
-        r = run(outer);
-        c = g - outer * (unsigned)st.cols;
-    }
-    if (r == nullptr) return;
-    // Columns begin at multiples of `vec` in memory, which are the same for all rows: a run's first may begin ahead of it.
-    const int64_t begin = (int64_t)c * st.vec - (int64_t)((uintptr_t)r & (unsigned)(st.vec - 1)), end = begin + st.vec;
+    constexpr int kCols = move_cols(MOVES), kTile = tile_cols(MOVES);
     const int n = moves.n;
-    if (begin >= limit) return;
-    if (begin < 0 || end > limit) {
-        move_part<MOVES>(r + max(begin, (int64_t)0), (int)(min(end, limit) - max(begin, (int64_t)0)), st.vec, moves, n);
-        return;
-    }
-    switch (st.vec) {
-        case 16:
-            if constexpr (move_bytes(MOVES) == 16) move_column<MOVES, uint4>(r + begin, moves, n);
-            break;
-        case 8: move_column<MOVES, uint2>(r + begin, moves, n); break;
-        case 4: move_column<MOVES, uint32_t>(r + begin, moves, n); break;
-        case 2: move_column<MOVES, uint16_t>(r + begin, moves, n); break;
-        default: move_column<MOVES, uint8_t>(r + begin, moves, n); break;
+    // Columns begin at multiples of `vec` in memory, which are the same for all rows: a run's first may begin ahead of it.
+    auto column = [&](int q, int64_t &begin) -> char * {
+        char *r;
+        unsigned c = tid + q * kMoveThreads;
+        if (st.run_tiles > 0) {
+            const unsigned outer = in_seq / (unsigned)st.run_tiles;
+            r = run(outer);
+            c += (in_seq - outer * (unsigned)st.run_tiles) * kTile;
+        } else {
+            const unsigned g = in_seq * kTile + c, outer = g / (unsigned)st.cols;
+            r = run(outer);
+            c = g - outer * (unsigned)st.cols;
+        }
+        begin = (int64_t)c * st.vec - (int64_t)((uintptr_t)r & (unsigned)(st.vec - 1));
+        return r == nullptr || begin >= limit ? nullptr : r;
+    };
+    auto move = [&](char *r, int64_t begin) {
+        const int64_t end = begin + st.vec;
+        if (begin < 0 || end > limit) {
+            move_part<MOVES>(r + max(begin, (int64_t)0), (int)(min(end, limit) - max(begin, (int64_t)0)), st.vec, moves, n);
+            return;
+        }
+        switch (st.vec) {
+            case 16:
+                if constexpr (move_bytes(MOVES) == 16) move_column<MOVES, uint4>(r + begin, moves, n);
+                break;
+            case 8: move_column<MOVES, uint2>(r + begin, moves, n); break;
+            case 4: move_column<MOVES, uint32_t>(r + begin, moves, n); break;
+            case 2: move_column<MOVES, uint16_t>(r + begin, moves, n); break;
+            default: move_column<MOVES, uint8_t>(r + begin, moves, n); break;
+        }
+    };
+    if constexpr (kCols == 1) {
+        int64_t begin;
+        char *const r = column(0, begin);
+        if (r != nullptr) move(r, begin);
+    } else {
+        int64_t b0, b1;
+        char *const r0 = column(0, b0), *const r1 = column(1, b1);
+        const bool in0 = r0 != nullptr && b0 >= 0 && b0 + 16 <= limit, in1 = r1 != nullptr && b1 >= 0 && b1 + 16 <= limit;
+        if (st.vec == 16 && in0 && in1) {
+            uint4 v0[MOVES], v1[MOVES];
+            load_rows(v0, r0 + b0, moves, n);
+            load_rows(v1, r1 + b1, moves, n);
+            store_rows(v0, r0 + b0, moves, n);
+            store_rows(v1, r1 + b1, moves, n);
+        } else {
+            if (r0 != nullptr) move(r0, b0);
+            if (r1 != nullptr) move(r1, b1);
+        }
     }
 }
 
@@ -278,13 +305,14 @@ static int reorder(StgHandle h, const StgBeamReorder *r, cudaStream_t stream)
         for (int j = 0; j < 3; j++)
             if (m.size[j] > 1) where |= (uint64_t)m.stride[j];
         const int64_t cols = (m.inner + m.vec - 1) / m.vec + (where % (uint64_t)m.vec != 0 ? 1 : 0), runs = (int64_t)m.size[0] * m.size[1];
+        const int64_t tile = tile_cols(r->n_beams);
         const bool too_many = cols > INT32_MAX / 2 || runs > INT32_MAX / m.size[2];
         int64_t per_seq = INT64_MAX;
         if (!too_many) {
-            const bool joined = cols < 4 * kMoveThreads && cols * (runs * m.size[2]) < INT32_MAX - kMoveThreads;
+            const bool joined = cols < 4 * tile && cols * (runs * m.size[2]) < INT32_MAX - tile;
             m.cols = (int32_t)cols;
-            m.run_tiles = joined ? 0 : (int32_t)((cols + kMoveThreads - 1) / kMoveThreads);
-            per_seq = joined ? (cols * (runs * m.size[2]) + kMoveThreads - 1) / kMoveThreads : m.run_tiles * (runs * m.size[2]);
+            m.run_tiles = joined ? 0 : (int32_t)((cols + tile - 1) / tile);
+            per_seq = joined ? (cols * (runs * m.size[2]) + tile - 1) / tile : m.run_tiles * (runs * m.size[2]);
         }
         if (per_seq > INT32_MAX / r->n_seq) return fail(h, STG_ERR_UNSUPPORTED, "stg_beam_reorder: state " + std::to_string(i) + " is too large");
         m.seq_tiles = (int32_t)per_seq;
@@ -299,7 +327,7 @@ static int reorder(StgHandle h, const StgBeamReorder *r, cudaStream_t stream)
     auto launch = [&]() -> int {
         if (a.n_states == 0) return STG_OK;
         const unsigned grid = (unsigned)tiles;
-        const auto fn = r->n_beams <= 4 ? k_beam_move<4> : r->n_beams <= 8 ? k_beam_move<8> : r->n_beams <= 16 ? k_beam_move<16> : k_beam_move<32>;
+        const auto fn = r->n_beams <= 2 ? k_beam_move<2> : r->n_beams <= 4 ? k_beam_move<4> : r->n_beams <= 8 ? k_beam_move<8> : r->n_beams <= 16 ? k_beam_move<16> : k_beam_move<32>;
         CK(launch_behind(fn, dim3(grid), kMoveThreads, 0, stream, a));
         h->stats.kernel_launches++;
         a.n_states = 0;

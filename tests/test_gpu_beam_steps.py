@@ -295,6 +295,31 @@ def test_reorder_layouts(bs, B, K, kind):
                 assert torch.equal(now, old)
 
 
+@pytest.mark.parametrize("K", [1, 2, 3])
+@pytest.mark.parametrize("kind", ["random", "one", "reverse"])
+def test_reorder_of_runs_of_several_tiles(bs, K, kind):
+    """Two columns to a thread of two beams, one of three: whole tiles, tiles that end within a run, runs that end within a vector."""
+    import torch
+    from opentail.stingray_b200 import BeamStates
+
+    B = 5
+    rng = np.random.default_rng(K + 10)
+    parents = _parents(kind, B, K, rng)
+    R = B * K
+    for shape, strides, dtype, pos in [((R, 2, 700, 80), None, torch.bfloat16, 2), ((R, 3, 500, 33), None, torch.float32, 2),
+                                       ((R, 5, 16, 1001), None, torch.bfloat16, 3), ((R, 40000), (40003, 1), torch.bfloat16, 1),
+                                       ((R, 8192), None, torch.float32, 1), ((R, 2, 4100, 4), (32816, 16404, 4, 1), torch.float32, 2),
+                                       ((R, 50000), (50001, 1), torch.uint8, 1)]:
+        x = _random(shape, dtype, K)
+        t = x.cuda() if strides is None else torch.as_strided(torch.zeros(R * strides[0] + 1, dtype=dtype, device="cuda"), shape, strides, 1).copy_(x)
+        room = shape[pos]
+        for used in (None, np.full(B, room - 1), rng.integers(0, room + 2, B)):
+            given = None if used is None else torch.from_numpy(used.astype(np.int32)).cuda()
+            want = _moved(t.cpu(), parents, 0, pos, used)
+            bs.beam_reorder(BeamStates([t], K, position_dim=pos), torch.from_numpy(parents).cuda(), positions=given)
+            assert torch.equal(t.cpu(), want), (shape, strides, used)
+
+
 def test_reorder_many_states_of_all_sizes_at_once(bs):
     """More states than one launch takes; some empty, some shared out over many tiles."""
     import torch
