@@ -544,7 +544,10 @@ typedef struct StgBeamReorder {
  * outside the beams, stay as they are, and so do positions beyond those in use and rows behind the last sequence.  The
  * rows and runs of a state must not overlap one another (STG_ERR_INVALID_ARGUMENT where the strides say that they do);
  * two states must not share memory.  With STG_MEM_HISTORY_RING the histories of one sequence's beams must be of one
- * length, as they are when every beam appends a token a step. */
+ * length, as they are when every beam appends a token a step (STG_ERR_INVALID_ARGUMENT where the host's lengths say that they are
+ * not).  A captured call moves what the histories hold at its replay, up to max_history tokens; the host's lengths say nothing
+ * then, and a sequence whose beams differ in length keeps its histories as they are.  Appending is not for a captured stream, as the
+ * host counts along: append between replays. */
 STG_API int stg_beam_reorder(StgHandle handle, const StgBeamReorder *reorder, void *stream);
 
 /* The tokens of n_hyps hypotheses per sequence (<= STG_BEAM_MAX_CANDIDATES) out of a trail of n_steps steps.

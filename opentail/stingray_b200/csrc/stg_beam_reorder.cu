@@ -29,6 +29,7 @@ struct MoveState {
     int32_t run_tiles;    // tiles of a run; 0: a tile's columns go on from run to run
     int32_t seq_tiles;    // tiles of one sequence
     int32_t first_tile;   // of this state
+    const int32_t *used;  // [n_seq * beams]: positions in use of every row, for which a sequence moves if they are one number; null: MoveArgs::positions
 };
 
 struct MoveArgs {
@@ -131,9 +132,11 @@ __global__ void __launch_bounds__(kMoveThreads, move_blocks(MOVES)) k_beam_move(
     const unsigned tile = blockIdx.x - (unsigned)st.first_tile, seq = tile / (unsigned)st.seq_tiles, in_seq = tile - seq * (unsigned)st.seq_tiles;
     pdl_release();
     pdl_wait();
-    const int64_t pos = a.positions ? (int64_t)max(a.positions[seq], 0) : 0;
+    const int32_t *const used = st.used ? st.used + (int64_t)seq * K : a.positions ? a.positions + seq : nullptr;
+    const int64_t pos = used ? (int64_t)max(*used, 0) : 0;
     if (tid < 32) {
-        const int p = tid < K ? a.parents[(int64_t)seq * K + tid] : -1;
+        const bool alike = __all_sync(0xFFFFFFFFu, st.used == nullptr || tid >= K || used[tid] == *used);
+        const int p = tid < K && alike ? a.parents[(int64_t)seq * K + tid] : -1;
         const int parent = p >= 0 && p < K && p != tid ? p : -1;
         uint32_t followers = 0u;
         for (int k = 0; k < K; k++)
@@ -156,7 +159,7 @@ __global__ void __launch_bounds__(kMoveThreads, move_blocks(MOVES)) k_beam_move(
     __syncthreads();
     if (moves.n == 0) return;
     char *const row = st.data + (int64_t)(seq * (unsigned)K) * st.row_stride;
-    const int64_t limit = a.positions && st.pos_dim == 3 ? min(st.inner, pos * st.pos_bytes) : st.inner;
+    const int64_t limit = used && st.pos_dim == 3 ? min(st.inner, pos * st.pos_bytes) : st.inner;
     // the run `outer`, or null where it is not to be moved
     auto run = [&](unsigned outer) -> char * {
         unsigned i0 = outer, i1 = 0u, i2 = 0u;
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__(kMoveThreads, move_blocks(MOVES)) k_beam_move(
             i2 = i1 / (unsigned)st.size[1]; i1 -= i2 * (unsigned)st.size[1];
         }
         if (i2 >= (unsigned)st.size[2] || i1 >= (unsigned)st.size[1] || i0 >= (unsigned)st.size[0]) return nullptr;
-        if (a.positions && st.pos_dim >= 0 && st.pos_dim < 3 && (int64_t)(st.pos_dim == 0 ? i0 : st.pos_dim == 1 ? i1 : i2) >= pos) return nullptr;
+        if (used && st.pos_dim >= 0 && st.pos_dim < 3 && (int64_t)(st.pos_dim == 0 ? i0 : st.pos_dim == 1 ? i1 : i2) >= pos) return nullptr;
         return row + i0 * st.stride[0] + i1 * st.stride[1] + i2 * st.stride[2];
     };
     constexpr int kCols = move_cols(MOVES), kTile = tile_cols(MOVES);
@@ -273,10 +276,20 @@ static int reorder(StgHandle h, const StgBeamReorder *r, cudaStream_t stream)
         if (!s.data) return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_beam_reorder: state " + std::to_string(i) + " has no data");
         if (!nested(s, rows)) return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_beam_reorder: rows or runs of state " + std::to_string(i) + " overlap");
     }
+    if (rows == 0 || r->n_beams == 1) return STG_OK;
+    if (!r->parents || misaligned(r->parents, 4) || misaligned(r->positions, 4))
+        return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_beam_reorder: parents are missing, or an array is not aligned to its elements");
+    const OnDevice on(h->cfg.device);
+    CK(on.error);
+    // The tokens in use of a history are read where they are appended, on the device: a captured call finds those of its replay.  The
+    // host's lengths say how many there can be, and refuse beams that differ; a captured call makes room for all there ever are.
     std::vector<StgBeamState> ring;
-    if (rows > 0 && (r->mem_flags & STG_MEM_HISTORY_RING)) {
-        int longest = 0;
-        for (int64_t x = 0; x < rows; x++) {
+    if (r->mem_flags & STG_MEM_HISTORY_RING) {
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        CK(cudaStreamIsCapturing(stream, &cap));
+        const bool captured = cap != cudaStreamCaptureStatusNone;
+        int longest = captured ? h->cfg.max_history : 0;
+        for (int64_t x = 0; x < rows && !captured; x++) {
             const int64_t first = x - x % r->n_beams;
             if (h->ring_len[x] != h->ring_len[first] || h->ring_dropped[x] != h->ring_dropped[first])
                 return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_beam_reorder: the histories of a sequence's beams differ in length");
@@ -288,19 +301,17 @@ static int reorder(StgHandle h, const StgBeamReorder *r, cudaStream_t stream)
         s.row_stride = (int64_t)std::max(h->cfg.max_history, 1) * 4;
         s.inner_bytes = (int64_t)longest * 4;
         s.size[0] = s.size[1] = s.size[2] = 1;
-        s.position_dim = -1;
+        s.position_dim = 3;
+        s.position_bytes = 4;
         ring.push_back(s);
     }
-    if (rows == 0 || r->n_beams == 1) return STG_OK;
-    if (!r->parents || misaligned(r->parents, 4) || misaligned(r->positions, 4))
-        return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_beam_reorder: parents are missing, or an array is not aligned to its elements");
-    const OnDevice on(h->cfg.device);
-    CK(on.error);
     const int total = r->n_states + (int)ring.size();
     std::vector<MoveState> moves;  // all of it is checked before any of it is moved
     for (int i = 0; i < total; i++) {
         MoveState m;
-        if (!move_state(i < r->n_states ? r->states[i] : ring[0], r->n_beams, r->positions ? -1 : r->n_positions, m)) continue;
+        const bool own = i >= r->n_states;
+        if (!move_state(own ? ring[0] : r->states[i], r->n_beams, own || r->positions ? -1 : r->n_positions, m)) continue;
+        if (own) m.used = (const int32_t *)h->ring_len_dev.p;
         uint64_t where = (uint64_t)(uintptr_t)m.data;
         for (int j = 0; j < 3; j++)
             if (m.size[j] > 1) where |= (uint64_t)m.stride[j];

@@ -575,7 +575,8 @@ class BatchSampler:
 
     def beam_reorder(self, states, parents, *, positions=None, history: bool = False, stream=None):
         """Row k of every sequence becomes what its row ``parents[seq, k]`` was, in place, in every tensor of ``states`` (a
-        ``BeamStates``, or None) and, with ``history``, in the handle's own histories (``stg_beam_reorder``).
+        ``BeamStates``, or None) and, with ``history``, in the handle's own histories (``stg_beam_reorder``), as
+        long as they are when a captured call is replayed.
         ``positions``: how many positions are in use - a number, or a device int32 tensor ``[n_seq]`` -
         in tensors that name a position dimension; None: all."""
         import torch

@@ -402,6 +402,80 @@ def test_reorder_of_the_handles_histories(bs):
     bs.history_reset()
 
 
+def _sampled_with(bs, hist, V, seed):
+    """Greedy tokens of random rows whose penalties see the handle's histories, and the same with `hist` handed over."""
+    import torch
+    from opentail.stingray_b200 import SamplingParams
+
+    x = torch.from_numpy(np.random.default_rng(seed).normal(0, 1, (len(hist), V)).astype(np.float32)).cuda()
+    params = [SamplingParams(Temperature=0.0, PresencePenalty=3.0, FrequencyPenalty=0.5, RepeatLastN=0)] * len(hist)
+    got = bs.sample_rows(x, params, history_ring=True)["tokens"]
+    ids, off = np.array([t for h in hist for t in h], np.int32), np.concatenate([[0], np.cumsum([len(h) for h in hist])]).astype(np.int32)
+    return got, bs.sample_rows(x, params, history_ids=torch.from_numpy(ids).cuda(), history_offsets=off)["tokens"]
+
+
+def test_a_captured_reorder_moves_histories_of_the_replays_length(bs):
+    """Captured while the histories are empty, replayed while direct appends make them longer."""
+    import torch
+    from opentail.stingray_b200 import BeamSearch
+
+    B, K, V, T = 3, 4, 30, 25
+    R = B * K
+    g = torch.Generator().manual_seed(4)
+    search = BeamSearch(B, K, T, eos=[2])
+    x = torch.zeros((R, V), device="cuda")
+    best = bs.beam_select(x, search.scores, search.n_candidates)
+    bs.history_reset()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        bs.beam_select(x, search.scores, search.n_candidates, out=best)
+        bs.beam_advance(search, best)
+        bs.beam_reorder(None, search.parents, history=True)
+    bs.beam_start(search)
+    hist = [[] for _ in range(R)]
+    moved = 0
+    for t in range(T):
+        x.copy_(torch.randn((R, V), generator=g) * 2)
+        graph.replay()
+        parents, tokens = search.parents.tolist(), search.tokens.flatten().tolist()
+        hist = [hist[b * K + parents[b][k]] + [tokens[b * K + k]] for b in range(B) for k in range(K)]
+        moved += sum(p != k for row in parents for k, p in enumerate(row))
+        bs.history_append(search.tokens.flatten())
+        if t % 8 == 7 or t == T - 1:
+            got, want = _sampled_with(bs, hist, V, t)
+            assert torch.equal(got, want), t
+    assert moved > T
+    # a direct call behind the replays
+    parents = _parents("reverse", B, K, None)
+    bs.beam_reorder(None, torch.from_numpy(parents).cuda(), history=True)
+    got, want = _sampled_with(bs, [hist[b * K + parents[b, k]] for b in range(B) for k in range(K)], V, 77)
+    assert torch.equal(got, want)
+    bs.history_reset()
+
+
+def test_a_replayed_reorder_leaves_histories_of_different_lengths(bs):
+    """What a direct call refuses: the sequence whose beams differ stays as it is, the others move."""
+    import torch
+
+    rng = np.random.default_rng(8)
+    B, K, V = 3, 4, 300
+    parents = _parents("cycle", B, K, None)
+    dev = torch.from_numpy(parents).cuda()
+    bs.history_reset()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        bs.beam_reorder(None, dev, history=True)
+    hist = [rng.integers(0, V, n).tolist() for n in [7] * 4 + [7, 9, 7, 7] + [30] * 4]
+    for r, h in enumerate(hist):
+        bs.history_load(r, np.array(h, np.int32))
+    graph.replay()
+    want = [hist[b * K + (k if b == 1 else parents[b, k])] for b in range(B) for k in range(K)]
+    got, ref = _sampled_with(bs, want, V, 1)
+    assert torch.equal(got, ref)
+    bs.history_reset()
+
+
 def test_refusals(bs):
     import ctypes as C
 
