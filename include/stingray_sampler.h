@@ -431,10 +431,12 @@ STG_API int stg_history_length(StgHandle handle, int32_t slot);
  * Every array is device memory unless it says otherwise, int32, float and double arrays aligned to their
  * elements, and no output may overlap an input.  n_seq * n_beams <= max_rows.
  *
- * Streams and captured graphs: the calls are enqueued on `stream` and wait for nothing.  Only
- * stg_beam_select uses workspace of the handle; it is ordered behind the handle's other calls as they are.  A
- * call on a stream that is being captured gets workspace of its own, held until stg_destroy, so graphs
- * captured from one handle may be replayed beside one another and beside direct calls. */
+ * Streams and captured graphs: the calls are enqueued on `stream` and the host waits for nothing.  stg_beam_select uses
+ * workspace of the handle, and stg_beam_reorder with STG_MEM_HISTORY_RING its histories; these two are ordered behind the handle's
+ * other calls, and those behind them, as sampling calls are among themselves (stg_history_*: by the caller, as ever).  A
+ * selection on a stream that is being captured gets workspace of its own, held until stg_destroy, so graphs
+ * captured from one handle may be replayed beside one another and beside direct calls; replays that move histories are ordered
+ * by the caller with what else uses them. */
 #define STG_BEAM_MAX_BEAMS 32
 #define STG_BEAM_MAX_CANDIDATES 128 /* per sequence; also the hypotheses of stg_beam_backtrace */
 #define STG_BEAM_MAX_EOS 8

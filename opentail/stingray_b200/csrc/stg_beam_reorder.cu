@@ -284,6 +284,7 @@ static int reorder(StgHandle h, const StgBeamReorder *r, cudaStream_t stream)
     // The tokens in use of a history are read where they are appended, on the device: a captured call finds those of its replay.  The
     // host's lengths say how many there can be, and refuse beams that differ; a captured call makes room for all there ever are.
     std::vector<StgBeamState> ring;
+    bool ordered = false;  // the histories are the handle's: what it has enqueued on another stream may read them still
     if (r->mem_flags & STG_MEM_HISTORY_RING) {
         cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
         CK(cudaStreamIsCapturing(stream, &cap));
@@ -304,6 +305,7 @@ static int reorder(StgHandle h, const StgBeamReorder *r, cudaStream_t stream)
         s.position_dim = 3;
         s.position_bytes = 4;
         ring.push_back(s);
+        ordered = !captured;
     }
     const int total = r->n_states + (int)ring.size();
     std::vector<MoveState> moves;  // all of it is checked before any of it is moved
@@ -328,6 +330,10 @@ static int reorder(StgHandle h, const StgBeamReorder *r, cudaStream_t stream)
         if (per_seq > INT32_MAX / r->n_seq) return fail(h, STG_ERR_UNSUPPORTED, "stg_beam_reorder: state " + std::to_string(i) + " is too large");
         m.seq_tiles = (int32_t)per_seq;
         moves.push_back(m);
+    }
+    if (ordered) {
+        rc = order_behind_last(h, stream);
+        if (rc) return rc;
     }
     MoveArgs a;
     a.n_states = 0;

@@ -476,6 +476,50 @@ def test_a_replayed_reorder_leaves_histories_of_different_lengths(bs):
     bs.history_reset()
 
 
+def test_histories_that_move_on_another_stream(bs):
+    """The handle's calls are put one behind the other: a step on one stream samples before, or behind, a reordering on another."""
+    import torch
+    from opentail.stingray_b200 import SamplingParams
+
+    rng = np.random.default_rng(2)
+    B, K, V = 2, 4, 400
+    R = B * K
+    parents = _parents("reverse", B, K, None)
+    dev = torch.from_numpy(parents).cuda()
+    hist = [rng.integers(0, V, 30).astype(np.int32) for _ in range(R)]
+    after = [hist[b * K + parents[b, k]] for b in range(B) for k in range(K)]
+    x = torch.from_numpy(rng.normal(0, 1, (R, V)).astype(np.float32)).cuda()
+    params = [SamplingParams(Temperature=0.0, PresencePenalty=3.0, FrequencyPenalty=0.5, RepeatLastN=0)] * R
+
+    def sampled(h):
+        ids, off = np.concatenate(h), np.arange(R + 1, dtype=np.int32) * 30
+        return bs.sample_rows(x, params, history_ids=torch.from_numpy(ids).cuda(), history_offsets=off)["tokens"]
+
+    want = [sampled(hist), sampled(after)]
+    assert not torch.equal(*want)
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    for first_moves in (False, True):
+        for r in range(R):
+            bs.history_load(r, hist[r])
+        torch.cuda.synchronize()
+        out = torch.full((R,), -1, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        with torch.cuda.stream(one):
+            torch.cuda._sleep(40_000_000)  # some 20 ms
+            if first_moves:
+                bs.beam_reorder(None, dev, history=True)
+            else:
+                bs.sample_rows(x, params, history_ring=True, out={"tokens": out})
+        with torch.cuda.stream(two):
+            if first_moves:
+                bs.sample_rows(x, params, history_ring=True, out={"tokens": out})
+            else:
+                bs.beam_reorder(None, dev, history=True)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[1 if first_moves else 0])
+    bs.history_reset()
+
+
 def test_refusals(bs):
     import ctypes as C
 
