@@ -9,10 +9,12 @@
 // candidates lie in the n best groups, whatever ties.  The CTA that ends last with a sequence finds those groups and
 // reads them once more.  One launch, no barrier and no list in the pass.
 //
-// The terms of S are computed and added up in 32 bits over the 16 or 32 elements that a thread holds, in 64 beyond, and
-// every warp's largest is put right in 64: the others' roundings (1e-7 each, either way) leave 1e-8 of S (measured on rows of
-// 151,936, N(0, 2.5^2) and peaked: 1.0e-8 and 1.5e-8 in the mean square, 1.2e-7 at most), so two beams' candidates change
-// places only if they lie closer than that.
+// The terms of S are computed in 32 bits.  The 16 or 32 that a thread holds are added up in 32 bits, halves to one another, and
+// in 64 beyond.  Where one of them makes next to nothing of the others - a logit far above the rest, as of a model that is sure -
+// 64 bits add them up from the first on, and every warp's largest term is put right in 64.  What that leaves of S: 1.0e-8 in the mean
+// square on rows of N(0, 2.5^2), up to 4.8e-8 with one logit 8 to 21 above a rest of N(0, 0.5^2) to N(0, 6^2), 5.9e-8 at most
+// (256 rows each of 50,257, 151,936 and 262,144, both types); the exponential's own error, 2^-22 at most, where most of S is
+// equal logits (1.4e-7 at most over flat rows).  Two beams' candidates change places only if they lie closer than that.
 //
 // What bounds it: the pass by HBM, 95 % of the copy rate on 256 rows of 151,936 fp32 (155 MB in 25 us); the join by latency,
 // 7 us for four beams and 13 for sixteen, of which only the last sequences' shows.
@@ -282,9 +284,41 @@ static __device__ __forceinline__ float warp_max(float v)
     asm("redux.sync.max.f32 %0, %0, 0xFFFFFFFF;" : "+f"(v));
     return v;
 }
+static __device__ __forceinline__ float warp_min(float v)
+{
+    asm("redux.sync.min.f32 %0, %0, 0xFFFFFFFF;" : "+f"(v));
+    return v;
+}
+
+// The sum of term(FIRST) .. term(FIRST + N - 1), halves added to one another: a large term takes part in log2(N) additions, not N, and
+// terms that are small beside it have been added to one another by then
+template <int FIRST, int N, class Term>
+static __device__ __forceinline__ f32x2 halves(const Term &term)
+{
+    if constexpr (N == 1) return term(FIRST);
+    else return add2(halves<FIRST, N / 2>(term), halves<FIRST + N / 2, N / 2>(term));
+}
+template <int N, class Term>
+static __device__ __forceinline__ double sum64(const Term &term)
+{
+    double a = 0.0, b = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        float x, y;
+        unpair(term(i), x, y);
+        a += (double)x;
+        b += (double)y;
+    }
+    return a + b;
+}
 
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr float kHuge = 1e6f;  // logits beyond take the slow way: c could not tell them apart
+// How far a thread's largest logit lies below the warp's where small terms may be lost beside large ones: what is less than
+// 2^-24 = e^-16.6 of a sum is, what a sum's own rounding can hide starts earlier.  At 10 a single logit 12 above a rest of
+// N(0, 0.5^2) leaves 2.5e-8 of S; at 12 it would 7e-8.  Rows of N(0, 2.5^2) never come here; of those of N(0, 4^2) 9 in 100 groups do, of N(0, 6^2) 30:
+// 512 bf16 rows of 256,000 take 62.3, 65.2 and 69.5 us, without this 62 all three; 256 fp32 rows of 151,936 36 to 36.4 us.
+constexpr float kApart = 10.f;
 
 // What a sum's terms are relative to: 2^c, c a whole number; or exp(logit) where that is not 0, -infinity as long as there
 // are none.
@@ -315,13 +349,13 @@ static __device__ __forceinline__ BeamRef warp_ref(BeamRef r)
 // The sum of exp(x - top) over a group with logits beyond kHuge, element by element, eight loads in flight (64 rows of 151,936
 // logits of some 1e6: 17.5 us, 27.9 one load after the other).
 template <bool BF16, bool VEC, bool CAP>
-static __device__ __noinline__ float huge_group(const LogitRow lr, const uint32_t *mrow, int base, int end, float top)
+static __device__ __noinline__ double huge_group(const LogitRow lr, const uint32_t *mrow, int base, int end, float top)
 {
-    float part = 0.f;
+    double part = 0.0;
 #pragma unroll 8
     for (int j = 0; j < BeamTile<BF16, VEC, CAP>::kGroup / 32; j++) {
         const int i = base + 32 * j + (int)(threadIdx.x & 31);
-        if (i < end && (mrow == nullptr || mask_bit(mrow, i))) part += expf(load_one<BF16>(lr, i) - top);
+        if (i < end && (mrow == nullptr || mask_bit(mrow, i))) part += (double)expf(load_one<BF16>(lr, i) - top);
     }
     return part;
 }
@@ -372,17 +406,17 @@ static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, 
             else next.load(lr, mrow != nullptr, ok, base + T::kLen, end);
             next_ok = T::allowed(mrow, base + 2 * T::kLen, end);
         }
-        float top = -CUDART_INF_F;
+        float own = -CUDART_INF_F;
         if (few < kDense) {
 #pragma unroll
             for (int q = 0; q < T::kFew; q += 2) {
                 if (q == T::kLeast && few == T::kLeast) break;
-                top = fmaxf(top, fmaxf(t.few(q), t.few(q + 1)));
+                own = fmaxf(own, fmaxf(t.few(q), t.few(q + 1)));
             }
         } else {
-            top = t.top();
+            own = t.top();
         }
-        top = warp_max(top);
+        const float top = warp_max(own);
         if (lane == 0) tops[base / T::kGroup] = top;
         if ((fabsf(top) > kHuge || ref.logit > kHuge) && top > -CUDART_INF_F) {
             if ((double)top > ref.natural()) {
@@ -391,9 +425,12 @@ static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, 
                 ref = now;
                 limit = -CUDART_INF_F;  // no c any more
             }
-            s += (double)huge_group<BF16, VEC, CAP>(lr, mrow, base, end, top) * exp64((double)top - ref.natural());
+            s += huge_group<BF16, VEC, CAP>(lr, mrow, base, end, top) * exp64((double)top - ref.natural());
             continue;
         }
+        // Terms that are next to nothing beside another of the same thread are lost in a sum of 32 bits, one after the other.  Where that
+        // is in sight and counts - the warp's largest so far is here, and some thread's largest lies far below it - 64 bits add up.
+        const bool apart = top >= best && top - warp_min(own > -CUDART_INF_F ? own : CUDART_INF_F) > kApart;
         best = fmaxf(best, top);
         if (top > limit) {
             const BeamRef now{floorf(top * 1.44269502f), 0.f};
@@ -401,22 +438,19 @@ static __device__ __forceinline__ void beam_piece(const BeamSelect &a, int row, 
             ref = now;
             limit = (now.c + 4.f) * 0.693147181f;
         }
-        f32x2 part = pair(0.f, 0.f);
         const f32x2 minus_c = pair(-ref.c, -ref.c);
-        if (few < kDense) {
-#pragma unroll
-            for (int q = 0; q < T::kFew; q += 2) {
-                if (q == T::kLeast && few == T::kLeast) break;
-                part = add2(part, exp_pair(pair(t.few(q), t.few(q + 1)), minus_c));
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < T::U; u++)
-#pragma unroll
-                for (int e = 0; e < T::E; e += 2) part = add2(part, exp_pair(pair(t.get(u, e), t.get(u, e + 1)), minus_c));
+        const auto few_term = [&](int i) { return exp_pair(pair(t.few(2 * i), t.few(2 * i + 1)), minus_c); };
+        const auto term = [&](int i) {
+            const int u = i / (T::E / 2), e = i % (T::E / 2) * 2;
+            return exp_pair(pair(t.get(u, e), t.get(u, e + 1)), minus_c);
+        };
+        constexpr int kPairs = T::U * T::E / 2;
+        if (apart) {
+            s += few == kDense ? sum64<kPairs>(term) : few == T::kFew ? sum64<T::kFew / 2>(few_term) : sum64<T::kLeast / 2>(few_term);
+            continue;
         }
         float p0, p1;
-        unpair(part, p0, p1);
+        unpair(few == kDense ? halves<0, kPairs>(term) : few == T::kFew ? halves<0, T::kFew / 2>(few_term) : halves<0, T::kLeast / 2>(few_term), p0, p1);
         s += (double)(p0 + p1);
     }
     // The largest term was made with the c that there is now.  Where a row's sum is little more than its largest term, that one's

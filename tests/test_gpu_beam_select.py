@@ -451,6 +451,51 @@ def test_normalisers_are_closer_than_their_bound(bs):
         assert ((got["scores"].view(64).double() - (norm.float().double() - norm)).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_one_logit_far_above_a_flat_rest(bs, dtype):
+    """Rows like a model that is sure: the best logit is 0, the others lie around -17 to -20.  Beams score what the row's normaliser
+    is as a float, so the best candidate's score shows the normaliser's error.  The largest term has no error of its own, and the
+    rest - q of the sum - is off by no more than LSE of itself, as long as the large term takes nothing away from the small ones that
+    are added up beside it (which would be up to 16 * 2^-24 of the sum).  In 64 bits the logarithm, the score and what is
+    compared are off by less than 1e-14 of numbers below 32."""
+    import torch
+
+    for V, peak, scale in ((262144, 17.0, 0.5), (262144, 18.0, 1.0), (151936, 17.0, 1.0), (151936, 18.0, 0.5), (262144, 19.0, 1.5), (50257, 17.5, 1.0),
+                           (50257, 20.0, 2.5)):
+        x = _normal(64, V, 3, scale=scale) - peak
+        at = torch.randint(0, V, (64,), generator=torch.Generator().manual_seed(V))
+        x[torch.arange(64), at] = 0.0
+        x = x.to(torch.bfloat16).cuda() if dtype == "bf16" else x.cuda()
+        d = x.double()
+        norm = torch.logsumexp(d, 1)
+        q = 1.0 - torch.exp(-norm)
+        got = bs.beam_select(x, norm.float().view(64, 1), 1)
+        assert torch.equal(got["tokens"].view(64).cpu(), at.int())
+        off = (got["scores"].view(64).double() - (norm.float().double() - norm)).abs()
+        assert (off <= q * LSE + 1e-12 + 2.0 ** -24 * (norm.float().double() - norm).abs()).all(), (V, peak, scale, float((off / (q * LSE)).max()))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("peak", [16.75, 17.0, 17.375, 18.0])
+def test_large_logits_do_not_swallow_the_small_ones_beside_them(bs, dtype, peak):
+    """One logit of 0 in every thread's share of a group, n elements, the others at -peak, of which one alone is less than half a
+    step of the sum.  The terms of a share are added pair by pair, so a large one takes part in log2(n) additions, each rounded by
+    2^-24 of it; the others' own errors are of no account, as all of them together are less than 1e-6 of the sum.  (Added
+    one after the other, each would be lost: n / 2 * e^-peak of the sum.)"""
+    import torch
+
+    V, n = 131072, 32 if dtype == "bf16" else 16
+    x = torch.full((8, V // (32 * n), 32 * n), -peak)
+    x[:, :, :8 * n:n // 4] = 0.0  # a thread reads n / 4 neighbours at a time
+    x = x.view(8, V).to(torch.bfloat16 if dtype == "bf16" else torch.float32).cuda()
+    norm = torch.logsumexp(x.double(), 1)
+    got = bs.beam_select(x, norm.float().view(8, 1), 1)
+    exact = norm.float().double() - norm  # the best candidate's score
+    off = (got["scores"].view(8).double() - exact).abs()
+    assert (got["tokens"] == 0).all()
+    assert (off <= np.log2(n) * 2.0 ** -24 + 1e-9 + 2.0 ** -24 * exact.abs()).all(), float(off.max())
+
+
 def test_more_rows_than_a_grid_has_in_one_dimension():
     import torch
 
