@@ -397,7 +397,8 @@ try {
     int cluster = 1;
     while (cluster < 8 && cluster * segment < n_steps) cluster *= 2;
     const size_t smem = trace_smem(n_beams);
-    if (smem > 24 * 1024) CK(cudaFuncSetAttribute(k_beam_backtrace, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // the limit is every thread's and handle's: only ever raised (20 KB are static, so 24 are below what needs no raising)
+    if (smem > 24 * 1024) CK(ensure_dynamic_smem((const void *)k_beam_backtrace, smem));
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)cluster;
