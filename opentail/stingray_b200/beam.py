@@ -28,7 +28,8 @@ class BeamSearch:
     """The device arrays of a search over ``n_seq`` sequences of ``num_beams`` beams, with a trail of ``max_steps`` tokens.
 
     A hypothesis of L tokens competes with its score divided by ``L ** length_penalty``.  ``n_candidates`` is how
-    many candidates ``beam_select`` has to find so that ``num_beams`` go on whatever ends.  Call
+    many candidates ``beam_select`` has to find so that ``num_beams`` go on whatever ends; a search that needs more than
+    there may be (128: 32 beams and four end tokens, 16 and eight) is refused.  Call
     ``BatchSampler.beam_start`` before the first step, also for single sequences that a new request takes over."""
 
     def __init__(self, n_seq: int, num_beams: int, max_steps: int, *, eos: Sequence[int] = (), pad: int = 0, length_penalty: float = 1.0,
@@ -42,6 +43,10 @@ class BeamSearch:
             raise ValueError("n_seq must be >= 0 and max_steps >= 1")
         if len(eos) > N.BEAM_MAX_EOS:
             raise ValueError(f"at most {N.BEAM_MAX_EOS} end tokens")
+        self.n_candidates = num_beams * (1 + len(set(eos)))
+        if self.n_candidates > N.BEAM_MAX_CANDIDATES:
+            raise ValueError(f"{num_beams} beams and {len(set(eos))} end tokens need {self.n_candidates} candidates a sequence so that {num_beams} go on "
+                             f"whatever ends, more than {N.BEAM_MAX_CANDIDATES}")
         dev = torch.device("cuda" if device is None else device)
         if dev.type != "cuda":
             raise ValueError("a search lies on a CUDA device")
@@ -49,7 +54,6 @@ class BeamSearch:
             dev = torch.device("cuda", torch.cuda.current_device())
         self.n_seq, self.num_beams, self.max_steps = n_seq, num_beams, max_steps
         self.eos, self.pad, self.device_index = eos, pad, dev.index
-        self.n_candidates = min(num_beams * (1 + len(set(eos))), N.BEAM_MAX_CANDIDATES)
 
         def ints(*shape):
             return torch.zeros(shape, dtype=torch.int32, device=dev)

@@ -80,6 +80,27 @@ def test_descriptions_are_short():
         BeamStates._describe(torch.zeros(8, 4, 4, 4, 4, 4)[:, ::2, ::2, ::2, ::2, ::2], 0, None)
 
 
+@pytest.mark.parametrize("beams,eos", [(32, 4), (32, 8), (16, 8), (26, 4), (22, 5)])
+def test_searches_that_need_more_candidates_than_there_may_be_are_refused(beams, eos):
+    """With fewer than num_beams * (1 + end tokens) of them, fewer beams than num_beams may go on."""
+    from opentail.stingray_b200 import BeamSearch
+
+    with pytest.raises(ValueError, match="candidates a sequence"):
+        BeamSearch(1, beams, 4, eos=range(2, 2 + eos))
+
+
+@pytest.mark.parametrize("beams,eos", [(32, [5, 6, 7]), (25, [5, 6, 7, 8]), (32, [5] * 8), (14, list(range(8))), (32, [])])
+def test_searches_of_as_many_candidates_as_there_may_be_are_not(beams, eos):
+    import torch
+    from opentail.stingray_b200 import BeamSearch
+
+    if torch.cuda.is_available():
+        assert BeamSearch(1, beams, 4, eos=eos).n_candidates == beams * (1 + len(set(eos)))
+    else:  # refused for its device alone
+        with pytest.raises(ValueError, match="CUDA device"):
+            BeamSearch(1, beams, 4, eos=eos, device="cpu")
+
+
 def test_states_and_searches_want_a_cuda_device():
     import torch
     from opentail.stingray_b200 import BeamSearch, BeamStates
