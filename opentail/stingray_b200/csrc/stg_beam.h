@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include "../../../include/stingray_sampler.h"
+#include "stg_beam_pieces.h"
 #include "stg_handle.h"
 
 namespace stg {
@@ -20,8 +21,6 @@ struct BeamWs {
     uint32_t *tickets;  // [n_seq]: CTAs of a sequence that have ended; zero between calls
 };
 
-// Pieces that all rows of a call together may be cut into beyond one each.
-constexpr int kBeamExtraPieces = 8192;
 inline size_t beam_ws_bytes(StgHandle h)
 {
     return ((size_t)h->cfg.max_rows + kBeamExtraPieces) * sizeof(BeamPart) + (size_t)h->cfg.max_rows * ((size_t)h->cfg.max_vocab / 512 + 1) * 4 + 1024;

@@ -931,7 +931,7 @@ static_assert(STG_BEAM_MAX_BEAMS == 32 && STG_BEAM_MAX_CANDIDATES <= kBeamThread
 // A CTA per piece of a row; like all kernels of a search launched while the one ahead of it ends.  The CTA that arrives last at
 // its sequence's ticket joins the sequence's rows and leaves the ticket at zero, as it was found.
 template <bool BF16, bool VEC, bool CAP, bool MASK>
-__global__ void __launch_bounds__(kBeamThreads, BF16 && CAP ? 1 : 2) k_beam_select(const __grid_constant__ BeamSelect a)
+__global__ void __launch_bounds__(kBeamThreads, kBeamCtas) k_beam_select(const __grid_constant__ BeamSelect a)
 {
     __shared__ MergeShared sh;
     __shared__ bool last;
@@ -974,25 +974,6 @@ static int captured_workspace(StgHandle h, size_t bytes, void **out)
     return STG_OK;
 }
 
-// How many CTAs share a row.  Two fit an SM; of the cuts into whole tiles the one with the least time, waves of CTAs
-// times tiles of each and about two tiles' worth for the rest of a CTA.  (256 rows of 151,936 fp32: one piece 33.6 us, two
-// 34.7, ten 49.0; 64 rows of 262,144 bf16 behind masks: four pieces 20.3, three 24.4, eight 22.0; 4 rows of 151,936: nineteen
-// pieces 10.3, ten 10.8.)
-static void beam_pieces(int rows, int vocab, int tile, int sms, int &pieces, int &len)
-{
-    const int tiles = (vocab + tile - 1) / tile;
-    const int most = std::max(1, std::min(tiles, kBeamExtraPieces / rows + 1));
-    int64_t least = INT64_MAX;
-    int each = tiles;
-    for (int c = 1; c <= most; c++) {
-        const int per = (tiles + c - 1) / c, got = (tiles + per - 1) / per;
-        const int64_t cost = (((int64_t)rows * got + 2 * sms - 1) / (2 * sms)) * (per + 2);
-        if (cost < least) { least = cost; each = per; }
-    }
-    pieces = (tiles + each - 1) / each;
-    len = each * tile;
-}
-
 static int beam_select(StgHandle h, const StgBeamBatch *b, cudaStream_t stream)
 {
     if (!b || b->struct_size != (int32_t)sizeof(StgBeamBatch)) return fail(h, STG_ERR_INVALID_ARGUMENT, "bad StgBeamBatch");
@@ -1025,7 +1006,8 @@ static int beam_select(StgHandle h, const StgBeamBatch *b, cudaStream_t stream)
     a.n_seq = b->n_seq; a.beams = b->n_beams; a.vocab = b->vocab; a.n = b->n_candidates;
     a.tokens = b->tokens; a.parents = b->parents; a.out_scores = b->candidate_scores; a.log_norms = b->log_norms; a.flags = b->seq_flags;
     const int rows = b->n_seq * b->n_beams;
-    const int group = b->logits_dtype == STG_DTYPE_BF16 ? 1024 : 512, tile = group * kBeamWarps;
+    const bool bf16 = b->logits_dtype == STG_DTYPE_BF16, capped = b->logit_softcap != 0.f;
+    const int group = bf16 ? 1024 : 512, tile = group * kBeamWarps;
     a.groups = (b->vocab + group - 1) / group;
     beam_pieces(rows, b->vocab, tile, h->sm_count, a.pieces, a.piece_len);
 
@@ -1057,7 +1039,7 @@ static int beam_select(StgHandle h, const StgBeamBatch *b, cudaStream_t stream)
          {{k_beam_select<false, true, false, false>, k_beam_select<false, true, false, true>}, {k_beam_select<false, true, true, false>, k_beam_select<false, true, true, true>}}},
         {{{k_beam_select<true, false, false, false>, k_beam_select<true, false, false, true>}, {k_beam_select<true, false, true, false>, k_beam_select<true, false, true, true>}},
          {{k_beam_select<true, true, false, false>, k_beam_select<true, true, false, true>}, {k_beam_select<true, true, true, false>, k_beam_select<true, true, true, true>}}}};
-    const Kernel fn = kernels[b->logits_dtype == STG_DTYPE_BF16][vec][b->logit_softcap != 0.f][b->mask != nullptr];
+    const Kernel fn = kernels[bf16][vec][capped][b->mask != nullptr];
     const cudaError_t e = launch_behind(fn, dim3((unsigned)a.pieces * (unsigned)rows), kBeamThreads, 0, stream, a);
     if (e != cudaSuccess) return cuda_fail(h, e, "k_beam_select launch");
     h->stats.calls++;
