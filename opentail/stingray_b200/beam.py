@@ -87,6 +87,12 @@ class BeamStates:
             raise ValueError("one position_dim per tensor")
         if not self.tensors:
             raise ValueError("no tensors")
+        if num_beams < 1:
+            raise ValueError("num_beams must be >= 1")
+        for t, p in zip(self.tensors, dims):  # a dimension that is not there would be taken for another one below
+            for name, d in (("beam_dim", beam_dim), ("position_dim", p)):
+                if d is not None and not -t.dim() <= d < t.dim():
+                    raise ValueError(f"{name} {d} is no dimension of a tensor of shape {tuple(t.shape)}")
         self.rows, self.device_index = None, self.tensors[0].get_device()
         described = []
         for t, p in zip(self.tensors, dims):

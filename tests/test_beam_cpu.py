@@ -101,6 +101,26 @@ def test_searches_of_as_many_candidates_as_there_may_be_are_not(beams, eos):
             BeamSearch(1, beams, 4, eos=eos, device="cpu")
 
 
+def test_dimensions_that_are_not_there_are_refused():
+    import torch
+    from opentail.stingray_b200 import BeamStates
+
+    t = torch.zeros(8, 2, 5, 4)
+    for kw in ({"beam_dim": 4}, {"beam_dim": -5}, {"position_dim": 4}, {"position_dim": 6}, {"position_dim": -5}, {"position_dim": [7]}):
+        with pytest.raises(ValueError, match="no dimension"):
+            BeamStates([t], 4, **kw)
+    with pytest.raises(ValueError, match="no dimension"):
+        BeamStates([torch.zeros(())], 1)
+    with pytest.raises(ValueError, match="no dimension"):
+        BeamStates([t, torch.zeros(8, 3)], 4, position_dim=2)
+    for beams in (0, -4):
+        with pytest.raises(ValueError, match="num_beams"):
+            BeamStates([t], beams)
+    for kw in ({"beam_dim": -4, "position_dim": -2}, {"beam_dim": 0, "position_dim": 3}):
+        with pytest.raises(ValueError, match="CUDA device"):  # nothing else is wrong with these
+            BeamStates([t], 4, **kw)
+
+
 def test_states_and_searches_want_a_cuda_device():
     import torch
     from opentail.stingray_b200 import BeamSearch, BeamStates
