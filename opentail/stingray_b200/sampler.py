@@ -523,7 +523,7 @@ class BatchSampler:
         mstride = 0
         if mask is not None:
             if mask.dtype != torch.int32 or mask.dim() != 2 or mask.shape[0] != rows or mask.shape[1] < (vocab + 31) // 32 or \
-                    mask.get_device() != self.device or mask.stride(1) != 1:
+                    mask.get_device() != self.device or (mask.shape[1] > 1 and mask.stride(1) != 1):
                 raise ValueError(f"mask must be int32 [{rows}, {(vocab + 31) // 32}] on cuda:{self.device} with contiguous rows")
             mp, mstride = mask.data_ptr(), mask.stride(0) if rows > 1 else mask.shape[1]
             if row_uses_mask is not None:

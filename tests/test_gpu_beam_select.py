@@ -295,6 +295,18 @@ def test_bits_behind_the_vocabulary_say_nothing(bs, dtype, V, stride):
         assert np.allclose(got["log_norms"].cpu().numpy()[on], norms[on], rtol=2.0 ** -24, atol=LSE)
 
 
+def test_masks_of_one_word_by_any_stride(bs):
+    """A dimension of one element has no stride to speak of."""
+    import torch
+
+    x, s = _normal(6, 29, 3).cuda(), torch.from_numpy(_scores(2, 3, 3)).cuda()
+    words = torch.from_numpy(_words(np.random.default_rng(1).random((6, 29)) < 0.4)).cuda()
+    want = bs.beam_select(x, s, 5, mask=words)
+    for m in (words.t().contiguous().t(), torch.as_strided(words.flatten(), (6, 1), (1, 6)), torch.stack([words, words], 1)[:, 0]):
+        got = bs.beam_select(x, s, 5, mask=m)
+        assert all(torch.equal(got[k], want[k]) for k in want)
+
+
 def test_mask_compose_feeds_the_selection():
     import torch
 
