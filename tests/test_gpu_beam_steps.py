@@ -520,6 +520,42 @@ def test_histories_that_move_on_another_stream(bs):
     bs.history_reset()
 
 
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("B,K", [(4, 2), (3, 5), (2, 20)])
+def test_histories_move_whatever_positions_the_states_have_in_use(bs, B, K, captured):
+    """The positions are the states'; a history goes by its own length."""
+    import torch
+    from opentail.stingray_b200 import BeamStates
+
+    rng = np.random.default_rng(K)
+    R, V = B * K, 300
+    hist = [rng.integers(0, V, n).tolist() for n in np.repeat(rng.integers(1, 41, B), K)]
+    parents = _parents("random", B, K, rng)
+    dev = torch.from_numpy(parents).cuda()
+    x = _random((R, 3, 12, 5), torch.float32, K)
+    each = torch.from_numpy(rng.integers(0, 14, B).astype(np.int32)).cuda()
+    for positions in (None, 0, 3, each):
+        bs.history_reset()
+        t = x.cuda()
+        states = BeamStates([t], K, position_dim=2)
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                bs.beam_reorder(states, dev, positions=positions, history=True)
+        for r, h in enumerate(hist):
+            bs.history_load(r, np.array(h, np.int32))
+        if captured:
+            graph.replay()
+        else:
+            bs.beam_reorder(states, dev, positions=positions, history=True)
+        want = [hist[b * K + (p if 0 <= (p := parents[b, k]) < K else k)] for b in range(B) for k in range(K)]
+        got, ref = _sampled_with(bs, want, V, K)
+        assert torch.equal(got, ref), positions
+        used = None if positions is None else each.tolist() if positions is each else [positions] * B
+        assert torch.equal(t.cpu(), _moved(x, parents, 0, 2, used))
+    bs.history_reset()
+
+
 def test_refusals(bs):
     import ctypes as C
 
