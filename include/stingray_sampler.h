@@ -436,7 +436,8 @@ STG_API int stg_history_length(StgHandle handle, int32_t slot);
  * other calls, and those behind them, as sampling calls are among themselves (stg_history_*: by the caller, as ever).  A
  * selection on a stream that is being captured gets workspace of its own, held until stg_destroy, so graphs
  * captured from one handle may be replayed beside one another and beside direct calls; replays that move histories are ordered
- * by the caller with what else uses them. */
+ * by the caller with what else uses them.  Every handle has the selection's workspace from stg_create on: 16 bytes for each of
+ * max_rows + 8192 pieces of rows, and 4 for each 512 of max_vocab logits of each of max_rows rows. */
 #define STG_BEAM_MAX_BEAMS 32
 #define STG_BEAM_MAX_CANDIDATES 128 /* per sequence; also the hypotheses of stg_beam_backtrace */
 #define STG_BEAM_MAX_EOS 8

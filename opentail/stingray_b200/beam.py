@@ -6,6 +6,7 @@ hands both to the library.  The reference has no beam search.
     search = BeamSearch(n_seq, beams, max_steps=256, eos=[2])
     states = BeamStates(key_value_caches, beams, position_dim=2)      # tensors [n_seq * beams, heads, room, width]
     bs.beam_start(search)
+    best = None
     for step in range(256):
         logits = model(search.tokens, ...)                            # [n_seq * beams, vocab]
         best = bs.beam_select(logits, search.scores, search.n_candidates, out=best)
