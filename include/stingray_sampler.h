@@ -65,7 +65,8 @@ enum {
 /* ---- element types of a logits buffer --------------------------------------------------------- */
 enum {
     STG_DTYPE_F32 = 0,
-    STG_DTYPE_BF16 = 1 /* widened exactly to fp32 on load; the reference has fp32 logits only */
+    STG_DTYPE_BF16 = 1, /* widened exactly to fp32 on load; the reference has fp32 logits only */
+    STG_DTYPE_F16 = 2   /* hidden states and weights of a head (stg_head_*) only: no logits are fp16 */
 };
 
 /* ---- where a caller array lives (bit set = host memory) ------------------------------------- */
@@ -566,6 +567,87 @@ STG_API int stg_beam_backtrace(StgHandle handle, const int32_t *trail_tokens, co
                                const int32_t *hyp_steps, const int32_t *hyp_parents, const int32_t *hyp_tokens,
                                int32_t pad_token, int32_t *sequences, int64_t out_stride, int32_t *lengths,
                                void *stream);
+
+/* ---- the head ----------------------------------------------------------------------------------------
+ * What makes rows of logits: hidden states [rows, width] times a weight [vocab, width].  stg_head_loss and
+ * stg_head_loss_backward score tokens and train a head (the reference's perplexity command sums such losses,
+ * src/OpenTail.Stingray.Cli/PerplexityCommand.cs:170-183); stg_head_logits makes a decode step's logits, in the layout that
+ * the sampling calls take, from a weight that stg_head_pack has laid out.  Every array is device memory, aligned to its elements
+ * unless it says otherwise, and no output may overlap an input or another output.  Sizes are not bounded by the handle's capacities.
+ *
+ * Streams and captured graphs: the calls are enqueued on `stream`, the host waits for nothing and nothing of the handle is
+ * written: what a call needs beside its arrays is its workspace, which the caller owns and which calls that may run at the same
+ * time must not share.  Its contents mean nothing between calls. */
+
+/* Softmax cross entropy.  With z[v] = hidden . weight[v], or cap * tanh(z / cap) of it, in fp32: log_norms = log(sum(exp(z))),
+ * loss = log_norms - z[target].  A target below 0 says that the row has no loss: both are 0, its hidden state is not read and it
+ * adds nothing to any gradient.  So does a target of vocab or beyond, but both are NaN.  Where a bounded wait of a kernel gives up,
+ * all losses (all of grad_hidden) are NaN. */
+typedef struct StgHeadLoss {
+    int32_t struct_size;            /* = sizeof(StgHeadLoss) */
+    int32_t rows;
+    int32_t vocab;
+    int32_t width;                  /* a multiple of 8 */
+    int32_t dtype;                  /* of hidden, weight and their gradients: STG_DTYPE_BF16 or STG_DTYPE_F16 */
+    float logit_softcap;            /* as StgSampleBatch.logit_softcap */
+    const void *hidden;             /* [rows, hidden_stride] */
+    int64_t hidden_stride;          /* elements between rows (>= width) */
+    const void *weight;             /* [vocab, weight_stride], rows begin at 16 bytes */
+    int64_t weight_stride;          /* elements, a multiple of 8 */
+    const int32_t *targets;         /* [rows] */
+    float *loss;                    /* stg_head_loss: out [rows] */
+    float *log_norms;               /* stg_head_loss: out [rows]; stg_head_loss_backward: what it wrote */
+    const float *grad_loss;         /* backward: gradient of loss [rows]; of rows without a loss not read */
+    const float *grad_log_norms;    /* backward: gradient of log_norms [rows] or NULL (none) */
+    void *grad_hidden;              /* backward: out [rows, width] contiguous, 16-byte aligned, or NULL */
+    void *grad_weight;              /* backward: out [vocab, width] contiguous, 16-byte aligned, or NULL; not both */
+    void *workspace;                /* 256-byte aligned */
+    uint64_t workspace_bytes;       /* >= stg_head_loss_workspace */
+} StgHeadLoss;
+/* Bytes of workspace for a call of these sizes (rows, vocab, width; other fields are only checked for what they allow). */
+STG_API int stg_head_loss_workspace(StgHandle handle, const StgHeadLoss *loss, int32_t backward, uint64_t *out_bytes);
+STG_API int stg_head_loss(StgHandle handle, const StgHeadLoss *loss, void *stream);
+/* Gradients of sum(grad_loss * loss + grad_log_norms * log_norms).  The gradients of the logits are rounded to `dtype` once, scaled by
+ * a power of two of their largest factor so that fp16 holds them too; sums are fp32 and outputs rounded once.  Deterministic. */
+STG_API int stg_head_loss_backward(StgHandle handle, const StgHeadLoss *loss, void *stream);
+
+/* A weight in 4 bits: weight[v][k] = (code[v][k] - zero[v][k / group]) * scale[v][k / group], codes 0 .. 15, two columns to a byte,
+ * the even one in the lower half. */
+typedef struct StgHeadPack {
+    int32_t struct_size;            /* = sizeof(StgHeadPack) */
+    int32_t vocab;
+    int32_t width;                  /* a multiple of group */
+    int32_t group;                  /* 32, 64 or 128 columns */
+    int32_t scale_dtype;            /* of scales and zeros: STG_DTYPE_BF16 or STG_DTYPE_F16 */
+    const void *codes;              /* uint8 [vocab, codes_stride] */
+    int64_t codes_stride;           /* bytes between rows (>= width / 2) */
+    const void *scales;             /* [vocab, width / group] contiguous */
+    const void *zeros;              /* the same shape, any value; NULL: 8 everywhere */
+    void *packed;                   /* out, 256-byte aligned */
+    uint64_t packed_bytes;          /* >= stg_head_pack_bytes */
+} StgHeadPack;
+STG_API int stg_head_pack_bytes(StgHandle handle, int32_t vocab, int32_t width, int32_t group, int32_t has_zeros, uint64_t *out_bytes);
+STG_API int stg_head_pack(StgHandle handle, const StgHeadPack *pack, void *stream);
+
+/* logits[r][v] = hidden[r] . weight[v]: group sums and scales in fp32, rounded once.  Any number of rows. */
+typedef struct StgHeadLogits {
+    int32_t struct_size;            /* = sizeof(StgHeadLogits) */
+    int32_t rows;
+    int32_t vocab;                  /* vocab, width, group, scale_dtype and has_zeros as the weight was packed */
+    int32_t width;
+    int32_t group;
+    int32_t scale_dtype;
+    int32_t has_zeros;
+    int32_t hidden_dtype;           /* STG_DTYPE_BF16 or STG_DTYPE_F16 */
+    int32_t logits_dtype;           /* STG_DTYPE_F32 or STG_DTYPE_BF16 */
+    const void *packed;             /* what stg_head_pack wrote */
+    uint64_t packed_bytes;          /* stg_head_pack_bytes of these sizes */
+    const void *hidden;             /* [rows, hidden_stride] */
+    int64_t hidden_stride;          /* elements between rows (>= width) */
+    void *logits;                   /* out [rows, row_stride] */
+    int64_t row_stride;             /* elements between rows (>= vocab); what lies behind vocab is not written */
+} StgHeadLogits;
+STG_API int stg_head_logits(StgHandle handle, const StgHeadLogits *logits, void *stream);
 
 /* ---- vocabulary-sharded mode (no counterpart in the reference, which is single-device:
  *      src/OpenTail.Stingray.Cli/RunCommand.cs:100) ------------------------------------------------

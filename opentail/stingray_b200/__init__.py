@@ -5,6 +5,7 @@ Importing this package never falls back to a CPU implementation: every operation
 ``libstingray_sampler.so`` and raises if the library or a CUDA device is missing.
 """
 from .beam import BeamSearch, BeamStates  # noqa: F401
+from .head import PackedHead  # noqa: F401
 from .sampler import (  # noqa: F401
     BatchSampler,
     Random,

@@ -12,7 +12,7 @@ ERR_NAMES = {
     1: "STG_ERR_INVALID_ARGUMENT", 2: "STG_ERR_CUDA", 3: "STG_ERR_CAPACITY", 4: "STG_ERR_UNSUPPORTED",
     5: "STG_ERR_TIMEOUT", 6: "STG_ERR_NCCL", 7: "STG_ERR_NO_DEVICE",
 }
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 MEM_HOST_LOGITS, MEM_HOST_HISTORY, MEM_HOST_MASK, MEM_HOST_BIAS = 1, 2, 4, 8
 MEM_HOST_UNIFORMS, MEM_HOST_OUTPUTS, MEM_HOST_DRAFT = 16, 32, 64
 MEM_HISTORY_RING = 128
@@ -32,6 +32,7 @@ EXPORTS = [
     "stg_mask_cache_put", "stg_mask_cache_contains", "stg_mask_compose",
     "stg_history_reset", "stg_history_load", "stg_history_append", "stg_history_length",
     "stg_beam_select", "stg_beam_start", "stg_beam_advance", "stg_beam_reorder", "stg_beam_backtrace",
+    "stg_head_loss_workspace", "stg_head_loss", "stg_head_loss_backward", "stg_head_pack_bytes", "stg_head_pack", "stg_head_logits",
 ]
 
 
@@ -113,6 +114,33 @@ class StgBeamReorder(C.Structure):
     ]
 
 
+class StgHeadLoss(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32), ("rows", C.c_int32), ("vocab", C.c_int32), ("width", C.c_int32), ("dtype", C.c_int32),
+        ("logit_softcap", C.c_float), ("hidden", C.c_void_p), ("hidden_stride", C.c_int64), ("weight", C.c_void_p),
+        ("weight_stride", C.c_int64), ("targets", C.c_void_p), ("loss", C.c_void_p), ("log_norms", C.c_void_p),
+        ("grad_loss", C.c_void_p), ("grad_log_norms", C.c_void_p), ("grad_hidden", C.c_void_p), ("grad_weight", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class StgHeadPack(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32), ("vocab", C.c_int32), ("width", C.c_int32), ("group", C.c_int32), ("scale_dtype", C.c_int32),
+        ("codes", C.c_void_p), ("codes_stride", C.c_int64), ("scales", C.c_void_p), ("zeros", C.c_void_p), ("packed", C.c_void_p),
+        ("packed_bytes", C.c_uint64),
+    ]
+
+
+class StgHeadLogits(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32), ("rows", C.c_int32), ("vocab", C.c_int32), ("width", C.c_int32), ("group", C.c_int32),
+        ("scale_dtype", C.c_int32), ("has_zeros", C.c_int32), ("hidden_dtype", C.c_int32), ("logits_dtype", C.c_int32),
+        ("packed", C.c_void_p), ("packed_bytes", C.c_uint64), ("hidden", C.c_void_p), ("hidden_stride", C.c_int64),
+        ("logits", C.c_void_p), ("row_stride", C.c_int64),
+    ]
+
+
 class StgStats(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in (
         "calls", "rows_sampled", "rows_greedy", "rows_topk_path", "rows_full_path",
@@ -173,6 +201,12 @@ def load() -> C.CDLL:
     lib.stg_beam_advance.argtypes = [vp, C.POINTER(StgBeamSearch), i32, vp, vp, vp, i32, vp]
     lib.stg_beam_reorder.argtypes = [vp, C.POINTER(StgBeamReorder), vp]
     lib.stg_beam_backtrace.argtypes = [vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, i32, vp, i64, vp, vp]
+    lib.stg_head_loss_workspace.argtypes = [vp, C.POINTER(StgHeadLoss), i32, C.POINTER(C.c_uint64)]
+    lib.stg_head_loss.argtypes = [vp, C.POINTER(StgHeadLoss), vp]
+    lib.stg_head_loss_backward.argtypes = [vp, C.POINTER(StgHeadLoss), vp]
+    lib.stg_head_pack_bytes.argtypes = [vp, i32, i32, i32, i32, C.POINTER(C.c_uint64)]
+    lib.stg_head_pack.argtypes = [vp, C.POINTER(StgHeadPack), vp]
+    lib.stg_head_logits.argtypes = [vp, C.POINTER(StgHeadLogits), vp]
     for name in EXPORTS:
         fn = getattr(lib, name)
         if name != "stg_last_error":

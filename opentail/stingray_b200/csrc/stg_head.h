@@ -1,0 +1,40 @@
+// The head (stg_head_*.cu): what its kernels share.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../../include/stingray_sampler.h"
+#include "stg_handle.h"
+
+namespace stg {
+
+constexpr int kHeadTileM = 128;
+
+// What the preparation of a call finds out, in device memory.
+struct HeadInfo {
+    int32_t used;       // rows that have a loss
+    int32_t failed;     // != 0: a bounded wait gave up; the outputs are NaN then
+    float scale;        // power of two that the logits' gradients are multiplied with where they are rounded to 16 bits
+    float unscale;      // its inverse
+};
+
+// A row that has a loss, in the order of the rows; behind the last one up to a multiple of kHeadTileM rows of zeros.
+struct HeadRow {
+    int32_t row, target;
+    float norm2;        // log2(e) * its normaliser
+    float a, b;         // the gradient of logit v is a * softmax[v] - b * [v == target]
+};
+
+struct HeadWs {
+    HeadInfo *info;
+    HeadRow *rows;      // [padded rows]
+    int32_t *place;     // [rows]: its place among the used rows, -1: no loss, -2: its target lies outside the vocabulary
+    void *hidden;       // [padded rows, width]: hidden states of the used rows
+    float *hit;         // [padded rows]: the target's logit
+    float2 *parts;      // [padded rows, two per tile of the vocabulary]: largest logit and the sum of exp relative to it
+    void *grads;        // [padded rows, piece]: gradients of a piece's logits
+    float *sums;        // [padded rows, width]: gradients of the hidden states so far
+};
+
+}  // namespace stg

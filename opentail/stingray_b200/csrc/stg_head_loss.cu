@@ -1,0 +1,397 @@
+// stg_head_loss, stg_head_loss_backward: softmax cross entropy of hidden states and a head's weight, in pieces of the vocabulary.
+//
+// With z = cap(hidden weight^T), a row's normaliser is log(sum(exp(z))), its loss the normaliser minus z[target], and the gradient of
+// z[v] is (dl + dn) exp(z[v] - normaliser) - dl [v == target], for gradients dl of the loss and dn of the normaliser.  Rows without a
+// loss take no part: the others are gathered first, so that nothing is computed for them and what their hidden states
+// hold reaches nothing.  The forward product keeps a maximum and a sum per row and tile; the backward forms a piece's logits
+// again, rounds their gradients to the operands' 16 bits (they are probabilities times a factor: a relative error of half a step
+// each, and the products' sums are fp32) and multiplies them with weight and hidden states.
+#include <cuda_runtime.h>
+#include <math_constants.h>
+#include <stdint.h>
+#include <string.h>
+
+#include <new>
+
+#include "stg_beam.h"
+#include "stg_head.h"
+#include "stg_head_gemm.cuh"
+#include "stg_launch.h"
+
+namespace stg {
+
+// ---- which rows have a loss ----
+
+struct HeadPrep {
+    HeadWs ws;
+    int rows, vocab;
+    const int32_t *targets;
+    const float *norms, *grad_loss, *grad_norms;  // NULL in the forward pass (grad_norms: also where there are none)
+};
+
+constexpr int kPrepThreads = 1024;
+
+__global__ void __launch_bounds__(kPrepThreads) k_head_prep(const __grid_constant__ HeadPrep p)
+{
+    __shared__ int warp_sum[32];
+    __shared__ float warp_most[32];
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    pdl_release();
+    pdl_wait();
+    int before = 0;
+    float most = 0.f;
+    for (int base = 0; base < p.rows; base += kPrepThreads) {
+        const int r = base + tid;
+        const int t = r < p.rows ? p.targets[r] : -1;
+        const bool on = t >= 0 && t < p.vocab;
+        const unsigned ballot = __ballot_sync(0xFFFFFFFFu, on);
+        if (lane == 0) warp_sum[w] = __popc(ballot);
+        __syncthreads();
+        int ahead = 0, all = 0;
+        for (int i = 0; i < 32; i++) {
+            if (i < w) ahead += warp_sum[i];
+            all += warp_sum[i];
+        }
+        const int at = before + ahead + __popc(ballot & ((1u << lane) - 1u));
+        if (r < p.rows) p.ws.place[r] = on ? at : t < 0 ? -1 : -2;
+        if (on) {
+            HeadRow row = {r, t, 0.f, 0.f, 0.f};
+            if (p.norms) {
+                row.b = p.grad_loss[r];
+                row.a = row.b + (p.grad_norms ? p.grad_norms[r] : 0.f);
+                row.norm2 = p.norms[r] * kLog2e;
+                most = fmaxf(most, fmaxf(fabsf(row.a), fabsf(row.b)));
+            }
+            p.ws.rows[at] = row;
+        }
+        before += all;
+        __syncthreads();
+    }
+    for (int i = before + tid; i < (before + kHeadTileM - 1) / kHeadTileM * kHeadTileM; i += kPrepThreads) p.ws.rows[i] = HeadRow{-1, -1, 0.f, 0.f, 0.f};
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+    if (lane == 0) warp_most[w] = most;
+    __syncthreads();
+    if (tid == 0) {
+        for (int i = 1; i < 32; i++) most = fmaxf(most, warp_most[i]);
+        // the largest factor comes to lie in [2^13, 2^14): a gradient of a logit is at most the sum of two, and fits
+        // fp16, of whose range the small ones then use as much as there is
+        int e = 0;
+        if (most > 0.f && most < CUDART_INF_F) e = max(-110, min(110, 13 - ilogbf(most)));
+        p.ws.info->used = before;
+        p.ws.info->failed = 0;
+        p.ws.info->scale = exp2f((float)e);
+        p.ws.info->unscale = exp2f((float)-e);
+    }
+}
+
+// Hidden states of the rows that have a loss, next to each other, zeros behind them up to whole tiles.
+__global__ void __launch_bounds__(128) k_head_gather(const __grid_constant__ HeadWs ws, const uint16_t *hidden, int64_t stride, int width, bool vec)
+{
+    pdl_release();
+    pdl_wait();
+    const int c = blockIdx.x, used = ws.info->used;
+    if (c >= (used + kHeadTileM - 1) / kHeadTileM * kHeadTileM) return;
+    uint4 *to = (uint4 *)((uint16_t *)ws.hidden + (int64_t)c * width);
+    const uint16_t *from = c < used ? hidden + (int64_t)ws.rows[c].row * stride : nullptr;
+    for (int i = threadIdx.x; i < width / 8; i += 128) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (from && vec) {
+            v = __ldg((const uint4 *)from + i);
+        } else if (from) {
+            uint32_t e[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) e[j] = from[8 * i + j];
+            v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        }
+        to[i] = v;
+    }
+}
+
+// A row's maxima and sums joined: its normaliser and loss.
+__global__ void __launch_bounds__(128) k_head_join(const __grid_constant__ HeadWs ws, int pieces, float *loss, float *norms)
+{
+    __shared__ float tops[4];
+    __shared__ double sums[4];
+    pdl_release();
+    pdl_wait();
+    const int r = blockIdx.x, tid = threadIdx.x, at = ws.place[r];
+    if (at < 0 || ws.info->failed != 0) {
+        if (tid == 0) loss[r] = norms[r] = at == -1 && ws.info->failed == 0 ? 0.f : CUDART_NAN_F;
+        return;
+    }
+    const float2 *parts = ws.parts + (int64_t)at * pieces;
+    float top = -CUDART_INF_F;
+    bool bad = false;
+    for (int i = tid; i < pieces; i += 128) {
+        top = fmaxf(top, parts[i].x);
+        bad |= parts[i].y != parts[i].y;
+    }
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if ((tid & 31) == 0) tops[tid >> 5] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    double sum = bad ? (double)CUDART_NAN_F : 0.0;
+    for (int i = tid; i < pieces; i += 128) {
+        const float2 v = parts[i];
+        if (v.x > -CUDART_INF_F) sum += (double)(v.y * expf(v.x - top));
+    }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if ((tid & 31) == 0) sums[tid >> 5] = sum;
+    __syncthreads();
+    if (tid == 0) {
+        const double norm = (double)top + log(sums[0] + sums[1] + sums[2] + sums[3]);
+        norms[r] = (float)norm;
+        loss[r] = (float)(norm - (double)ws.hit[at]);
+    }
+}
+
+// Gradients of the hidden states: rounded, back in their rows; zeros where a row has no loss.
+template <bool BF16>
+__global__ void __launch_bounds__(128) k_head_spread(const __grid_constant__ HeadWs ws, int width, uint16_t *out)
+{
+    pdl_release();
+    pdl_wait();
+    const int r = blockIdx.x, at = ws.place[r];
+    const float unscale = ws.info->failed != 0 ? CUDART_NAN_F : ws.info->unscale;
+    const float *from = ws.sums + (int64_t)at * width;
+    for (int i = threadIdx.x; i < width / 8; i += 128) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (at >= 0) {
+            const float4 x = ((const float4 *)from)[2 * i], y = ((const float4 *)from)[2 * i + 1];
+            v = make_uint4(pack2<BF16>(x.x * unscale, x.y * unscale), pack2<BF16>(x.z * unscale, x.w * unscale), pack2<BF16>(y.x * unscale, y.y * unscale),
+                           pack2<BF16>(y.z * unscale, y.w * unscale));
+        }
+        ((uint4 *)(out + (int64_t)r * width))[i] = v;
+    }
+}
+
+// ---- host ----
+
+struct HeadPlan {
+    int rows_pad, tile_n, tiles_n, piece, pieces;
+    size_t bytes;
+};
+
+// Offsets of the workspace; `base` NULL: only its size.
+static HeadWs head_layout(const StgHeadLoss *b, bool backward, HeadPlan &p, char *base)
+{
+    HeadWs ws;
+    memset(&ws, 0, sizeof(ws));
+    size_t at = 0;
+    auto take = [&](size_t bytes) { char *x = base ? base + at : nullptr; at += round_up(bytes, 256); return x; };
+    const size_t R = (size_t)p.rows_pad;
+    ws.info = (HeadInfo *)take(sizeof(HeadInfo));
+    ws.rows = (HeadRow *)take(R * sizeof(HeadRow));
+    ws.place = (int32_t *)take(R * 4);
+    ws.hidden = take(R * (size_t)b->width * 2);
+    if (backward) {
+        ws.grads = take(R * (size_t)p.piece * 2);
+        ws.sums = (float *)take(R * (size_t)b->width * 4);
+    } else {
+        ws.hit = (float *)take(R * 4);
+        ws.parts = (float2 *)take(R * 2 * (size_t)p.tiles_n * sizeof(float2));
+    }
+    p.bytes = at;
+    return ws;
+}
+
+static HeadPlan head_plan(StgHandle h, const StgHeadLoss *b, bool backward)
+{
+    HeadPlan p;
+    memset(&p, 0, sizeof(p));
+    p.rows_pad = (b->rows + kHeadTileM - 1) / kHeadTileM * kHeadTileM;
+    p.tile_n = 256;
+    p.tiles_n = (b->vocab + 255) / 256;
+    const int64_t whole = (int64_t)p.tiles_n * 256;
+    // a piece of the gradients takes 256 MB at most, or 2048 columns
+    int64_t piece = std::max<int64_t>(2048, (int64_t)(1 << 27) / std::max(1, p.rows_pad) / 256 * 256);
+    piece = std::min<int64_t>(std::min<int64_t>(piece, 16384), whole);
+    p.pieces = (int)((whole + piece - 1) / piece);
+    p.piece = (int)((whole / 256 + p.pieces - 1) / p.pieces * 256);
+    p.pieces = (int)((whole + p.piece - 1) / p.piece);
+    head_layout(b, backward, p, nullptr);
+    return p;
+}
+
+static int head_check(StgHandle h, const StgHeadLoss *b, const char *who)
+{
+    const std::string at = std::string(who) + ": ";
+    if (!b || b->struct_size != (int32_t)sizeof(StgHeadLoss)) return fail(h, STG_ERR_INVALID_ARGUMENT, "bad StgHeadLoss");
+    if (b->rows < 0 || b->vocab <= 0 || b->width <= 0) return fail(h, STG_ERR_INVALID_ARGUMENT, at + "rows must be >= 0, vocab and width > 0");
+    if (b->rows > (1 << 20) || b->vocab > (1 << 26) || b->width > (1 << 16)) return fail(h, STG_ERR_CAPACITY, at + "more than 2^20 rows, 2^26 vocabulary entries or a width of 2^16");
+    if (b->dtype != STG_DTYPE_BF16 && b->dtype != STG_DTYPE_F16) return fail(h, STG_ERR_INVALID_ARGUMENT, at + "dtype must be STG_DTYPE_BF16 or STG_DTYPE_F16");
+    if (b->width % 8 != 0) return fail(h, STG_ERR_UNSUPPORTED, at + "width must be a multiple of 8");
+    if (b->hidden_stride < b->width || b->weight_stride < b->width) return fail(h, STG_ERR_INVALID_ARGUMENT, at + "a row stride smaller than width");
+    if (!(b->logit_softcap >= 0.f) || b->logit_softcap > 3.0e38f) return fail(h, STG_ERR_INVALID_ARGUMENT, at + "logit_softcap must be 0 (off) or a finite positive cap");
+    return STG_OK;
+}
+
+static int head_check_arrays(StgHandle h, const StgHeadLoss *b, const char *who, bool backward, const HeadPlan &p)
+{
+    const std::string at = std::string(who) + ": ";
+    if (!b->hidden || !b->weight || !b->targets || !b->log_norms || (!backward && !b->loss) || (backward && !b->grad_loss))
+        return fail(h, STG_ERR_INVALID_ARGUMENT, at + "hidden, weight, targets, log_norms and loss (backward: grad_loss) are required");
+    if (misaligned(b->hidden, 2) || misaligned(b->targets, 4) || misaligned(b->log_norms, 4) || misaligned(b->loss, 4) || misaligned(b->grad_loss, 4) ||
+        misaligned(b->grad_log_norms, 4) || misaligned(b->grad_hidden, 16) || misaligned(b->grad_weight, 16))
+        return fail(h, STG_ERR_INVALID_ARGUMENT, at + "an array is not aligned to its elements, or a gradient not to 16 bytes");
+    if (misaligned(b->weight, 16) || b->weight_stride % 8 != 0) return fail(h, STG_ERR_UNSUPPORTED, at + "the weight's rows must begin at 16 bytes");
+    if (!b->workspace || misaligned(b->workspace, 256) || b->workspace_bytes < p.bytes)
+        return fail(h, STG_ERR_CAPACITY, at + "workspace missing, not aligned to 256 bytes or smaller than stg_head_loss_workspace says");
+    return STG_OK;
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A map of 16-bit rows: boxes of 64 columns (128 bytes, swizzled) by `box_rows` rows, zeros outside.
+static int head_map(StgHandle h, CUtensorMap *map, bool bf16, const void *p, int64_t columns, int64_t rows, int64_t stride, int box_rows)
+{
+    static const EncodeTiled encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) fn = nullptr;
+        return (EncodeTiled)fn;
+    }();
+    if (!encode) return fail(h, STG_ERR_CUDA, "cuTensorMapEncodeTiled is not there");
+    const cuuint64_t size[2] = {(cuuint64_t)columns, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, step[2] = {1, 1};
+    const CUresult e = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void *)p, size, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return e == CUDA_SUCCESS ? STG_OK : fail(h, STG_ERR_CUDA, "cuTensorMapEncodeTiled failed with " + std::to_string((int)e));
+}
+
+template <int MODE>
+static cudaError_t head_gemm(StgHandle h, bool bf16, cudaStream_t stream, const CUtensorMap &a, const CUtensorMap &b, const HeadGemm &g, int64_t tiles)
+{
+    using Kernel = void (*)(CUtensorMap, CUtensorMap, HeadGemm);
+    static const Kernel kernels[2][2] = {{k_head_gemm<MODE, false, false>, k_head_gemm<MODE, false, (MODE < kHidden)>},
+                                         {k_head_gemm<MODE, true, false>, k_head_gemm<MODE, true, (MODE < kHidden)>}};
+    const Kernel fn = kernels[bf16][g.cap != 0.f];
+    const cudaError_t e = ensure_dynamic_smem((const void *)fn, kGemmSmem);
+    if (e != cudaSuccess) return e;
+    h->stats.kernel_launches++;
+    return launch_behind(fn, dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, h->sm_count))), kGemmThreads, kGemmSmem, stream, a, b, g);
+}
+
+static int head_begin(StgHandle h, const StgHeadLoss *b, const HeadWs &ws, const HeadPlan &p, bool backward, cudaStream_t stream)
+{
+    const HeadPrep prep = {ws, b->rows, b->vocab, b->targets, backward ? b->log_norms : nullptr, b->grad_loss, b->grad_log_norms};
+    CK(launch_behind(k_head_prep, dim3(1), kPrepThreads, 0, stream, prep));
+    const bool vec = !misaligned(b->hidden, 16) && (b->rows == 1 || b->hidden_stride % 8 == 0);
+    CK(launch_behind(k_head_gather, dim3((unsigned)p.rows_pad), 128, 0, stream, ws, (const uint16_t *)b->hidden, b->hidden_stride, b->width, vec));
+    h->stats.kernel_launches += 2;
+    return STG_OK;
+}
+
+static int head_forward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
+{
+    int rc = head_check(h, b, "stg_head_loss");
+    if (rc || b->rows == 0) return rc;
+    HeadPlan p = head_plan(h, b, false);
+    rc = head_check_arrays(h, b, "stg_head_loss", false, p);
+    if (rc) return rc;
+    const OnDevice on(h->cfg.device);
+    CK(on.error);
+    const HeadWs ws = head_layout(b, false, p, (char *)b->workspace);
+    const bool bf16 = b->dtype == STG_DTYPE_BF16;
+    CUtensorMap rows, weight;
+    if ((rc = head_map(h, &rows, bf16, ws.hidden, b->width, p.rows_pad, b->width, kHeadTileM))) return rc;
+    if ((rc = head_map(h, &weight, bf16, b->weight, b->width, b->vocab, b->weight_stride, p.tile_n))) return rc;
+    if ((rc = head_begin(h, b, ws, p, false, stream))) return rc;
+    HeadGemm g;
+    memset(&g, 0, sizeof(g));
+    g.info = ws.info; g.rows = ws.rows; g.n = b->vocab; g.k = b->width; g.tile_n = p.tile_n; g.cap = b->logit_softcap;
+    g.parts = ws.parts; g.hit = ws.hit; g.pieces = 2 * p.tiles_n;
+    CK(head_gemm<kStats>(h, bf16, stream, rows, weight, g, (int64_t)p.rows_pad / kHeadTileM * p.tiles_n));
+    CK(launch_behind(k_head_join, dim3((unsigned)b->rows), 128, 0, stream, ws, 2 * p.tiles_n, b->loss, b->log_norms));
+    h->stats.kernel_launches++;
+    h->stats.calls++;
+    return STG_OK;
+}
+
+static int head_backward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
+{
+    int rc = head_check(h, b, "stg_head_loss_backward");
+    if (rc) return rc;
+    if (!b->grad_hidden && !b->grad_weight) return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_head_loss_backward: neither grad_hidden nor grad_weight");
+    const OnDevice on(h->cfg.device);
+    CK(on.error);
+    const size_t weight_bytes = (size_t)b->vocab * b->width * 2;
+    if (b->rows == 0) {
+        if (b->grad_weight) CK(cudaMemsetAsync(b->grad_weight, 0, weight_bytes, stream));
+        return STG_OK;
+    }
+    HeadPlan p = head_plan(h, b, true);
+    rc = head_check_arrays(h, b, "stg_head_loss_backward", true, p);
+    if (rc) return rc;
+    const HeadWs ws = head_layout(b, true, p, (char *)b->workspace);
+    const bool bf16 = b->dtype == STG_DTYPE_BF16;
+    CUtensorMap rows_k, weight_k, grads_k, weight_mn, grads_mn, rows_mn;  // how the operands' boxes of 64 columns are cut
+    if ((rc = head_map(h, &rows_k, bf16, ws.hidden, b->width, p.rows_pad, b->width, kHeadTileM))) return rc;
+    if ((rc = head_map(h, &weight_k, bf16, b->weight, b->width, b->vocab, b->weight_stride, 256))) return rc;
+    if ((rc = head_map(h, &grads_k, bf16, ws.grads, p.piece, p.rows_pad, p.piece, kHeadTileM))) return rc;
+    if ((rc = head_map(h, &weight_mn, bf16, b->weight, b->width, b->vocab, b->weight_stride, kGemmK))) return rc;
+    if ((rc = head_map(h, &grads_mn, bf16, ws.grads, p.piece, p.rows_pad, p.piece, kGemmK))) return rc;
+    if ((rc = head_map(h, &rows_mn, bf16, ws.hidden, b->width, p.rows_pad, b->width, kGemmK))) return rc;
+    if ((rc = head_begin(h, b, ws, p, true, stream))) return rc;
+    const int64_t tiles_m = p.rows_pad / kHeadTileM, tiles_w = (b->width + 255) / 256;
+    for (int i = 0; i < p.pieces; i++) {
+        HeadGemm g;
+        memset(&g, 0, sizeof(g));
+        g.info = ws.info; g.rows = ws.rows; g.tile_n = 256; g.cap = b->logit_softcap;
+        g.first = i * p.piece;
+        const int count = std::min(p.piece, b->vocab - g.first);
+        g.n = count; g.k = b->width;
+        g.grads = ws.grads; g.grads_stride = p.piece;
+        CK(head_gemm<kGrad>(h, bf16, stream, rows_k, weight_k, g, tiles_m * ((count + 255) / 256)));
+        g.n = b->width;
+        if (b->grad_hidden) {
+            g.k = count;
+            g.sums = ws.sums; g.sums_stride = b->width;
+            CK(head_gemm<kHidden>(h, bf16, stream, grads_k, weight_mn, g, tiles_m * tiles_w));
+        }
+        if (b->grad_weight) {
+            g.m = count;
+            g.out = b->grad_weight; g.out_stride = b->width;
+            CK(head_gemm<kWeight>(h, bf16, stream, grads_mn, rows_mn, g, (int64_t)((count + kHeadTileM - 1) / kHeadTileM) * tiles_w));
+        }
+    }
+    if (b->grad_hidden) {
+        CK(launch_behind(bf16 ? k_head_spread<true> : k_head_spread<false>, dim3((unsigned)b->rows), 128, 0, stream, ws, b->width, (uint16_t *)b->grad_hidden));
+        h->stats.kernel_launches++;
+    }
+    h->stats.calls++;
+    return STG_OK;
+}
+
+}  // namespace stg
+
+extern "C" {
+
+int stg_head_loss_workspace(StgHandle h, const StgHeadLoss *loss, int32_t backward, uint64_t *out_bytes)
+try {
+    if (!h) return STG_ERR_INVALID_ARGUMENT;
+    const int rc = stg::head_check(h, loss, "stg_head_loss_workspace");
+    if (rc) return rc;
+    if (!out_bytes) return stg::fail(h, STG_ERR_INVALID_ARGUMENT, "stg_head_loss_workspace: out_bytes is required");
+    *out_bytes = stg::head_plan(h, loss, backward != 0).bytes;
+    return STG_OK;
+} catch (const std::bad_alloc &) {
+    return STG_ERR_CAPACITY;
+}
+
+int stg_head_loss(StgHandle h, const StgHeadLoss *loss, void *stream)
+try {
+    return h ? stg::head_forward(h, loss, (cudaStream_t)stream) : STG_ERR_INVALID_ARGUMENT;
+} catch (const std::bad_alloc &) {
+    return STG_ERR_CAPACITY;
+}
+
+int stg_head_loss_backward(StgHandle h, const StgHeadLoss *loss, void *stream)
+try {
+    return h ? stg::head_backward(h, loss, (cudaStream_t)stream) : STG_ERR_INVALID_ARGUMENT;
+} catch (const std::bad_alloc &) {
+    return STG_ERR_CAPACITY;
+}
+
+}  // extern "C"

@@ -21,6 +21,7 @@ from typing import Dict, List, Optional, Sequence
 import numpy as np
 
 from . import _native as N
+from .head import PackedHead
 
 PARAMS_DTYPE = np.dtype([
     ("temperature", "<f4"), ("top_p", "<f4"), ("min_p", "<f4"), ("repetition_penalty", "<f4"),
@@ -30,6 +31,7 @@ PARAMS_DTYPE = np.dtype([
 
 
 _BEAM_DTYPES = {"torch.float32": N.DTYPE_F32, "torch.bfloat16": N.DTYPE_BF16}
+_HALF_DTYPES = {"torch.bfloat16": N.DTYPE_BF16, "torch.float16": N.DTYPE_F16}
 
 
 class StingrayError(RuntimeError):
@@ -615,6 +617,137 @@ class BatchSampler:
             n_steps, n_seq, beams, hyps, self._beam_array("steps", steps, i32, shape), self._beam_array("parents", parents, i32, shape),
             self._beam_array("tokens", tokens, i32, shape), pad, self._beam_array("out['sequences']", out["sequences"], i32, (n_seq, hyps, n_steps)),
             n_steps, self._beam_array("out['lengths']", out["lengths"], i32, shape), self._stream_here(stream)))
+        return out
+
+    # -- the head -------------------------------------------------------------------------------------
+    def _head_rows(self, name, x, dtypes, columns=None):
+        """Address, row stride and type of a CUDA matrix with contiguous rows on the handle's device."""
+        dtype = dtypes.get(str(x.dtype))
+        if dtype is None or x.dim() != 2 or x.get_device() != self.device or (x.shape[1] > 1 and x.stride(1) != 1) or \
+                (columns is not None and x.shape[1] != columns):
+            raise ValueError(f"{name} must be a matrix of {' or '.join(dtypes)} with {'contiguous rows' if columns is None else f'contiguous rows of {columns}'} "
+                             f"on cuda:{self.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+        return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else x.shape[1], dtype
+
+    def _head_workspace(self, b, backward: bool, stream):
+        """A call's own workspace, in the order of the stream that uses it; in a graph's memory where that stream is captured."""
+        import torch
+
+        n = C.c_uint64(0)
+        self._check(self._lib.stg_head_loss_workspace(self._h, C.byref(b), 1 if backward else 0, C.byref(n)))
+        dev = torch.device("cuda", self.device)
+        if stream is None:
+            ws = torch.empty(int(n.value), dtype=torch.uint8, device=dev)
+        else:
+            if not isinstance(stream, torch.cuda.Stream):
+                stream = torch.cuda.ExternalStream(stream, device=dev)
+            with torch.cuda.stream(stream):
+                ws = torch.empty(int(n.value), dtype=torch.uint8, device=dev)
+        b.workspace, b.workspace_bytes = ws.data_ptr(), int(n.value)
+        return ws
+
+    def _head_loss(self, hidden, weight, targets, softcap):
+        import torch
+
+        b = N.StgHeadLoss()
+        b.struct_size = C.sizeof(N.StgHeadLoss)
+        b.weight, b.weight_stride, b.dtype = self._head_rows("weight", weight, _HALF_DTYPES)
+        b.vocab, b.width = weight.shape
+        b.hidden, b.hidden_stride, _ = self._head_rows("hidden", hidden, {str(weight.dtype): b.dtype}, b.width)
+        b.rows, b.logit_softcap = hidden.shape[0], softcap
+        b.targets = self._beam_array("targets", targets, torch.int32, (b.rows,))
+        return b
+
+    def head_loss(self, hidden, weight, targets, *, softcap: float = 0.0, stream=None, out: Optional[dict] = None):
+        """Softmax cross entropy straight from a head (``stg_head_loss``), in pieces of the vocabulary: ``hidden`` ``[rows,
+        width]`` and ``weight`` ``[vocab, width]`` bf16 or fp16, ``targets`` ``[rows]`` int32; below 0: the row has no
+        loss.  Returns a dict with ``loss`` ``[rows]`` - minus the log-probability of the target - and ``log_norms`` ``[rows]``, the
+        logarithm of the softmax's denominator, float32.  ``softcap`` as in ``sample_rows``.  ``out``: the dict of a
+        previous call with as many rows, whose tensors are written again."""
+        import torch
+
+        b = self._head_loss(hidden, weight, targets, softcap)
+        if out is None:
+            out = {n: torch.empty(b.rows, dtype=torch.float32, device=hidden.device) for n in ("loss", "log_norms")}
+        b.loss = self._beam_array("out['loss']", out["loss"], torch.float32, (b.rows,))
+        b.log_norms = self._beam_array("out['log_norms']", out["log_norms"], torch.float32, (b.rows,))
+        ws = self._head_workspace(b, False, stream)  # noqa: F841 (held until the call is enqueued)
+        self._check(self._lib.stg_head_loss(self._h, C.byref(b), self._stream_here(stream)))
+        return out
+
+    def head_loss_backward(self, hidden, weight, targets, log_norms, grad_loss, *, grad_log_norms=None, softcap: float = 0.0,
+                           want_hidden: bool = True, want_weight: bool = True, stream=None, out: Optional[dict] = None):
+        """Gradients of ``sum(grad_loss * loss + grad_log_norms * log_norms)`` of a ``head_loss`` call with the same
+        ``hidden``, ``weight``, ``targets`` and ``softcap``, whose ``log_norms`` are given (``stg_head_loss_backward``); ``grad_loss`` and
+        ``grad_log_norms`` ``[rows]`` float32.  Returns a dict with ``grad_hidden`` and ``grad_weight`` where wanted, in the
+        inputs' type; rows without a loss have gradient 0.  ``out``: the dict of a previous call with the same
+        shapes and options, whose tensors are written again."""
+        import torch
+
+        b = self._head_loss(hidden, weight, targets, softcap)
+        f32, rows = torch.float32, (b.rows,)
+        b.log_norms = self._beam_array("log_norms", log_norms, f32, rows)
+        b.grad_loss = self._beam_array("grad_loss", grad_loss, f32, rows)
+        if grad_log_norms is not None:
+            b.grad_log_norms = self._beam_array("grad_log_norms", grad_log_norms, f32, rows)
+        shapes = {}
+        if want_hidden:
+            shapes["grad_hidden"] = (b.rows, b.width)
+        if want_weight:
+            shapes["grad_weight"] = (b.vocab, b.width)
+        if out is None:
+            out = {n: torch.empty(s, dtype=weight.dtype, device=weight.device) for n, s in shapes.items()}
+        for n, s in shapes.items():
+            setattr(b, n, self._beam_array(f"out[{n!r}]", out[n], weight.dtype, s))
+        ws = self._head_workspace(b, True, stream)  # noqa: F841
+        self._check(self._lib.stg_head_loss_backward(self._h, C.byref(b), self._stream_here(stream)))
+        return out
+
+    def head_pack(self, codes, scales, zeros=None, *, stream=None) -> PackedHead:
+        """Lays out a weight in 4 bits for ``head_logits`` (``stg_head_pack``): ``codes`` uint8 ``[vocab, width / 2]``, two
+        columns to a byte, the even one in the lower half; ``scales`` bf16 or fp16 ``[vocab, width / group]``; ``zeros`` the
+        same, or None: 8.  ``weight = (code - zero) * scale``; groups of 32, 64 or 128 columns."""
+        import torch
+
+        b = N.StgHeadPack()
+        b.struct_size = C.sizeof(N.StgHeadPack)
+        b.codes, b.codes_stride, _ = self._head_rows("codes", codes, {"torch.uint8": 0})
+        b.vocab, b.width = codes.shape[0], 2 * codes.shape[1]
+        dtype = _HALF_DTYPES.get(str(scales.dtype))
+        if dtype is None or scales.dim() != 2 or scales.shape[0] != b.vocab or scales.shape[1] < 1 or b.width % scales.shape[1] != 0:
+            raise ValueError(f"scales must be a bfloat16 or float16 matrix of {b.vocab} rows with one column per group of a width of {b.width}, "
+                             f"got {scales.dtype} {tuple(scales.shape)}")
+        b.group, b.scale_dtype = b.width // scales.shape[1], dtype
+        b.scales = self._beam_array("scales", scales, scales.dtype, scales.shape)
+        if zeros is not None:
+            b.zeros = self._beam_array("zeros", zeros, scales.dtype, scales.shape)
+        n = C.c_uint64(0)
+        self._check(self._lib.stg_head_pack_bytes(self._h, b.vocab, b.width, b.group, 0 if zeros is None else 1, C.byref(n)))
+        packed = torch.empty(int(n.value), dtype=torch.uint8, device=codes.device)
+        b.packed, b.packed_bytes = packed.data_ptr(), int(n.value)
+        self._check(self._lib.stg_head_pack(self._h, C.byref(b), self._stream_here(stream)))
+        return PackedHead(packed, b.vocab, b.width, b.group, dtype, zeros is not None)
+
+    def head_logits(self, hidden, head: PackedHead, *, dtype=None, stream=None, out=None):
+        """Logits ``[rows, vocab]`` of a decode step (``stg_head_logits``): ``hidden`` ``[rows, width]`` bf16 or fp16 times a
+        weight in 4 bits (``head_pack``), float32 or, with ``dtype=torch.bfloat16``, bf16.  ``out``: a matrix with
+        contiguous rows to write them to."""
+        import torch
+
+        if head.device_index != self.device:
+            raise ValueError(f"the head lies on cuda:{head.device_index}, the handle on cuda:{self.device}")
+        b = N.StgHeadLogits()
+        b.struct_size = C.sizeof(N.StgHeadLogits)
+        b.vocab, b.width, b.group, b.scale_dtype, b.has_zeros = head.vocab, head.width, head.group, head.scale_dtype, 1 if head.has_zeros else 0
+        b.packed, b.packed_bytes = head.packed.data_ptr(), head.nbytes
+        b.hidden, b.hidden_stride, b.hidden_dtype = self._head_rows("hidden", hidden, _HALF_DTYPES, head.width)
+        b.rows = hidden.shape[0]
+        if out is None:
+            out = torch.empty((b.rows, head.vocab), dtype=torch.float32 if dtype is None else dtype, device=hidden.device)
+        elif dtype is not None and out.dtype != dtype or out.shape[0] != b.rows:
+            raise ValueError(f"out must be {dtype or out.dtype} with {b.rows} rows, got {out.dtype} {tuple(out.shape)}")
+        b.logits, b.row_stride, b.logits_dtype = self._head_rows("out", out, _BEAM_DTYPES, head.vocab)
+        self._check(self._lib.stg_head_logits(self._h, C.byref(b), self._stream_here(stream)))
         return out
 
     # -- vocabulary-sharded mode ---------------------------------------------------------------------
