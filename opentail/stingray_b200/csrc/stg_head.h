@@ -14,7 +14,7 @@ constexpr int kHeadTileM = 128;
 // What the preparation of a call finds out, in device memory.
 struct HeadInfo {
     int32_t used;       // rows that have a loss
-    int32_t failed;     // != 0: a bounded wait gave up; the outputs are NaN then
+    int32_t splits;     // backward: parts of a piece of the vocabulary whose gradients of the hidden states are kept apart
     float scale;        // power of two that the logits' gradients are multiplied with where they are rounded to 16 bits
     float unscale;      // its inverse
 };
@@ -34,7 +34,7 @@ struct HeadWs {
     float *hit;         // [padded rows]: the target's logit
     float2 *parts;      // [padded rows, two per tile of the vocabulary]: largest logit and the sum of exp relative to it
     void *grads;        // [padded rows, piece]: gradients of a piece's logits
-    float *sums;        // [padded rows, width]: gradients of the hidden states so far
+    float *sums;        // [splits, used rows up to whole tiles, width]: gradients of the hidden states so far
 };
 
 }  // namespace stg

@@ -27,6 +27,7 @@ struct HeadPrep {
     int rows, vocab;
     const int32_t *targets;
     const float *norms, *grad_loss, *grad_norms;  // NULL in the forward pass (grad_norms: also where there are none)
+    int width, tile_m, workers, blocks, sums_rows;  // backward: for the number of splits
 };
 
 constexpr int kPrepThreads = 1024;
@@ -77,8 +78,19 @@ __global__ void __launch_bounds__(kPrepThreads) k_head_prep(const __grid_constan
         // fp16, of whose range the small ones then use as much as there is
         int e = 0;
         if (most > 0.f && most < CUDART_INF_F) e = max(-110, min(110, 13 - ilogbf(most)));
+        // few tiles of the hidden states' gradients: pieces of the vocabulary are split, so that the tiles' parts fill the chip
+        int splits = 1;
+        if (p.norms && before > 0) {
+            const int tiles = (before + p.tile_m - 1) / p.tile_m * ((p.width + 255) / 256);
+            int64_t least = 1ll << 62;
+            for (int n = 1; n <= 64 && n <= p.blocks && (int64_t)n * before <= p.sums_rows; n++) {
+                // waves of tiles times their blocks, and some six blocks' time for a tile's sums to be written and read
+                const int64_t cost = (int64_t)((tiles * n + p.workers - 1) / p.workers) * ((p.blocks + n - 1) / n + 6);
+                if (cost < least) { least = cost; splits = n; }
+            }
+        }
         p.ws.info->used = before;
-        p.ws.info->failed = 0;
+        p.ws.info->splits = splits;
         p.ws.info->scale = exp2f((float)e);
         p.ws.info->unscale = exp2f((float)-e);
     }
@@ -107,16 +119,16 @@ __global__ void __launch_bounds__(128) k_head_gather(const __grid_constant__ Hea
     }
 }
 
-// A row's maxima and sums joined: its normaliser and loss.
-__global__ void __launch_bounds__(128) k_head_join(const __grid_constant__ HeadWs ws, int pieces, float *loss, float *norms)
+// A row's maxima and sums joined: its normaliser and loss.  `targets`: the rows are the caller's own, else they have been gathered.
+__global__ void __launch_bounds__(128) k_head_join(const __grid_constant__ HeadWs ws, int pieces, const int32_t *targets, int vocab, float *loss, float *norms)
 {
     __shared__ float tops[4];
     __shared__ double sums[4];
     pdl_release();
     pdl_wait();
-    const int r = blockIdx.x, tid = threadIdx.x, at = ws.place[r];
-    if (at < 0 || ws.info->failed != 0) {
-        if (tid == 0) loss[r] = norms[r] = at == -1 && ws.info->failed == 0 ? 0.f : CUDART_NAN_F;
+    const int r = blockIdx.x, tid = threadIdx.x, at = !targets ? ws.place[r] : targets[r] < 0 ? -1 : targets[r] >= vocab ? -2 : r;
+    if (at < 0) {
+        if (tid == 0) loss[r] = norms[r] = at == -1 ? 0.f : CUDART_NAN_F;
         return;
     }
     const float2 *parts = ws.parts + (int64_t)at * pieces;
@@ -145,19 +157,26 @@ __global__ void __launch_bounds__(128) k_head_join(const __grid_constant__ HeadW
     }
 }
 
-// Gradients of the hidden states: rounded, back in their rows; zeros where a row has no loss.
+// Gradients of the hidden states: the splits' sums added up and rounded, back in their rows; zeros where a row has no loss.
 template <bool BF16>
 __global__ void __launch_bounds__(128) k_head_spread(const __grid_constant__ HeadWs ws, int width, uint16_t *out)
 {
     pdl_release();
     pdl_wait();
-    const int r = blockIdx.x, at = ws.place[r];
-    const float unscale = ws.info->failed != 0 ? CUDART_NAN_F : ws.info->unscale;
-    const float *from = ws.sums + (int64_t)at * width;
+    const int r = blockIdx.x, at = ws.place[r], splits = ws.info->splits;
+    const float unscale = ws.info->unscale;
+    const int64_t slab = (int64_t)ws.info->used * width;
     for (int i = threadIdx.x; i < width / 8; i += 128) {
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (at >= 0) {
-            const float4 x = ((const float4 *)from)[2 * i], y = ((const float4 *)from)[2 * i + 1];
+            const float *from = ws.sums + (int64_t)at * width + 8 * i;
+            float4 x = *(const float4 *)from, y = *(const float4 *)(from + 4);
+#pragma unroll 4
+            for (int s = 1; s < splits; s++) {
+                const float4 u = *(const float4 *)(from + s * slab), w = *(const float4 *)(from + s * slab + 4);
+                x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
+                y.x += w.x; y.y += w.y; y.z += w.z; y.w += w.w;
+            }
             v = make_uint4(pack2<BF16>(x.x * unscale, x.y * unscale), pack2<BF16>(x.z * unscale, x.w * unscale), pack2<BF16>(y.x * unscale, y.y * unscale),
                            pack2<BF16>(y.z * unscale, y.w * unscale));
         }
@@ -168,7 +187,11 @@ __global__ void __launch_bounds__(128) k_head_spread(const __grid_constant__ Hea
 // ---- host ----
 
 struct HeadPlan {
-    int rows_pad, tile_n, tiles_n, piece, pieces;
+    bool pair;              // tiles of 256 rows by two CTAs
+    int tile_m, rows_pad;
+    int tile_n, tiles_n;    // of the vocabulary
+    int piece, pieces;      // backward: vocabulary entries whose gradients are there at a time; a multiple of 64
+    int grads_stride, sums_rows;
     size_t bytes;
 };
 
@@ -185,8 +208,8 @@ static HeadWs head_layout(const StgHeadLoss *b, bool backward, HeadPlan &p, char
     ws.place = (int32_t *)take(R * 4);
     ws.hidden = take(R * (size_t)b->width * 2);
     if (backward) {
-        ws.grads = take(R * (size_t)p.piece * 2);
-        ws.sums = (float *)take(R * (size_t)b->width * 4);
+        ws.grads = take(R * (size_t)p.grads_stride * 2);
+        ws.sums = (float *)take((size_t)p.sums_rows * (size_t)b->width * 4);
     } else {
         ws.hit = (float *)take(R * 4);
         ws.parts = (float2 *)take(R * 2 * (size_t)p.tiles_n * sizeof(float2));
@@ -199,16 +222,29 @@ static HeadPlan head_plan(StgHandle h, const StgHeadLoss *b, bool backward)
 {
     HeadPlan p;
     memset(&p, 0, sizeof(p));
+    p.pair = b->rows > kHeadTileM;
+    p.tile_m = p.pair ? 2 * kHeadTileM : kHeadTileM;
     p.rows_pad = (b->rows + kHeadTileM - 1) / kHeadTileM * kHeadTileM;
+    // One row of tiles reads the weight once, and its time is that of the CTA with the most of it: the width of a
+    // tile is the one whose waves take the fewest vocabulary entries, the widest of those (64 x 4096 x 151,936: 5 waves of 208, 1040
+    // entries per CTA, in place of 5 of 256)
     p.tile_n = 256;
-    p.tiles_n = (b->vocab + 255) / 256;
-    const int64_t whole = (int64_t)p.tiles_n * 256;
+    if (!p.pair)
+        for (int64_t n = 256, least = INT64_MAX; n >= 64; n -= 16) {
+            const int64_t tiles = (b->vocab + n - 1) / n, most = (tiles + h->sm_count - 1) / h->sm_count * n;
+            if (most < least) { least = most; p.tile_n = (int)n; }
+        }
+    p.tiles_n = (b->vocab + p.tile_n - 1) / p.tile_n;
     // a piece of the gradients takes 256 MB at most, or 2048 columns
-    int64_t piece = std::max<int64_t>(2048, (int64_t)(1 << 27) / std::max(1, p.rows_pad) / 256 * 256);
-    piece = std::min<int64_t>(std::min<int64_t>(piece, 16384), whole);
-    p.pieces = (int)((whole + piece - 1) / piece);
-    p.piece = (int)((whole / 256 + p.pieces - 1) / p.pieces * 256);
+    const int64_t whole = ((int64_t)b->vocab + 63) / 64 * 64;
+    const int64_t most = std::min<int64_t>(std::max<int64_t>(2048, (int64_t)(1 << 27) / std::max(1, p.rows_pad)), whole);
+    p.pieces = (int)((whole + most - 1) / most);
+    // whole tiles, of the row of CTAs that the rows take at most
+    const int64_t each = ((whole + p.pieces - 1) / p.pieces + 255) / 256 * 256;
+    p.piece = (int)std::min(each, whole);
     p.pieces = (int)((whole + p.piece - 1) / p.piece);
+    p.grads_stride = (p.piece + p.tile_n - 1) / p.tile_n * p.tile_n;
+    p.sums_rows = (int)std::max<int64_t>(p.rows_pad, (int64_t)2 * h->sm_count * kHeadTileM * 256 / b->width);
     head_layout(b, backward, p, nullptr);
     return p;
 }
@@ -261,26 +297,57 @@ static int head_map(StgHandle h, CUtensorMap *map, bool bf16, const void *p, int
 }
 
 template <int MODE>
-static cudaError_t head_gemm(StgHandle h, bool bf16, cudaStream_t stream, const CUtensorMap &a, const CUtensorMap &b, const HeadGemm &g, int64_t tiles)
+static cudaError_t head_gemm(StgHandle h, bool bf16, bool pair, cudaStream_t stream, const CUtensorMap &a, const CUtensorMap &b, const HeadGemm &g, int64_t tiles)
 {
     using Kernel = void (*)(CUtensorMap, CUtensorMap, HeadGemm);
-    static const Kernel kernels[2][2] = {{k_head_gemm<MODE, false, false>, k_head_gemm<MODE, false, (MODE < kHidden)>},
-                                         {k_head_gemm<MODE, true, false>, k_head_gemm<MODE, true, (MODE < kHidden)>}};
-    const Kernel fn = kernels[bf16][g.cap != 0.f];
-    const cudaError_t e = ensure_dynamic_smem((const void *)fn, kGemmSmem);
+    constexpr bool C = MODE == kStats || MODE == kGrad;  // the others have no soft cap
+    static const Kernel kernels[2][2][2] = {{{k_head_gemm<MODE, false, false, false>, k_head_gemm<MODE, false, false, true>}, {k_head_gemm<MODE, false, C, false>, k_head_gemm<MODE, false, C, true>}},
+                                            {{k_head_gemm<MODE, true, false, false>, k_head_gemm<MODE, true, false, true>}, {k_head_gemm<MODE, true, C, false>, k_head_gemm<MODE, true, C, true>}}};
+    const Kernel fn = kernels[bf16][g.cap != 0.f][pair];
+    const size_t smem = pair ? GemmRing<true>::kSmem : GemmRing<false>::kSmem;
+    const cudaError_t e = ensure_dynamic_smem((const void *)fn, smem);
     if (e != cudaSuccess) return e;
     h->stats.kernel_launches++;
-    return launch_behind(fn, dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, h->sm_count))), kGemmThreads, kGemmSmem, stream, a, b, g);
+    const int ctas = pair ? 2 : 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = 2;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(ctas * std::max<int64_t>(1, std::min<int64_t>(tiles, h->sm_count / ctas))));
+    cfg.blockDim = dim3(kGemmThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = at;
+    cfg.numAttrs = pair ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, fn, a, b, g);
 }
+
+static bool head_rows_aligned(const StgHeadLoss *b) { return !misaligned(b->hidden, 16) && (b->rows == 1 || b->hidden_stride % 8 == 0); }
 
 static int head_begin(StgHandle h, const StgHeadLoss *b, const HeadWs &ws, const HeadPlan &p, bool backward, cudaStream_t stream)
 {
-    const HeadPrep prep = {ws, b->rows, b->vocab, b->targets, backward ? b->log_norms : nullptr, b->grad_loss, b->grad_log_norms};
+    const HeadPrep prep = {ws, b->rows, b->vocab, b->targets, backward ? b->log_norms : nullptr, b->grad_loss, b->grad_log_norms,
+                           b->width, p.tile_m, h->sm_count * kHeadTileM / p.tile_m, (p.piece + kGemmK - 1) / kGemmK, p.sums_rows};
     CK(launch_behind(k_head_prep, dim3(1), kPrepThreads, 0, stream, prep));
-    const bool vec = !misaligned(b->hidden, 16) && (b->rows == 1 || b->hidden_stride % 8 == 0);
-    CK(launch_behind(k_head_gather, dim3((unsigned)p.rows_pad), 128, 0, stream, ws, (const uint16_t *)b->hidden, b->hidden_stride, b->width, vec));
+    CK(launch_behind(k_head_gather, dim3((unsigned)p.rows_pad), 128, 0, stream, ws, (const uint16_t *)b->hidden, b->hidden_stride, b->width, head_rows_aligned(b)));
     h->stats.kernel_launches += 2;
     return STG_OK;
+}
+
+// Tiles are taken in groups of rows, so that what runs at a time reads few rows and columns over and over in L2: 8192 x 4096 x 151,936 in
+// 7.9 ms with groups of 16 x 256 rows, 8.3 with all rows, 8.5 with 6; its gradients' products over pieces of 15,360 with groups of 8 in
+// 24.5 ms, 27.6 with all rows.
+constexpr int kGroupLogits = 16, kGroupGrads = 8;
+
+static HeadGemm head_args(const StgHeadLoss *b, const HeadWs &ws, const HeadPlan &p)
+{
+    HeadGemm g;
+    memset(&g, 0, sizeof(g));
+    g.info = ws.info; g.rows = ws.rows; g.rows_pad = p.rows_pad; g.tile_n = p.tile_n; g.group = kGroupLogits; g.cap = b->logit_softcap;
+    return g;
 }
 
 static int head_forward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
@@ -294,16 +361,19 @@ static int head_forward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
     CK(on.error);
     const HeadWs ws = head_layout(b, false, p, (char *)b->workspace);
     const bool bf16 = b->dtype == STG_DTYPE_BF16;
+    // one row of tiles takes no less time for fewer rows: they are read where they are
+    const bool direct = !p.pair && head_rows_aligned(b);
     CUtensorMap rows, weight;
-    if ((rc = head_map(h, &rows, bf16, ws.hidden, b->width, p.rows_pad, b->width, kHeadTileM))) return rc;
-    if ((rc = head_map(h, &weight, bf16, b->weight, b->width, b->vocab, b->weight_stride, p.tile_n))) return rc;
-    if ((rc = head_begin(h, b, ws, p, false, stream))) return rc;
-    HeadGemm g;
-    memset(&g, 0, sizeof(g));
-    g.info = ws.info; g.rows = ws.rows; g.n = b->vocab; g.k = b->width; g.tile_n = p.tile_n; g.cap = b->logit_softcap;
+    if ((rc = direct ? head_map(h, &rows, bf16, b->hidden, b->width, b->rows, b->rows == 1 ? b->width : b->hidden_stride, kHeadTileM)
+                     : head_map(h, &rows, bf16, ws.hidden, b->width, p.rows_pad, b->width, kHeadTileM))) return rc;
+    if ((rc = head_map(h, &weight, bf16, b->weight, b->width, b->vocab, b->weight_stride, p.pair ? p.tile_n / 2 : p.tile_n))) return rc;
+    if (!direct && (rc = head_begin(h, b, ws, p, false, stream))) return rc;
+    HeadGemm g = head_args(b, ws, p);
+    g.targets = direct ? b->targets : nullptr; g.used_rows = b->rows;
+    g.n = b->vocab; g.k = b->width;
     g.parts = ws.parts; g.hit = ws.hit; g.pieces = 2 * p.tiles_n;
-    CK(head_gemm<kStats>(h, bf16, stream, rows, weight, g, (int64_t)p.rows_pad / kHeadTileM * p.tiles_n));
-    CK(launch_behind(k_head_join, dim3((unsigned)b->rows), 128, 0, stream, ws, 2 * p.tiles_n, b->loss, b->log_norms));
+    CK(head_gemm<kStats>(h, bf16, p.pair, stream, rows, weight, g, (int64_t)((b->rows + p.tile_m - 1) / p.tile_m) * p.tiles_n));
+    CK(launch_behind(k_head_join, dim3((unsigned)b->rows), 128, 0, stream, ws, 2 * p.tiles_n, g.targets, b->vocab, b->loss, b->log_norms));
     h->stats.kernel_launches++;
     h->stats.calls++;
     return STG_OK;
@@ -328,32 +398,31 @@ static int head_backward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
     const bool bf16 = b->dtype == STG_DTYPE_BF16;
     CUtensorMap rows_k, weight_k, grads_k, weight_mn, grads_mn, rows_mn;  // how the operands' boxes of 64 columns are cut
     if ((rc = head_map(h, &rows_k, bf16, ws.hidden, b->width, p.rows_pad, b->width, kHeadTileM))) return rc;
-    if ((rc = head_map(h, &weight_k, bf16, b->weight, b->width, b->vocab, b->weight_stride, 256))) return rc;
-    if ((rc = head_map(h, &grads_k, bf16, ws.grads, p.piece, p.rows_pad, p.piece, kHeadTileM))) return rc;
+    if ((rc = head_map(h, &weight_k, bf16, b->weight, b->width, b->vocab, b->weight_stride, p.pair ? p.tile_n / 2 : p.tile_n))) return rc;
     if ((rc = head_map(h, &weight_mn, bf16, b->weight, b->width, b->vocab, b->weight_stride, kGemmK))) return rc;
-    if ((rc = head_map(h, &grads_mn, bf16, ws.grads, p.piece, p.rows_pad, p.piece, kGemmK))) return rc;
     if ((rc = head_map(h, &rows_mn, bf16, ws.hidden, b->width, p.rows_pad, b->width, kGemmK))) return rc;
     if ((rc = head_begin(h, b, ws, p, true, stream))) return rc;
-    const int64_t tiles_m = p.rows_pad / kHeadTileM, tiles_w = (b->width + 255) / 256;
+    const int64_t tiles_m = (b->rows + p.tile_m - 1) / p.tile_m, tiles_w = (b->width + 255) / 256;
     for (int i = 0; i < p.pieces; i++) {
-        HeadGemm g;
-        memset(&g, 0, sizeof(g));
-        g.info = ws.info; g.rows = ws.rows; g.tile_n = 256; g.cap = b->logit_softcap;
-        g.first = i * p.piece;
-        const int count = std::min(p.piece, b->vocab - g.first);
+        const int first = i * p.piece, count = std::min(p.piece, b->vocab - first);
+        // what lies behind the piece's columns is read as zeros
+        if ((rc = head_map(h, &grads_k, bf16, ws.grads, count, p.rows_pad, p.grads_stride, kHeadTileM))) return rc;
+        if ((rc = head_map(h, &grads_mn, bf16, ws.grads, count, p.rows_pad, p.grads_stride, kGemmK))) return rc;
+        HeadGemm g = head_args(b, ws, p);
+        g.first = first;
         g.n = count; g.k = b->width;
-        g.grads = ws.grads; g.grads_stride = p.piece;
-        CK(head_gemm<kGrad>(h, bf16, stream, rows_k, weight_k, g, tiles_m * ((count + 255) / 256)));
-        g.n = b->width;
+        g.grads = ws.grads; g.grads_stride = p.grads_stride;
+        CK(head_gemm<kGrad>(h, bf16, p.pair, stream, rows_k, weight_k, g, tiles_m * ((count + p.tile_n - 1) / p.tile_n)));
+        g.n = b->width; g.tile_n = 256; g.group = kGroupGrads; g.cap = 0.f;
         if (b->grad_hidden) {
             g.k = count;
-            g.sums = ws.sums; g.sums_stride = b->width;
-            CK(head_gemm<kHidden>(h, bf16, stream, grads_k, weight_mn, g, tiles_m * tiles_w));
+            g.sums = ws.sums;
+            CK(head_gemm<kHidden>(h, bf16, p.pair, stream, grads_k, weight_mn, g, tiles_m * tiles_w * 64));
         }
         if (b->grad_weight) {
             g.m = count;
             g.out = b->grad_weight; g.out_stride = b->width;
-            CK(head_gemm<kWeight>(h, bf16, stream, grads_mn, rows_mn, g, (int64_t)((count + kHeadTileM - 1) / kHeadTileM) * tiles_w));
+            CK(head_gemm<kWeight>(h, bf16, p.pair, stream, grads_mn, rows_mn, g, (int64_t)((count + p.tile_m - 1) / p.tile_m) * tiles_w));
         }
     }
     if (b->grad_hidden) {

@@ -15,6 +15,7 @@ native status, ``CudaBackend.cs:4110-4111``) when the library reports a failure.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence
 
@@ -31,7 +32,21 @@ PARAMS_DTYPE = np.dtype([
 
 
 _BEAM_DTYPES = {"torch.float32": N.DTYPE_F32, "torch.bfloat16": N.DTYPE_BF16}
-_HALF_DTYPES = {"torch.bfloat16": N.DTYPE_BF16, "torch.float16": N.DTYPE_F16}
+
+
+@functools.lru_cache(None)
+def _half_dtypes():
+    """Types of hidden states, weights and scales."""
+    import torch
+
+    return {torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_F16}
+
+
+@functools.lru_cache(None)
+def _logits_dtypes():
+    import torch
+
+    return {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16}
 
 
 class StingrayError(RuntimeError):
@@ -117,6 +132,7 @@ class BatchSampler:
             raise StingrayError(rc, self._error(None))
         self._h = h
         self.device = device
+        self._head_sizes = {}
         self.max_rows, self.max_vocab, self.max_top_k = max_rows, max_vocab, max_top_k
 
     # -- plumbing -------------------------------------------------------------------------------
@@ -622,41 +638,46 @@ class BatchSampler:
     # -- the head -------------------------------------------------------------------------------------
     def _head_rows(self, name, x, dtypes, columns=None):
         """Address, row stride and type of a CUDA matrix with contiguous rows on the handle's device."""
-        dtype = dtypes.get(str(x.dtype))
-        if dtype is None or x.dim() != 2 or x.get_device() != self.device or (x.shape[1] > 1 and x.stride(1) != 1) or \
-                (columns is not None and x.shape[1] != columns):
-            raise ValueError(f"{name} must be a matrix of {' or '.join(dtypes)} with {'contiguous rows' if columns is None else f'contiguous rows of {columns}'} "
-                             f"on cuda:{self.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
-        return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else x.shape[1], dtype
+        dtype, shape = dtypes.get(x.dtype), x.shape
+        if dtype is None or len(shape) != 2 or x.get_device() != self.device or (columns is not None and shape[1] != columns) or \
+                (shape[1] > 1 and x.stride(1) != 1):
+            raise ValueError(f"{name} must be a matrix of {' or '.join(str(d) for d in dtypes)} with "
+                             f"{'contiguous rows' if columns is None else f'contiguous rows of {columns}'} on cuda:{self.device}, "
+                             f"got {x.dtype} {tuple(shape)} on {x.device}")
+        return x.data_ptr(), x.stride(0) if shape[0] > 1 else shape[1], dtype
 
     def _head_workspace(self, b, backward: bool, stream):
         """A call's own workspace, in the order of the stream that uses it; in a graph's memory where that stream is captured."""
         import torch
 
-        n = C.c_uint64(0)
-        self._check(self._lib.stg_head_loss_workspace(self._h, C.byref(b), 1 if backward else 0, C.byref(n)))
-        dev = torch.device("cuda", self.device)
+        key = (b.rows, b.vocab, b.width, backward)
+        size = self._head_sizes.get(key)
+        if size is None:  # 3 us of a call
+            n = C.c_uint64(0)
+            self._check(self._lib.stg_head_loss_workspace(self._h, C.byref(b), 1 if backward else 0, C.byref(n)))
+            if len(self._head_sizes) > 1000:
+                self._head_sizes.clear()
+            size = self._head_sizes[key] = int(n.value)
+        dev = f"cuda:{self.device}"
         if stream is None:
-            ws = torch.empty(int(n.value), dtype=torch.uint8, device=dev)
+            ws = torch.empty(size, dtype=torch.uint8, device=dev)
         else:
             if not isinstance(stream, torch.cuda.Stream):
                 stream = torch.cuda.ExternalStream(stream, device=dev)
             with torch.cuda.stream(stream):
-                ws = torch.empty(int(n.value), dtype=torch.uint8, device=dev)
-        b.workspace, b.workspace_bytes = ws.data_ptr(), int(n.value)
+                ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        b.workspace, b.workspace_bytes = ws.data_ptr(), size
         return ws
 
     def _head_loss(self, hidden, weight, targets, softcap):
         import torch
 
-        b = N.StgHeadLoss()
-        b.struct_size = C.sizeof(N.StgHeadLoss)
-        b.weight, b.weight_stride, b.dtype = self._head_rows("weight", weight, _HALF_DTYPES)
-        b.vocab, b.width = weight.shape
-        b.hidden, b.hidden_stride, _ = self._head_rows("hidden", hidden, {str(weight.dtype): b.dtype}, b.width)
-        b.rows, b.logit_softcap = hidden.shape[0], softcap
-        b.targets = self._beam_array("targets", targets, torch.int32, (b.rows,))
-        return b
+        wp, ws, dtype = self._head_rows("weight", weight, _half_dtypes())
+        vocab, width = weight.shape
+        hp, hs, _ = self._head_rows("hidden", hidden, {weight.dtype: dtype}, width)
+        rows = hidden.shape[0]
+        return N.StgHeadLoss(C.sizeof(N.StgHeadLoss), rows, vocab, width, dtype, softcap, hp, hs, wp, ws,
+                             self._beam_array("targets", targets, torch.int32, (rows,)))
 
     def head_loss(self, hidden, weight, targets, *, softcap: float = 0.0, stream=None, out: Optional[dict] = None):
         """Softmax cross entropy straight from a head (``stg_head_loss``), in pieces of the vocabulary: ``hidden`` ``[rows,
@@ -711,9 +732,9 @@ class BatchSampler:
 
         b = N.StgHeadPack()
         b.struct_size = C.sizeof(N.StgHeadPack)
-        b.codes, b.codes_stride, _ = self._head_rows("codes", codes, {"torch.uint8": 0})
+        b.codes, b.codes_stride, _ = self._head_rows("codes", codes, {torch.uint8: 0})
         b.vocab, b.width = codes.shape[0], 2 * codes.shape[1]
-        dtype = _HALF_DTYPES.get(str(scales.dtype))
+        dtype = _half_dtypes().get(scales.dtype)
         if dtype is None or scales.dim() != 2 or scales.shape[0] != b.vocab or scales.shape[1] < 1 or b.width % scales.shape[1] != 0:
             raise ValueError(f"scales must be a bfloat16 or float16 matrix of {b.vocab} rows with one column per group of a width of {b.width}, "
                              f"got {scales.dtype} {tuple(scales.shape)}")
@@ -736,17 +757,15 @@ class BatchSampler:
 
         if head.device_index != self.device:
             raise ValueError(f"the head lies on cuda:{head.device_index}, the handle on cuda:{self.device}")
-        b = N.StgHeadLogits()
-        b.struct_size = C.sizeof(N.StgHeadLogits)
-        b.vocab, b.width, b.group, b.scale_dtype, b.has_zeros = head.vocab, head.width, head.group, head.scale_dtype, 1 if head.has_zeros else 0
-        b.packed, b.packed_bytes = head.packed.data_ptr(), head.nbytes
-        b.hidden, b.hidden_stride, b.hidden_dtype = self._head_rows("hidden", hidden, _HALF_DTYPES, head.width)
-        b.rows = hidden.shape[0]
+        hp, hs, hd = self._head_rows("hidden", hidden, _half_dtypes(), head.width)
+        rows = hidden.shape[0]
         if out is None:
-            out = torch.empty((b.rows, head.vocab), dtype=torch.float32 if dtype is None else dtype, device=hidden.device)
-        elif dtype is not None and out.dtype != dtype or out.shape[0] != b.rows:
-            raise ValueError(f"out must be {dtype or out.dtype} with {b.rows} rows, got {out.dtype} {tuple(out.shape)}")
-        b.logits, b.row_stride, b.logits_dtype = self._head_rows("out", out, _BEAM_DTYPES, head.vocab)
+            out = torch.empty((rows, head.vocab), dtype=torch.float32 if dtype is None else dtype, device=hidden.device)
+        elif dtype is not None and out.dtype != dtype or out.shape[0] != rows:
+            raise ValueError(f"out must be {dtype or out.dtype} with {rows} rows, got {out.dtype} {tuple(out.shape)}")
+        op, os_, od = self._head_rows("out", out, _logits_dtypes(), head.vocab)
+        b = N.StgHeadLogits(C.sizeof(N.StgHeadLogits), rows, head.vocab, head.width, head.group, head.scale_dtype, 1 if head.has_zeros else 0, hd, od,
+                            head.packed.data_ptr(), head.nbytes, hp, hs, op, os_)
         self._check(self._lib.stg_head_logits(self._h, C.byref(b), self._stream_here(stream)))
         return out
 
