@@ -629,7 +629,8 @@ typedef struct StgHeadPack {
 STG_API int stg_head_pack_bytes(StgHandle handle, int32_t vocab, int32_t width, int32_t group, int32_t has_zeros, uint64_t *out_bytes);
 STG_API int stg_head_pack(StgHandle handle, const StgHeadPack *pack, void *stream);
 
-/* logits[r][v] = hidden[r] . weight[v]: group sums and scales in fp32, rounded once.  Any number of rows. */
+/* logits[r][v] = hidden[r] . weight[v]: sums of groups and their scaling in fp32, rounded once.  Any number of rows.  A hidden state that is
+ * not finite leaves none of its row's logits finite, a scale or zero point that is not, none of its entry's. */
 typedef struct StgHeadLogits {
     int32_t struct_size;            /* = sizeof(StgHeadLogits) */
     int32_t rows;
@@ -646,7 +647,11 @@ typedef struct StgHeadLogits {
     int64_t hidden_stride;          /* elements between rows (>= width) */
     void *logits;                   /* out [rows, row_stride] */
     int64_t row_stride;             /* elements between rows (>= vocab); what lies behind vocab is not written */
+    void *workspace;                /* 256-byte aligned, or NULL where stg_head_logits_workspace says 0 */
+    uint64_t workspace_bytes;       /* >= stg_head_logits_workspace */
 } StgHeadLogits;
+/* Bytes of workspace for a call of these sizes and types: 0 for a few rows. */
+STG_API int stg_head_logits_workspace(StgHandle handle, const StgHeadLogits *logits, uint64_t *out_bytes);
 STG_API int stg_head_logits(StgHandle handle, const StgHeadLogits *logits, void *stream);
 
 /* ---- vocabulary-sharded mode (no counterpart in the reference, which is single-device:

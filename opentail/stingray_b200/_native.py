@@ -32,7 +32,7 @@ EXPORTS = [
     "stg_mask_cache_put", "stg_mask_cache_contains", "stg_mask_compose",
     "stg_history_reset", "stg_history_load", "stg_history_append", "stg_history_length",
     "stg_beam_select", "stg_beam_start", "stg_beam_advance", "stg_beam_reorder", "stg_beam_backtrace",
-    "stg_head_loss_workspace", "stg_head_loss", "stg_head_loss_backward", "stg_head_pack_bytes", "stg_head_pack", "stg_head_logits",
+    "stg_head_loss_workspace", "stg_head_loss", "stg_head_loss_backward", "stg_head_pack_bytes", "stg_head_pack", "stg_head_logits_workspace", "stg_head_logits",
 ]
 
 
@@ -137,7 +137,7 @@ class StgHeadLogits(C.Structure):
         ("struct_size", C.c_int32), ("rows", C.c_int32), ("vocab", C.c_int32), ("width", C.c_int32), ("group", C.c_int32),
         ("scale_dtype", C.c_int32), ("has_zeros", C.c_int32), ("hidden_dtype", C.c_int32), ("logits_dtype", C.c_int32),
         ("packed", C.c_void_p), ("packed_bytes", C.c_uint64), ("hidden", C.c_void_p), ("hidden_stride", C.c_int64),
-        ("logits", C.c_void_p), ("row_stride", C.c_int64),
+        ("logits", C.c_void_p), ("row_stride", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
     ]
 
 
@@ -206,6 +206,7 @@ def load() -> C.CDLL:
     lib.stg_head_loss_backward.argtypes = [vp, C.POINTER(StgHeadLoss), vp]
     lib.stg_head_pack_bytes.argtypes = [vp, i32, i32, i32, i32, C.POINTER(C.c_uint64)]
     lib.stg_head_pack.argtypes = [vp, C.POINTER(StgHeadPack), vp]
+    lib.stg_head_logits_workspace.argtypes = [vp, C.POINTER(StgHeadLogits), C.POINTER(C.c_uint64)]
     lib.stg_head_logits.argtypes = [vp, C.POINTER(StgHeadLogits), vp]
     for name in EXPORTS:
         fn = getattr(lib, name)

@@ -37,4 +37,8 @@ struct HeadWs {
     float *sums;        // [splits, used rows up to whole tiles, width]: gradients of the hidden states so far
 };
 
+// A tensor map (stg_head_loss.cu): sizes and boxes from the innermost dimension on, strides in bytes between the others; zeros outside.
+int head_map_of(StgHandle h, CUtensorMap *map, CUtensorMapDataType type, int dims, const void *p, const cuuint64_t *size, const cuuint64_t *stride, const cuuint32_t *box,
+                CUtensorMapSwizzle swizzle);
+
 }  // namespace stg

@@ -6,43 +6,19 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <math_constants.h>
 #include <stdint.h>
 #include <string.h>
 
 #include <new>
 
 #include "stg_beam.h"
-#include "stg_head.h"
+#include "stg_head4.cuh"
 #include "stg_launch.h"
 #include "stg_pdl.cuh"
 #include "stg_tc.cuh"
 
 namespace stg {
-
-// The packed weight: units of 16 vocabulary entries by 128 columns, a tile's units (16 entries, all columns, zeros behind the last)
-// next to each other.  A unit: twice 512 bytes of codes, of which a lane of a warp holds 16 - what it needs of 64 columns in four
-// steps of mma.m16n8k16 (word s: step s); the columns of a step are chosen such that a lane's share of a hidden state are eight
-// neighbours for two steps: step s, columns 32 (s / 2) + 8 t + 4 (s % 2) + 0..3 for t = lane % 4.  Then the scales, and in the same way
-// the zero points: for entry g = 0..7 the unit's groups, for each of them entries g and g + 8.
-constexpr int kHeadRows4 = 16, kUnitCols = 128, kUnitCodes = 1024;
-
-struct Head4 {
-    const unsigned char *units;
-    int vocab, width, group, tiles, units_per_tile, unit_bytes, groups_per_unit;
-};
-
-static Head4 head4_shape(int vocab, int width, int group, bool zeros)
-{
-    Head4 w;
-    memset(&w, 0, sizeof(w));
-    w.vocab = vocab; w.width = width; w.group = group;
-    w.groups_per_unit = kUnitCols / group;
-    w.unit_bytes = kUnitCodes + 32 * w.groups_per_unit * (zeros ? 2 : 1);
-    w.units_per_tile = (width + kUnitCols - 1) / kUnitCols;
-    w.tiles = (vocab + kHeadRows4 - 1) / kHeadRows4;
-    return w;
-}
-static size_t head4_bytes(const Head4 &w) { return (size_t)w.tiles * w.units_per_tile * w.unit_bytes; }
 
 struct HeadPack {
     Head4 w;
@@ -76,7 +52,7 @@ __global__ void __launch_bounds__(256) k_head_pack(const __grid_constant__ HeadP
                 const uint32_t a = code(g, col), b = code(g + 8, col), c = code(g, col + 2), d = code(g + 8, col + 2);
                 word[s] = (a & 15u) | (b & 15u) << 4 | (c & 15u) << 8 | (d & 15u) << 12 | (a >> 4) << 16 | (b >> 4) << 20 | (c >> 4) << 24 | (d >> 4) << 28;
             }
-            ((uint4 *)(out + block * 512))[lane] = make_uint4(word[0], word[1], word[2], word[3]);
+            ((uint4 *)(out + block * 512))[code_place(lane)] = make_uint4(word[0] ^ kCodeSigns, word[1] ^ kCodeSigns, word[2] ^ kCodeSigns, word[3] ^ kCodeSigns);
         }
         const int n = 16 * w.groups_per_unit, groups = w.width / w.group;
         for (int i = lane; i < n; i += 32) {
@@ -89,101 +65,67 @@ __global__ void __launch_bounds__(256) k_head_pack(const __grid_constant__ HeadP
     }
 }
 
-struct HeadLogits {
-    Head4 w;
-    const uint16_t *hidden;
-    int64_t hidden_stride;
-    bool vec;
-    int rows;
-    void *out;
-    int64_t out_stride;
-    bool out_bf16;
-};
-
-template <bool BF16>
-__device__ __forceinline__ float half_at(uint16_t x)
-{
-    return BF16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
-}
-
-// Eight codes of a word as the four registers of an A fragment, q - 8 each.  A code is put below the bits of a number
-// whose last bits count in ones (fp16: 1024, or 1024 with the code times 16; bf16: 128), and that number is taken off; both are exact.
-template <bool BF16>
+// Eight codes of a word as the four registers of an fp16 A fragment, q - 8 each.  A code, its highest bit turned back, is put below
+// the bits of 1024, plain or times 16, and what is too much is taken off; all of it is exact.
 __device__ __forceinline__ void codes_to_a(uint32_t w, uint32_t (&a)[4])
 {
-    if (BF16) {
-        const uint32_t one = 0x3F803F80u, less = 0xC308C308u;  // 1, -136
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t v = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
-            asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(a[i]) : "r"(v), "r"(one), "r"(less));
-        }
+    const uint32_t sixteenth = 0x2C002C00u, low = 0xE408E408u, high = 0xD480D480u;  // 1/16, -1032, -72
+    const uint32_t u = w >> 8;
+    const uint32_t v0 = bits_of(w, 0x000F000Fu, 0x64086408u), v1 = bits_of(w, 0x00F000F0u, 0x64806480u);
+    const uint32_t v2 = bits_of(u, 0x000F000Fu, 0x64086408u), v3 = bits_of(u, 0x00F000F0u, 0x64806480u);
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(a[0]) : "r"(v0), "r"(low));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(a[1]) : "r"(v1), "r"(sixteenth), "r"(high));
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(a[2]) : "r"(v2), "r"(low));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(a[3]) : "r"(v3), "r"(sixteenth), "r"(high));
+}
+
+// d = a b + c
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+
+// Entry g's and g + 8's scales or zero points of a unit's groups.
+template <int G>
+__device__ __forceinline__ void group_words(uint32_t (&to)[G], const unsigned char *from, int g)
+{
+    if constexpr (G == 4) {
+        const uint4 v = ((const uint4 *)from)[g];
+        to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+    } else if constexpr (G == 2) {
+        const uint2 v = ((const uint2 *)from)[g];
+        to[0] = v.x; to[1] = v.y;
     } else {
-        const uint32_t sixteenth = 0x2C002C00u, low = 0xE408E408u, high = 0xD480D480u;  // 1/16, -1032, -72
-        const uint32_t u = w >> 8;
-        const uint32_t v0 = (w & 0x000F000Fu) | 0x64006400u, v1 = (w & 0x00F000F0u) | 0x64006400u;
-        const uint32_t v2 = (u & 0x000F000Fu) | 0x64006400u, v3 = (u & 0x00F000F0u) | 0x64006400u;
-        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(a[0]) : "r"(v0), "r"(low));
-        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(a[1]) : "r"(v1), "r"(sixteenth), "r"(high));
-        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(a[2]) : "r"(v2), "r"(low));
-        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(a[3]) : "r"(v3), "r"(sixteenth), "r"(high));
+        to[0] = ((const uint32_t *)from)[g];
     }
-}
-
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-{
-    if (BF16)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Eight neighbouring hidden states.
-__device__ __forceinline__ uint4 eight_states(const uint16_t *from, bool vec)
-{
-    if (vec) return __ldg((const uint4 *)from);
-    uint32_t e[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) e[j] = from[j];
-    return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
 }
 
 // A unit's part of 16 logits for 8 NT rows of hidden states.  x: this lane's share of the first row group's row lane / 4 at the unit's first
 // column; sums: of the unit's first group, per group 8 NT of them.
-template <bool BF16, bool SBF16, bool ZEROS, int G, int NT>
+template <bool SBF16, bool ZEROS, int G, int NT>
 __device__ __forceinline__ void unit_logits(float (&acc)[NT][4], const unsigned char *unit, const unsigned char *x, int pitch, const float *sums)
 {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint4 q[2] = {((const uint4 *)unit)[lane], ((const uint4 *)(unit + 512))[lane]};
+    const uint4 q[2] = {((const uint4 *)unit)[code_place(lane)], ((const uint4 *)(unit + 512))[code_place(lane)]};
     const uint32_t word[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
     uint32_t scale[G], zero[G];
-    auto words = [&](uint32_t (&to)[G], const unsigned char *from) {
-        if constexpr (G == 4) { const uint4 v = ((const uint4 *)from)[g]; to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w; }
-        else if constexpr (G == 2) { const uint2 v = ((const uint2 *)from)[g]; to[0] = v.x; to[1] = v.y; }
-        else to[0] = ((const uint32_t *)from)[g];
-    };
-    words(scale, unit + kUnitCodes);
-    if (ZEROS) words(zero, unit + kUnitCodes + 32 * G);
+    group_words<G>(scale, unit + kUnitCodes, g);
+    if (ZEROS) group_words<G>(zero, unit + kUnitCodes + 32 * G, g);
 #pragma unroll
     for (int gr = 0; gr < G; gr++) {
         float part[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) part[n][i] = 0.f;
-#pragma unroll
         for (int h = gr * (4 / G); h < (gr + 1) * (4 / G); h++) {  // 32 columns each
             uint32_t a0[4], a1[4];
-            codes_to_a<BF16>(word[2 * h], a0);
-            codes_to_a<BF16>(word[2 * h + 1], a1);
+            codes_to_a(word[2 * h], a0);
+            codes_to_a(word[2 * h + 1], a1);
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const uint4 v = *(const uint4 *)(x + n * 8 * pitch + h * 64);
-                mma16816<BF16>(part[n], a0, v.x, v.y);
-                mma16816<BF16>(part[n], a1, v.z, v.w);
+                if (h == gr * (4 / G)) mma16816(part[n], a0, v.x, v.y, 0.f, 0.f, 0.f, 0.f);
+                else mma16816(part[n], a0, v.x, v.y, part[n][0], part[n][1], part[n][2], part[n][3]);
+                mma16816(part[n], a1, v.z, v.w, part[n][0], part[n][1], part[n][2], part[n][3]);
             }
         }
         const float s0 = half_at<SBF16>((uint16_t)scale[gr]), s1 = half_at<SBF16>((uint16_t)(scale[gr] >> 16));
@@ -205,8 +147,53 @@ __device__ __forceinline__ void unit_logits(float (&acc)[NT][4], const unsigned 
     }
 }
 
+// The same for two rows of hidden states as integers of four digits, base 256, which are eight columns of mma.m16n8k32 over 8-bit integers:
+// 16 (q - 8) of eight codes takes three instructions, where fp16 takes nine.  Sums of a group are exact; they come out on top of
+// 1.5 * 2^23, as whose last bits they can be read in fp32 (below 2^21 each).
+template <bool SBF16, bool ZEROS, int G>
+__device__ __forceinline__ void unit_logits_int(float (&acc)[4], const unsigned char *unit, const unsigned char *x, const float *sums)
+{
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint4 q[2] = {((const uint4 *)unit)[code_place(lane)], ((const uint4 *)(unit + 512))[code_place(lane)]};
+    const uint32_t word[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
+    const uint4 b[2] = {((const uint4 *)x)[0], ((const uint4 *)x)[1]};
+    const uint32_t digits[8] = {b[0].x, b[0].y, b[0].z, b[0].w, b[1].x, b[1].y, b[1].z, b[1].w};
+    uint32_t scale[G], zero[G];
+    group_words<G>(scale, unit + kUnitCodes, g);
+    if (ZEROS) group_words<G>(zero, unit + kUnitCodes + 32 * G, g);
+    constexpr int kTop = 0x4B400000;
+#pragma unroll
+    for (int gr = 0; gr < G; gr++) {
+        int part[4] = {kTop, kTop, kTop, kTop};
+#pragma unroll
+        for (int h = gr * (4 / G); h < (gr + 1) * (4 / G); h++) {
+            const uint32_t a0 = (word[2 * h] * 16u) & 0xF0F0F0F0u, a1 = word[2 * h] & 0xF0F0F0F0u;
+            const uint32_t a2 = (word[2 * h + 1] * 16u) & 0xF0F0F0F0u, a3 = word[2 * h + 1] & 0xF0F0F0F0u;
+            asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                : "=r"(part[0]), "=r"(part[1]), "=r"(part[2]), "=r"(part[3])
+                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(digits[2 * h]), "r"(digits[2 * h + 1]), "r"(part[0]), "r"(part[1]), "r"(part[2]), "r"(part[3]));
+        }
+        const float s0 = half_at<SBF16>((uint16_t)scale[gr]), s1 = half_at<SBF16>((uint16_t)(scale[gr] >> 16));
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) f[i] = __int_as_float(part[i]) - 12582912.f;
+        if (ZEROS) {
+            const float z0 = 8.f - half_at<SBF16>((uint16_t)zero[gr]), z1 = 8.f - half_at<SBF16>((uint16_t)(zero[gr] >> 16));
+            const float2 u = *(const float2 *)(sums + gr * 8 + 2 * t);
+            f[0] = fmaf(z0, u.x, f[0]);
+            f[1] = fmaf(z0, u.y, f[1]);
+            f[2] = fmaf(z1, u.x, f[2]);
+            f[3] = fmaf(z1, u.y, f[3]);
+        }
+        acc[0] = fmaf(s0, f[0], acc[0]);
+        acc[1] = fmaf(s0, f[1], acc[1]);
+        acc[2] = fmaf(s1, f[2], acc[2]);
+        acc[3] = fmaf(s1, f[3], acc[3]);
+    }
+}
+
 template <int NT>
-__device__ __forceinline__ void write_logits(const HeadLogits &p, const float (&acc)[NT][4], int64_t tile, int r0)
+__device__ __forceinline__ void write_logits(const HeadLogits &p, const float (&acc)[NT][4], int64_t tile, const float2 *unscale)
 {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
@@ -214,43 +201,171 @@ __device__ __forceinline__ void write_logits(const HeadLogits &p, const float (&
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int64_t v = tile * kHeadRows4 + g + (i >= 2 ? 8 : 0);
-            const int r = r0 + n * 8 + 2 * t + (i & 1);
+            const int r = n * 8 + 2 * t + (i & 1);
             if (v >= p.w.vocab || r >= p.rows) continue;
-            if (p.out_bf16) ((__nv_bfloat16 *)p.out)[r * p.out_stride + v] = __float2bfloat16_rn(acc[n][i]);
-            else ((float *)p.out)[r * p.out_stride + v] = acc[n][i];
+            const float2 u = unscale[r];
+            const float x = acc[n][i] * u.x * u.y;
+            if (p.out_bf16) ((__nv_bfloat16 *)p.out)[r * p.out_stride + v] = __float2bfloat16_rn(x);
+            else ((float *)p.out)[r * p.out_stride + v] = x;
         }
 }
 
-// Hidden states of rows [r0, r0 + 8 NT) and columns [k0, k0 + cols) into shared memory, zeros where there are none; `cols` whole units.
-// The sums of their groups too, for zero points.
-template <bool BF16, bool ZEROS, int G, int NT>
-__device__ __forceinline__ void stage_states(const HeadLogits &p, int r0, int k0, int cols, unsigned char *xs, int pitch, float *sums)
+// The sums of groups of hidden states that lie in shared memory, for zero points; `cols` whole units.
+template <int G, int NT>
+__device__ __forceinline__ void sum_groups(int cols, const unsigned char *xs, int pitch, float *sums)
 {
-    for (int i = threadIdx.x; i < 8 * NT * (cols / 8); i += blockDim.x) {
-        const int n = i / (cols / 8), k = (i - n * (cols / 8)) * 8;
+    constexpr int kGroup = kUnitCols / G;
+    for (int i = threadIdx.x; i < cols / kGroup * 8 * NT; i += blockDim.x) {
+        const int n = i % (8 * NT), gr = i / (8 * NT);
+        float s = 0.f;
+        for (int k = 0; k < kGroup; k += 8) {
+            const uint4 v = *(const uint4 *)(xs + n * pitch + (gr * kGroup + k) * 2);
+            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) s += half_at<false>((uint16_t)e[j]) + half_at<false>((uint16_t)(e[j] >> 16));
+        }
+        sums[i] = s;
+    }
+}
+
+// Hidden states of up to 8 NT rows into shared memory in fp16, zeros where there are none, `cols` whole units: bf16 ones times a power of two that
+// takes a row's largest finite one to [2^14, 2^15).  That is exact down to 2^-29 of it, and 2^-40 of it off below.  `unscale`: the
+// inverse, in two factors.
+template <bool ZEROS, int G, int NT>
+__device__ __forceinline__ void stage_rows(const HeadLogits &p, int cols, unsigned char *xs, int pitch, float *sums, float2 *unscale, uint32_t *most)
+{
+    const int per = cols / 8;  // a multiple of 16
+    if (threadIdx.x < 8 * NT) most[threadIdx.x] = 0u;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 8 * NT * per; i += blockDim.x) {
+        const int n = i / per, k = (i - n * per) * 8;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r0 + n < p.rows && k0 + k < p.w.width) v = eight_states(p.hidden + (int64_t)(r0 + n) * p.hidden_stride + k0 + k, p.vec);
+        if (n < p.rows && k < p.w.width) v = eight_states(p.hidden + (int64_t)n * p.hidden_stride + k, p.vec);
         *(uint4 *)(xs + n * pitch + k * 2) = v;
+        if (p.hidden_bf16 && n < p.rows) {  // half warps have one row
+            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+            uint32_t m = 0u;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t lo = e[j] & 0x7FFFu, hi = e[j] >> 16 & 0x7FFFu;
+                m = max(m, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
+            }
+            m = __reduce_max_sync(0xFFFFu << (threadIdx.x & 16), m);
+            if ((threadIdx.x & 15) == 0) atomicMax(&most[n], m);
+        }
+    }
+    __syncthreads();
+    if (p.hidden_bf16) {
+        for (int i = threadIdx.x; i < min(8 * NT, p.rows) * per; i += blockDim.x) {
+            const int n = i / per;
+            const float top = __uint_as_float(most[n] << 16);
+            const int e = top > 0.f ? 14 - ilogbf(top) : 0, half = e / 2;
+            const float s1 = __uint_as_float((uint32_t)(127 + half) << 23), s2 = __uint_as_float((uint32_t)(127 + e - half) << 23);
+            uint4 *at = (uint4 *)(xs + n * pitch + (i - n * per) * 16);
+            const uint4 v = *at;
+            uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x[j]) : "f"(half_at<true>((uint16_t)(x[j] >> 16)) * s1 * s2), "f"(half_at<true>((uint16_t)x[j]) * s1 * s2));
+            *at = make_uint4(x[0], x[1], x[2], x[3]);
+        }
+    }
+    if (threadIdx.x < 8 * NT) {
+        const float top = __uint_as_float(most[threadIdx.x] << 16);
+        const int e = top > 0.f ? 14 - ilogbf(top) : 0, half = e / 2;
+        unscale[threadIdx.x] = make_float2(__uint_as_float((uint32_t)(127 - half) << 23), __uint_as_float((uint32_t)(127 - (e - half)) << 23));
+    }
+    __syncthreads();
+    if (ZEROS) {
+        sum_groups<G, NT>(cols, xs, pitch, sums);
+        __syncthreads();
+    }
+}
+
+// Up to two rows as integers: hidden state x is X * 2^(e - 30), e the exponent above the row's largest finite one, X rounded - exact down to
+// 2^-22 of the largest, 2^-31 of it off below - and X four digits of -128 .. 127.  Column 4 r + d of `xs` (pitch bytes between columns) has
+// digit d of row r, the highest first; of a unit's 128 columns a lane's are next to each other: byte 32 t + 8 h + i is column
+// 32 h + 8 t + i, the middle two of every four exchanged.  A row with a hidden state that is not finite comes out NaN or infinite by `bad`, the
+// sum of what such hidden states are times zero, which is added to its logits.
+template <bool ZEROS, int G>
+__device__ __forceinline__ void stage_digits(const HeadLogits &p, int cols, unsigned char *xs, int pitch, float *sums, float2 *unscale, uint32_t *most)
+{
+    const int per = cols / 8;
+    if (threadIdx.x < 8) most[threadIdx.x] = 0u;
+    __syncthreads();
+    float bad[2] = {0.f, 0.f};
+    // twice over the rows, which are in L2 or L1: for the largest, and for the digits
+    for (int pass = 0; pass < 2; pass++) {
+        for (int i = threadIdx.x; i < 2 * per; i += blockDim.x) {
+            const int r = i >= per ? 1 : 0, k = (i - r * per) * 8;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (r < p.rows && k < p.w.width) v = eight_states(p.hidden + (int64_t)r * p.hidden_stride + k, p.vec);
+            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint16_t h = (uint16_t)(e[j / 2] >> (16 * (j & 1)));
+                x[j] = p.hidden_bf16 ? half_at<true>(h) : half_at<false>(h);
+                if (!(fabsf(x[j]) < CUDART_INF_F)) {
+                    bad[r] += x[j] * 0.f;
+                    x[j] = 0.f;
+                }
+            }
+            if (pass == 0) {
+                float m = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(x[j]));
+                const uint32_t u = __reduce_max_sync(0xFFFFu << (threadIdx.x & 16), __float_as_uint(m));
+                if ((threadIdx.x & 15) == 0) atomicMax(&most[r], u);
+            } else {
+                const float top = __uint_as_float(most[r]);
+                const int e2 = top > 0.f ? 29 - ilogbf(top) : 0, half = e2 / 2;  // |X| < 2^30
+                const float s1 = __uint_as_float((uint32_t)(127 + half) << 23), s2 = __uint_as_float((uint32_t)(127 + e2 - half) << 23);
+                uint32_t d[4][2] = {};
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    int X = __float2int_rn(x[j] * s1 * s2);
+                    const int byte = (j & 3) == 1 ? 2 : (j & 3) == 2 ? 1 : (j & 3);
+#pragma unroll
+                    for (int n = 3; n >= 0; n--) {
+                        const int digit = (int)(int8_t)X;
+                        d[n][j / 4] |= (uint32_t)(uint8_t)digit << (8 * byte);
+                        X = (X - digit) >> 8;
+                    }
+                }
+                const int in = k & 127, at = (k & ~127) + (in >> 3 & 3) * 32 + (in >> 5) * 8;
+#pragma unroll
+                for (int n = 0; n < 4; n++) *(uint2 *)(xs + (4 * r + n) * pitch + at) = make_uint2(d[n][0], d[n][1]);
+            }
+        }
+        __syncthreads();
+    }
+    // (most[4 + r], behind the rows' largest: what is added to a row's logits)
+#pragma unroll
+    for (int r = 0; r < 2; r++)
+        if (bad[r] != 0.f) ((volatile uint32_t *)most)[4 + r] = 0x7FC00000u;  // NaN: times zero, so is an infinity
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const float top = __uint_as_float(most[threadIdx.x]);
+        const int e2 = top > 0.f ? 29 - ilogbf(top) + 4 : 4, half = e2 / 2;  // 16 (q - 8)
+        const float nan = __uint_as_float(most[4 + threadIdx.x]);
+        unscale[threadIdx.x] = make_float2(__uint_as_float((uint32_t)(127 - half) << 23) + nan, __uint_as_float((uint32_t)(127 - (e2 - half)) << 23));
     }
     if (ZEROS) {
-        __syncthreads();
         constexpr int kGroup = kUnitCols / G;
-        for (int i = threadIdx.x; i < cols / kGroup * 8 * NT; i += blockDim.x) {
-            const int n = i % (8 * NT), gr = i / (8 * NT);
-            float s = 0.f;
-            for (int k = 0; k < kGroup; k += 8) {
-                const uint4 v = *(const uint4 *)(xs + n * pitch + (gr * kGroup + k) * 2);
-                const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < 4; j++) s += half_at<BF16>((uint16_t)e[j]) + half_at<BF16>((uint16_t)(e[j] >> 16));
-            }
-            sums[i] = s;
+        for (int i = threadIdx.x; i < cols / kGroup * 8; i += blockDim.x) {  // column n of group gr: a group is bytes 8 h .. of every 32
+            const int n = i % 8, gr = i / 8;
+            const unsigned char *from = xs + n * pitch + gr / G * kUnitCols + (gr % G) * (32 / G);
+            int sum = 0;
+            for (int t = 0; t < 4; t++)
+                for (int j = 0; j < 32 / G; j += 4) sum = __dp4a(*(const int *)(from + 32 * t + j), 0x01010101, sum);
+            sums[i] = 16.f * (float)sum;
         }
     }
     __syncthreads();
 }
 
-// Up to 16 rows: the weight streams through, once.  Hidden states lie in shared memory whole.  A CTA per SM has a run of tiles, whose
+// Up to 16 rows at a time: the weight streams through, once.  Hidden states lie in shared memory whole.  A CTA per SM has a run of tiles, whose
 // units its 16 warps share out evenly, each a run of neighbours that it copies into a ring of its own (bulk copies, one per stage), so no
 // warp waits for another before the end.  A tile that several warps have units of is added up there, by the warp that has its first.
 constexpr int kStreamWarps = 16, kStreamStages = 2;
@@ -258,10 +373,32 @@ constexpr int kStreamWarps = 16, kStreamStages = 2;
 struct StreamShape {
     int pitch;          // bytes between rows of hidden states
     int chunk;          // units of a stage
-    size_t sums, slots, ring, bars, smem;  // offsets, and bytes in all
+    size_t sums, unscale, slots, ring, bars, smem;  // offsets, and bytes in all
 };
 
-template <bool BF16, bool SBF16, bool ZEROS, int G, int NT>
+template <int NT, bool INT>
+__device__ __forceinline__ void stream_write(const HeadLogits &p, const float (&acc)[NT][4], int64_t tile, const float2 *unscale)
+{
+    if constexpr (INT) {  // two lanes have a row's digits: columns 2 t and 2 t + 1
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, r = t >> 1;
+        const float s1 = (t & 1) ? 256.f : 16777216.f, s2 = (t & 1) ? 1.f : 65536.f;
+        float low = acc[0][0] * s1 + acc[0][1] * s2, high = acc[0][2] * s1 + acc[0][3] * s2;
+        low += __shfl_xor_sync(0xFFFFFFFFu, low, 1);
+        high += __shfl_xor_sync(0xFFFFFFFFu, high, 1);
+        const int64_t v = tile * kHeadRows4 + g + 8 * (t & 1);
+        if (r < p.rows && v < p.w.vocab) {
+            const float2 u = unscale[r];
+            const float x = ((t & 1) ? high : low) * u.x * u.y;
+            if (p.out_bf16) ((__nv_bfloat16 *)p.out)[r * p.out_stride + v] = __float2bfloat16_rn(x);
+            else ((float *)p.out)[r * p.out_stride + v] = x;
+        }
+    } else {
+        write_logits<NT>(p, acc, tile, unscale);
+    }
+}
+
+// INT: up to two rows as integers, NT 1.
+template <bool SBF16, bool ZEROS, int G, int NT, bool INT>
 __global__ void __launch_bounds__(kStreamWarps * 32, 1) k_head_stream(const __grid_constant__ HeadLogits p, const __grid_constant__ StreamShape s)
 {
     extern __shared__ __align__(128) unsigned char sm[];
@@ -293,9 +430,12 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1) k_head_stream(const __gr
     if (lane == 0)
         for (int c = 0; c < kStreamStages && c < chunks; c++) load(c);
     float *sums = (float *)(sm + s.sums);
-    stage_states<BF16, ZEROS, G, NT>(p, 0, 0, per * kUnitCols, sm, s.pitch, sums);
+    const float2 *unscale = (const float2 *)(sm + s.unscale);
+    __shared__ uint32_t most[8 * NT];
+    if (INT) stage_digits<ZEROS, G>(p, per * kUnitCols, sm, s.pitch, sums, (float2 *)(sm + s.unscale), most);
+    else stage_rows<ZEROS, G, NT>(p, per * kUnitCols, sm, s.pitch, sums, (float2 *)(sm + s.unscale), most);
 
-    const unsigned char *x = sm + (lane >> 2) * s.pitch + (lane & 3) * 16;
+    const unsigned char *x = sm + (lane >> 2) * s.pitch + (lane & 3) * (INT ? 32 : 16);
     float *slot = (float *)(sm + s.slots) + (size_t)warp * NT * 128;
     float acc[NT][4];
 #pragma unroll
@@ -311,11 +451,13 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1) k_head_stream(const __gr
         if (!__all_sync(0xFFFFFFFFu, bar_wait(bar + 8 * stage, (c / kStreamStages) & 1, dead))) break;
         const int n = min(s.chunk, u1 - u0 - c * s.chunk);
         for (int j = 0; j < n; j++) {
-            unit_logits<BF16, SBF16, ZEROS, G, NT>(acc, ring + stage * ring_bytes + j * w.unit_bytes, x + ku * (kUnitCols * 2), s.pitch, sums + ku * G * 8 * NT);
+            const unsigned char *unit = ring + stage * ring_bytes + j * w.unit_bytes;
+            if constexpr (INT) unit_logits_int<SBF16, ZEROS, G>(acc[0], unit, x + ku * kUnitCols, sums + ku * G * 8);
+            else unit_logits<SBF16, ZEROS, G, NT>(acc, unit, x + ku * (kUnitCols * 2), s.pitch, sums + ku * G * 8 * NT);
             left = true;
             if (++ku == per) {
                 if (own) {
-                    write_logits<NT>(p, acc, t0 + tile, 0);
+                    stream_write<NT, INT>(p, acc, t0 + tile, unscale);
                 } else {
 #pragma unroll
                     for (int m = 0; m < NT; m++) ((float4 *)slot)[m * 32 + lane] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
@@ -348,7 +490,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1) k_head_stream(const __gr
                 acc[m][0] += v.x; acc[m][1] += v.y; acc[m][2] += v.z; acc[m][3] += v.w;
             }
         }
-        write_logits<NT>(p, acc, t0 + tile, 0);
+        stream_write<NT, INT>(p, acc, t0 + tile, unscale);
     }
     if (dead_ != 0) {  // a wait has given up: the copies under way end, and the CTA's logits are NaN
         if (lane == 0)
@@ -362,38 +504,6 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1) k_head_stream(const __gr
             else ((float *)p.out)[r * p.out_stride + v] = __uint_as_float(0x7FFFFFFFu);
         }
     }
-}
-
-// More rows than the stream takes: blocks of 16 rows, each of which reads the weight.
-constexpr int kLogitsCols = 2048;  // columns of the hidden states that a CTA has in shared memory at a time
-constexpr int kLogitsPitch = kLogitsCols * 2 + 64;
-
-template <bool BF16, bool SBF16, bool ZEROS, int G, int NT>
-__global__ void __launch_bounds__(256) k_head_logits(const __grid_constant__ HeadLogits p)
-{
-    extern __shared__ __align__(128) unsigned char sm[];
-    float *sums = (float *)(sm + 8 * NT * kLogitsPitch);
-    const int lane = threadIdx.x & 31, tile = blockIdx.x * 8 + (threadIdx.x >> 5), r0 = blockIdx.y * 8 * NT;
-    const Head4 &w = p.w;
-    pdl_release();
-    pdl_wait();
-    float acc[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[n][i] = 0.f;
-    const unsigned char *x = sm + (lane >> 2) * kLogitsPitch + (lane & 3) * 16;
-    for (int k0 = 0; k0 < w.width; k0 += kLogitsCols) {
-        const int cols = min(kLogitsCols, w.units_per_tile * kUnitCols - k0);
-        __syncthreads();
-        stage_states<BF16, ZEROS, G, NT>(p, r0, k0, cols, sm, kLogitsPitch, sums);
-        if (tile >= w.tiles) continue;
-        const unsigned char *from = w.units + ((int64_t)tile * w.units_per_tile + k0 / kUnitCols) * w.unit_bytes;
-#pragma unroll 2
-        for (int u = 0; u < cols / kUnitCols; u++)
-            unit_logits<BF16, SBF16, ZEROS, G, NT>(acc, from + (int64_t)u * w.unit_bytes, x + u * kUnitCols * 2, kLogitsPitch, sums + u * G * 8 * NT);
-    }
-    if (tile < w.tiles) write_logits<NT>(p, acc, tile, r0);
 }
 
 // ---- host ----
@@ -432,54 +542,75 @@ static int head_pack(StgHandle h, const StgHeadPack *b, cudaStream_t stream)
     return STG_OK;
 }
 
-static StreamShape stream_shape(const HeadLogits &p, int nt, bool zeros, size_t most)
+// `chunk` 0: it does not fit.
+constexpr int kIntRows = 2;
+static StreamShape stream_shape(const Head4 &w, int rows, bool zeros, size_t most)
 {
+    const int nt = rows <= 8 ? 1 : 2;
+    const bool ints = rows <= kIntRows;
     StreamShape s;
     memset(&s, 0, sizeof(s));
-    const size_t cols = (size_t)p.w.units_per_tile * kUnitCols;
-    s.pitch = (int)(cols * 2 + 64);  // rows g and g + 1 of a fragment in different banks
+    const size_t cols = (size_t)w.units_per_tile * kUnitCols;
+    s.pitch = (int)(ints ? cols + 16 : cols * 2 + 64);  // rows g and g + 1 of a fragment in different banks
     s.sums = (size_t)8 * nt * s.pitch;
-    s.slots = s.sums + (zeros ? cols / p.w.group * 8 * nt * 4 : 0);
+    s.unscale = s.sums + (zeros ? cols / w.group * 8 * nt * 4 : 0);
+    s.slots = round_up(s.unscale + (size_t)8 * nt * 8, 16);
     s.bars = s.slots + (size_t)kStreamWarps * nt * 512;
     s.ring = round_up(s.bars + kStreamWarps * kStreamStages * 8, 128);
-    const size_t unit = (size_t)kStreamWarps * kStreamStages * p.w.unit_bytes;
+    const size_t unit = (size_t)kStreamWarps * kStreamStages * w.unit_bytes;
     s.chunk = s.ring + unit <= most ? (int)std::min<size_t>(4, (most - s.ring) / unit) : 0;
     s.smem = s.ring + s.chunk * unit;
     return s;
 }
 
-template <bool BF16, bool SBF16, bool ZEROS, int G>
-static cudaError_t launch_logits(StgHandle h, const HeadLogits &p, cudaStream_t stream)
+// Up to 32 rows stream, where 16 of them fit into shared memory beside the rings; more than 16 in two calls of half of them, each of which reads
+// the weight (17 x 4096 x 151,936: 2 x 97 us, stg_head_tiles.cu 207 with groups of 128, 333 with groups of 32).
+constexpr int kStreamRows = 32;
+static bool streams(StgHandle h, const Head4 &w, int rows, bool zeros)
 {
-    const int nt = p.rows <= 8 ? 1 : 2;
-    const StreamShape s = stream_shape(p, nt, ZEROS, h->smem_optin);
-    if (p.rows <= 16 && s.chunk > 0) {
-        void (*fn)(HeadLogits, StreamShape) = nt == 1 ? k_head_stream<BF16, SBF16, ZEROS, G, 1> : k_head_stream<BF16, SBF16, ZEROS, G, 2>;
-        const cudaError_t e = ensure_dynamic_smem((const void *)fn, s.smem);
-        return e != cudaSuccess ? e : launch_behind(fn, dim3((unsigned)std::min(h->sm_count, p.w.tiles)), kStreamWarps * 32, s.smem, stream, p, s);
-    }
-    const size_t smem = (size_t)8 * nt * (kLogitsPitch + (ZEROS ? kLogitsCols / 32 * 4 : 0));
-    void (*fn)(HeadLogits) = nt == 1 ? k_head_logits<BF16, SBF16, ZEROS, G, 1> : k_head_logits<BF16, SBF16, ZEROS, G, 2>;
-    const cudaError_t e = ensure_dynamic_smem((const void *)fn, smem);
-    return e != cudaSuccess ? e : launch_behind(fn, dim3((unsigned)(p.w.tiles + 7) / 8, (unsigned)(p.rows + 8 * nt - 1) / (8 * nt)), 256, smem, stream, p);
+    return rows <= kStreamRows && stream_shape(w, std::min(rows, 16), zeros, h->smem_optin).chunk > 0;
 }
 
-template <bool BF16, bool SBF16, bool ZEROS>
-static cudaError_t launch_logits_of(StgHandle h, const HeadLogits &p, cudaStream_t stream)
+template <bool SBF16, bool ZEROS, int G>
+static cudaError_t launch_stream(StgHandle h, const HeadLogits &p, cudaStream_t stream)
 {
-    return p.w.group == 32 ? launch_logits<BF16, SBF16, ZEROS, 4>(h, p, stream) : p.w.group == 64 ? launch_logits<BF16, SBF16, ZEROS, 2>(h, p, stream)
-                                                                                : launch_logits<BF16, SBF16, ZEROS, 1>(h, p, stream);
+    const StreamShape s = stream_shape(p.w, p.rows, ZEROS, h->smem_optin);
+    void (*fn)(HeadLogits, StreamShape) = p.rows <= kIntRows ? k_head_stream<SBF16, ZEROS, G, 1, true> : p.rows <= 8 ? k_head_stream<SBF16, ZEROS, G, 1, false>
+                                                                                                                    : k_head_stream<SBF16, ZEROS, G, 2, false>;
+    const cudaError_t e = ensure_dynamic_smem((const void *)fn, s.smem);
+    return e != cudaSuccess ? e : launch_behind(fn, dim3((unsigned)std::min(h->sm_count, p.w.tiles)), kStreamWarps * 32, s.smem, stream, p, s);
+}
+
+template <bool SBF16, bool ZEROS>
+static cudaError_t launch_stream_of(StgHandle h, const HeadLogits &p, cudaStream_t stream)
+{
+    return p.w.group == 32 ? launch_stream<SBF16, ZEROS, 4>(h, p, stream) : p.w.group == 64 ? launch_stream<SBF16, ZEROS, 2>(h, p, stream)
+                                                                                : launch_stream<SBF16, ZEROS, 1>(h, p, stream);
+}
+
+static int head_logits_check(StgHandle h, const StgHeadLogits *b, const char *who)
+{
+    const std::string at = std::string(who) + ": ";
+    if (!b || b->struct_size != (int32_t)sizeof(StgHeadLogits)) return fail(h, STG_ERR_INVALID_ARGUMENT, "bad StgHeadLogits");
+    const int rc = head4_check(h, who, b->vocab, b->width, b->group, b->scale_dtype);
+    if (rc) return rc;
+    if (b->rows < 0) return fail(h, STG_ERR_INVALID_ARGUMENT, at + "rows must be >= 0");
+    if (b->rows > (1 << 20)) return fail(h, STG_ERR_CAPACITY, at + "more than 2^20 rows");
+    if (b->hidden_dtype != STG_DTYPE_BF16 && b->hidden_dtype != STG_DTYPE_F16) return fail(h, STG_ERR_INVALID_ARGUMENT, at + "hidden_dtype must be STG_DTYPE_BF16 or STG_DTYPE_F16");
+    if (b->logits_dtype != STG_DTYPE_F32 && b->logits_dtype != STG_DTYPE_BF16) return fail(h, STG_ERR_INVALID_ARGUMENT, at + "logits_dtype must be STG_DTYPE_F32 or STG_DTYPE_BF16");
+    return STG_OK;
+}
+
+static size_t head_logits_workspace(StgHandle h, const StgHeadLogits *b)
+{
+    const Head4 w = head4_shape(b->vocab, b->width, b->group, b->has_zeros != 0);
+    return b->rows == 0 || streams(h, w, b->rows, b->has_zeros != 0) ? 0 : head_tiles_workspace(h, w, b->rows);
 }
 
 static int head_logits(StgHandle h, const StgHeadLogits *b, cudaStream_t stream)
 {
-    if (!b || b->struct_size != (int32_t)sizeof(StgHeadLogits)) return fail(h, STG_ERR_INVALID_ARGUMENT, "bad StgHeadLogits");
-    int rc = head4_check(h, "stg_head_logits", b->vocab, b->width, b->group, b->scale_dtype);
+    const int rc = head_logits_check(h, b, "stg_head_logits");
     if (rc) return rc;
-    if (b->rows < 0) return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_head_logits: rows must be >= 0");
-    if (b->rows > (1 << 20)) return fail(h, STG_ERR_CAPACITY, "stg_head_logits: more than 2^20 rows");
-    if (b->hidden_dtype != STG_DTYPE_BF16 && b->hidden_dtype != STG_DTYPE_F16) return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_head_logits: hidden_dtype must be STG_DTYPE_BF16 or STG_DTYPE_F16");
-    if (b->logits_dtype != STG_DTYPE_F32 && b->logits_dtype != STG_DTYPE_BF16) return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_head_logits: logits_dtype must be STG_DTYPE_F32 or STG_DTYPE_BF16");
     if (b->hidden_stride < b->width || b->row_stride < b->vocab) return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_head_logits: a row stride smaller than the row");
     if (b->rows == 0) return STG_OK;
     if (!b->packed || !b->hidden || !b->logits) return fail(h, STG_ERR_INVALID_ARGUMENT, "stg_head_logits: packed, hidden and logits are required");
@@ -492,14 +623,27 @@ static int head_logits(StgHandle h, const StgHeadLogits *b, cudaStream_t stream)
     p.w.units = (const unsigned char *)b->packed;
     p.hidden = (const uint16_t *)b->hidden; p.hidden_stride = b->hidden_stride;
     p.vec = !misaligned(b->hidden, 16) && (b->rows == 1 || b->hidden_stride % 8 == 0);
-    p.rows = b->rows; p.out = b->logits; p.out_stride = b->row_stride; p.out_bf16 = b->logits_dtype == STG_DTYPE_BF16;
+    p.rows = b->rows; p.hidden_bf16 = b->hidden_dtype == STG_DTYPE_BF16; p.out = b->logits; p.out_stride = b->row_stride; p.out_bf16 = b->logits_dtype == STG_DTYPE_BF16;
     const OnDevice on(h->cfg.device);
     CK(on.error);
-    using Launch = cudaError_t (*)(StgHandle, const HeadLogits &, cudaStream_t);
-    static const Launch launch[2][2][2] = {{{launch_logits_of<false, false, false>, launch_logits_of<false, false, true>}, {launch_logits_of<false, true, false>, launch_logits_of<false, true, true>}},
-                                           {{launch_logits_of<true, false, false>, launch_logits_of<true, false, true>}, {launch_logits_of<true, true, false>, launch_logits_of<true, true, true>}}};
-    CK(launch[b->hidden_dtype == STG_DTYPE_BF16][b->scale_dtype == STG_DTYPE_BF16][b->has_zeros != 0](h, p, stream));
-    h->stats.kernel_launches++;
+    if (!streams(h, p.w, p.rows, b->has_zeros != 0)) {
+        if (!b->workspace || misaligned(b->workspace, 256) || b->workspace_bytes < head_tiles_workspace(h, p.w, p.rows))
+            return fail(h, STG_ERR_CAPACITY, "stg_head_logits: workspace missing, not aligned to 256 bytes or smaller than stg_head_logits_workspace says");
+        const int rc2 = head_tiles(h, p, b->scale_dtype == STG_DTYPE_BF16, b->workspace, stream);
+        if (rc2) return rc2;
+    } else {
+        using Launch = cudaError_t (*)(StgHandle, const HeadLogits &, cudaStream_t);
+        static const Launch launch[2][2] = {{launch_stream_of<false, false>, launch_stream_of<false, true>}, {launch_stream_of<true, false>, launch_stream_of<true, true>}};
+        const int calls = (p.rows + 15) / 16, rows = p.rows, each = (rows + calls - 1) / calls;
+        for (int r = 0; r < rows; r += each) {
+            HeadLogits q = p;
+            q.rows = std::min(each, rows - r);
+            q.hidden += (int64_t)r * p.hidden_stride;
+            q.out = (char *)p.out + (int64_t)r * p.out_stride * (p.out_bf16 ? 2 : 4);
+            CK(launch[b->scale_dtype == STG_DTYPE_BF16][b->has_zeros != 0](h, q, stream));
+            h->stats.kernel_launches++;
+        }
+    }
     h->stats.calls++;
     return STG_OK;
 }
@@ -523,6 +667,18 @@ try {
 int stg_head_pack(StgHandle h, const StgHeadPack *pack, void *stream)
 try {
     return h ? stg::head_pack(h, pack, (cudaStream_t)stream) : STG_ERR_INVALID_ARGUMENT;
+} catch (const std::bad_alloc &) {
+    return STG_ERR_CAPACITY;
+}
+
+int stg_head_logits_workspace(StgHandle h, const StgHeadLogits *logits, uint64_t *out_bytes)
+try {
+    if (!h) return STG_ERR_INVALID_ARGUMENT;
+    const int rc = stg::head_logits_check(h, logits, "stg_head_logits_workspace");
+    if (rc) return rc;
+    if (!out_bytes) return stg::fail(h, STG_ERR_INVALID_ARGUMENT, "stg_head_logits_workspace: out_bytes is required");
+    *out_bytes = stg::head_logits_workspace(h, logits);
+    return STG_OK;
 } catch (const std::bad_alloc &) {
     return STG_ERR_CAPACITY;
 }

@@ -279,8 +279,8 @@ static int head_check_arrays(StgHandle h, const StgHeadLoss *b, const char *who,
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// A map of 16-bit rows: boxes of 64 columns (128 bytes, swizzled) by `box_rows` rows, zeros outside.
-static int head_map(StgHandle h, CUtensorMap *map, bool bf16, const void *p, int64_t columns, int64_t rows, int64_t stride, int box_rows)
+int head_map_of(StgHandle h, CUtensorMap *map, CUtensorMapDataType type, int dims, const void *p, const cuuint64_t *size, const cuuint64_t *stride, const cuuint32_t *box,
+                CUtensorMapSwizzle swizzle)
 {
     static const EncodeTiled encode = [] {
         void *fn = nullptr;
@@ -289,11 +289,18 @@ static int head_map(StgHandle h, CUtensorMap *map, bool bf16, const void *p, int
         return (EncodeTiled)fn;
     }();
     if (!encode) return fail(h, STG_ERR_CUDA, "cuTensorMapEncodeTiled is not there");
-    const cuuint64_t size[2] = {(cuuint64_t)columns, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, step[2] = {1, 1};
-    const CUresult e = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void *)p, size, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint32_t step[3] = {1, 1, 1};
+    const CUresult e = encode(map, type, (cuuint32_t)dims, (void *)p, size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return e == CUDA_SUCCESS ? STG_OK : fail(h, STG_ERR_CUDA, "cuTensorMapEncodeTiled failed with " + std::to_string((int)e));
+}
+
+// A map of 16-bit rows: boxes of 64 columns (128 bytes, swizzled) by `box_rows` rows.
+static int head_map(StgHandle h, CUtensorMap *map, bool bf16, const void *p, int64_t columns, int64_t rows, int64_t stride, int box_rows)
+{
+    const cuuint64_t size[2] = {(cuuint64_t)columns, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    return head_map_of(h, map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p, size, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int MODE>

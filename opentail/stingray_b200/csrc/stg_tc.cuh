@@ -19,6 +19,7 @@ __device__ __forceinline__ bool one_lane()
 // ---- mbarriers ----
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void bar_arrive_times(uint32_t bar, uint32_t n) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n) : "memory"); }
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes)
 {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -31,6 +32,15 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
     return done != 0u;
 }
 
+// The same, asleep for up to some ten microseconds: a loop of short tries takes issue slots and power from the warps that work.
+__device__ __forceinline__ bool bar_try_long(uint32_t bar, uint32_t parity)
+{
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
+    return done != 0u;
+}
+
 // Waits for the phase of this parity to end.  Bounded: after about two seconds, or when another of the CTA's waits has
 // given up (*dead), it returns false, and the caller leaves what it is doing.
 constexpr uint32_t kBarTries = 1u << 26;
@@ -40,8 +50,8 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     if (bar_try(bar, parity)) return true;
     const long long begin = clock64();
     for (uint32_t i = 0; i < kBarTries; i++) {
-        if (bar_try(bar, parity)) return true;
-        if ((i & 63u) == 63u && (*dead != 0 || clock64() - begin > kBarCycles)) break;
+        if (bar_try_long(bar, parity)) return true;
+        if (*dead != 0 || clock64() - begin > kBarCycles) break;
     }
     *dead = 1;
     return false;
@@ -60,6 +70,12 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, i
     else
         asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
                      "r"(x), "r"(y), "r"(bar) : "memory");
+}
+// The same of a three-dimensional map.
+__device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x),
+                 "r"(y), "r"(z), "r"(bar) : "memory");
 }
 // `bytes` from global memory, both 16-byte aligned and a multiple of 16 bytes.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
@@ -132,6 +148,26 @@ __device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t (&v)[16])
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
                    "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
                  : "r"(at));
+}
+__device__ __forceinline__ void tmem_load8(uint32_t at, uint32_t (&v)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(at));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&v)[32])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+                 "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+                 "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+                 "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// d (+)= a b with a in tensor memory: a row per lane, two elements to a column.
+__device__ __forceinline__ void tc_mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add)
+{
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+                 "r"((uint32_t)add) : "memory");
 }
 __device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 

@@ -646,18 +646,20 @@ class BatchSampler:
                              f"got {x.dtype} {tuple(shape)} on {x.device}")
         return x.data_ptr(), x.stride(0) if shape[0] > 1 else shape[1], dtype
 
-    def _head_workspace(self, b, backward: bool, stream):
-        """A call's own workspace, in the order of the stream that uses it; in a graph's memory where that stream is captured."""
+    def _head_workspace(self, key, ask, b, stream):
+        """A call's own workspace, in the order of the stream that uses it; in a graph's memory where that stream is captured.
+        ``key``: what its size depends on, which the library is asked for once."""
         import torch
 
-        key = (b.rows, b.vocab, b.width, backward)
         size = self._head_sizes.get(key)
-        if size is None:  # 3 us of a call
+        if size is None:
             n = C.c_uint64(0)
-            self._check(self._lib.stg_head_loss_workspace(self._h, C.byref(b), 1 if backward else 0, C.byref(n)))
+            self._check(ask(n))
             if len(self._head_sizes) > 1000:
                 self._head_sizes.clear()
             size = self._head_sizes[key] = int(n.value)
+        if size == 0:
+            return None
         dev = f"cuda:{self.device}"
         if stream is None:
             ws = torch.empty(size, dtype=torch.uint8, device=dev)
@@ -668,6 +670,10 @@ class BatchSampler:
                 ws = torch.empty(size, dtype=torch.uint8, device=dev)
         b.workspace, b.workspace_bytes = ws.data_ptr(), size
         return ws
+
+    def _loss_workspace(self, b, backward: bool, stream):
+        return self._head_workspace((b.rows, b.vocab, b.width, backward),
+                                    lambda n: self._lib.stg_head_loss_workspace(self._h, C.byref(b), 1 if backward else 0, C.byref(n)), b, stream)
 
     def _head_loss(self, hidden, weight, targets, softcap):
         import torch
@@ -692,7 +698,7 @@ class BatchSampler:
             out = {n: torch.empty(b.rows, dtype=torch.float32, device=hidden.device) for n in ("loss", "log_norms")}
         b.loss = self._beam_array("out['loss']", out["loss"], torch.float32, (b.rows,))
         b.log_norms = self._beam_array("out['log_norms']", out["log_norms"], torch.float32, (b.rows,))
-        ws = self._head_workspace(b, False, stream)  # noqa: F841 (held until the call is enqueued)
+        ws = self._loss_workspace(b, False, stream)  # noqa: F841 (held until the call is enqueued)
         self._check(self._lib.stg_head_loss(self._h, C.byref(b), self._stream_here(stream)))
         return out
 
@@ -720,7 +726,7 @@ class BatchSampler:
             out = {n: torch.empty(s, dtype=weight.dtype, device=weight.device) for n, s in shapes.items()}
         for n, s in shapes.items():
             setattr(b, n, self._beam_array(f"out[{n!r}]", out[n], weight.dtype, s))
-        ws = self._head_workspace(b, True, stream)  # noqa: F841
+        ws = self._loss_workspace(b, True, stream)  # noqa: F841
         self._check(self._lib.stg_head_loss_backward(self._h, C.byref(b), self._stream_here(stream)))
         return out
 
@@ -766,6 +772,8 @@ class BatchSampler:
         op, os_, od = self._head_rows("out", out, _logits_dtypes(), head.vocab)
         b = N.StgHeadLogits(C.sizeof(N.StgHeadLogits), rows, head.vocab, head.width, head.group, head.scale_dtype, 1 if head.has_zeros else 0, hd, od,
                             head.packed.data_ptr(), head.nbytes, hp, hs, op, os_)
+        ws = self._head_workspace((rows, head.vocab, head.width, head.group, head.has_zeros),  # noqa: F841
+                                  lambda n: self._lib.stg_head_logits_workspace(self._h, C.byref(b), C.byref(n)), b, stream)
         self._check(self._lib.stg_head_logits(self._h, C.byref(b), self._stream_here(stream)))
         return out
 
