@@ -34,7 +34,7 @@ struct HeadWs {
     float *hit;         // [padded rows]: the target's logit
     float2 *parts;      // [padded rows, two per tile of the vocabulary]: largest logit and the sum of exp relative to it
     void *grads;        // [padded rows, piece]: gradients of a piece's logits
-    float *sums;        // [splits, used rows up to whole tiles, width]: gradients of the hidden states so far
+    float *sums;        // [splits, used rows up to a multiple of kHeadTileM, width]: gradients of the hidden states so far
 };
 
 // A tensor map (stg_head_loss.cu): sizes and boxes from the innermost dimension on, strides in bytes between the others; zeros outside.

@@ -43,11 +43,9 @@ struct HeadGemm {
     float2 *parts;      // [rows, pieces]
     int pieces;
     float *hit;
-    void *grads;
-    int64_t grads_stride;
-    float *sums;
-    void *out;
+    void *out;          // where map_out's rows lie, and elements between them
     int64_t out_stride;
+    int a_rows;         // rows of the first operand's boxes: fewer than 128 where there are fewer rows
 };
 
 constexpr int kGemmEpiWarps = 8;
@@ -62,6 +60,7 @@ struct GemmRing {
     static constexpr int kStageBytes = kGemmABytes + kBBytes;
     static constexpr int kSmem = 1024 + kStages * kStageBytes;
 };
+constexpr int kGemmOut = 4096;                              // bytes that each of the eight warps writes its results from: 32 rows of 128 bytes
 constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ __forceinline__ float exp2_fast(float x)
@@ -115,7 +114,7 @@ struct HeadTile {
 
 template <int MODE, bool BF16, bool CAP, bool PAIR>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                                                               const __grid_constant__ HeadGemm g)
+                                                               const __grid_constant__ CUtensorMap map_out, const __grid_constant__ HeadGemm g)
 {
     using Ring = GemmRing<PAIR>;
     constexpr bool kAMn = MODE == kWeight, kBMn = MODE == kHidden || MODE == kWeight;
@@ -133,6 +132,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
     if (warp == 0 && one_lane()) {
         tma_prefetch(&map_a);
         tma_prefetch(&map_b);
+        if (MODE != kStats) tma_prefetch(&map_out);
         for (int i = 0; i < kStages; i++) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
         for (int i = 0; i < 2; i++) { bar_init(acc_full + 8 * i, 1); bar_init(acc_empty + 8 * i, kCtas * kGemmEpiWarps); }
         dead_ = 0;
@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
     const uint32_t tmem = tmem_slot;
     pdl_release();
     pdl_wait();
+    asm volatile("fence.proxy.async;" ::: "memory");  // what the kernels ahead have written is read by TMA
 
     const int used = MODE == kStats && g.targets ? g.used_rows : g.info->used;
     const int tiles_m = ((MODE == kWeight ? g.m : used) + kTileM - 1) / kTileM;
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
             uint32_t at = 0;  // stages filled so far
             bool ok = true;
             const int own_n = g.tile_n / kCtas, chunks = (own_n + 63) / 64;
-            const uint32_t bytes = kCtas * (kGemmABytes + (kBMn ? (uint32_t)chunks * 8192u : (uint32_t)own_n * 128u));
+            const uint32_t bytes = kCtas * ((kAMn ? kGemmABytes : (uint32_t)g.a_rows * 128u) + (kBMn ? (uint32_t)chunks * 8192u : (uint32_t)own_n * 128u));
             for (int t = first_tile; ok && t < tiles; t += step) {
                 const HeadTile tile(t, tiles_m, tiles_n, g.group, splits, blocks);
                 const int m0 = tile.m * kTileM + rank * kHeadTileM, n0 = tile.n * g.tile_n + rank * own_n;
@@ -228,6 +229,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
         const int chunks = g.tile_n / 16, c_begin = half == 0 ? 0 : (chunks + 1) / 2, c_end = half == 0 ? (chunks + 1) / 2 : chunks;  // 8 at most
         const float unscale = MODE == kWeight ? g.info->unscale : 1.f, scale = MODE == kGrad ? g.info->scale : 1.f;
         const uint32_t free_bar = PAIR ? cluster_at(acc_empty, 0) : acc_empty;
+        const uint32_t out = ring + kStages * Ring::kStageBytes + (warp - 2) * kGemmOut;
         const float by_cap = CAP ? 1.f / g.cap : 0.f;
         uint32_t unit = 0;
         bool ok = true;
@@ -253,6 +255,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                 unit++;
             };
             if constexpr (MODE == kStats) {
+                const bool rows_here = m0 + quarter * 32 < used;  // of this warp
                 const int target = r >= used ? -1 : g.targets ? g.targets[r] : g.rows[r].target;
                 float z[8][16];
                 for (int k0 = 0; k0 < blocks; k0 += kAccBlocks) {
@@ -260,7 +263,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                     if (!ok) break;
 #pragma unroll
                     for (int c = 0; c < 8; c++) {
-                        if (c_begin + c >= c_end) break;
+                        if (c_begin + c >= c_end || !rows_here) break;
                         HeadCols x;
                         tmem_load16(from + (c_begin + c) * 16, x.v);
                         tmem_loaded();
@@ -270,6 +273,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                     read_unit();
                 }
                 if (!ok) break;
+                if (!rows_here) continue;
                 float top = -CUDART_INF_F;
                 float most[4] = {top, top, top, top};
 #pragma unroll
@@ -292,68 +296,85 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                     for (int i = 0; i < 16; i++) sum[i & 3] += exp2_fast(fmaf(z[c][i], kLog2e, -ref));
                 if (r < used) g.parts[(int64_t)r * g.pieces + 2 * tn + half] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
             } else {
+                // what 128 bytes of a row hold goes through shared memory and out as a box of the warp's 32 rows
+                // (one row of tiles, whose widths are not whole boxes, has few gradients: each thread writes its own)
+                constexpr bool kDirect = MODE == kGrad && !PAIR;
+                constexpr int kOutCols = MODE == kHidden ? 32 : 64, kOutChunks = kOutCols / 16;
+                const int slab = (used + kHeadTileM - 1) / kHeadTileM * kHeadTileM;  // rows of a split
+                const int r0 = m0 + quarter * 32;
+                const bool rows_here = r0 < (MODE == kWeight ? g.m : MODE == kHidden ? slab : g.rows_pad) && (some || MODE != kHidden || g.first == 0);
                 HeadRow row = {};
-                if (MODE == kGrad && r < g.rows_pad) row = g.rows[r];
+                if (MODE == kGrad && rows_here) row = g.rows[r];
                 const uint32_t from = some ? full_unit() : 0u;
                 if (!ok) break;
-                for (int c = c_begin; c < c_end; c++) {
-                    const int col = n0 + c * 16;
-                    HeadCols x;
-                    if (some) {
-                        tmem_load16(from + c * 16, x.v);
-                        tmem_loaded();
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; i++) x.v[i] = 0u;
+                for (int c0 = c_begin; c0 < c_end && rows_here; c0 += kOutChunks) {
+                    if (n0 + c0 * 16 >= g.n) break;
+                    if (!kDirect) {
+                        if (lane == 0) store_read();
+                        __syncwarp();
                     }
-                    if (MODE == kGrad) {
-                        uint32_t o[8];
-                        float d[16];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            float slope = scale, z = x.f(i);
-                            if (CAP) {
-                                const float th = tanh_fast(z * by_cap);
-                                z = th * g.cap;
-                                slope *= 1.f - th * th;
+                    for (int c = 0; c < kOutChunks; c++) {
+                        const int col = n0 + (c0 + c) * 16;
+                        if (c0 + c >= c_end) break;
+                        HeadCols x;
+                        if (some) {
+                            tmem_load16(from + (c0 + c) * 16, x.v);
+                            tmem_loaded();
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; i++) x.v[i] = 0u;
+                        }
+                        const uint32_t to = out + lane * 128;  // its 16 bytes are exchanged as a 128-byte swizzle wants them
+                        if constexpr (MODE == kHidden) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) shared_store(to + (((4 * c + i) ^ (lane & 7)) << 4), x.v[4 * i], x.v[4 * i + 1], x.v[4 * i + 2], x.v[4 * i + 3]);
+                        } else {
+                            uint32_t o[8];
+                            if constexpr (MODE == kGrad) {
+                                float d[16];
+#pragma unroll
+                                for (int i = 0; i < 16; i++) {
+                                    float slope = scale, z = x.f(i);
+                                    if (CAP) {
+                                        const float th = tanh_fast(z * by_cap);
+                                        z = th * g.cap;
+                                        slope *= 1.f - th * th;
+                                    }
+                                    d[i] = row.a * exp2_fast(fmaf(z, kLog2e, -row.norm2));
+                                    if (g.first + col + i == row.target) d[i] -= row.b;
+                                    d[i] = r < used ? d[i] * slope : 0.f;
+                                }
+#pragma unroll
+                                for (int i = 0; i < 8; i++) o[i] = pack2<BF16>(d[2 * i], d[2 * i + 1]);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 8; i++) o[i] = pack2<BF16>(x.f(2 * i) * unscale, x.f(2 * i + 1) * unscale);
                             }
-                            d[i] = row.a * exp2_fast(fmaf(z, kLog2e, -row.norm2));
-                            if (g.first + col + i == row.target) d[i] -= row.b;
-                            d[i] = col + i < g.n ? d[i] * slope : 0.f;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 8; i++) o[i] = pack2<BF16>(d[2 * i], d[2 * i + 1]);
-                        if (r < g.rows_pad) {
-                            uint4 *to = (uint4 *)((uint16_t *)g.grads + (int64_t)r * g.grads_stride + col);
-                            to[0] = make_uint4(o[0], o[1], o[2], o[3]);
-                            to[1] = make_uint4(o[4], o[5], o[6], o[7]);
-                        }
-                    } else if (MODE == kHidden) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            if (col + 4 * i >= g.n || r >= used) break;  // width is a multiple of 8
-                            float4 *to = (float4 *)(g.sums + ((int64_t)tile.split * used + r) * g.n + col + 4 * i);
-                            float4 v = make_float4(x.f(4 * i), x.f(4 * i + 1), x.f(4 * i + 2), x.f(4 * i + 3));
-                            if (g.first > 0) {
-                                const float4 w = *to;
-                                v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+                            if constexpr (kDirect) {
+                                uint4 *at = (uint4 *)((uint16_t *)g.out + (int64_t)r * g.out_stride + col);
+                                at[0] = make_uint4(o[0], o[1], o[2], o[3]);
+                                at[1] = make_uint4(o[4], o[5], o[6], o[7]);
+                            } else {
+                                shared_store(to + (((2 * c) ^ (lane & 7)) << 4), o[0], o[1], o[2], o[3]);
+                                shared_store(to + (((2 * c + 1) ^ (lane & 7)) << 4), o[4], o[5], o[6], o[7]);
                             }
-                            *to = v;
                         }
-                    } else if (r < g.m) {
-#pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            if (col + 8 * i >= g.n) break;
-                            uint32_t o[4];
-#pragma unroll
-                            for (int j = 0; j < 4; j++) o[j] = pack2<BF16>(x.f(8 * i + 2 * j) * unscale, x.f(8 * i + 2 * j + 1) * unscale);
-                            *(uint4 *)((uint16_t *)g.out + (int64_t)(g.first + r) * g.out_stride + col + 8 * i) = make_uint4(o[0], o[1], o[2], o[3]);
-                        }
+                    }
+                    if (kDirect) continue;
+                    async_proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) {
+                        const int x = n0 + c0 * 16, y = (MODE == kWeight ? g.first : MODE == kHidden ? tile.split * slab : 0) + r0;
+                        if (MODE == kHidden && g.first > 0) tma_store<true>(&map_out, x, y, out);
+                        else tma_store<false>(&map_out, x, y, out);
+                        store_commit();
                     }
                 }
                 if (some) read_unit();
             }
         }
+        if (MODE != kStats && lane == 0) store_done();
     }
     __syncwarp();
     tc_fence_before();
@@ -367,9 +388,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
             for (int i = threadIdx.x; i < kHeadTileM * g.tile_n; i += kGemmThreads) {
                 const int r = tile.m * kTileM + (int)rank * kHeadTileM + i / g.tile_n, c = tile.n * g.tile_n + i % g.tile_n;
                 if (MODE == kStats && r < used && i % g.tile_n < 2) g.parts[(int64_t)r * g.pieces + 2 * tile.n + i % g.tile_n] = make_float2(0.f, CUDART_NAN_F);
-                if (MODE == kGrad && r < used && c < g.n) ((uint16_t *)g.grads)[(int64_t)r * g.grads_stride + c] = 0x7FFFu;
-                if (MODE == kHidden && r < used && c < g.n) g.sums[((int64_t)tile.split * used + r) * g.n + c] = CUDART_NAN_F;
-                if (MODE == kWeight && r < g.m && c < g.n) ((uint16_t *)g.out)[(int64_t)(g.first + r) * g.out_stride + c] = 0x7FFFu;
+                if (MODE == kHidden && r < used && c < g.n) ((float *)g.out)[((int64_t)tile.split * ((used + kHeadTileM - 1) / kHeadTileM * kHeadTileM) + r) * g.out_stride + c] = CUDART_NAN_F;
+                if ((MODE == kGrad && r < used && c < g.n) || (MODE == kWeight && r < g.m && c < g.n))
+                    ((uint16_t *)g.out)[(int64_t)((MODE == kWeight ? g.first : 0) + r) * g.out_stride + c] = 0x7FFFu;
             }
         }
     }

@@ -31,6 +31,7 @@ struct HeadPrep {
 };
 
 constexpr int kPrepThreads = 1024;
+constexpr int kMostSplits = 64;
 
 __global__ void __launch_bounds__(kPrepThreads) k_head_prep(const __grid_constant__ HeadPrep p)
 {
@@ -72,25 +73,26 @@ __global__ void __launch_bounds__(kPrepThreads) k_head_prep(const __grid_constan
     for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
     if (lane == 0) warp_most[w] = most;
     __syncthreads();
+    if (w == 1 && p.norms) {
+        // few tiles of the hidden states' gradients: pieces of the vocabulary are split, so that the tiles' parts fill the chip
+        const int tiles = (before + p.tile_m - 1) / p.tile_m * ((p.width + 255) / 256), slab = (before + kHeadTileM - 1) / kHeadTileM * kHeadTileM;
+        uint64_t least = ~0ull;
+        for (int n = lane + 1; n <= kMostSplits; n += 32)
+            if (n == 1 || (n <= p.blocks && (int64_t)n * slab <= p.sums_rows)) {
+                // waves of tiles times their blocks, and some six blocks' time for a tile's sums to be written and read
+                const uint32_t cost = (uint32_t)((tiles * n + p.workers - 1) / p.workers) * (uint32_t)((p.blocks + n - 1) / n + 6);
+                least = min(least, (uint64_t)cost << 32 | (uint32_t)n);
+            }
+        for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xFFFFFFFFu, least, o));
+        if (lane == 0) p.ws.info->splits = (int)(uint32_t)least;
+    }
     if (tid == 0) {
         for (int i = 1; i < 32; i++) most = fmaxf(most, warp_most[i]);
         // the largest factor comes to lie in [2^13, 2^14): a gradient of a logit is at most the sum of two, and fits
         // fp16, of whose range the small ones then use as much as there is
         int e = 0;
         if (most > 0.f && most < CUDART_INF_F) e = max(-110, min(110, 13 - ilogbf(most)));
-        // few tiles of the hidden states' gradients: pieces of the vocabulary are split, so that the tiles' parts fill the chip
-        int splits = 1;
-        if (p.norms && before > 0) {
-            const int tiles = (before + p.tile_m - 1) / p.tile_m * ((p.width + 255) / 256);
-            int64_t least = 1ll << 62;
-            for (int n = 1; n <= 64 && n <= p.blocks && (int64_t)n * before <= p.sums_rows; n++) {
-                // waves of tiles times their blocks, and some six blocks' time for a tile's sums to be written and read
-                const int64_t cost = (int64_t)((tiles * n + p.workers - 1) / p.workers) * ((p.blocks + n - 1) / n + 6);
-                if (cost < least) { least = cost; splits = n; }
-            }
-        }
         p.ws.info->used = before;
-        p.ws.info->splits = splits;
         p.ws.info->scale = exp2f((float)e);
         p.ws.info->unscale = exp2f((float)-e);
     }
@@ -132,56 +134,69 @@ __global__ void __launch_bounds__(128) k_head_join(const __grid_constant__ HeadW
         return;
     }
     const float2 *parts = ws.parts + (int64_t)at * pieces;
+    // each thread joins its own as they come; they are joined relative to the largest of all then
     float top = -CUDART_INF_F;
-    bool bad = false;
-    for (int i = tid; i < pieces; i += 128) {
-        top = fmaxf(top, parts[i].x);
-        bad |= parts[i].y != parts[i].y;
-    }
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    if ((tid & 31) == 0) tops[tid >> 5] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    double sum = bad ? (double)CUDART_NAN_F : 0.0;
+    double sum = 0.0;
+#pragma unroll 4
     for (int i = tid; i < pieces; i += 128) {
         const float2 v = parts[i];
-        if (v.x > -CUDART_INF_F) sum += (double)(v.y * expf(v.x - top));
+        if (v.x > top) {
+            sum = sum * (double)expf(top - v.x) + (double)v.y;
+            top = v.x;
+        } else {  // a NaN of either stays
+            sum += v.x > -CUDART_INF_F ? (double)(v.y * expf(v.x - top)) : (double)v.y;
+        }
     }
+    float all = top;
+    for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
+    if ((tid & 31) == 0) tops[tid >> 5] = all;
+    __syncthreads();
+    all = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    if (top > -CUDART_INF_F) sum *= (double)expf(top - all);
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     if ((tid & 31) == 0) sums[tid >> 5] = sum;
     __syncthreads();
     if (tid == 0) {
-        const double norm = (double)top + log(sums[0] + sums[1] + sums[2] + sums[3]);
+        const double norm = (double)all + log(sums[0] + sums[1] + sums[2] + sums[3]);
         norms[r] = (float)norm;
         loss[r] = (float)(norm - (double)ws.hit[at]);
     }
 }
 
-// Gradients of the hidden states: the splits' sums added up and rounded, back in their rows; zeros where a row has no loss.
+// Gradients of the hidden states: the splits' sums added up and rounded, back in their rows; zeros where a row has no loss.  A CTA has 256 columns
+// of a row, and eight threads share out the splits of each eight columns.
 template <bool BF16>
-__global__ void __launch_bounds__(128) k_head_spread(const __grid_constant__ HeadWs ws, int width, uint16_t *out)
+__global__ void __launch_bounds__(256) k_head_spread(const __grid_constant__ HeadWs ws, int width, uint16_t *out)
 {
+    __shared__ float4 parts[8][32][2];
     pdl_release();
     pdl_wait();
-    const int r = blockIdx.x, at = ws.place[r], splits = ws.info->splits;
+    const int r = blockIdx.x, at = ws.place[r], splits = ws.info->splits, tid = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.y * 256 + tid * 8;
     const float unscale = ws.info->unscale;
-    const int64_t slab = (int64_t)ws.info->used * width;
-    for (int i = threadIdx.x; i < width / 8; i += 128) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (at >= 0) {
-            const float *from = ws.sums + (int64_t)at * width + 8 * i;
-            float4 x = *(const float4 *)from, y = *(const float4 *)(from + 4);
+    const int64_t slab = (int64_t)((ws.info->used + kHeadTileM - 1) / kHeadTileM * kHeadTileM) * width;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+    if (at >= 0 && col < width) {
+        const float *from = ws.sums + (int64_t)at * width + col;
 #pragma unroll 4
-            for (int s = 1; s < splits; s++) {
-                const float4 u = *(const float4 *)(from + s * slab), w = *(const float4 *)(from + s * slab + 4);
-                x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
-                y.x += w.x; y.y += w.y; y.z += w.z; y.w += w.w;
-            }
-            v = make_uint4(pack2<BF16>(x.x * unscale, x.y * unscale), pack2<BF16>(x.z * unscale, x.w * unscale), pack2<BF16>(y.x * unscale, y.y * unscale),
-                           pack2<BF16>(y.z * unscale, y.w * unscale));
+        for (int s = w; s < splits; s += 8) {
+            const float4 u = *(const float4 *)(from + s * slab), v = *(const float4 *)(from + s * slab + 4);
+            x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
+            y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
         }
-        ((uint4 *)(out + (int64_t)r * width))[i] = v;
     }
+    if (splits > 1) {
+        parts[w][tid][0] = x;
+        parts[w][tid][1] = y;
+        __syncthreads();
+        for (int i = 1; w == 0 && i < min(8, splits); i++) {
+            const float4 u = parts[i][tid][0], v = parts[i][tid][1];
+            x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
+            y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
+        }
+    }
+    if (w == 0 && col < width)
+        *(uint4 *)(out + (int64_t)r * width + col) = make_uint4(pack2<BF16>(x.x * unscale, x.y * unscale), pack2<BF16>(x.z * unscale, x.w * unscale),
+                                                                pack2<BF16>(y.x * unscale, y.y * unscale), pack2<BF16>(y.z * unscale, y.w * unscale));
 }
 
 // ---- host ----
@@ -304,14 +319,15 @@ static int head_map(StgHandle h, CUtensorMap *map, bool bf16, const void *p, int
 }
 
 template <int MODE>
-static cudaError_t head_gemm(StgHandle h, bool bf16, bool pair, cudaStream_t stream, const CUtensorMap &a, const CUtensorMap &b, const HeadGemm &g, int64_t tiles)
+static cudaError_t head_gemm(StgHandle h, bool bf16, bool pair, cudaStream_t stream, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &out,
+                             const HeadGemm &g, int64_t tiles)
 {
-    using Kernel = void (*)(CUtensorMap, CUtensorMap, HeadGemm);
+    using Kernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, HeadGemm);
     constexpr bool C = MODE == kStats || MODE == kGrad;  // the others have no soft cap
     static const Kernel kernels[2][2][2] = {{{k_head_gemm<MODE, false, false, false>, k_head_gemm<MODE, false, false, true>}, {k_head_gemm<MODE, false, C, false>, k_head_gemm<MODE, false, C, true>}},
                                             {{k_head_gemm<MODE, true, false, false>, k_head_gemm<MODE, true, false, true>}, {k_head_gemm<MODE, true, C, false>, k_head_gemm<MODE, true, C, true>}}};
     const Kernel fn = kernels[bf16][g.cap != 0.f][pair];
-    const size_t smem = pair ? GemmRing<true>::kSmem : GemmRing<false>::kSmem;
+    const size_t smem = (pair ? GemmRing<true>::kSmem : GemmRing<false>::kSmem) + (MODE == kStats ? 0 : kGemmEpiWarps * kGemmOut);
     const cudaError_t e = ensure_dynamic_smem((const void *)fn, smem);
     if (e != cudaSuccess) return e;
     h->stats.kernel_launches++;
@@ -329,7 +345,7 @@ static cudaError_t head_gemm(StgHandle h, bool bf16, bool pair, cudaStream_t str
     cfg.stream = stream;
     cfg.attrs = at;
     cfg.numAttrs = pair ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, fn, a, b, g);
+    return cudaLaunchKernelEx(&cfg, fn, a, b, out, g);
 }
 
 static bool head_rows_aligned(const StgHeadLoss *b) { return !misaligned(b->hidden, 16) && (b->rows == 1 || b->hidden_stride % 8 == 0); }
@@ -349,11 +365,14 @@ static int head_begin(StgHandle h, const StgHeadLoss *b, const HeadWs &ws, const
 // 24.5 ms, 27.6 with all rows.
 constexpr int kGroupLogits = 16, kGroupGrads = 8;
 
+static int head_box_rows(int rows) { return std::min(kHeadTileM, (rows + 7) / 8 * 8); }
+
 static HeadGemm head_args(const StgHeadLoss *b, const HeadWs &ws, const HeadPlan &p)
 {
     HeadGemm g;
     memset(&g, 0, sizeof(g));
     g.info = ws.info; g.rows = ws.rows; g.rows_pad = p.rows_pad; g.tile_n = p.tile_n; g.group = kGroupLogits; g.cap = b->logit_softcap;
+    g.a_rows = head_box_rows(b->rows);
     return g;
 }
 
@@ -371,15 +390,15 @@ static int head_forward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
     // one row of tiles takes no less time for fewer rows: they are read where they are
     const bool direct = !p.pair && head_rows_aligned(b);
     CUtensorMap rows, weight;
-    if ((rc = direct ? head_map(h, &rows, bf16, b->hidden, b->width, b->rows, b->rows == 1 ? b->width : b->hidden_stride, kHeadTileM)
-                     : head_map(h, &rows, bf16, ws.hidden, b->width, p.rows_pad, b->width, kHeadTileM))) return rc;
+    if ((rc = direct ? head_map(h, &rows, bf16, b->hidden, b->width, b->rows, b->rows == 1 ? b->width : b->hidden_stride, head_box_rows(b->rows))
+                     : head_map(h, &rows, bf16, ws.hidden, b->width, p.rows_pad, b->width, head_box_rows(b->rows)))) return rc;
     if ((rc = head_map(h, &weight, bf16, b->weight, b->width, b->vocab, b->weight_stride, p.pair ? p.tile_n / 2 : p.tile_n))) return rc;
     if (!direct && (rc = head_begin(h, b, ws, p, false, stream))) return rc;
     HeadGemm g = head_args(b, ws, p);
     g.targets = direct ? b->targets : nullptr; g.used_rows = b->rows;
     g.n = b->vocab; g.k = b->width;
     g.parts = ws.parts; g.hit = ws.hit; g.pieces = 2 * p.tiles_n;
-    CK(head_gemm<kStats>(h, bf16, p.pair, stream, rows, weight, g, (int64_t)((b->rows + p.tile_m - 1) / p.tile_m) * p.tiles_n));
+    CK(head_gemm<kStats>(h, bf16, p.pair, stream, rows, weight, rows, g, (int64_t)((b->rows + p.tile_m - 1) / p.tile_m) * p.tiles_n));
     CK(launch_behind(k_head_join, dim3((unsigned)b->rows), 128, 0, stream, ws, 2 * p.tiles_n, g.targets, b->vocab, b->loss, b->log_norms));
     h->stats.kernel_launches++;
     h->stats.calls++;
@@ -404,10 +423,16 @@ static int head_backward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
     const HeadWs ws = head_layout(b, true, p, (char *)b->workspace);
     const bool bf16 = b->dtype == STG_DTYPE_BF16;
     CUtensorMap rows_k, weight_k, grads_k, weight_mn, grads_mn, rows_mn;  // how the operands' boxes of 64 columns are cut
-    if ((rc = head_map(h, &rows_k, bf16, ws.hidden, b->width, p.rows_pad, b->width, kHeadTileM))) return rc;
+    CUtensorMap grads_out, sums_out, weight_out;                          // results: boxes of 32 rows
+    if ((rc = head_map(h, &rows_k, bf16, ws.hidden, b->width, p.rows_pad, b->width, head_box_rows(b->rows)))) return rc;
     if ((rc = head_map(h, &weight_k, bf16, b->weight, b->width, b->vocab, b->weight_stride, p.pair ? p.tile_n / 2 : p.tile_n))) return rc;
     if ((rc = head_map(h, &weight_mn, bf16, b->weight, b->width, b->vocab, b->weight_stride, kGemmK))) return rc;
     if ((rc = head_map(h, &rows_mn, bf16, ws.hidden, b->width, p.rows_pad, b->width, kGemmK))) return rc;
+    if (b->grad_hidden) {
+        const cuuint64_t size[2] = {(cuuint64_t)b->width, (cuuint64_t)p.sums_rows}, stride[1] = {(cuuint64_t)b->width * 4};
+        const cuuint32_t box[2] = {32, 32};
+        if ((rc = head_map_of(h, &sums_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, ws.sums, size, stride, box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+    }
     if ((rc = head_begin(h, b, ws, p, true, stream))) return rc;
     const int64_t tiles_m = (b->rows + p.tile_m - 1) / p.tile_m, tiles_w = (b->width + 255) / 256;
     for (int i = 0; i < p.pieces; i++) {
@@ -415,25 +440,27 @@ static int head_backward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
         // what lies behind the piece's columns is read as zeros
         if ((rc = head_map(h, &grads_k, bf16, ws.grads, count, p.rows_pad, p.grads_stride, kHeadTileM))) return rc;
         if ((rc = head_map(h, &grads_mn, bf16, ws.grads, count, p.rows_pad, p.grads_stride, kGemmK))) return rc;
+        if ((rc = head_map(h, &grads_out, bf16, ws.grads, count, p.rows_pad, p.grads_stride, 32))) return rc;
         HeadGemm g = head_args(b, ws, p);
         g.first = first;
         g.n = count; g.k = b->width;
-        g.grads = ws.grads; g.grads_stride = p.grads_stride;
-        CK(head_gemm<kGrad>(h, bf16, p.pair, stream, rows_k, weight_k, g, tiles_m * ((count + p.tile_n - 1) / p.tile_n)));
+        g.out = ws.grads; g.out_stride = p.grads_stride;
+        CK(head_gemm<kGrad>(h, bf16, p.pair, stream, rows_k, weight_k, grads_out, g, tiles_m * ((count + p.tile_n - 1) / p.tile_n)));
         g.n = b->width; g.tile_n = 256; g.group = kGroupGrads; g.cap = 0.f;
         if (b->grad_hidden) {
-            g.k = count;
-            g.sums = ws.sums;
-            CK(head_gemm<kHidden>(h, bf16, p.pair, stream, grads_k, weight_mn, g, tiles_m * tiles_w * 64));
+            g.k = count; g.a_rows = kHeadTileM;
+            g.out = ws.sums; g.out_stride = b->width;
+            CK(head_gemm<kHidden>(h, bf16, p.pair, stream, grads_k, weight_mn, sums_out, g, tiles_m * tiles_w * 64));
         }
         if (b->grad_weight) {
             g.m = count;
             g.out = b->grad_weight; g.out_stride = b->width;
-            CK(head_gemm<kWeight>(h, bf16, p.pair, stream, grads_mn, rows_mn, g, (int64_t)((count + p.tile_m - 1) / p.tile_m) * tiles_w));
+            if ((rc = head_map(h, &weight_out, bf16, b->grad_weight, b->width, first + count, b->width, 32))) return rc;
+            CK(head_gemm<kWeight>(h, bf16, p.pair, stream, grads_mn, rows_mn, weight_out, g, (int64_t)((count + p.tile_m - 1) / p.tile_m) * tiles_w));
         }
     }
     if (b->grad_hidden) {
-        CK(launch_behind(bf16 ? k_head_spread<true> : k_head_spread<false>, dim3((unsigned)b->rows), 128, 0, stream, ws, b->width, (uint16_t *)b->grad_hidden));
+        CK(launch_behind(bf16 ? k_head_spread<true> : k_head_spread<false>, dim3((unsigned)b->rows, (unsigned)(b->width + 255) / 256), 256, 0, stream, ws, b->width, (uint16_t *)b->grad_hidden));
         h->stats.kernel_launches++;
     }
     h->stats.calls++;
