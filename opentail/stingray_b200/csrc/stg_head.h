@@ -6,14 +6,14 @@
 
 #include "../../../include/stingray_sampler.h"
 #include "stg_handle.h"
+#include "stg_head_plan.h"
 
 namespace stg {
 
-constexpr int kHeadTileM = 128;
-
 // What the preparation of a call finds out, in device memory.
 struct HeadInfo {
-    int32_t used;       // rows that have a loss
+    int32_t used;       // rows that have a loss, and those of their remainders
+    int32_t low;        // backward: how many rows there are ahead of the remainders', or 0: there are none
     int32_t splits;     // backward: parts of a piece of the vocabulary whose gradients of the hidden states are kept apart
     float scale;        // power of two that the logits' gradients are multiplied with where they are rounded to 16 bits
     float unscale;      // its inverse
@@ -24,6 +24,7 @@ struct HeadRow {
     int32_t row, target;
     float norm2;        // log2(e) * its normaliser
     float a, b;         // the gradient of logit v is a * softmax[v] - b * [v == target]
+    int32_t low;        // != 0: the row of what rounding to 16 bits takes from another one's gradients
 };
 
 struct HeadWs {
@@ -31,7 +32,9 @@ struct HeadWs {
     HeadRow *rows;      // [padded rows]
     int32_t *place;     // [rows]: its place among the used rows, -1: no loss, -2: its target lies outside the vocabulary
     void *hidden;       // [padded rows, width]: hidden states of the used rows
-    float *hit;         // [padded rows]: the target's logit
+    float *hit;         // [padded rows]: the target's logit; backward: what rounding takes from its gradient
+    int32_t *first;     // backward, more than 64 rows: [vocab]: the last of the used rows with this target, -1: none; and
+    int32_t *next;      // [padded rows]: the one ahead of it with the same target
     float2 *parts;      // [padded rows, two per tile of the vocabulary]: largest logit and the sum of exp relative to it
     void *grads;        // [padded rows, piece]: gradients of a piece's logits
     float *sums;        // [splits, used rows up to a multiple of kHeadTileM, width]: gradients of the hidden states so far

@@ -5,7 +5,7 @@
 //   kHidden  gradients of the hidden states += gradients weight, over a piece of the vocabulary, in fp32
 //   kWeight  gradients of the weight = gradients^T hidden, for a piece of the vocabulary, rounded once
 //
-// Persistent pairs of CTAs take tiles of 256 x 256 (PAIR; up to 128 rows: single CTAs take tiles of 128 x tile_n).  Each CTA loads 64 columns
+// Persistent pairs of CTAs take tiles of 256 x tile_n (PAIR; up to 128 rows: single CTAs take tiles of 128 x tile_n).  Each CTA loads 64 columns
 // of its 128 rows of the one operand and of its half of the other at a time by TMA, into a ring of six stages; one thread of the pair
 // issues tcgen05.mma into one of two accumulators in tensor memory, and eight warps of each CTA work on the other one meanwhile: a
 // thread has one row.  Operands lie in shared memory with their rows along K (hidden, weight, gradients) or along M or N
@@ -25,8 +25,6 @@
 
 namespace stg {
 
-enum HeadMode { kStats = 0, kGrad = 1, kHidden = 2, kWeight = 3 };
-
 struct HeadGemm {
     HeadInfo *info;
     const HeadRow *rows;
@@ -45,22 +43,15 @@ struct HeadGemm {
     float *hit;
     void *out;          // where map_out's rows lie, and elements between them
     int64_t out_stride;
+    const int32_t *first_of, *next;  // kWeight: HeadWs, or NULL
+    const uint16_t *hidden;       // kWeight: [rows, n]
     int a_rows;         // rows of the first operand's boxes: fewer than 128 where there are fewer rows
+    int stages, stage_bytes;  // the second operand's boxes ahead of the first's
+    int a_at;
 };
 
-constexpr int kGemmEpiWarps = 8;
 constexpr int kAccBlocks = 16;
 constexpr int kGemmThreads = 64 + 32 * kGemmEpiWarps;
-constexpr int kGemmK = 64;                                  // columns of a stage: 128 bytes, the swizzle's width
-constexpr int kGemmABytes = kHeadTileM * kGemmK * 2;
-template <bool PAIR>
-struct GemmRing {
-    static constexpr int kStages = PAIR ? 6 : 4;
-    static constexpr int kBBytes = (PAIR ? 128 : 256) * kGemmK * 2;
-    static constexpr int kStageBytes = kGemmABytes + kBBytes;
-    static constexpr int kSmem = 1024 + kStages * kStageBytes;
-};
-constexpr int kGemmOut = 4096;                              // bytes that each of the eight warps writes its results from: 32 rows of 128 bytes
 constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ __forceinline__ float exp2_fast(float x)
@@ -77,6 +68,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
     if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+}
+
+template <bool BF16>
+__device__ __forceinline__ float half_of(uint32_t x)  // its lower half
+{
+    return BF16 ? __uint_as_float(x << 16) : __half2float(__ushort_as_half((unsigned short)x));
 }
 
 // Sixteen accumulators of a row.
@@ -116,16 +113,15 @@ template <int MODE, bool BF16, bool CAP, bool PAIR>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                const __grid_constant__ CUtensorMap map_out, const __grid_constant__ HeadGemm g)
 {
-    using Ring = GemmRing<PAIR>;
     constexpr bool kAMn = MODE == kWeight, kBMn = MODE == kHidden || MODE == kWeight;
-    constexpr int kStages = Ring::kStages, kCtas = PAIR ? 2 : 1, kTileM = kCtas * kHeadTileM;
+    constexpr int kCtas = PAIR ? 2 : 1, kTileM = kCtas * kHeadTileM;
     extern __shared__ unsigned char raw[];
-    __shared__ alignas(8) uint64_t bars[2 * kStages + 4];
+    __shared__ alignas(8) uint64_t bars[2 * kGemmStages + 4];
     __shared__ uint32_t tmem_slot;
     __shared__ int dead_;
     volatile int *dead = &dead_;
     const uint32_t ring = (smem_at(raw) + 1023u) & ~1023u;
-    const uint32_t full = smem_at(bars), empty = full + 8 * kStages, acc_full = empty + 8 * kStages, acc_empty = acc_full + 16;
+    const uint32_t full = smem_at(bars), empty = full + 8 * kGemmStages, acc_full = empty + 8 * kGemmStages, acc_empty = acc_full + 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? cluster_rank() : 0u;
 
@@ -133,7 +129,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
         tma_prefetch(&map_a);
         tma_prefetch(&map_b);
         if (MODE != kStats) tma_prefetch(&map_out);
-        for (int i = 0; i < kStages; i++) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
+        for (int i = 0; i < g.stages; i++) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
         for (int i = 0; i < 2; i++) { bar_init(acc_full + 8 * i, 1); bar_init(acc_empty + 8 * i, kCtas * kGemmEpiWarps); }
         dead_ = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -160,18 +156,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
 
     if (warp == 0) {
         if (one_lane()) {
-            uint32_t at = 0;  // stages filled so far
+            uint32_t loaded = 0, phase = 1;
+            int s = 0;
             bool ok = true;
             const int own_n = g.tile_n / kCtas, chunks = (own_n + 63) / 64;
             const uint32_t bytes = kCtas * ((kAMn ? kGemmABytes : (uint32_t)g.a_rows * 128u) + (kBMn ? (uint32_t)chunks * 8192u : (uint32_t)own_n * 128u));
             for (int t = first_tile; ok && t < tiles; t += step) {
                 const HeadTile tile(t, tiles_m, tiles_n, g.group, splits, blocks);
                 const int m0 = tile.m * kTileM + rank * kHeadTileM, n0 = tile.n * g.tile_n + rank * own_n;
-                for (int kb = tile.begin; kb < tile.end; kb++, at++) {
-                    const uint32_t s = at % kStages;
-                    ok = bar_wait(empty + 8 * s, ((at / kStages) & 1u) ^ 1u, dead);
+                for (int kb = tile.begin; kb < tile.end; kb++, loaded++) {
+                    ok = bar_wait(empty + 8 * s, phase, dead);
                     if (!ok) break;
-                    const uint32_t a = ring + s * Ring::kStageBytes, b = a + kGemmABytes;
+                    const uint32_t b = ring + s * g.stage_bytes, a = b + g.a_at;
                     const uint32_t bar = PAIR ? cluster_at(full + 8 * s, 0) : full + 8 * s;  // both CTAs' bytes count on the first one's barrier
                     const int k0 = kb * kGemmK;
                     if (rank == 0) bar_expect(full + 8 * s, bytes);
@@ -186,17 +182,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                     } else {
                         tma_load<PAIR>(b, &map_b, k0, g.first + n0, bar);
                     }
+                    if (++s == g.stages) { s = 0; phase ^= 1u; }
                 }
             }
             // copies in flight end before the CTA does
-            for (uint32_t i = at < kStages ? 0 : at - kStages; rank == 0 && i < at; i++)
-                for (uint32_t j = 0; j < (1u << 20) && !bar_try(full + 8 * (i % kStages), (i / kStages) & 1u); j++) {}
+            const uint32_t n = (uint32_t)g.stages;
+            for (uint32_t i = loaded < n ? 0 : loaded - n; rank == 0 && i < loaded; i++)
+                for (uint32_t j = 0; j < (1u << 20) && !bar_try(full + 8 * (i % n), (i / n) & 1u); j++) {}
         }
     } else if (warp == 1) {
         if (rank == 0 && one_lane()) {
             const uint32_t idesc = tc_idesc(BF16, kAMn, kBMn, kTileM, (uint32_t)g.tile_n);
             const uint64_t da = tc_desc_base(kAMn ? 8192u : 16u), db = tc_desc_base(kBMn ? 8192u : 16u);
-            uint32_t at = 0, unit = 0;
+            uint32_t at = 0, unit = 0, phase = 0;
+            int s = 0;
             bool ok = true;
             for (int t = first_tile; ok && t < tiles; t += step) {
                 const HeadTile tile(t, tiles_m, tiles_n, g.group, splits, blocks);
@@ -207,32 +206,41 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                     if (!ok) break;
                     tc_fence_after();
                     for (int kb = k0; kb < k1; kb++, at++) {
-                        const uint32_t s = at % kStages;
-                        ok = bar_wait(full + 8 * s, (at / kStages) & 1u, dead);
+                        ok = bar_wait(full + 8 * s, phase, dead);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t a = ring + s * Ring::kStageBytes, b = a + kGemmABytes;
+                        const uint32_t b = ring + s * g.stage_bytes, a = b + g.a_at;
 #pragma unroll
                         for (int k = 0; k < kGemmK / 16; k++)
                             tc_mma<PAIR>(tmem + acc * 256, tc_desc(da, a + k * (kAMn ? 2048 : 32)), tc_desc(db, b + k * (kBMn ? 2048 : 32)), idesc, kb > k0 || k > 0);
                         tc_commit<PAIR>(empty + 8 * s);
+                        if (++s == g.stages) { s = 0; phase ^= 1u; }
                     }
                     if (ok) tc_commit<PAIR>(acc_full + 8 * acc);
                 }
             }
             // what was issued ends before tensor memory is given back: the last commits arrive on `empty`
-            for (uint32_t i = at < kStages ? 0 : at - kStages; i < at; i++)
-                for (uint32_t j = 0; j < (1u << 20) && !bar_try(empty + 8 * (i % kStages), (i / kStages) & 1u); j++) {}
+            const uint32_t n = (uint32_t)g.stages;
+            for (uint32_t i = at < n ? 0 : at - n; i < at; i++)
+                for (uint32_t j = 0; j < (1u << 20) && !bar_try(empty + 8 * (i % n), (i / n) & 1u); j++) {}
         }
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         const int chunks = g.tile_n / 16, c_begin = half == 0 ? 0 : (chunks + 1) / 2, c_end = half == 0 ? (chunks + 1) / 2 : chunks;  // 8 at most
         const float unscale = MODE == kWeight ? g.info->unscale : 1.f, scale = MODE == kGrad ? g.info->scale : 1.f;
         const uint32_t free_bar = PAIR ? cluster_at(acc_empty, 0) : acc_empty;
-        const uint32_t out = ring + kStages * Ring::kStageBytes + (warp - 2) * kGemmOut;
-        const float by_cap = CAP ? 1.f / g.cap : 0.f;
+        const uint32_t out = ring + kGemmRingBytes + (warp - 2) * kGemmOut;
+        const float by_cap = CAP ? fminf(1.f / g.cap, 3.0e38f) : 0.f;  // a cap of almost nothing: 0 stays 0
         uint32_t unit = 0;
         bool ok = true;
+        // kWeight: the last row whose target this thread's entry of a tile is
+        const bool links = MODE == kWeight && g.first_of && g.info->low == 0;
+        auto link_of = [&](int t) {
+            if (t >= tiles) return -1;
+            const int entry = HeadTile(t, tiles_m, tiles_n, g.group, splits, blocks).m * kTileM + (int)rank * kHeadTileM + quarter * 32 + lane;
+            return entry < g.m ? g.first_of[g.first + entry] : -1;
+        };
+        int next_link = links ? link_of(first_tile) : -1;
         for (int t = first_tile; ok && t < tiles; t += step) {
             const HeadTile tile(t, tiles_m, tiles_n, g.group, splits, blocks);
             const int m0 = tile.m * kTileM + rank * kHeadTileM, tn = tile.n, n0 = tn * g.tile_n;
@@ -298,70 +306,109 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
             } else {
                 // what 128 bytes of a row hold goes through shared memory and out as a box of the warp's 32 rows
                 // (one row of tiles, whose widths are not whole boxes, has few gradients: each thread writes its own)
-                constexpr bool kDirect = MODE == kGrad && !PAIR;
+                const bool direct = MODE == kGrad && (!PAIR || g.tile_n != 256);
                 constexpr int kOutCols = MODE == kHidden ? 32 : 64, kOutChunks = kOutCols / 16;
                 const int slab = (used + kHeadTileM - 1) / kHeadTileM * kHeadTileM;  // rows of a split
                 const int r0 = m0 + quarter * 32;
                 const bool rows_here = r0 < (MODE == kWeight ? g.m : MODE == kHidden ? slab : g.rows_pad) && (some || MODE != kHidden || g.first == 0);
                 HeadRow row = {};
                 if (MODE == kGrad && rows_here) row = g.rows[r];
+                int link = -1;
+                if (MODE == kWeight && links) {  // read a tile ahead
+                    link = next_link;
+                    next_link = link_of(t + step);
+                }
+                const bool linked = MODE == kWeight && __any_sync(0xFFFFFFFFu, link >= 0);
                 const uint32_t from = some ? full_unit() : 0u;
                 if (!ok) break;
                 for (int c0 = c_begin; c0 < c_end && rows_here; c0 += kOutChunks) {
                     if (n0 + c0 * 16 >= g.n) break;
-                    if (!kDirect) {
+                    // all of a box's columns on their way before the first is waited for, and the last box's shared memory waited for last
+                    HeadCols x[kOutChunks];
+#pragma unroll
+                    for (int c = 0; c < kOutChunks; c++) {
+                        if (some && c0 + c < c_end) {
+                            tmem_load16(from + (c0 + c) * 16, x[c].v);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; i++) x[c].v[i] = 0u;
+                        }
+                    }
+                    if (some) tmem_loaded();
+                    if (MODE == kWeight && linked) {  // what rounding has taken from the gradients of the rows whose target this is
+                        for (int q = link; q >= 0; q = g.next[q]) {
+                            const float rest = g.hit[q];
+                            const uint16_t *h = g.hidden + (int64_t)q * g.n + n0 + c0 * 16;
+#pragma unroll
+                            for (int c = 0; c < 2 * kOutChunks; c++) {
+                                if (n0 + c0 * 16 + 8 * c >= g.n) break;
+                                const uint4 e = ((const uint4 *)h)[c];
+                                const uint32_t w[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+                                for (int i = 0; i < 8; i++)
+                                    x[c / 2].v[8 * (c & 1) + i] = __float_as_uint(fmaf(rest, half_of<BF16>(w[i / 2] >> (16 * (i & 1))), x[c / 2].f(8 * (c & 1) + i)));
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    uint32_t o[kOutChunks][MODE == kHidden ? 1 : 8];
+#pragma unroll
+                    for (int c = 0; c < kOutChunks; c++) {
+                        const int col = n0 + (c0 + c) * 16;
+                        if constexpr (MODE == kGrad) {
+                            float d[16];
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                float slope = scale, z = x[c].f(i);
+                                if (CAP) {
+                                    const float th = tanh_fast(z * by_cap);
+                                    z = th * g.cap;
+                                    slope *= 1.f - th * th;
+                                }
+                                d[i] = row.a * exp2_fast(fmaf(z, kLog2e, -row.norm2));
+                                if (g.first + col + i == row.target) d[i] -= row.b;
+                                d[i] = r < used ? d[i] * slope : 0.f;
+                            }
+                            const unsigned at = (unsigned)(row.target - g.first - col);
+                            if (at < 16u && r < used && c0 + c < c_end) {
+                                float hit = 0.f;
+#pragma unroll
+                                for (int i = 0; i < 16; i++) hit = at == (unsigned)i ? d[i] : hit;
+                                g.hit[r] = hit - (BF16 ? __bfloat162float(__float2bfloat16_rn(hit)) : __half2float(__float2half_rn(hit)));
+                            }
+                            if (row.low != 0) {
+#pragma unroll
+                                for (int i = 0; i < 16; i++) d[i] -= BF16 ? __bfloat162float(__float2bfloat16_rn(d[i])) : __half2float(__float2half_rn(d[i]));
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; i++) o[c][i] = pack2<BF16>(d[2 * i], d[2 * i + 1]);
+                        } else if constexpr (MODE == kWeight) {
+#pragma unroll
+                            for (int i = 0; i < 8; i++) o[c][i] = pack2<BF16>(x[c].f(2 * i) * unscale, x[c].f(2 * i + 1) * unscale);
+                        }
+                    }
+                    if (!direct) {
                         if (lane == 0) store_read();
                         __syncwarp();
                     }
 #pragma unroll
                     for (int c = 0; c < kOutChunks; c++) {
-                        const int col = n0 + (c0 + c) * 16;
-                        if (c0 + c >= c_end) break;
-                        HeadCols x;
-                        if (some) {
-                            tmem_load16(from + (c0 + c) * 16, x.v);
-                            tmem_loaded();
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 16; i++) x.v[i] = 0u;
-                        }
                         const uint32_t to = out + lane * 128;  // its 16 bytes are exchanged as a 128-byte swizzle wants them
                         if constexpr (MODE == kHidden) {
 #pragma unroll
-                            for (int i = 0; i < 4; i++) shared_store(to + (((4 * c + i) ^ (lane & 7)) << 4), x.v[4 * i], x.v[4 * i + 1], x.v[4 * i + 2], x.v[4 * i + 3]);
+                            for (int i = 0; i < 4; i++) shared_store(to + (((4 * c + i) ^ (lane & 7)) << 4), x[c].v[4 * i], x[c].v[4 * i + 1], x[c].v[4 * i + 2], x[c].v[4 * i + 3]);
+                        } else if (direct) {
+                            if (c0 + c < c_end) {
+                                uint4 *at = (uint4 *)((uint16_t *)g.out + (int64_t)r * g.out_stride + n0 + (c0 + c) * 16);
+                                at[0] = make_uint4(o[c][0], o[c][1], o[c][2], o[c][3]);
+                                at[1] = make_uint4(o[c][4], o[c][5], o[c][6], o[c][7]);
+                            }
                         } else {
-                            uint32_t o[8];
-                            if constexpr (MODE == kGrad) {
-                                float d[16];
-#pragma unroll
-                                for (int i = 0; i < 16; i++) {
-                                    float slope = scale, z = x.f(i);
-                                    if (CAP) {
-                                        const float th = tanh_fast(z * by_cap);
-                                        z = th * g.cap;
-                                        slope *= 1.f - th * th;
-                                    }
-                                    d[i] = row.a * exp2_fast(fmaf(z, kLog2e, -row.norm2));
-                                    if (g.first + col + i == row.target) d[i] -= row.b;
-                                    d[i] = r < used ? d[i] * slope : 0.f;
-                                }
-#pragma unroll
-                                for (int i = 0; i < 8; i++) o[i] = pack2<BF16>(d[2 * i], d[2 * i + 1]);
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 8; i++) o[i] = pack2<BF16>(x.f(2 * i) * unscale, x.f(2 * i + 1) * unscale);
-                            }
-                            if constexpr (kDirect) {
-                                uint4 *at = (uint4 *)((uint16_t *)g.out + (int64_t)r * g.out_stride + col);
-                                at[0] = make_uint4(o[0], o[1], o[2], o[3]);
-                                at[1] = make_uint4(o[4], o[5], o[6], o[7]);
-                            } else {
-                                shared_store(to + (((2 * c) ^ (lane & 7)) << 4), o[0], o[1], o[2], o[3]);
-                                shared_store(to + (((2 * c + 1) ^ (lane & 7)) << 4), o[4], o[5], o[6], o[7]);
-                            }
+                            shared_store(to + (((2 * c) ^ (lane & 7)) << 4), o[c][0], o[c][1], o[c][2], o[c][3]);
+                            shared_store(to + (((2 * c + 1) ^ (lane & 7)) << 4), o[c][4], o[c][5], o[c][6], o[c][7]);
                         }
                     }
-                    if (kDirect) continue;
+                    if (direct) continue;
                     async_proxy_fence();
                     __syncwarp();
                     if (lane == 0) {

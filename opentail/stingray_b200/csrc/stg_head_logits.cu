@@ -67,16 +67,22 @@ __global__ void __launch_bounds__(256) k_head_pack(const __grid_constant__ HeadP
 
 // Eight codes of a word as the four registers of an fp16 A fragment, q - 8 each.  A code, its highest bit turned back, is put below
 // the bits of 1024, plain or times 16, and what is too much is taken off; all of it is exact.
-__device__ __forceinline__ void codes_to_a(uint32_t w, uint32_t (&a)[4])
+struct CodeBits {  // held in registers: an instruction has room for one constant at most
+    uint32_t low, high, low_base, high_base, low_less, high_less, sixteenth;
+    __device__ __forceinline__ CodeBits()
+    {
+        asm volatile("mov.b32 %0, 0x000F000F;\nmov.b32 %1, 0x00F000F0;\nmov.b32 %2, 0x64086408;\nmov.b32 %3, 0x64806480;" : "=r"(low), "=r"(high), "=r"(low_base), "=r"(high_base));
+        asm volatile("mov.b32 %0, 0xE408E408;\nmov.b32 %1, 0xD480D480;\nmov.b32 %2, 0x2C002C00;" : "=r"(low_less), "=r"(high_less), "=r"(sixteenth));  // -1032, -72, 1/16
+    }
+};
+__device__ __forceinline__ void codes_to_a(const CodeBits &k, uint32_t w, uint32_t (&a)[4])
 {
-    const uint32_t sixteenth = 0x2C002C00u, low = 0xE408E408u, high = 0xD480D480u;  // 1/16, -1032, -72
     const uint32_t u = w >> 8;
-    const uint32_t v0 = bits_of(w, 0x000F000Fu, 0x64086408u), v1 = bits_of(w, 0x00F000F0u, 0x64806480u);
-    const uint32_t v2 = bits_of(u, 0x000F000Fu, 0x64086408u), v3 = bits_of(u, 0x00F000F0u, 0x64806480u);
-    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(a[0]) : "r"(v0), "r"(low));
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(a[1]) : "r"(v1), "r"(sixteenth), "r"(high));
-    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(a[2]) : "r"(v2), "r"(low));
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(a[3]) : "r"(v3), "r"(sixteenth), "r"(high));
+    const uint32_t v0 = bits_of(w, k.low, k.low_base), v1 = bits_of(w, k.high, k.high_base), v2 = bits_of(u, k.low, k.low_base), v3 = bits_of(u, k.high, k.high_base);
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(a[0]) : "r"(v0), "r"(k.low_less));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(a[1]) : "r"(v1), "r"(k.sixteenth), "r"(k.high_less));
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(a[2]) : "r"(v2), "r"(k.low_less));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(a[3]) : "r"(v3), "r"(k.sixteenth), "r"(k.high_less));
 }
 
 // d = a b + c
@@ -104,7 +110,7 @@ __device__ __forceinline__ void group_words(uint32_t (&to)[G], const unsigned ch
 // A unit's part of 16 logits for 8 NT rows of hidden states.  x: this lane's share of the first row group's row lane / 4 at the unit's first
 // column; sums: of the unit's first group, per group 8 NT of them.
 template <bool SBF16, bool ZEROS, int G, int NT>
-__device__ __forceinline__ void unit_logits(float (&acc)[NT][4], const unsigned char *unit, const unsigned char *x, int pitch, const float *sums)
+__device__ __forceinline__ void unit_logits(const CodeBits &bits, float (&acc)[NT][4], const unsigned char *unit, const unsigned char *x, int pitch, const float *sums)
 {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint4 q[2] = {((const uint4 *)unit)[code_place(lane)], ((const uint4 *)(unit + 512))[code_place(lane)]};
@@ -118,8 +124,8 @@ __device__ __forceinline__ void unit_logits(float (&acc)[NT][4], const unsigned 
 #pragma unroll
         for (int h = gr * (4 / G); h < (gr + 1) * (4 / G); h++) {  // 32 columns each
             uint32_t a0[4], a1[4];
-            codes_to_a(word[2 * h], a0);
-            codes_to_a(word[2 * h + 1], a1);
+            codes_to_a(bits, word[2 * h], a0);
+            codes_to_a(bits, word[2 * h + 1], a1);
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const uint4 v = *(const uint4 *)(x + n * 8 * pitch + h * 64);
@@ -368,14 +374,6 @@ __device__ __forceinline__ void stage_digits(const HeadLogits &p, int cols, unsi
 // Up to 16 rows at a time: the weight streams through, once.  Hidden states lie in shared memory whole.  A CTA per SM has a run of tiles, whose
 // units its 16 warps share out evenly, each a run of neighbours that it copies into a ring of its own (bulk copies, one per stage), so no
 // warp waits for another before the end.  A tile that several warps have units of is added up there, by the warp that has its first.
-constexpr int kStreamWarps = 16, kStreamStages = 2;
-
-struct StreamShape {
-    int pitch;          // bytes between rows of hidden states
-    int chunk;          // units of a stage
-    size_t sums, unscale, slots, ring, bars, smem;  // offsets, and bytes in all
-};
-
 template <int NT, bool INT>
 __device__ __forceinline__ void stream_write(const HeadLogits &p, const float (&acc)[NT][4], int64_t tile, const float2 *unscale)
 {
@@ -442,6 +440,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1) k_head_stream(const __gr
     for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[n][i] = 0.f;
+    const CodeBits bits;
     int ku = u0 % per, tile = u0 / per;      // the next unit's place
     bool own = ku == 0;                      // this warp has the tile's first unit
     bool left = false;                       // what is in acc belongs to a tile that is not at its end
@@ -453,7 +452,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1) k_head_stream(const __gr
         for (int j = 0; j < n; j++) {
             const unsigned char *unit = ring + stage * ring_bytes + j * w.unit_bytes;
             if constexpr (INT) unit_logits_int<SBF16, ZEROS, G>(acc[0], unit, x + ku * kUnitCols, sums + ku * G * 8);
-            else unit_logits<SBF16, ZEROS, G, NT>(acc, unit, x + ku * (kUnitCols * 2), s.pitch, sums + ku * G * 8 * NT);
+            else unit_logits<SBF16, ZEROS, G, NT>(bits, acc, unit, x + ku * (kUnitCols * 2), s.pitch, sums + ku * G * 8 * NT);
             left = true;
             if (++ku == per) {
                 if (own) {
@@ -542,35 +541,6 @@ static int head_pack(StgHandle h, const StgHeadPack *b, cudaStream_t stream)
     return STG_OK;
 }
 
-// `chunk` 0: it does not fit.
-constexpr int kIntRows = 2;
-static StreamShape stream_shape(const Head4 &w, int rows, bool zeros, size_t most)
-{
-    const int nt = rows <= 8 ? 1 : 2;
-    const bool ints = rows <= kIntRows;
-    StreamShape s;
-    memset(&s, 0, sizeof(s));
-    const size_t cols = (size_t)w.units_per_tile * kUnitCols;
-    s.pitch = (int)(ints ? cols + 16 : cols * 2 + 64);  // rows g and g + 1 of a fragment in different banks
-    s.sums = (size_t)8 * nt * s.pitch;
-    s.unscale = s.sums + (zeros ? cols / w.group * 8 * nt * 4 : 0);
-    s.slots = round_up(s.unscale + (size_t)8 * nt * 8, 16);
-    s.bars = s.slots + (size_t)kStreamWarps * nt * 512;
-    s.ring = round_up(s.bars + kStreamWarps * kStreamStages * 8, 128);
-    const size_t unit = (size_t)kStreamWarps * kStreamStages * w.unit_bytes;
-    s.chunk = s.ring + unit <= most ? (int)std::min<size_t>(4, (most - s.ring) / unit) : 0;
-    s.smem = s.ring + s.chunk * unit;
-    return s;
-}
-
-// Up to 32 rows stream, where 16 of them fit into shared memory beside the rings; more than 16 in two calls of half of them, each of which reads
-// the weight (17 x 4096 x 151,936: 2 x 97 us, stg_head_tiles.cu 207 with groups of 128, 333 with groups of 32).
-constexpr int kStreamRows = 32;
-static bool streams(StgHandle h, const Head4 &w, int rows, bool zeros)
-{
-    return rows <= kStreamRows && stream_shape(w, std::min(rows, 16), zeros, h->smem_optin).chunk > 0;
-}
-
 template <bool SBF16, bool ZEROS, int G>
 static cudaError_t launch_stream(StgHandle h, const HeadLogits &p, cudaStream_t stream)
 {
@@ -604,7 +574,7 @@ static int head_logits_check(StgHandle h, const StgHeadLogits *b, const char *wh
 static size_t head_logits_workspace(StgHandle h, const StgHeadLogits *b)
 {
     const Head4 w = head4_shape(b->vocab, b->width, b->group, b->has_zeros != 0);
-    return b->rows == 0 || streams(h, w, b->rows, b->has_zeros != 0) ? 0 : head_tiles_workspace(h, w, b->rows);
+    return b->rows == 0 || streams(w, b->rows, b->has_zeros != 0, h->smem_optin) ? 0 : head_tiles_workspace(h, w, b->rows);
 }
 
 static int head_logits(StgHandle h, const StgHeadLogits *b, cudaStream_t stream)
@@ -626,7 +596,7 @@ static int head_logits(StgHandle h, const StgHeadLogits *b, cudaStream_t stream)
     p.rows = b->rows; p.hidden_bf16 = b->hidden_dtype == STG_DTYPE_BF16; p.out = b->logits; p.out_stride = b->row_stride; p.out_bf16 = b->logits_dtype == STG_DTYPE_BF16;
     const OnDevice on(h->cfg.device);
     CK(on.error);
-    if (!streams(h, p.w, p.rows, b->has_zeros != 0)) {
+    if (!streams(p.w, p.rows, b->has_zeros != 0, h->smem_optin)) {
         if (!b->workspace || misaligned(b->workspace, 256) || b->workspace_bytes < head_tiles_workspace(h, p.w, p.rows))
             return fail(h, STG_ERR_CAPACITY, "stg_head_logits: workspace missing, not aligned to 256 bytes or smaller than stg_head_logits_workspace says");
         const int rc2 = head_tiles(h, p, b->scale_dtype == STG_DTYPE_BF16, b->workspace, stream);

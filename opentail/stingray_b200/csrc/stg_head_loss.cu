@@ -31,7 +31,6 @@ struct HeadPrep {
 };
 
 constexpr int kPrepThreads = 1024;
-constexpr int kMostSplits = 64;
 
 __global__ void __launch_bounds__(kPrepThreads) k_head_prep(const __grid_constant__ HeadPrep p)
 {
@@ -57,7 +56,7 @@ __global__ void __launch_bounds__(kPrepThreads) k_head_prep(const __grid_constan
         const int at = before + ahead + __popc(ballot & ((1u << lane) - 1u));
         if (r < p.rows) p.ws.place[r] = on ? at : t < 0 ? -1 : -2;
         if (on) {
-            HeadRow row = {r, t, 0.f, 0.f, 0.f};
+            HeadRow row = {r, t, 0.f, 0.f, 0.f, 0};
             if (p.norms) {
                 row.b = p.grad_loss[r];
                 row.a = row.b + (p.grad_norms ? p.grad_norms[r] : 0.f);
@@ -69,7 +68,20 @@ __global__ void __launch_bounds__(kPrepThreads) k_head_prep(const __grid_constan
         before += all;
         __syncthreads();
     }
-    for (int i = before + tid; i < (before + kHeadTileM - 1) / kHeadTileM * kHeadTileM; i += kPrepThreads) p.ws.rows[i] = HeadRow{-1, -1, 0.f, 0.f, 0.f};
+    // Up to 64 rows have room for as many more in the one row of tiles that they take.  They get what the rounding of the logits' gradients
+    // leaves, as rows of their own, at no cost: a row's largest gradient is its target's, and its rounding shows in both results
+    // (one row: up to 2^-8 of them).
+    const int low = p.norms && p.rows <= kLowRows ? before : 0;
+    if (low > 0) {
+        __syncthreads();
+        if (tid < low) {
+            HeadRow row = p.ws.rows[tid];
+            row.low = 1;
+            p.ws.rows[low + tid] = row;
+        }
+        before += low;
+    }
+    for (int i = before + tid; i < (before + kHeadTileM - 1) / kHeadTileM * kHeadTileM; i += kPrepThreads) p.ws.rows[i] = HeadRow{-1, -1, 0.f, 0.f, 0.f, 0};
     for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
     if (lane == 0) warp_most[w] = most;
     __syncthreads();
@@ -93,17 +105,20 @@ __global__ void __launch_bounds__(kPrepThreads) k_head_prep(const __grid_constan
         int e = 0;
         if (most > 0.f && most < CUDART_INF_F) e = max(-110, min(110, 13 - ilogbf(most)));
         p.ws.info->used = before;
+        p.ws.info->low = low;
         p.ws.info->scale = exp2f((float)e);
         p.ws.info->unscale = exp2f((float)-e);
     }
 }
 
 // Hidden states of the rows that have a loss, next to each other, zeros behind them up to whole tiles.
-__global__ void __launch_bounds__(128) k_head_gather(const __grid_constant__ HeadWs ws, const uint16_t *hidden, int64_t stride, int width, bool vec)
+__global__ void __launch_bounds__(128) k_head_gather(const __grid_constant__ HeadWs ws, const uint16_t *hidden, int64_t stride, int width, bool vec, bool links, int vocab)
 {
     pdl_release();
     pdl_wait();
     const int c = blockIdx.x, used = ws.info->used;
+    if (links)  // no row has a target yet (k_head_links)
+        for (int64_t i = (int64_t)c * 128 + threadIdx.x; i < vocab; i += (int64_t)gridDim.x * 128) ws.first[i] = -1;
     if (c >= (used + kHeadTileM - 1) / kHeadTileM * kHeadTileM) return;
     uint4 *to = (uint4 *)((uint16_t *)ws.hidden + (int64_t)c * width);
     const uint16_t *from = c < used ? hidden + (int64_t)ws.rows[c].row * stride : nullptr;
@@ -121,6 +136,38 @@ __global__ void __launch_bounds__(128) k_head_gather(const __grid_constant__ Hea
     }
 }
 
+// For each used row the one ahead of it with the same target, and for each target its last row.  Every thread looks through all rows ahead of its
+// own, 1024 at a time in shared memory (8192 rows: 33 million comparisons, 13 us).
+constexpr int kLinkThreads = 64, kLinkRows = 1024;
+
+__global__ void __launch_bounds__(kLinkThreads) k_head_links(const __grid_constant__ HeadWs ws)
+{
+    __shared__ int4 targets[kLinkRows / 4];
+    pdl_release();
+    pdl_wait();
+    const int used = ws.info->used, first = blockIdx.x * kLinkThreads, r = first + threadIdx.x;
+    if (ws.info->low > 0 || first >= used) return;
+    const int mine = r < used ? ws.rows[r].target : -1;
+    int found = -1;
+    for (int from = 0; from < min(used, first + kLinkThreads); from += kLinkRows) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < kLinkRows; i += kLinkThreads) ((int *)targets)[i] = from + i < used ? ws.rows[from + i].target : -2;
+        __syncthreads();
+        const int n = min(kLinkRows, r - from);  // rows ahead
+#pragma unroll 4
+        for (int i = 0; i < n; i += 4) {
+            const int4 t = targets[i / 4];
+            if (t.x == mine) found = from + i;
+            if (t.y == mine && i + 1 < n) found = from + i + 1;
+            if (t.z == mine && i + 2 < n) found = from + i + 2;
+            if (t.w == mine && i + 3 < n) found = from + i + 3;
+        }
+    }
+    if (r >= used) return;
+    ws.next[r] = found;
+    atomicMax(ws.first + mine, r);
+}
+
 // A row's maxima and sums joined: its normaliser and loss.  `targets`: the rows are the caller's own, else they have been gathered.
 __global__ void __launch_bounds__(128) k_head_join(const __grid_constant__ HeadWs ws, int pieces, const int32_t *targets, int vocab, float *loss, float *norms)
 {
@@ -134,18 +181,22 @@ __global__ void __launch_bounds__(128) k_head_join(const __grid_constant__ HeadW
         return;
     }
     const float2 *parts = ws.parts + (int64_t)at * pieces;
-    // each thread joins its own as they come; they are joined relative to the largest of all then
+    // each thread joins its own as they come, eight at a time; they are joined relative to the largest of all then.  A NaN sum stays.
     float top = -CUDART_INF_F;
     double sum = 0.0;
-#pragma unroll 4
-    for (int i = tid; i < pieces; i += 128) {
-        const float2 v = parts[i];
-        if (v.x > top) {
-            sum = sum * (double)expf(top - v.x) + (double)v.y;
-            top = v.x;
-        } else {  // a NaN of either stays
-            sum += v.x > -CUDART_INF_F ? (double)(v.y * expf(v.x - top)) : (double)v.y;
-        }
+    for (int base = tid; base < pieces; base += 8 * 128) {
+        float2 v[8];
+        float most = top;
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = base + i * 128 < pieces ? parts[base + i * 128] : make_float2(-CUDART_INF_F, 0.f);
+#pragma unroll
+        for (int i = 0; i < 8; i++) most = fmaxf(most, v[i].x);
+        const float ref = most > -CUDART_INF_F ? most : 0.f;
+        float part = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) part += v[i].y * expf(v[i].x - ref);
+        sum = (top > -CUDART_INF_F ? sum * (double)expf(top - ref) : sum) + (double)part;
+        top = most;
     }
     float all = top;
     for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
@@ -163,10 +214,13 @@ __global__ void __launch_bounds__(128) k_head_join(const __grid_constant__ HeadW
     }
 }
 
-// Gradients of the hidden states: the splits' sums added up and rounded, back in their rows; zeros where a row has no loss.  A CTA has 256 columns
+// Gradients of the hidden states: the splits' sums added up and rounded, back in their rows; zeros where a row has no loss.  Where the logits'
+// gradients have no remainders of their own, the target's - the largest of a row, mostly - is multiplied here (without it a bf16 gradient is 2.4e-3
+// off in place of 1.7e-3, which is its own rounding).  A CTA has 256 columns
 // of a row, and eight threads share out the splits of each eight columns.
 template <bool BF16>
-__global__ void __launch_bounds__(256) k_head_spread(const __grid_constant__ HeadWs ws, int width, uint16_t *out)
+__global__ void __launch_bounds__(256) k_head_spread(const __grid_constant__ HeadWs ws, int width, const uint16_t *weight, int64_t weight_stride,
+                                                              uint16_t *out)
 {
     __shared__ float4 parts[8][32][2];
     pdl_release();
@@ -175,8 +229,9 @@ __global__ void __launch_bounds__(256) k_head_spread(const __grid_constant__ Hea
     const float unscale = ws.info->unscale;
     const int64_t slab = (int64_t)((ws.info->used + kHeadTileM - 1) / kHeadTileM * kHeadTileM) * width;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-    if (at >= 0 && col < width) {
-        const float *from = ws.sums + (int64_t)at * width + col;
+    const int low = ws.info->low;
+    for (int part = 0; at >= 0 && col < width && part < (low > 0 ? 2 : 1); part++) {  // the row's, and its remainders'
+        const float *from = ws.sums + (int64_t)(at + part * low) * width + col;
 #pragma unroll 4
         for (int s = w; s < splits; s += 8) {
             const float4 u = *(const float4 *)(from + s * slab), v = *(const float4 *)(from + s * slab + 4);
@@ -194,21 +249,20 @@ __global__ void __launch_bounds__(256) k_head_spread(const __grid_constant__ Hea
             y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
         }
     }
+    if (w == 0 && at >= 0 && low == 0 && col < width) {
+        const float rest = ws.hit[at];
+        const uint4 t = *(const uint4 *)(weight + (int64_t)ws.rows[at].target * weight_stride + col);
+        x.x = fmaf(rest, half_of<BF16>(t.x), x.x); x.y = fmaf(rest, half_of<BF16>(t.x >> 16), x.y);
+        x.z = fmaf(rest, half_of<BF16>(t.y), x.z); x.w = fmaf(rest, half_of<BF16>(t.y >> 16), x.w);
+        y.x = fmaf(rest, half_of<BF16>(t.z), y.x); y.y = fmaf(rest, half_of<BF16>(t.z >> 16), y.y);
+        y.z = fmaf(rest, half_of<BF16>(t.w), y.z); y.w = fmaf(rest, half_of<BF16>(t.w >> 16), y.w);
+    }
     if (w == 0 && col < width)
         *(uint4 *)(out + (int64_t)r * width + col) = make_uint4(pack2<BF16>(x.x * unscale, x.y * unscale), pack2<BF16>(x.z * unscale, x.w * unscale),
                                                                 pack2<BF16>(y.x * unscale, y.y * unscale), pack2<BF16>(y.z * unscale, y.w * unscale));
 }
 
 // ---- host ----
-
-struct HeadPlan {
-    bool pair;              // tiles of 256 rows by two CTAs
-    int tile_m, rows_pad;
-    int tile_n, tiles_n;    // of the vocabulary
-    int piece, pieces;      // backward: vocabulary entries whose gradients are there at a time; a multiple of 64
-    int grads_stride, sums_rows;
-    size_t bytes;
-};
 
 // Offsets of the workspace; `base` NULL: only its size.
 static HeadWs head_layout(const StgHeadLoss *b, bool backward, HeadPlan &p, char *base)
@@ -222,11 +276,15 @@ static HeadWs head_layout(const StgHeadLoss *b, bool backward, HeadPlan &p, char
     ws.rows = (HeadRow *)take(R * sizeof(HeadRow));
     ws.place = (int32_t *)take(R * 4);
     ws.hidden = take(R * (size_t)b->width * 2);
+    ws.hit = (float *)take(R * 4);
     if (backward) {
         ws.grads = take(R * (size_t)p.grads_stride * 2);
         ws.sums = (float *)take((size_t)p.sums_rows * (size_t)b->width * 4);
+        if (b->rows > kLowRows) {
+            ws.first = (int32_t *)take((size_t)b->vocab * 4);
+            ws.next = (int32_t *)take(R * 4);
+        }
     } else {
-        ws.hit = (float *)take(R * 4);
         ws.parts = (float2 *)take(R * 2 * (size_t)p.tiles_n * sizeof(float2));
     }
     p.bytes = at;
@@ -235,31 +293,7 @@ static HeadWs head_layout(const StgHeadLoss *b, bool backward, HeadPlan &p, char
 
 static HeadPlan head_plan(StgHandle h, const StgHeadLoss *b, bool backward)
 {
-    HeadPlan p;
-    memset(&p, 0, sizeof(p));
-    p.pair = b->rows > kHeadTileM;
-    p.tile_m = p.pair ? 2 * kHeadTileM : kHeadTileM;
-    p.rows_pad = (b->rows + kHeadTileM - 1) / kHeadTileM * kHeadTileM;
-    // One row of tiles reads the weight once, and its time is that of the CTA with the most of it: the width of a
-    // tile is the one whose waves take the fewest vocabulary entries, the widest of those (64 x 4096 x 151,936: 5 waves of 208, 1040
-    // entries per CTA, in place of 5 of 256)
-    p.tile_n = 256;
-    if (!p.pair)
-        for (int64_t n = 256, least = INT64_MAX; n >= 64; n -= 16) {
-            const int64_t tiles = (b->vocab + n - 1) / n, most = (tiles + h->sm_count - 1) / h->sm_count * n;
-            if (most < least) { least = most; p.tile_n = (int)n; }
-        }
-    p.tiles_n = (b->vocab + p.tile_n - 1) / p.tile_n;
-    // a piece of the gradients takes 256 MB at most, or 2048 columns
-    const int64_t whole = ((int64_t)b->vocab + 63) / 64 * 64;
-    const int64_t most = std::min<int64_t>(std::max<int64_t>(2048, (int64_t)(1 << 27) / std::max(1, p.rows_pad)), whole);
-    p.pieces = (int)((whole + most - 1) / most);
-    // whole tiles, of the row of CTAs that the rows take at most
-    const int64_t each = ((whole + p.pieces - 1) / p.pieces + 255) / 256 * 256;
-    p.piece = (int)std::min(each, whole);
-    p.pieces = (int)((whole + p.piece - 1) / p.piece);
-    p.grads_stride = (p.piece + p.tile_n - 1) / p.tile_n * p.tile_n;
-    p.sums_rows = (int)std::max<int64_t>(p.rows_pad, (int64_t)2 * h->sm_count * kHeadTileM * 256 / b->width);
+    HeadPlan p = head_shape(b->rows, b->vocab, b->width, h->sm_count, backward);
     head_layout(b, backward, p, nullptr);
     return p;
 }
@@ -320,14 +354,16 @@ static int head_map(StgHandle h, CUtensorMap *map, bool bf16, const void *p, int
 
 template <int MODE>
 static cudaError_t head_gemm(StgHandle h, bool bf16, bool pair, cudaStream_t stream, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &out,
-                             const HeadGemm &g, int64_t tiles)
+                             HeadGemm g, int64_t tiles)
 {
     using Kernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, HeadGemm);
     constexpr bool C = MODE == kStats || MODE == kGrad;  // the others have no soft cap
     static const Kernel kernels[2][2][2] = {{{k_head_gemm<MODE, false, false, false>, k_head_gemm<MODE, false, false, true>}, {k_head_gemm<MODE, false, C, false>, k_head_gemm<MODE, false, C, true>}},
                                             {{k_head_gemm<MODE, true, false, false>, k_head_gemm<MODE, true, false, true>}, {k_head_gemm<MODE, true, C, false>, k_head_gemm<MODE, true, C, true>}}};
     const Kernel fn = kernels[bf16][g.cap != 0.f][pair];
-    const size_t smem = (pair ? GemmRing<true>::kSmem : GemmRing<false>::kSmem) + (MODE == kStats ? 0 : kGemmEpiWarps * kGemmOut);
+    const GemmRing ring = gemm_ring(MODE, pair, g.tile_n, g.a_rows);
+    g.a_at = ring.a_at; g.stage_bytes = ring.stage_bytes; g.stages = ring.stages;
+    const size_t smem = 1024 + kGemmRingBytes + (MODE == kStats ? 0 : kGemmEpiWarps * kGemmOut);
     const cudaError_t e = ensure_dynamic_smem((const void *)fn, smem);
     if (e != cudaSuccess) return e;
     h->stats.kernel_launches++;
@@ -350,13 +386,18 @@ static cudaError_t head_gemm(StgHandle h, bool bf16, bool pair, cudaStream_t str
 
 static bool head_rows_aligned(const StgHeadLoss *b) { return !misaligned(b->hidden, 16) && (b->rows == 1 || b->hidden_stride % 8 == 0); }
 
-static int head_begin(StgHandle h, const StgHeadLoss *b, const HeadWs &ws, const HeadPlan &p, bool backward, cudaStream_t stream)
+static int head_begin(StgHandle h, const StgHeadLoss *b, const HeadWs &ws, const HeadPlan &p, bool backward, bool links, cudaStream_t stream)
 {
     const HeadPrep prep = {ws, b->rows, b->vocab, b->targets, backward ? b->log_norms : nullptr, b->grad_loss, b->grad_log_norms,
                            b->width, p.tile_m, h->sm_count * kHeadTileM / p.tile_m, (p.piece + kGemmK - 1) / kGemmK, p.sums_rows};
     CK(launch_behind(k_head_prep, dim3(1), kPrepThreads, 0, stream, prep));
-    CK(launch_behind(k_head_gather, dim3((unsigned)p.rows_pad), 128, 0, stream, ws, (const uint16_t *)b->hidden, b->hidden_stride, b->width, head_rows_aligned(b)));
+    CK(launch_behind(k_head_gather, dim3((unsigned)p.rows_pad), 128, 0, stream, ws, (const uint16_t *)b->hidden, b->hidden_stride, b->width, head_rows_aligned(b), links,
+                     b->vocab));
     h->stats.kernel_launches += 2;
+    if (links) {
+        CK(launch_behind(k_head_links, dim3((unsigned)(p.rows_pad + kLinkThreads - 1) / kLinkThreads), kLinkThreads, 0, stream, ws));
+        h->stats.kernel_launches++;
+    }
     return STG_OK;
 }
 
@@ -372,7 +413,7 @@ static HeadGemm head_args(const StgHeadLoss *b, const HeadWs &ws, const HeadPlan
     HeadGemm g;
     memset(&g, 0, sizeof(g));
     g.info = ws.info; g.rows = ws.rows; g.rows_pad = p.rows_pad; g.tile_n = p.tile_n; g.group = kGroupLogits; g.cap = b->logit_softcap;
-    g.a_rows = head_box_rows(b->rows);
+    g.a_rows = head_box_rows(b->rows);  // backward: twice as many, below
     return g;
 }
 
@@ -393,7 +434,7 @@ static int head_forward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
     if ((rc = direct ? head_map(h, &rows, bf16, b->hidden, b->width, b->rows, b->rows == 1 ? b->width : b->hidden_stride, head_box_rows(b->rows))
                      : head_map(h, &rows, bf16, ws.hidden, b->width, p.rows_pad, b->width, head_box_rows(b->rows)))) return rc;
     if ((rc = head_map(h, &weight, bf16, b->weight, b->width, b->vocab, b->weight_stride, p.pair ? p.tile_n / 2 : p.tile_n))) return rc;
-    if (!direct && (rc = head_begin(h, b, ws, p, false, stream))) return rc;
+    if (!direct && (rc = head_begin(h, b, ws, p, false, false, stream))) return rc;
     HeadGemm g = head_args(b, ws, p);
     g.targets = direct ? b->targets : nullptr; g.used_rows = b->rows;
     g.n = b->vocab; g.k = b->width;
@@ -424,7 +465,8 @@ static int head_backward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
     const bool bf16 = b->dtype == STG_DTYPE_BF16;
     CUtensorMap rows_k, weight_k, grads_k, weight_mn, grads_mn, rows_mn;  // how the operands' boxes of 64 columns are cut
     CUtensorMap grads_out, sums_out, weight_out;                          // results: boxes of 32 rows
-    if ((rc = head_map(h, &rows_k, bf16, ws.hidden, b->width, p.rows_pad, b->width, head_box_rows(b->rows)))) return rc;
+    const int box_rows = head_box_rows(2 * b->rows);  // with the remainders'
+    if ((rc = head_map(h, &rows_k, bf16, ws.hidden, b->width, p.rows_pad, b->width, box_rows))) return rc;
     if ((rc = head_map(h, &weight_k, bf16, b->weight, b->width, b->vocab, b->weight_stride, p.pair ? p.tile_n / 2 : p.tile_n))) return rc;
     if ((rc = head_map(h, &weight_mn, bf16, b->weight, b->width, b->vocab, b->weight_stride, kGemmK))) return rc;
     if ((rc = head_map(h, &rows_mn, bf16, ws.hidden, b->width, p.rows_pad, b->width, kGemmK))) return rc;
@@ -433,8 +475,9 @@ static int head_backward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
         const cuuint32_t box[2] = {32, 32};
         if ((rc = head_map_of(h, &sums_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, ws.sums, size, stride, box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
     }
-    if ((rc = head_begin(h, b, ws, p, true, stream))) return rc;
-    const int64_t tiles_m = (b->rows + p.tile_m - 1) / p.tile_m, tiles_w = (b->width + 255) / 256;
+    const bool links = b->grad_weight && ws.first;
+    if ((rc = head_begin(h, b, ws, p, true, links, stream))) return rc;
+    const int64_t tiles_m = (p.rows_pad + p.tile_m - 1) / p.tile_m, tiles_w = (b->width + 255) / 256;
     for (int i = 0; i < p.pieces; i++) {
         const int first = i * p.piece, count = std::min(p.piece, b->vocab - first);
         // what lies behind the piece's columns is read as zeros
@@ -443,8 +486,8 @@ static int head_backward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
         if ((rc = head_map(h, &grads_out, bf16, ws.grads, count, p.rows_pad, p.grads_stride, 32))) return rc;
         HeadGemm g = head_args(b, ws, p);
         g.first = first;
-        g.n = count; g.k = b->width;
-        g.out = ws.grads; g.out_stride = p.grads_stride;
+        g.n = count; g.k = b->width; g.a_rows = box_rows;
+        g.out = ws.grads; g.out_stride = p.grads_stride; g.hit = ws.hit;
         CK(head_gemm<kGrad>(h, bf16, p.pair, stream, rows_k, weight_k, grads_out, g, tiles_m * ((count + p.tile_n - 1) / p.tile_n)));
         g.n = b->width; g.tile_n = 256; g.group = kGroupGrads; g.cap = 0.f;
         if (b->grad_hidden) {
@@ -454,13 +497,15 @@ static int head_backward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
         }
         if (b->grad_weight) {
             g.m = count;
+            g.first_of = links ? ws.first : nullptr; g.next = ws.next; g.hidden = (const uint16_t *)ws.hidden;
             g.out = b->grad_weight; g.out_stride = b->width;
             if ((rc = head_map(h, &weight_out, bf16, b->grad_weight, b->width, first + count, b->width, 32))) return rc;
             CK(head_gemm<kWeight>(h, bf16, p.pair, stream, grads_mn, rows_mn, weight_out, g, (int64_t)((count + p.tile_m - 1) / p.tile_m) * tiles_w));
         }
     }
     if (b->grad_hidden) {
-        CK(launch_behind(bf16 ? k_head_spread<true> : k_head_spread<false>, dim3((unsigned)b->rows, (unsigned)(b->width + 255) / 256), 256, 0, stream, ws, b->width, (uint16_t *)b->grad_hidden));
+        CK(launch_behind(bf16 ? k_head_spread<true> : k_head_spread<false>, dim3((unsigned)b->rows, (unsigned)(b->width + 255) / 256), 256, 0, stream, ws, b->width, (const uint16_t *)b->weight, b->weight_stride,
+                         (uint16_t *)b->grad_hidden));
         h->stats.kernel_launches++;
     }
     h->stats.calls++;

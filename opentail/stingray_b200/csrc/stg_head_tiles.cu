@@ -24,9 +24,7 @@ struct HeadTiles {
     uint16_t *states;       // [blocks * n, padded width] fp16, zeros where there are no rows
     float2 *unscale;        // [blocks * n]: the inverse of what a row was multiplied with, in two factors
     float *sums;            // [blocks][groups of the padded width][n]: sums of groups, for zero points
-    int n, blocks;          // rows of a block (16, 32, 64 or 128) and their number
-    int per_item, items_v;  // tiles of an item, and items of the vocabulary
-    int code_stages, state_stages, slots;
+    int n, blocks, per_item, items_v, code_stages, state_stages, slots;  // TilesShape
     bool scale_bf16;
 };
 
@@ -92,16 +90,6 @@ struct TilesWarps {
     static constexpr int kTeams = C == 8 ? 1 : 2, kSets = 2, kUnpack = 3, kAdd = 3 + 4 * kTeams;
     static constexpr int kThreads = 32 * (3 + 4 * kTeams + 4 * kSets);
 };
-constexpr int kTilesMost = 8;        // tiles of an item
-constexpr int kTilesChunk = 4;       // units of a stage: copies of one unit each kept the copying warp busy for 1400 cycles a unit
-constexpr int kTilesStages = 6;      // of either ring at most
-constexpr int kTilesSlots = 8;       // accumulators at most
-__host__ __device__ constexpr int tiles_buffers(int n) { return n <= 64 ? 4 : 2; }  // of unpacked weights, 64 columns of tensor memory each, behind the accumulators
-static __host__ __device__ size_t tiles_code_stage(const Head4 &w, int n)
-{
-    return ((size_t)kTilesChunk * (kTilesMost * w.unit_bytes + w.groups_per_unit * n * 4) + 1023) / 1024 * 1024;
-}
-
 // a b + c, two at a time.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 {
@@ -127,7 +115,7 @@ __global__ void __launch_bounds__(TilesWarps<C>::kThreads, 1) k_head_tiles(const
     const Head4 &w = a.p.w;
     // the rings: hidden states, then codes, in each stage with the groups' sums ahead
     unsigned char *const states_p = raw + ((1024u - (smem_at(raw) & 1023u)) & 1023u), *const codes_p = states_p + a.state_stages * kStateBytes;
-    const uint32_t code_stage = (uint32_t)tiles_code_stage(w, N), tile_stage = kTilesChunk * (uint32_t)w.unit_bytes;
+    const uint32_t code_stage = (uint32_t)tiles_code_stage(w.unit_bytes, w.groups_per_unit, N), tile_stage = kTilesChunk * (uint32_t)w.unit_bytes;
     constexpr uint32_t kSumBytes = ZEROS ? G * N * 4 : 0, kCodesAt = kTilesChunk * kSumBytes;
     const uint32_t c_full = smem_at(bars), c_empty = c_full + 8 * kTilesStages, s_full = c_empty + 8 * kTilesStages, s_empty = s_full + 8 * kTilesStages,
                    a_full = s_empty + 8 * kTilesStages, a_empty = a_full + 8 * kBuffers, d_full = a_empty + 8 * kBuffers, d_empty = d_full + 8 * kTilesSlots;
@@ -389,26 +377,13 @@ __global__ void __launch_bounds__(TilesWarps<C>::kThreads, 1) k_head_tiles(const
 
 // ---- host ----
 
-static HeadTiles tiles_shape(StgHandle h, const Head4 &w, int rows)
+static HeadTiles tiles_args(StgHandle h, const Head4 &w, int rows)
 {
+    const TilesShape s = tiles_shape(w, rows, h->sm_count, h->smem_optin);
     HeadTiles a;
     memset(&a, 0, sizeof(a));
-    a.blocks = (rows + 127) / 128;
-    const int each = (rows + a.blocks - 1) / a.blocks;
-    a.n = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : 128;
-    // Few rows: the time is that of the CTA with the most of the weight, and smaller items share it out more evenly.  Many: an item takes
-    // its time however few tiles it has.
-    a.per_item = kTilesMost;
-    if (a.n <= 32)
-        for (int64_t n = kTilesMost, least = INT64_MAX; n >= 5; n--) {
-            const int64_t items = (w.tiles + n - 1) / n, most = (items + h->sm_count - 1) / h->sm_count * n;
-            if (most < least) { least = most; a.per_item = (int)n; }
-        }
-    a.items_v = (w.tiles + a.per_item - 1) / a.per_item;
-    a.slots = std::min(kTilesSlots, (512 - 64 * tiles_buffers(a.n)) / a.n);
-    const size_t code = tiles_code_stage(w, a.n), state = (size_t)2 * a.n * 128, room = h->smem_optin - 1024;
-    a.code_stages = a.n <= 64 ? 3 : 2;
-    a.state_stages = (int)std::min<size_t>(kTilesStages, (room - a.code_stages * code) / state);
+    a.n = s.n; a.blocks = s.blocks; a.per_item = s.per_item; a.items_v = s.items_v;
+    a.code_stages = s.code_stages; a.state_stages = s.state_stages; a.slots = s.slots;
     return a;
 }
 
@@ -425,7 +400,7 @@ static size_t tiles_layout(const Head4 &w, HeadTiles &a, char *base)
 
 size_t head_tiles_workspace(StgHandle h, const Head4 &w, int rows)
 {
-    HeadTiles a = tiles_shape(h, w, rows);
+    HeadTiles a = tiles_args(h, w, rows);
     return tiles_layout(w, a, nullptr);
 }
 
@@ -434,14 +409,14 @@ static cudaError_t launch_tiles(const HeadTiles &a, const CUtensorMap &states, i
 {
     void (*fn)(CUtensorMap, HeadTiles) = a.n == 16 ? k_head_tiles<ZEROS, G, 1> : a.n == 32 ? k_head_tiles<ZEROS, G, 2> : a.n == 64 ? k_head_tiles<ZEROS, G, 4> : k_head_tiles<ZEROS, G, 8>;
     const int threads = a.n == 128 ? TilesWarps<8>::kThreads : TilesWarps<1>::kThreads;
-    const size_t smem = 1024 + a.code_stages * tiles_code_stage(a.p.w, a.n) + (size_t)a.state_stages * 2 * a.n * 128;
+    const size_t smem = 1024 + a.code_stages * tiles_code_stage(a.p.w.unit_bytes, a.p.w.groups_per_unit, a.n) + (size_t)a.state_stages * 2 * a.n * 128;
     const cudaError_t e = ensure_dynamic_smem((const void *)fn, smem);
     return e != cudaSuccess ? e : launch_behind(fn, dim3((unsigned)std::min(sms, a.items_v * a.blocks)), threads, smem, stream, states, a);
 }
 
 int head_tiles(StgHandle h, const HeadLogits &p, bool scale_bf16, void *workspace, cudaStream_t stream)
 {
-    HeadTiles a = tiles_shape(h, p.w, p.rows);
+    HeadTiles a = tiles_args(h, p.w, p.rows);
     tiles_layout(p.w, a, (char *)workspace);
     a.p = p;
     a.scale_bf16 = scale_bf16;

@@ -50,7 +50,8 @@ class Loss:
         hot = torch.zeros_like(p)
         hot.scatter_(1, self.t[:, None], 1.0)
         g = (a[:, None] * p - b[:, None] * hot) * self.slope
-        # the probability is as far off as its exponent, the gradient is rounded once; fp16 ends 2^-38 below the largest factor
+        # the probability is as far off as its exponent, the gradient is rounded once (up to 64 rows keep the remainders, rounded in turn);
+        # fp16 ends 2^-38 below the largest factor
         factor = torch.maximum(a.abs(), b.abs())
         most = factor.max() if factor.numel() else 0.0
         dp = self.dz + self.d_norm[:, None] + 2e-5

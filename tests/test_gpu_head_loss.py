@@ -77,6 +77,35 @@ def test_longer_sums(bs):
     _check(bs, h, w, t, dl)
 
 
+@pytest.mark.parametrize("rows,vocab", [(70, 5), (200, 3), (1500, 40), (2500, 1), (65, 900)])
+def test_many_rows_with_one_target(bs, rows, vocab):
+    """Rows that share targets: the remainders of their gradients are added up in their order, repeatably."""
+    import torch
+
+    h, w, t, dl, dn = _inputs(rows, 72, vocab, torch.bfloat16, ignored=0.1)
+    _, b = _check(bs, h, w, t, dl, dn)
+    n = bs.head_loss(h, w, t)["log_norms"]
+    for _ in range(2):
+        b2 = bs.head_loss_backward(h, w, t, n, dl, grad_log_norms=dn)
+        assert torch.equal(b["grad_weight"], b2["grad_weight"]) and torch.equal(b["grad_hidden"], b2["grad_hidden"])
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("rows", [1, 64, 65, 300])
+def test_gradients_are_nearly_their_own_rounding(bs, rows, dtype):
+    """The roundings of the logits' gradients even out or are made good: both results are about as far off as their own rounding, which
+    is evenly spread below half a step: 0.29 steps of 2 U relative to the value's power of two, 0.42 U of the value on average (0.58 at worst)."""
+    import torch
+
+    h, w, t, _, _ = _inputs(rows, 256, 3000, getattr(torch, dtype))
+    n = bs.head_loss(h, w, t)["log_norms"]
+    one = torch.full((rows,), 1.0 / rows, device="cuda")
+    b = bs.head_loss_backward(h, w, t, n, one)
+    gh, _, gw, _ = O.Loss(h, w, t).grads(one)
+    for got, want in ((b["grad_hidden"], gh), (b["grad_weight"], gw)):
+        assert ((got.double() - want).norm() / want.norm()).item() <= 0.58 * O.U[h.dtype]
+
+
 def test_strided_and_unaligned_rows(bs):
     import torch
 
@@ -220,6 +249,21 @@ def test_gradients_against_differences(bs):
     quotient = (f[2]["loss"].double() - f[0]["loss"].double()) / (2 * e)
     bound = e * e / 3 * spread ** 3 + (want[0].d_loss + want[1].d_loss) / (2 * e) + (dh * d.abs().double()).sum(1)
     _near("difference", (gh.double() * d.double()).sum(1), quotient, bound)
+
+
+@pytest.mark.parametrize("cap", [1e-40, 1e-6, 1e30])
+def test_soft_caps_of_any_size(bs, cap):
+    """A cap of almost nothing leaves equal logits, a large one leaves them as they are."""
+    import torch
+
+    h, w, t, dl, _ = _inputs(40, 64, 900, torch.bfloat16)
+    h[3] = 0
+    f = bs.head_loss(h, w, t, softcap=cap)
+    if cap < 1:
+        assert ((f["log_norms"].double() - math.log(900)).abs() <= 2 * cap + 2e-6).all() and ((f["loss"].double() - math.log(900)).abs() <= 4 * cap + 2e-6).all()
+    else:
+        want = O.Loss(h, w, t)  # tanh's own error is 2^-22 of the cap: nothing is left of the logits
+        assert torch.isfinite(f["loss"]).all() and (f["loss"].double() - want.loss).abs().max() <= cap
 
 
 def test_repeats_are_equal(bs):
