@@ -138,6 +138,48 @@ public:
                                  n_hyps, steps, parents, tokens, search.pad_token, sequences, search.max_steps, lengths, stream),
               "stg_beam_backtrace");
     }
+    // The head: losses of tokens and their gradients without logits; logits from a weight in 4 bits.  `workspace`: device memory of the
+    // bytes that the *_workspace call says, one for each call that may run at the same time
+    uint64_t head_loss_workspace(StgHeadLoss loss, bool backward) const
+    {
+        uint64_t n = 0;
+        loss.struct_size = (int32_t)sizeof(StgHeadLoss);
+        check(stg_head_loss_workspace(h_, &loss, backward ? 1 : 0, &n), "stg_head_loss_workspace");
+        return n;
+    }
+    void head_loss(StgHeadLoss loss, void *stream = nullptr)
+    {
+        loss.struct_size = (int32_t)sizeof(StgHeadLoss);
+        check(stg_head_loss(h_, &loss, stream), "stg_head_loss");
+    }
+    void head_loss_backward(StgHeadLoss loss, void *stream = nullptr)
+    {
+        loss.struct_size = (int32_t)sizeof(StgHeadLoss);
+        check(stg_head_loss_backward(h_, &loss, stream), "stg_head_loss_backward");
+    }
+    uint64_t head_pack_bytes(int vocab, int width, int group, bool has_zeros) const
+    {
+        uint64_t n = 0;
+        check(stg_head_pack_bytes(h_, vocab, width, group, has_zeros ? 1 : 0, &n), "stg_head_pack_bytes");
+        return n;
+    }
+    void head_pack(StgHeadPack pack, void *stream = nullptr)
+    {
+        pack.struct_size = (int32_t)sizeof(StgHeadPack);
+        check(stg_head_pack(h_, &pack, stream), "stg_head_pack");
+    }
+    uint64_t head_logits_workspace(StgHeadLogits logits) const
+    {
+        uint64_t n = 0;
+        logits.struct_size = (int32_t)sizeof(StgHeadLogits);
+        check(stg_head_logits_workspace(h_, &logits, &n), "stg_head_logits_workspace");
+        return n;
+    }
+    void head_logits(StgHeadLogits logits, void *stream = nullptr)
+    {
+        logits.struct_size = (int32_t)sizeof(StgHeadLogits);
+        check(stg_head_logits(h_, &logits, stream), "stg_head_logits");
+    }
     StgStats stats() const
     {
         StgStats s{};

@@ -91,8 +91,9 @@ __global__ void __launch_bounds__(kPrepThreads) k_head_prep(const __grid_constan
         uint64_t least = ~0ull;
         for (int n = lane + 1; n <= kMostSplits; n += 32)
             if (n == 1 || (n <= p.blocks && (int64_t)n * slab <= p.sums_rows)) {
-                // waves of tiles times their blocks, and some six blocks' time for a tile's sums to be written and read
-                const uint32_t cost = (uint32_t)((tiles * n + p.workers - 1) / p.workers) * (uint32_t)((p.blocks + n - 1) / n + 6);
+                // waves of tiles times their blocks, and some sixteen blocks' time for a tile's sums to be written and read (with six, 819 rows of
+                // 2048 x 151,936 were split in nine in place of two: fuller waves, but 1.59 ms in place of 1.55 at the card's power limit)
+                const uint32_t cost = (uint32_t)((tiles * n + p.workers - 1) / p.workers) * (uint32_t)((p.blocks + n - 1) / n + 16);
                 least = min(least, (uint64_t)cost << 32 | (uint32_t)n);
             }
         for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xFFFFFFFFu, least, o));

@@ -61,7 +61,8 @@ inline HeadPlan head_shape(int rows, int vocab, int width, int sms, bool backwar
     p.piece = (int)std::min(each, whole);
     p.pieces = (int)((whole + p.piece - 1) / p.piece);
     p.grads_stride = (p.piece + p.tile_n - 1) / p.tile_n * p.tile_n;
-    p.sums_rows = (int)std::max<int64_t>(p.rows_pad, (int64_t)2 * sms * kHeadTileM * 256 / width);
+    // room for splits: eight tiles per SM (155 MB), which leaves k_head_prep the choice of waves that are nearly full
+    p.sums_rows = (int)std::max<int64_t>(p.rows_pad, std::min<int64_t>((int64_t)kMostSplits * p.rows_pad, (int64_t)8 * sms * kHeadTileM * 256 / width));
     return p;
 }
 
