@@ -374,6 +374,10 @@ __device__ __forceinline__ void stage_digits(const HeadLogits &p, int cols, unsi
 // Up to 16 rows at a time: the weight streams through, once.  Hidden states lie in shared memory whole.  A CTA per SM has a run of tiles, whose
 // units its 16 warps share out evenly, each a run of neighbours that it copies into a ring of its own (bulk copies, one per stage), so no
 // warp waits for another before the end.  A tile that several warps have units of is added up there, by the warp that has its first.
+//
+// One row x 4096 x 151,936, groups of 32: 60 us for 351 MB (5.9 TB/s, 89 % of the copy rate; 84 as fp16, 250 with plain loads and fp16);
+// groups of 128: 56.  Three to eight rows 65 to 73, bound by instructions (154 for a unit of 2048 weights, of which unpacking is 72 and
+// the products 8); 16 rows 98 to 104, where the products' pipe and the unpacking's share the time.
 template <int NT, bool INT>
 __device__ __forceinline__ void stream_write(const HeadLogits &p, const float (&acc)[NT][4], int64_t tile, const float2 *unscale)
 {

@@ -6,6 +6,11 @@
 // numbers q - 8, exactly, each of them the units in turn, a thread one entry, and store them to tensor memory, a few buffers in turn.  One
 // thread multiplies, each group of columns into an accumulator of its own (a ring of them), and more warps add them up, scaled by the
 // entry's scale: a thread's numbers all have the same.  So the weight is not rounded, and scales meet fp32 sums.
+//
+// What bounds it is the way into tensor memory and out of it: a unit of eight tiles is 32 KB of unpacked weight, and each of its groups
+// 512 bytes of sums per row, at what measures as some 30 and 60 bytes a cycle.  256 rows x 4096 x 151,936 take 440 us with groups of 128
+// (720 TFLOP/s; the library's bf16 product of that size would be 193 at its best rate), 509 with zero points too, 704 with
+// groups of 32; 64 rows 173 and 282.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
