@@ -8,8 +8,8 @@
 // entry's scale: a thread's numbers all have the same.  So the weight is not rounded, and scales meet fp32 sums.
 //
 // What bounds it is the way into tensor memory and out of it: a unit of eight tiles is 32 KB of unpacked weight, and each of its groups
-// 512 bytes of sums per row, at what measures as some 30 and 60 bytes a cycle.  256 rows x 4096 x 151,936 take 440 us with groups of 128
-// (720 TFLOP/s; the library's bf16 product of that size would be 193 at its best rate), 509 with zero points too, 704 with
+// 512 bytes of sums per row, at what measures as some 30 and 60 bytes a cycle.  256 rows x 4096 x 151,936 take 410 us with groups of 128
+// (780 TFLOP/s; the library's bf16 product of that size would be 193 at its best rate), 509 with zero points too, 704 with
 // groups of 32; 64 rows 173 and 282.
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -87,14 +87,18 @@ __global__ void __launch_bounds__(256) k_head_states(const __grid_constant__ Hea
     }
 }
 
-// Two warps load, one multiplies; teams of four unpack, and two sets of four add up, each half of the columns.  Every warp's waits and
+// Two warps load, one multiplies; teams of four unpack, and sets of four add up, each some of the columns.  Every warp's waits and
 // arrivals cost it about a hundred instructions a unit, so few warps with many columns each take less time than many with few: 128 rows have
-// one team, whose registers the sums then get.
-template <int C>
+// one team, whose registers the sums then get, and two sets - but where a unit is one group without zero points, which leaves the adding
+// warps less to do than the unpacking ones, two teams and four sets (4096 x 151,936, 256 rows: 410 us in place of 439; with zero points
+// 689 in place of 487, with groups of 64 526 in place of 511).
+template <bool ZEROS, int G, int C>
 struct TilesWarps {
-    static constexpr int kTeams = C == 8 ? 1 : 2, kSets = 2, kUnpack = 3, kAdd = 3 + 4 * kTeams;
+    static constexpr bool kMany = C == 8 && G == 1 && !ZEROS;
+    static constexpr int kTeams = C == 8 && !kMany ? 1 : 2, kSets = kMany ? 4 : 2, kUnpack = 3, kAdd = 3 + 4 * kTeams;
     static constexpr int kThreads = 32 * (3 + 4 * kTeams + 4 * kSets);
 };
+
 // a b + c, two at a time.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 {
@@ -106,9 +110,9 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 
 // G groups to a unit; 16 C rows to a block.
 template <bool ZEROS, int G, int C>
-__global__ void __launch_bounds__(TilesWarps<C>::kThreads, 1) k_head_tiles(const __grid_constant__ CUtensorMap states, const __grid_constant__ HeadTiles a)
+__global__ void __launch_bounds__(TilesWarps<ZEROS, G, C>::kThreads, 1) k_head_tiles(const __grid_constant__ CUtensorMap states, const __grid_constant__ HeadTiles a)
 {
-    using Warps = TilesWarps<C>;
+    using Warps = TilesWarps<ZEROS, G, C>;
     constexpr int N = 16 * C, kTeams = Warps::kTeams, kSets = Warps::kSets, kThreads = Warps::kThreads, kCols = N / kSets;
     constexpr int kBuffers = tiles_buffers(N);
     constexpr uint32_t kUnpacked = 512 - 64 * kBuffers, kStateBytes = 2 * N * 128;
@@ -413,7 +417,7 @@ template <bool ZEROS, int G>
 static cudaError_t launch_tiles(const HeadTiles &a, const CUtensorMap &states, int sms, cudaStream_t stream)
 {
     void (*fn)(CUtensorMap, HeadTiles) = a.n == 16 ? k_head_tiles<ZEROS, G, 1> : a.n == 32 ? k_head_tiles<ZEROS, G, 2> : a.n == 64 ? k_head_tiles<ZEROS, G, 4> : k_head_tiles<ZEROS, G, 8>;
-    const int threads = a.n == 128 ? TilesWarps<8>::kThreads : TilesWarps<1>::kThreads;
+    const int threads = a.n == 128 ? TilesWarps<ZEROS, G, 8>::kThreads : TilesWarps<ZEROS, G, 1>::kThreads;
     const size_t smem = 1024 + a.code_stages * tiles_code_stage(a.p.w.unit_bytes, a.p.w.groups_per_unit, a.n) + (size_t)a.state_stages * 2 * a.n * 128;
     const cudaError_t e = ensure_dynamic_smem((const void *)fn, smem);
     return e != cudaSuccess ? e : launch_behind(fn, dim3((unsigned)std::min(sms, a.items_v * a.blocks)), threads, smem, stream, states, a);

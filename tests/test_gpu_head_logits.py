@@ -70,24 +70,25 @@ def test_every_code(bs, dtype):
     assert torch.equal(got.T.double(), w)
 
 
-def test_strides_and_places_behind(bs):
+@pytest.mark.parametrize("rows", [1, 5, 20, 40])
+def test_strides_and_places_behind(bs, rows):
     """Rows of hidden states, codes and logits inside wider ones: what lies behind is neither read nor written."""
     import torch
 
-    h, c, s, z = _inputs(20, 192, 1001, 64, torch.bfloat16, torch.float16, True)
+    h, c, s, z = _inputs(rows, 192, 1001, 64, torch.bfloat16, torch.float16, True)
     ref = bs.head_logits(h, bs.head_pack(c, s, z))
     codes = torch.full((1001, 131), 255, dtype=torch.uint8, device="cuda")
     codes[:, 3:99] = c
     head = bs.head_pack(codes[:, 3:99], s, z)
     for shift in (0, 1, 8):
-        wide = torch.full((20, 215), float("nan"), dtype=h.dtype, device="cuda")
+        wide = torch.full((rows, 215), float("nan"), dtype=h.dtype, device="cuda")
         wide[:, shift:shift + 192] = h
         for dtype in (torch.float32, torch.bfloat16):
-            room = torch.full((22, 1009), 7.0, dtype=dtype, device="cuda")
-            view = room[1:21, 1:1002]
+            room = torch.full((rows + 2, 1009), 7.0, dtype=dtype, device="cuda")
+            view = room[1:rows + 1, 1:1002]
             assert bs.head_logits(wide[:, shift:shift + 192], head, out=view) is view
             assert torch.equal(view, ref.to(dtype))
-            assert (room[[0, 21]] == 7).all() and (room[:, 0] == 7).all() and (room[:, 1002:] == 7).all()
+            assert (room[[0, rows + 1]] == 7).all() and (room[:, 0] == 7).all() and (room[:, 1002:] == 7).all()
 
 
 @pytest.mark.parametrize("rows", [3, 40, 140])
