@@ -26,29 +26,49 @@ struct HeadPack {
     int64_t codes_stride;
     const uint16_t *scales, *zeros;
     unsigned char *out;
+    bool vec;           // rows of codes begin at 16 bytes
 };
 
-// One warp per unit.
+// One warp per unit, whose codes - 64 bytes of each of 16 rows - it brings into shared memory first: 16 bytes at a time where rows begin at 16
+// bytes (4096 x 151,936: 256 us, 378 with bytes read where they are needed).
 __global__ void __launch_bounds__(256) k_head_pack(const __grid_constant__ HeadPack p)
 {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    __shared__ uint4 codes[8][16][5];  // a row's 64 bytes, and 16 that keep rows out of each other's banks
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warp = threadIdx.x >> 5;
     const Head4 &w = p.w;
     const int64_t units = (int64_t)w.tiles * w.units_per_tile;
     pdl_release();
     pdl_wait();
-    for (int64_t unit = blockIdx.x * 8ll + (threadIdx.x >> 5); unit < units; unit += gridDim.x * 8ll) {
+    for (int64_t unit = blockIdx.x * 8ll + warp; unit < units; unit += gridDim.x * 8ll) {
         const int64_t v0 = unit / w.units_per_tile * kHeadRows4;
         const int k0 = (int)(unit % w.units_per_tile) * kUnitCols;
         unsigned char *out = p.out + unit * w.unit_bytes;
-        auto code = [&](int row, int col) -> uint32_t {  // col is even: two codes of a byte; 8 where there is no weight
-            return v0 + row < w.vocab && col < w.width ? p.codes[(v0 + row) * p.codes_stride + col / 2] : 0x88u;
-        };
+        __syncwarp();
+#pragma unroll
+        for (int i = lane; i < 64; i += 32) {
+            const int row = i >> 2, part = i & 3;
+            uint4 x = make_uint4(kCodeSigns, kCodeSigns, kCodeSigns, kCodeSigns);  // codes of 8 where there is no weight
+            if (v0 + row < w.vocab && k0 + part * 32 < w.width) {  // the width is a multiple of 32
+                const uint8_t *from = p.codes + (v0 + row) * p.codes_stride + k0 / 2 + part * 16;
+                if (p.vec) {
+                    x = __ldcs((const uint4 *)from);
+                } else {
+                    uint32_t e[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) e[j] = from[4 * j] | from[4 * j + 1] << 8 | from[4 * j + 2] << 16 | (uint32_t)from[4 * j + 3] << 24;
+                    x = make_uint4(e[0], e[1], e[2], e[3]);
+                }
+            }
+            codes[warp][row][part] = x;
+        }
+        __syncwarp();
+        auto code = [&](int row, int col) -> uint32_t { return ((const uint8_t *)codes[warp][row])[col / 2]; };  // col is even: two codes of a byte
 #pragma unroll
         for (int block = 0; block < 2; block++) {
             uint32_t word[4];
 #pragma unroll
             for (int s = 0; s < 4; s++) {
-                const int col = k0 + block * 64 + 32 * (s / 2) + 8 * t + 4 * (s % 2);
+                const int col = block * 64 + 32 * (s / 2) + 8 * t + 4 * (s % 2);
                 const uint32_t a = code(g, col), b = code(g + 8, col), c = code(g, col + 2), d = code(g + 8, col + 2);
                 word[s] = (a & 15u) | (b & 15u) << 4 | (c & 15u) << 8 | (d & 15u) << 12 | (a >> 4) << 16 | (b >> 4) << 20 | (c >> 4) << 24 | (d >> 4) << 28;
             }
@@ -538,6 +558,7 @@ static int head_pack(StgHandle h, const StgHeadPack *b, cudaStream_t stream)
     const OnDevice on(h->cfg.device);
     CK(on.error);
     p.codes = (const uint8_t *)b->codes; p.codes_stride = b->codes_stride;
+    p.vec = !misaligned(b->codes, 16) && b->codes_stride % 16 == 0;
     p.scales = (const uint16_t *)b->scales; p.zeros = (const uint16_t *)b->zeros;
     p.out = (unsigned char *)b->packed;
     CK(launch_behind(k_head_pack, dim3((unsigned)h->sm_count * 8), 256, 0, stream, p));
