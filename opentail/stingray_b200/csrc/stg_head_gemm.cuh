@@ -12,8 +12,9 @@
 // (weight and hidden states of the two gradients' products, gradients transposed): nothing is transposed in memory.
 //
 // The tensor cores' additions lose up to a step of the running sum each, always towards zero.  For the losses a sum is therefore
-// kept for kAccBlocks * 64 columns at most and the parts are added up in registers, which costs nothing next to the products
-// (8192 x 4096 x 151,936: the normalisers' error 1.7e-6 without, relative).
+// kept for kAccBlocks * 64 columns at most and the parts are added up in registers (8192 x 4096 x 151,936: the normalisers are 3.7e-7 off,
+// 1.7e-6 without, relative).  Pairs take 1024 columns, which costs nothing next to their products (512: 7.9 ms in place of 7.3); single CTAs,
+// which wait for memory, 512 (64 x 4096 x 151,936: 1.8e-7 off).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -50,7 +51,8 @@ struct HeadGemm {
     int a_at;
 };
 
-constexpr int kAccBlocks = 16;
+template <bool PAIR>
+constexpr int kAccBlocks = PAIR ? 16 : 8;
 constexpr int kGemmThreads = 64 + 32 * kGemmEpiWarps;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -151,7 +153,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
     const int splits = MODE == kHidden ? g.info->splits : 1;
     const int tiles = tiles_m * tiles_n * splits;
     const int blocks = ((MODE == kWeight ? used : g.k) + kGemmK - 1) / kGemmK;
-    const int part = MODE == kStats ? kAccBlocks : 1 << 30;  // blocks of an accumulator
+    const int part = MODE == kStats ? kAccBlocks<PAIR> : 1 << 30;  // blocks of an accumulator
     const int first_tile = blockIdx.x / kCtas, step = gridDim.x / kCtas;
 
     if (warp == 0) {
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                 const bool rows_here = m0 + quarter * 32 < used;  // of this warp
                 const int target = r >= used ? -1 : g.targets ? g.targets[r] : g.rows[r].target;
                 float z[8][16];
-                for (int k0 = 0; k0 < blocks; k0 += kAccBlocks) {
+                for (int k0 = 0; k0 < blocks; k0 += kAccBlocks<PAIR>) {
                     const uint32_t from = full_unit();
                     if (!ok) break;
 #pragma unroll
