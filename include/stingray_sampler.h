@@ -607,8 +607,9 @@ typedef struct StgHeadLoss {
 /* Bytes of workspace for a call of these sizes (rows, vocab, width; other fields are only checked for what they allow). */
 STG_API int stg_head_loss_workspace(StgHandle handle, const StgHeadLoss *loss, int32_t backward, uint64_t *out_bytes);
 STG_API int stg_head_loss(StgHandle handle, const StgHeadLoss *loss, void *stream);
-/* Gradients of sum(grad_loss * loss + grad_log_norms * log_norms).  The gradients of the logits are rounded to `dtype` once, scaled by
- * a power of two of their largest factor so that fp16 holds them too; sums are fp32 and outputs rounded once.  Deterministic. */
+/* Gradients of sum(grad_loss * loss + grad_log_norms * log_norms).  The gradients of the logits are rounded to `dtype`, scaled by a power
+ * of two of their largest factor so that fp16 holds them too; what that takes from the target's of each row - up to 64 rows: from
+ * all - is made good.  Sums are fp32, outputs rounded once.  Deterministic. */
 STG_API int stg_head_loss_backward(StgHandle handle, const StgHeadLoss *loss, void *stream);
 
 /* A weight in 4 bits: weight[v][k] = (code[v][k] - zero[v][k / group]) * scale[v][k / group], codes 0 .. 15, two columns to a byte,
