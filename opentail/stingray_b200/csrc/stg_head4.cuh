@@ -37,10 +37,10 @@ __device__ __forceinline__ uint32_t bits_of(uint32_t x, uint32_t mask, uint32_t 
     return r;
 }
 
-// Eight neighbouring hidden states.
+// Eight neighbouring hidden states.  (Not as read-only data: the kernel ahead may still have been writing them when this one began.)
 __device__ __forceinline__ uint4 eight_states(const uint16_t *from, bool vec)
 {
-    if (vec) return __ldg((const uint4 *)from);
+    if (vec) return *(const uint4 *)from;
     uint32_t e[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) e[j] = from[j];

@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
     const uint32_t tmem = tmem_slot;
     pdl_release();
     pdl_wait();
-    asm volatile("fence.proxy.async;" ::: "memory");  // what the kernels ahead have written is read by TMA
+    async_fence();  // what the kernels ahead have written is read by TMA
 
     const int used = MODE == kStats && g.targets ? g.used_rows : g.info->used;
     const int tiles_m = ((MODE == kWeight ? g.m : used) + kTileM - 1) / kTileM;

@@ -444,6 +444,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1) k_head_stream(const __gr
     }
     pdl_release();
     pdl_wait();
+    async_fence();  // the weight may have been packed by the kernel ahead
     auto load = [&](int c) {  // lane 0
         const int n = min(s.chunk, u1 - u0 - c * s.chunk), stage = c % kStreamStages;
         bar_expect(bar + 8 * stage, (uint32_t)(n * w.unit_bytes));

@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(128) k_head_gather(const __grid_constant__ Hea
     for (int i = threadIdx.x; i < width / 8; i += 128) {
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (from && vec) {
-            v = __ldg((const uint4 *)from + i);
+            v = ((const uint4 *)from)[i];  // (not as read-only data: a kernel ahead may still have been writing it when this one began)
         } else if (from) {
             uint32_t e[8];
 #pragma unroll

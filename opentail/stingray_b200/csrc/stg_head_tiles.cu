@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(TilesWarps<ZEROS, G, C>::kThreads, 1) k_head_t
     const uint32_t tmem = tmem_slot;
     pdl_release();
     pdl_wait();
+    async_fence();  // what the kernels ahead have written - hidden states, groups' sums, the packed weight - is read by bulk copies
     const int items = a.items_v * a.blocks, per = w.units_per_tile;
 
     if (warp == 0) {  // hidden states
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(TilesWarps<ZEROS, G, C>::kThreads, 1) k_head_t
             for (int i = 0; i < kCols; i++) {
                 const int r = r0 + i;
                 if (mine && r < a.p.rows) {
-                    const float2 un = __ldg(a.unscale + r);
+                    const float2 un = a.unscale[r];
                     const float x = ((i & 1) ? acc[i / 2].y : acc[i / 2].x) * un.x * un.y;
                     if (a.p.out_bf16) ((__nv_bfloat16 *)a.p.out)[r * a.p.out_stride + v] = __float2bfloat16_rn(x);
                     else ((float *)a.p.out)[r * a.p.out_stride + v] = x;

@@ -87,6 +87,8 @@ __device__ __forceinline__ void tma_store(const CUtensorMap *map, int x, int y, 
 __device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }  // the thread's stores have read shared memory
 __device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// What other kernels or threads have written with ordinary stores, as far as this thread sees it, is seen by the copies that it issues from here on.
+__device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async;" ::: "memory"); }
 __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void shared_store(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 {
