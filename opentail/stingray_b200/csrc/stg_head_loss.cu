@@ -209,9 +209,9 @@ __global__ void __launch_bounds__(128) k_head_join(const __grid_constant__ HeadW
     if ((tid & 31) == 0) sums[tid >> 5] = sum;
     __syncthreads();
     if (tid == 0) {
-        const double norm = (double)all + log(sums[0] + sums[1] + sums[2] + sums[3]);
-        norms[r] = (float)norm;
-        loss[r] = (float)(norm - (double)ws.hit[at]);
+        const double rest = log(sums[0] + sums[1] + sums[2] + sums[3]);
+        norms[r] = (float)((double)all + rest);
+        loss[r] = (float)((double)all - (double)ws.hit[at] + rest);  // what the target lacks to the largest logit, exactly, and nothing of either's size
     }
 }
 
