@@ -502,6 +502,46 @@ class BatchSampler:
             raise StingrayError(-n, self._error(self._h))
         return n
 
+    # -- streams --------------------------------------------------------------------------------------
+    def _aside(self, stream):
+        """torch's object of the stream that a call is given, or None where that is the current one, or none."""
+        if stream is None:
+            return None
+        import torch
+
+        raw = getattr(stream, "cuda_stream", stream)
+        if raw == torch._C._cuda_getCurrentRawStream(self.device):
+            return None
+        if isinstance(stream, torch.cuda.Stream):
+            return stream
+        # (an ExternalStream of handle 0 would be some other stream)
+        return torch.cuda.ExternalStream(raw, device=f"cuda:{self.device}") if raw else torch.cuda.default_stream(self.device)
+
+    def _result(self, shape, dtype, aside):
+        """A tensor that a call writes on the stream ``aside`` (None: the current one).  Its memory is taken in that stream's order,
+        so that nothing enqueued elsewhere still has it, and does not come back before what the current stream - the caller's, who
+        reads it there - had enqueued by the time it is dropped."""
+        import torch
+
+        if aside is None:
+            return torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
+        current = torch.cuda.current_stream(self.device)
+        with torch.cuda.stream(aside):
+            x = torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
+        x.record_stream(current)
+        return x
+
+    @staticmethod
+    def _lend(aside, *tensors):
+        """What a call reads or writes on ``aside`` does not come back before that stream is through with it, also where the caller
+        drops it at once.  Not for a handle of the caller's own stream, which may be gone by the time."""
+        import torch
+
+        if aside is not None and not isinstance(aside, torch.cuda.ExternalStream):
+            for x in tensors:
+                if x is not None and x.numel() > 0:
+                    x.record_stream(aside)
+
     # -- beam search ----------------------------------------------------------------------------------
     def _stream_here(self, stream) -> Optional[int]:
         if stream is not None:
@@ -646,7 +686,7 @@ class BatchSampler:
                              f"got {x.dtype} {tuple(shape)} on {x.device}")
         return x.data_ptr(), x.stride(0) if shape[0] > 1 else shape[1], dtype
 
-    def _head_workspace(self, key, ask, b, stream):
+    def _head_workspace(self, key, ask, b, aside):
         """A call's own workspace, in the order of the stream that uses it; in a graph's memory where that stream is captured.
         ``key``: what its size depends on, which the library is asked for once."""
         import torch
@@ -660,20 +700,17 @@ class BatchSampler:
             size = self._head_sizes[key] = int(n.value)
         if size == 0:
             return None
-        dev = f"cuda:{self.device}"
-        if stream is None:
-            ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        if aside is None:
+            ws = torch.empty(size, dtype=torch.uint8, device=f"cuda:{self.device}")
         else:
-            if not isinstance(stream, torch.cuda.Stream):
-                stream = torch.cuda.ExternalStream(stream, device=dev)
-            with torch.cuda.stream(stream):
-                ws = torch.empty(size, dtype=torch.uint8, device=dev)
+            with torch.cuda.stream(aside):
+                ws = torch.empty(size, dtype=torch.uint8, device=f"cuda:{self.device}")
         b.workspace, b.workspace_bytes = ws.data_ptr(), size
         return ws
 
-    def _loss_workspace(self, b, backward: bool, stream):
+    def _loss_workspace(self, b, backward: bool, aside):
         return self._head_workspace((b.rows, b.vocab, b.width, backward),
-                                    lambda n: self._lib.stg_head_loss_workspace(self._h, C.byref(b), 1 if backward else 0, C.byref(n)), b, stream)
+                                    lambda n: self._lib.stg_head_loss_workspace(self._h, C.byref(b), 1 if backward else 0, C.byref(n)), b, aside)
 
     def _head_loss(self, hidden, weight, targets, softcap):
         import torch
@@ -693,13 +730,14 @@ class BatchSampler:
         previous call with as many rows, whose tensors are written again."""
         import torch
 
-        b = self._head_loss(hidden, weight, targets, softcap)
+        b, aside = self._head_loss(hidden, weight, targets, softcap), self._aside(stream)
         if out is None:
-            out = {n: torch.empty(b.rows, dtype=torch.float32, device=hidden.device) for n in ("loss", "log_norms")}
+            out = {n: self._result((b.rows,), torch.float32, aside) for n in ("loss", "log_norms")}
         b.loss = self._beam_array("out['loss']", out["loss"], torch.float32, (b.rows,))
         b.log_norms = self._beam_array("out['log_norms']", out["log_norms"], torch.float32, (b.rows,))
-        ws = self._loss_workspace(b, False, stream)  # noqa: F841 (held until the call is enqueued)
+        ws = self._loss_workspace(b, False, aside)  # noqa: F841 (held until the call is enqueued)
         self._check(self._lib.stg_head_loss(self._h, C.byref(b), self._stream_here(stream)))
+        self._lend(aside, hidden, weight, targets, out["loss"], out["log_norms"])
         return out
 
     def head_loss_backward(self, hidden, weight, targets, log_norms, grad_loss, *, grad_log_norms=None, softcap: float = 0.0,
@@ -711,7 +749,7 @@ class BatchSampler:
         shapes and options, whose tensors are written again."""
         import torch
 
-        b = self._head_loss(hidden, weight, targets, softcap)
+        b, aside = self._head_loss(hidden, weight, targets, softcap), self._aside(stream)
         f32, rows = torch.float32, (b.rows,)
         b.log_norms = self._beam_array("log_norms", log_norms, f32, rows)
         b.grad_loss = self._beam_array("grad_loss", grad_loss, f32, rows)
@@ -723,11 +761,12 @@ class BatchSampler:
         if want_weight:
             shapes["grad_weight"] = (b.vocab, b.width)
         if out is None:
-            out = {n: torch.empty(s, dtype=weight.dtype, device=weight.device) for n, s in shapes.items()}
+            out = {n: self._result(s, weight.dtype, aside) for n, s in shapes.items()}
         for n, s in shapes.items():
             setattr(b, n, self._beam_array(f"out[{n!r}]", out[n], weight.dtype, s))
-        ws = self._loss_workspace(b, True, stream)  # noqa: F841
+        ws = self._loss_workspace(b, True, aside)  # noqa: F841
         self._check(self._lib.stg_head_loss_backward(self._h, C.byref(b), self._stream_here(stream)))
+        self._lend(aside, hidden, weight, targets, log_norms, grad_loss, grad_log_norms, *(out[n] for n in shapes))
         return out
 
     def head_pack(self, codes, scales, zeros=None, *, stream=None) -> PackedHead:
@@ -750,9 +789,11 @@ class BatchSampler:
             b.zeros = self._beam_array("zeros", zeros, scales.dtype, scales.shape)
         n = C.c_uint64(0)
         self._check(self._lib.stg_head_pack_bytes(self._h, b.vocab, b.width, b.group, 0 if zeros is None else 1, C.byref(n)))
-        packed = torch.empty(int(n.value), dtype=torch.uint8, device=codes.device)
+        aside = self._aside(stream)
+        packed = self._result((int(n.value),), torch.uint8, aside)
         b.packed, b.packed_bytes = packed.data_ptr(), int(n.value)
         self._check(self._lib.stg_head_pack(self._h, C.byref(b), self._stream_here(stream)))
+        self._lend(aside, codes, scales, zeros, packed)
         return PackedHead(packed, b.vocab, b.width, b.group, dtype, zeros is not None)
 
     def head_logits(self, hidden, head: PackedHead, *, dtype=None, stream=None, out=None):
@@ -764,17 +805,18 @@ class BatchSampler:
         if head.device_index != self.device:
             raise ValueError(f"the head lies on cuda:{head.device_index}, the handle on cuda:{self.device}")
         hp, hs, hd = self._head_rows("hidden", hidden, _half_dtypes(), head.width)
-        rows = hidden.shape[0]
+        rows, aside = hidden.shape[0], self._aside(stream)
         if out is None:
-            out = torch.empty((rows, head.vocab), dtype=torch.float32 if dtype is None else dtype, device=hidden.device)
+            out = self._result((rows, head.vocab), torch.float32 if dtype is None else dtype, aside)
         elif dtype is not None and out.dtype != dtype or out.shape[0] != rows:
             raise ValueError(f"out must be {dtype or out.dtype} with {rows} rows, got {out.dtype} {tuple(out.shape)}")
         op, os_, od = self._head_rows("out", out, _logits_dtypes(), head.vocab)
         b = N.StgHeadLogits(C.sizeof(N.StgHeadLogits), rows, head.vocab, head.width, head.group, head.scale_dtype, 1 if head.has_zeros else 0, hd, od,
                             head.packed.data_ptr(), head.nbytes, hp, hs, op, os_)
         ws = self._head_workspace((rows, head.vocab, head.width, head.group, head.has_zeros),  # noqa: F841
-                                  lambda n: self._lib.stg_head_logits_workspace(self._h, C.byref(b), C.byref(n)), b, stream)
+                                  lambda n: self._lib.stg_head_logits_workspace(self._h, C.byref(b), C.byref(n)), b, aside)
         self._check(self._lib.stg_head_logits(self._h, C.byref(b), self._stream_here(stream)))
+        self._lend(aside, hidden, head.packed, out)
         return out
 
     # -- vocabulary-sharded mode ---------------------------------------------------------------------
