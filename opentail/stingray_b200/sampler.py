@@ -169,13 +169,13 @@ class BatchSampler:
 
         return torch.cuda.current_stream().cuda_stream
 
-    def _alloc(self, shape, dtype, host: bool):
+    def _alloc(self, shape, dtype, host: bool, stream=None):
         if host:
             return np.empty(shape, dtype)
         import torch
 
         td = {np.int32: torch.int32, np.float32: torch.float32, np.uint32: torch.int32}[dtype]
-        return torch.empty(shape, dtype=td, device=f"cuda:{self.device}")
+        return self._result(shape, td, self._aside(stream))
 
     def _batch(self, logits, params, history_ids, history_offsets, mask, row_uses_mask, bias,
                uniforms, softcap: float = 0.0, history_ring: bool = False):
@@ -254,7 +254,7 @@ class BatchSampler:
         rows, width = logits.shape
         vocab = width if valid_len is None else valid_len
         dtype = {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16}[logits.dtype]
-        out = torch.empty((rows, 2), dtype=torch.int32, device=logits.device)
+        out = self._result((rows, 2), torch.int32, self._aside(stream))
         self._check(self._lib.stg_argmax_rows(self._h, logits.data_ptr(), dtype, rows, vocab,
                                               logits.stride(0) if rows > 1 else width,
                                               out.data_ptr(), self._stream(stream)))
@@ -286,7 +286,7 @@ class BatchSampler:
                 if tuple(arr.shape) != tuple(shape):
                     raise ValueError(f"out[{name!r}] has shape {tuple(arr.shape)}, this call needs {tuple(shape)}")
                 return arr
-            return self._alloc(shape, dtype, host)
+            return self._alloc(shape, dtype, host, stream)
 
         out = {"tokens": take("tokens", (rows,), np.int32)}
         b.tokens = _ptr(out["tokens"])
@@ -313,7 +313,7 @@ class BatchSampler:
         """``Sampler.BuildFilteredDistribution`` for every row: returns ``[rows, vocab]`` float32."""
         b, keep = self._batch(logits, params, history_ids, history_offsets, mask, None, bias, None, softcap)
         host = (not _is_torch(logits)) if host_outputs is None else host_outputs
-        probs = self._alloc((b.rows, b.vocab), np.float32, host)
+        probs = self._alloc((b.rows, b.vocab), np.float32, host, stream)
         if host:
             b.mem_flags |= N.MEM_HOST_OUTPUTS
         self._check(self._lib.stg_build_distribution(self._h, C.byref(b), _ptr(probs),
@@ -326,9 +326,9 @@ class BatchSampler:
         full-vocabulary pipeline whatever ``TopK`` is.  ``logits`` is a CUDA tensor; returns
         (tokens, probs ``[rows, vocab]`` or None), both on the device."""
         b, keep = self._batch(logits, params, history_ids, history_offsets, mask, None, None, uniforms, softcap)
-        tokens = self._alloc((b.rows,), np.int32, False)
+        tokens = self._alloc((b.rows,), np.int32, False, stream)
         b.tokens = _ptr(tokens)
-        probs = self._alloc((b.rows, b.vocab), np.float32, False) if want_probs else None
+        probs = self._alloc((b.rows, b.vocab), np.float32, False, stream) if want_probs else None
         self._check(self._lib.stg_sample_with_distribution(self._h, C.byref(b), _ptr(probs), self._stream(stream)))
         return tokens, probs
 
@@ -342,8 +342,8 @@ class BatchSampler:
         if not _is_torch(uniforms):
             uniforms = np.ascontiguousarray(uniforms, dtype=np.float32)
             flags |= N.MEM_HOST_UNIFORMS
-        tokens = self._alloc((rows,), np.int32, False)
-        rf = self._alloc((rows,), np.uint32, False)
+        tokens = self._alloc((rows,), np.int32, False, stream)
+        rf = self._alloc((rows,), np.uint32, False, stream)
         self._check(self._lib.stg_sample_from_probs(self._h, probs.data_ptr(), rows, vocab, probs.stride(0) if rows > 1 else vocab,
                                                     _ptr(uniforms), _ptr(tokens), _ptr(rf), flags, self._stream(stream)))
         return tokens, rf
@@ -363,8 +363,8 @@ class BatchSampler:
         if not _is_torch(uniforms):
             uniforms = np.ascontiguousarray(uniforms, dtype=np.float32).reshape(rows, 2)
             flags |= N.MEM_HOST_UNIFORMS
-        tokens = self._alloc((rows,), np.int32, False)
-        rf = self._alloc((rows,), np.uint32, False)
+        tokens = self._alloc((rows,), np.int32, False, stream)
+        rf = self._alloc((rows,), np.uint32, False, stream)
         self._check(self._lib.stg_resample_residual(self._h, p.data_ptr(), q.data_ptr(), rows, vocab,
                                                     p.stride(0) if rows > 1 else vocab, _ptr(uniforms), _ptr(tokens),
                                                     _ptr(rf), flags, self._stream(stream)))
@@ -389,11 +389,9 @@ class BatchSampler:
         if not _is_torch(uniforms):
             uniforms = np.ascontiguousarray(uniforms, dtype=np.float64)
             flags |= N.MEM_HOST_UNIFORMS
-        dev = target_logits.device
-        accepted = torch.empty(n_seq, dtype=torch.int32, device=dev)
-        correction = torch.empty(n_seq, dtype=torch.int32, device=dev)
-        aprobs = torch.empty((n_seq, max(L, 1)), dtype=torch.float32, device=dev)
-        sflags = torch.empty(n_seq, dtype=torch.int32, device=dev)
+        aside = self._aside(stream)
+        accepted, correction, sflags = (self._result((n_seq,), torch.int32, aside) for _ in range(3))
+        aprobs = self._result((n_seq, max(L, 1)), torch.float32, aside)
         b = N.StgSpecBatch()
         b.struct_size = C.sizeof(N.StgSpecBatch)
         b.n_seq, b.n_draft, b.vocab, b.logits_dtype, b.mode = n_seq, L, vocab, dtype, mode
@@ -417,9 +415,8 @@ class BatchSampler:
 
         rows, vocab = logits.shape
         dtype = {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16}[logits.dtype]
-        acc = torch.empty(rows, dtype=torch.int32, device=logits.device)
-        am = torch.empty(rows, dtype=torch.int32, device=logits.device)
-        pr = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        aside = self._aside(stream)
+        acc, am, pr = (self._result((rows,), t, aside) for t in (torch.int32, torch.int32, torch.float32))
         self._check(self._lib.stg_mtp_accept(self._h, logits.data_ptr(), dtype, rows, vocab,
                                              logits.stride(0) if rows > 1 else vocab,
                                              draft_tokens.data_ptr(), p_min, acc.data_ptr(),
@@ -434,8 +431,8 @@ class BatchSampler:
 
         n_masks, rows, words = masks.shape
         assert masks.is_contiguous() and masks.dtype == torch.int32
-        out = torch.empty((rows, words), dtype=torch.int32, device=masks.device)
-        uses = torch.empty(rows, dtype=torch.uint8, device=masks.device)
+        aside = self._aside(stream)
+        out, uses = self._result((rows, words), torch.int32, aside), self._result((rows,), torch.uint8, aside)
         self._check(self._lib.stg_and_masks(self._h, C.c_void_p(masks.data_ptr()), n_masks, rows, vocab,
                                             C.c_int64(words), C.c_void_p(out.data_ptr()), C.c_int64(words),
                                             C.c_void_p(uses.data_ptr()), self._stream(stream)))
@@ -472,9 +469,8 @@ class BatchSampler:
         k = np.ascontiguousarray(keys, dtype=np.uint64)
         rows, per = k.shape
         words = (vocab + 31) // 32
-        dev = f"cuda:{self.device}"
-        out = torch.empty((rows, words), dtype=torch.int32, device=dev)
-        uses = torch.empty(rows, dtype=torch.uint8, device=dev)
+        aside = self._aside(stream)
+        out, uses = self._result((rows, words), torch.int32, aside), self._result((rows,), torch.uint8, aside)
         self._check(self._lib.stg_mask_compose(self._h, k.ctypes.data, per, rows, vocab,
                                                {"and": N.MASK_AND, "or": N.MASK_OR}[op], C.c_void_p(out.data_ptr()),
                                                C.c_int64(words), C.c_void_p(uses.data_ptr()), self._stream(stream)))
@@ -589,14 +585,14 @@ class BatchSampler:
         elif row_uses_mask is not None:
             raise ValueError("row_uses_mask without a mask")
         if out is None:
-            dev = logits.device
-            out = {"tokens": torch.empty((n_seq, n), dtype=torch.int32, device=dev),
-                   "parents": torch.empty((n_seq, n), dtype=torch.int32, device=dev),
-                   "scores": torch.empty((n_seq, n), dtype=torch.float32, device=dev)}
+            aside = self._aside(stream)
+            out = {"tokens": self._result((n_seq, n), torch.int32, aside),
+                   "parents": self._result((n_seq, n), torch.int32, aside),
+                   "scores": self._result((n_seq, n), torch.float32, aside)}
             if want_norms:
-                out["log_norms"] = torch.empty((n_seq, beams), dtype=torch.float32, device=dev)
+                out["log_norms"] = self._result((n_seq, beams), torch.float32, aside)
             if want_flags:
-                out["flags"] = torch.empty(n_seq, dtype=torch.int32, device=dev)
+                out["flags"] = self._result((n_seq,), torch.int32, aside)
         b = N.StgBeamBatch(
             C.sizeof(N.StgBeamBatch), n_seq, beams, vocab, dtype, n, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, sp, mp, mstride, up,
             softcap, self._beam_array("out['tokens']", out["tokens"], torch.int32, (n_seq, n)),
@@ -665,8 +661,9 @@ class BatchSampler:
         n_steps, n_seq, beams = trail_tokens.shape
         hyps = steps.shape[1]
         if out is None:
-            out = {"sequences": torch.empty((n_seq, hyps, n_steps), dtype=torch.int32, device=trail_tokens.device),
-                   "lengths": torch.empty((n_seq, hyps), dtype=torch.int32, device=trail_tokens.device)}
+            aside = self._aside(stream)
+            out = {"sequences": self._result((n_seq, hyps, n_steps), torch.int32, aside),
+                   "lengths": self._result((n_seq, hyps), torch.int32, aside)}
         i32, shape, trail = torch.int32, (n_seq, hyps), (n_steps, n_seq, beams)
         self._check(self._lib.stg_beam_backtrace(
             self._h, self._beam_array("trail_tokens", trail_tokens, i32, trail), self._beam_array("trail_parents", trail_parents, i32, trail),
@@ -879,18 +876,18 @@ class BatchSampler:
             keep.append(uniforms)
             b.uniforms = _ptr(uniforms)
         b.mem_flags = flags
-        out = {"tokens": self._alloc((rows,), np.int32, False)}
+        out = {"tokens": self._alloc((rows,), np.int32, False, stream)}
         b.tokens = _ptr(out["tokens"])
         if want_probs:
-            out["probs"] = self._alloc((rows,), np.float32, False)
+            out["probs"] = self._alloc((rows,), np.float32, False, stream)
             b.token_probs = _ptr(out["probs"])
         if want_flags:
-            out["flags"] = self._alloc((rows,), np.uint32, False)
+            out["flags"] = self._alloc((rows,), np.uint32, False, stream)
             b.row_flags = _ptr(out["flags"])
         if want_topk:
-            out["topk_ids"] = self._alloc((rows, want_topk), np.int32, False)
-            out["topk_logits"] = self._alloc((rows, want_topk), np.float32, False)
-            out["topk_probs"] = self._alloc((rows, want_topk), np.float32, False)
+            out["topk_ids"] = self._alloc((rows, want_topk), np.int32, False, stream)
+            out["topk_logits"] = self._alloc((rows, want_topk), np.float32, False, stream)
+            out["topk_probs"] = self._alloc((rows, want_topk), np.float32, False, stream)
             b.topk_ids, b.topk_logits = _ptr(out["topk_ids"]), _ptr(out["topk_logits"])
             b.topk_probs, b.topk_stride = _ptr(out["topk_probs"]), want_topk
         self._check(self._lib.stg_shard_finish(self._h, C.byref(b), global_vocab, self._stream(stream)))
