@@ -33,8 +33,9 @@ struct HeadWs {
     int32_t *place;     // [rows]: its place among the used rows, -1: no loss, -2: its target lies outside the vocabulary
     void *hidden;       // [padded rows, width]: hidden states of the used rows
     float *hit;         // [padded rows]: the target's logit; backward: what rounding takes from its gradient
-    int32_t *first;     // backward, more than 64 rows: [vocab]: the last of the used rows with this target, -1: none; and
-    int32_t *next;      // [padded rows]: the one ahead of it with the same target
+    int32_t *first;     // backward, more than 64 rows: [vocab]: where the used rows with this target begin in `order`, -1: there are none;
+    int32_t *order;     // [padded rows]: the used rows by their targets, those of one target in their order; and
+    int32_t *count;     // [padded rows]: where a target's rows begin, their number
     float2 *parts;      // [padded rows, two per tile of the vocabulary]: largest logit and the sum of exp relative to it
     void *grads;        // [padded rows, piece]: gradients of a piece's logits
     float *sums;        // [splits, used rows up to a multiple of kHeadTileM, width]: gradients of the hidden states so far

@@ -44,7 +44,7 @@ struct HeadGemm {
     float *hit;
     void *out;          // where map_out's rows lie, and elements between them
     int64_t out_stride;
-    const int32_t *first_of, *next;  // kWeight: HeadWs, or NULL
+    const int32_t *first_of, *order, *count;  // kWeight: HeadWs, or NULL
     const uint16_t *hidden;       // kWeight: [rows, n]
     int a_rows;         // rows of the first operand's boxes: fewer than 128 where there are fewer rows
     int stages, stage_bytes;  // the second operand's boxes ahead of the first's
@@ -114,6 +114,20 @@ struct HeadTile {
         end = (int)((int64_t)blocks * (split + 1) / splits);
     }
 };
+
+// kWeight: the lanes whose entries' rows - `n` of this lane's - the warp goes through together, a lane's after another's.  A lane by itself takes one
+// row after another, at kRestAlone cycles each beside the products' traffic, all lanes at the same time; the warp takes kRestLane for a lane's and
+// kRestRow more for each row.  So no accumulator is held for longer than a bounded wait lasts, however many rows have one target: 8192 rows x
+// 2048 x 32,000 take 2430 us with targets spread evenly, 3150 with the k-th token 1 / k as often as the first (4100 where each lane walked through
+// its own) and 4150 with one target (16,840).
+constexpr unsigned kRestsAlone = 4, kRestAlone = 2000, kRestLane = 2500, kRestRow = 200;
+__device__ __forceinline__ uint32_t rests_together(int n)
+{
+    const uint32_t many = __ballot_sync(0xFFFFFFFFu, n > (int)kRestsAlone);
+    if (many == 0u) return 0u;
+    const unsigned most = __reduce_max_sync(0xFFFFFFFFu, (unsigned)n), all = __reduce_add_sync(0xFFFFFFFFu, n > (int)kRestsAlone ? (unsigned)n : 0u);
+    return (uint64_t)most * kRestAlone > (uint64_t)__popc(many) * kRestLane + (uint64_t)all * kRestRow ? many : 0u;
+}
 
 template <int MODE, bool BF16, bool CAP, bool PAIR>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -239,14 +253,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
         const float by_cap = CAP ? fminf(1.f / g.cap, 3.0e38f) : 0.f;  // a cap of almost nothing: 0 stays 0
         uint32_t unit = 0;
         bool ok = true;
-        // kWeight: the last row whose target this thread's entry of a tile is
-        const bool links = MODE == kWeight && g.first_of && g.info->low == 0;
-        auto link_of = [&](int t) {
-            if (t >= tiles) return -1;
+        // kWeight: the rows whose target this thread's entry of a tile is: where they begin in g.order, and their number
+        const bool rests = MODE == kWeight && g.first_of && g.info->low == 0;
+        auto rests_of = [&](int t) {
+            if (t >= tiles) return make_int2(0, 0);
             const int entry = HeadTile(t, tiles_m, tiles_n, g.group, splits, blocks).m * kTileM + (int)rank * kHeadTileM + quarter * 32 + lane;
-            return entry < g.m ? g.first_of[g.first + entry] : -1;
+            const int first = entry < g.m ? g.first_of[g.first + entry] : -1;
+            return first < 0 ? make_int2(0, 0) : make_int2(first, g.count[first]);
         };
-        int next_link = links ? link_of(first_tile) : -1;
+        int2 next_rests = rests ? rests_of(first_tile) : make_int2(0, 0);
         for (int t = first_tile; ok && t < tiles; t += step) {
             const HeadTile tile(t, tiles_m, tiles_n, g.group, splits, blocks);
             const int m0 = tile.m * kTileM + rank * kHeadTileM, tn = tile.n, n0 = tn * g.tile_n;
@@ -327,12 +342,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                 const bool rows_here = r0 < (MODE == kWeight ? g.m : MODE == kHidden ? slab : g.rows_pad) && (some || MODE != kHidden || g.first == 0);
                 HeadRow row = {};
                 if (MODE == kGrad && rows_here) row = g.rows[r];
-                int link = -1;
-                if (MODE == kWeight && links) {  // read a tile ahead
-                    link = next_link;
-                    next_link = link_of(t + step);
+                int2 mine = make_int2(0, 0);
+                uint32_t together = 0u;
+                if (MODE == kWeight && rests) {  // read a tile ahead
+                    mine = next_rests;
+                    next_rests = rests_of(t + step);
+                    together = rests_together(mine.y);
                 }
-                const bool linked = MODE == kWeight && __any_sync(0xFFFFFFFFu, link >= 0);
+                const bool any_rests = MODE == kWeight && __any_sync(0xFFFFFFFFu, mine.y > 0);
                 const uint32_t from = some ? full_unit() : 0u;
                 if (!ok) break;
                 for (int c0 = c_begin; c0 < c_end && rows_here; c0 += kOutChunks) {
@@ -349,8 +366,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                         }
                     }
                     if (some) tmem_loaded();
-                    if (MODE == kWeight && linked) {  // what rounding has taken from the gradients of the rows whose target this is
-                        for (int q = link; q >= 0; q = g.next[q]) {
+                    if (MODE == kWeight && any_rests) {  // what rounding has taken from the gradients of the rows whose target this is
+                        const int own = together >> lane & 1u ? 0 : mine.y;
+                        for (int k = 0; k < own; k++) {
+                            const int q = g.order[mine.x + k];
                             const float rest = g.hit[q];
                             const uint16_t *h = g.hidden + (int64_t)q * g.n + n0 + c0 * 16;
 #pragma unroll
@@ -364,6 +383,39 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                             }
                         }
                         __syncwarp();
+                        for (uint32_t left = together; left != 0u; left &= left - 1u) {  // by the warp: a lane has two columns
+                            const int to = __ffs(left) - 1, begin = __shfl_sync(0xFFFFFFFFu, mine.x, to), n = __shfl_sync(0xFFFFFFFFu, mine.y, to), col = n0 + c0 * 16 + 2 * lane;
+                            float2 sum = make_float2(0.f, 0.f);
+                            for (int k0 = 0; k0 < n; k0 += 32) {  // a lane looks up a row
+                                const int q = k0 + lane < n ? g.order[begin + k0 + lane] : 0;
+                                const float rest = k0 + lane < n ? g.hit[q] : 0.f;
+                                const int here = min(32, n - k0);
+#pragma unroll 8
+                                for (int k = 0; k < here; k++) {
+                                    const int row = __shfl_sync(0xFFFFFFFFu, q, k);
+                                    const float by = __shfl_sync(0xFFFFFFFFu, rest, k);
+                                    const uint32_t e = col < g.n ? *(const uint32_t *)(g.hidden + (int64_t)row * g.n + col) : 0u;
+                                    sum.x = fmaf(by, half_of<BF16>(e), sum.x);
+                                    sum.y = fmaf(by, half_of<BF16>(e >> 16), sum.y);
+                                }
+                            }
+                            if (lane == 0) store_read();
+                            __syncwarp();
+                            shared_store2(out + lane * 8, __float_as_uint(sum.x), __float_as_uint(sum.y));
+                            __syncwarp();
+                            if (lane == to) {
+#pragma unroll
+                                for (int i = 0; i < 16 * kOutChunks; i += 4) {
+                                    const float4 v = shared_load(out + i * 4);
+                                    uint32_t *at = x[i / 16].v + i % 16;
+                                    at[0] = __float_as_uint(__uint_as_float(at[0]) + v.x);
+                                    at[1] = __float_as_uint(__uint_as_float(at[1]) + v.y);
+                                    at[2] = __float_as_uint(__uint_as_float(at[2]) + v.z);
+                                    at[3] = __float_as_uint(__uint_as_float(at[3]) + v.w);
+                                }
+                            }
+                            __syncwarp();
+                        }
                     }
                     uint32_t o[kOutChunks][MODE == kHidden ? 1 : 8];
 #pragma unroll

@@ -113,12 +113,12 @@ __global__ void __launch_bounds__(kPrepThreads) k_head_prep(const __grid_constan
 }
 
 // Hidden states of the rows that have a loss, next to each other, zeros behind them up to whole tiles.
-__global__ void __launch_bounds__(128) k_head_gather(const __grid_constant__ HeadWs ws, const uint16_t *hidden, int64_t stride, int width, bool vec, bool links, int vocab)
+__global__ void __launch_bounds__(128) k_head_gather(const __grid_constant__ HeadWs ws, const uint16_t *hidden, int64_t stride, int width, bool vec, bool order, int vocab)
 {
     pdl_release();
     pdl_wait();
     const int c = blockIdx.x, used = ws.info->used;
-    if (links)  // no row has a target yet (k_head_links)
+    if (order)  // no row has a target yet (k_head_order)
         for (int64_t i = (int64_t)c * 128 + threadIdx.x; i < vocab; i += (int64_t)gridDim.x * 128) ws.first[i] = -1;
     if (c >= (used + kHeadTileM - 1) / kHeadTileM * kHeadTileM) return;
     uint4 *to = (uint4 *)((uint16_t *)ws.hidden + (int64_t)c * width);
@@ -137,36 +137,56 @@ __global__ void __launch_bounds__(128) k_head_gather(const __grid_constant__ Hea
     }
 }
 
-// For each used row the one ahead of it with the same target, and for each target its last row.  Every thread looks through all rows ahead of its
-// own, 1024 at a time in shared memory (8192 rows: 33 million comparisons, 13 us).
-constexpr int kLinkThreads = 64, kLinkRows = 1024;
+// The used rows by their targets, for the remainders in the weight's gradient: a row's place is the number of rows with a smaller target and of those
+// ahead of it with its own.  Four threads to a row look through all rows, 4096 at a time in shared memory.
+constexpr int kOrderThreads = 256, kOrderRows = 4096;
 
-__global__ void __launch_bounds__(kLinkThreads) k_head_links(const __grid_constant__ HeadWs ws)
+__global__ void __launch_bounds__(kOrderThreads) k_head_order(const __grid_constant__ HeadWs ws)
 {
-    __shared__ int4 targets[kLinkRows / 4];
+    __shared__ int4 targets[kOrderRows / 4];
     pdl_release();
     pdl_wait();
-    const int used = ws.info->used, first = blockIdx.x * kLinkThreads, r = first + threadIdx.x;
+    const int used = ws.info->used, first = blockIdx.x * (kOrderThreads / 4), r = first + threadIdx.x / 4, part = threadIdx.x & 3;
     if (ws.info->low > 0 || first >= used) return;
     const int mine = r < used ? ws.rows[r].target : -1;
-    int found = -1;
-    for (int from = 0; from < min(used, first + kLinkThreads); from += kLinkRows) {
+    int smaller = 0, ahead = 0, behind = 0;  // rows with a smaller target, and those with this one ahead of the row and behind it
+    for (int from = 0; from < used; from += kOrderRows) {
         __syncthreads();
-        for (int i = threadIdx.x; i < kLinkRows; i += kLinkThreads) ((int *)targets)[i] = from + i < used ? ws.rows[from + i].target : -2;
+        for (int i = threadIdx.x; i < kOrderRows; i += kOrderThreads) ((int *)targets)[i] = from + i < used ? ws.rows[from + i].target : 0x7FFFFFFF;
         __syncthreads();
-        const int n = min(kLinkRows, r - from);  // rows ahead
+        const int n = (min(kOrderRows, used - from) + 3) / 4, at = r - from, own = at >> 2;  // the row itself is number `at`, if it is among these
+        auto count = [&](int begin, int end, int &same) {
+            int less[4] = {0, 0, 0, 0}, equal[4] = {0, 0, 0, 0};
 #pragma unroll 4
-        for (int i = 0; i < n; i += 4) {
-            const int4 t = targets[i / 4];
-            if (t.x == mine) found = from + i;
-            if (t.y == mine && i + 1 < n) found = from + i + 1;
-            if (t.z == mine && i + 2 < n) found = from + i + 2;
-            if (t.w == mine && i + 3 < n) found = from + i + 3;
+            for (int i = begin + ((part - begin) & 3); i < end; i += 4) {
+                const int4 t = targets[i];
+                less[0] += t.x < mine; equal[0] += t.x == mine;
+                less[1] += t.y < mine; equal[1] += t.y == mine;
+                less[2] += t.z < mine; equal[2] += t.z == mine;
+                less[3] += t.w < mine; equal[3] += t.w == mine;
+            }
+            smaller += (less[0] + less[1]) + (less[2] + less[3]);
+            same += (equal[0] + equal[1]) + (equal[2] + equal[3]);
+        };
+        count(0, min(max(own, 0), n), ahead);
+        count(max(own + 1, 0), n, behind);
+        if (own >= 0 && own < n) {
+            const int i = 4 * own + part, t = ((const int *)targets)[i];
+            smaller += t < mine;
+            ahead += t == mine && i < at;
+            behind += t == mine && i > at;
         }
     }
-    if (r >= used) return;
-    ws.next[r] = found;
-    atomicMax(ws.first + mine, r);
+    for (int o = 1; o < 4; o *= 2) {
+        smaller += __shfl_xor_sync(0xFFFFFFFFu, smaller, o);
+        ahead += __shfl_xor_sync(0xFFFFFFFFu, ahead, o);
+        behind += __shfl_xor_sync(0xFFFFFFFFu, behind, o);
+    }
+    if (r >= used || part != 0) return;
+    ws.order[smaller + ahead] = r;
+    if (ahead > 0) return;
+    ws.first[mine] = smaller;
+    ws.count[smaller] = 1 + behind;
 }
 
 // A row's maxima and sums joined: its normaliser and loss.  `targets`: the rows are the caller's own, else they have been gathered.
@@ -283,7 +303,8 @@ static HeadWs head_layout(const StgHeadLoss *b, bool backward, HeadPlan &p, char
         ws.sums = (float *)take((size_t)p.sums_rows * (size_t)b->width * 4);
         if (b->rows > kLowRows) {
             ws.first = (int32_t *)take((size_t)b->vocab * 4);
-            ws.next = (int32_t *)take(R * 4);
+            ws.order = (int32_t *)take(R * 4);
+            ws.count = (int32_t *)take(R * 4);
         }
     } else {
         ws.parts = (float2 *)take(R * 2 * (size_t)p.tiles_n * sizeof(float2));
@@ -387,16 +408,16 @@ static cudaError_t head_gemm(StgHandle h, bool bf16, bool pair, cudaStream_t str
 
 static bool head_rows_aligned(const StgHeadLoss *b) { return !misaligned(b->hidden, 16) && (b->rows == 1 || b->hidden_stride % 8 == 0); }
 
-static int head_begin(StgHandle h, const StgHeadLoss *b, const HeadWs &ws, const HeadPlan &p, bool backward, bool links, cudaStream_t stream)
+static int head_begin(StgHandle h, const StgHeadLoss *b, const HeadWs &ws, const HeadPlan &p, bool backward, bool order, cudaStream_t stream)
 {
     const HeadPrep prep = {ws, b->rows, b->vocab, b->targets, backward ? b->log_norms : nullptr, b->grad_loss, b->grad_log_norms,
                            b->width, p.tile_m, h->sm_count * kHeadTileM / p.tile_m, (p.piece + kGemmK - 1) / kGemmK, p.sums_rows};
     CK(launch_behind(k_head_prep, dim3(1), kPrepThreads, 0, stream, prep));
-    CK(launch_behind(k_head_gather, dim3((unsigned)p.rows_pad), 128, 0, stream, ws, (const uint16_t *)b->hidden, b->hidden_stride, b->width, head_rows_aligned(b), links,
+    CK(launch_behind(k_head_gather, dim3((unsigned)p.rows_pad), 128, 0, stream, ws, (const uint16_t *)b->hidden, b->hidden_stride, b->width, head_rows_aligned(b), order,
                      b->vocab));
     h->stats.kernel_launches += 2;
-    if (links) {
-        CK(launch_behind(k_head_links, dim3((unsigned)(p.rows_pad + kLinkThreads - 1) / kLinkThreads), kLinkThreads, 0, stream, ws));
+    if (order) {
+        CK(launch_behind(k_head_order, dim3((unsigned)(p.rows_pad + kOrderThreads / 4 - 1) / (kOrderThreads / 4)), kOrderThreads, 0, stream, ws));
         h->stats.kernel_launches++;
     }
     return STG_OK;
@@ -476,8 +497,8 @@ static int head_backward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
         const cuuint32_t box[2] = {32, 32};
         if ((rc = head_map_of(h, &sums_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, ws.sums, size, stride, box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
     }
-    const bool links = b->grad_weight && ws.first;
-    if ((rc = head_begin(h, b, ws, p, true, links, stream))) return rc;
+    const bool order = b->grad_weight && ws.first;
+    if ((rc = head_begin(h, b, ws, p, true, order, stream))) return rc;
     const int64_t tiles_m = (p.rows_pad + p.tile_m - 1) / p.tile_m, tiles_w = (b->width + 255) / 256;
     for (int i = 0; i < p.pieces; i++) {
         const int first = i * p.piece, count = std::min(p.piece, b->vocab - first);
@@ -498,7 +519,7 @@ static int head_backward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
         }
         if (b->grad_weight) {
             g.m = count;
-            g.first_of = links ? ws.first : nullptr; g.next = ws.next; g.hidden = (const uint16_t *)ws.hidden;
+            g.first_of = order ? ws.first : nullptr; g.order = ws.order; g.count = ws.count; g.hidden = (const uint16_t *)ws.hidden;
             g.out = b->grad_weight; g.out_stride = b->width;
             if ((rc = head_map(h, &weight_out, bf16, b->grad_weight, b->width, first + count, b->width, 32))) return rc;
             CK(head_gemm<kWeight>(h, bf16, p.pair, stream, grads_mn, rows_mn, weight_out, g, (int64_t)((count + p.tile_m - 1) / p.tile_m) * tiles_w));
