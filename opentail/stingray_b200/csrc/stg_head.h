@@ -22,7 +22,7 @@ struct HeadInfo {
 // A row that has a loss, in the order of the rows; behind the last one up to a multiple of kHeadTileM rows of zeros.
 struct HeadRow {
     int32_t row, target;
-    float norm2;        // log2(e) * its normaliser
+    float norm;         // its normaliser
     float a, b;         // the gradient of logit v is a * softmax[v] - b * [v == target]
     int32_t low;        // != 0: the row of what rounding to 16 bits takes from another one's gradients
 };

@@ -342,6 +342,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                 const bool rows_here = r0 < (MODE == kWeight ? g.m : MODE == kHidden ? slab : g.rows_pad) && (some || MODE != kHidden || g.first == 0);
                 HeadRow row = {};
                 if (MODE == kGrad && rows_here) row = g.rows[r];
+                row.a *= scale;
+                row.b *= scale;
                 int2 mine = make_int2(0, 0);
                 uint32_t together = 0u;
                 if (MODE == kWeight && rests) {  // read a tile ahead
@@ -422,32 +424,36 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                     for (int c = 0; c < kOutChunks; c++) {
                         const int col = n0 + (c0 + c) * 16;
                         if constexpr (MODE == kGrad) {
-                            float d[16];
+                            float d[16], slope[16];
 #pragma unroll
                             for (int i = 0; i < 16; i++) {
-                                float slope = scale, z = x[c].f(i);
+                                float logit = x[c].f(i);
                                 if (CAP) {
-                                    const Capped capped = head_cap(z, g.cap, by_cap);
-                                    z = capped.z;
-                                    slope *= 1.f - capped.tanh * capped.tanh;
+                                    const Capped capped = head_cap(logit, g.cap, by_cap);
+                                    logit = capped.z;
+                                    slope[i] = 1.f - capped.tanh * capped.tanh;
                                 }
-                                d[i] = row.a * exp2_fast(fmaf(z, kLog2e, -row.norm2));
-                                if (g.first + col + i == row.target) d[i] -= row.b;
-                                d[i] = r < used ? d[i] * slope : 0.f;
+                                d[i] = row.a * exp2_fast((logit - row.norm) * kLog2e);
                             }
                             const unsigned at = (unsigned)(row.target - g.first - col);
-                            if (at < 16u && r < used && c0 + c < c_end) {
+                            if (at < 16u && c0 + c < c_end) {
                                 float hit = 0.f;
 #pragma unroll
-                                for (int i = 0; i < 16; i++) hit = at == (unsigned)i ? d[i] : hit;
-                                g.hit[r] = hit - (BF16 ? __bfloat162float(__float2bfloat16_rn(hit)) : __half2float(__float2half_rn(hit)));
+                                for (int i = 0; i < 16; i++)
+                                    if (at == (unsigned)i) {
+                                        d[i] -= row.b;
+                                        hit = CAP ? d[i] * slope[i] : d[i];
+                                    }
+                                if (r < used) g.hit[r] = hit - (BF16 ? __bfloat162float(__float2bfloat16_rn(hit)) : __half2float(__float2half_rn(hit)));
                             }
+#pragma unroll
+                            for (int i = 0; i < 16 && CAP; i++) d[i] *= slope[i];
                             if (row.low != 0) {
 #pragma unroll
                                 for (int i = 0; i < 16; i++) d[i] -= BF16 ? __bfloat162float(__float2bfloat16_rn(d[i])) : __half2float(__float2half_rn(d[i]));
                             }
 #pragma unroll
-                            for (int i = 0; i < 8; i++) o[c][i] = pack2<BF16>(d[2 * i], d[2 * i + 1]);
+                            for (int i = 0; i < 8; i++) o[c][i] = r < used ? pack2<BF16>(d[2 * i], d[2 * i + 1]) : 0u;
                         } else if constexpr (MODE == kWeight) {
 #pragma unroll
                             for (int i = 0; i < 8; i++) o[c][i] = pack2<BF16>(x[c].f(2 * i) * unscale, x[c].f(2 * i + 1) * unscale);

@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kPrepThreads) k_head_prep(const __grid_constan
             if (p.norms) {
                 row.b = p.grad_loss[r];
                 row.a = row.b + (p.grad_norms ? p.grad_norms[r] : 0.f);
-                row.norm2 = p.norms[r] * kLog2e;
+                row.norm = p.norms[r];
                 most = fmaxf(most, fmaxf(fabsf(row.a), fabsf(row.b)));
             }
             p.ws.rows[at] = row;
