@@ -11,10 +11,14 @@
 // thread has one row.  Operands lie in shared memory with their rows along K (hidden, weight, gradients) or along M or N
 // (weight and hidden states of the two gradients' products, gradients transposed): nothing is transposed in memory.
 //
-// The tensor cores' additions lose up to a step of the running sum each, always towards zero.  For the losses a sum is therefore
-// kept for kAccBlocks * 64 columns at most and the parts are added up in registers (8192 x 4096 x 151,936: the normalisers are 3.7e-7 off,
-// 1.7e-6 without, relative).  Pairs take 1024 columns, which costs nothing next to their products (512: 7.9 ms in place of 7.3); single CTAs,
-// which wait for memory, 512 (64 x 4096 x 151,936: 1.8e-7 off).
+// The tensor cores' additions lose up to a step of the running sum each, always towards zero, some 1e-7 of it on average.  For the losses a sum is
+// therefore kept for 1024 columns at most and the parts are added up in registers (8192 x 4096 x 151,936: the normalisers are 3.7e-7 off,
+// 1.7e-6 without, relative; 512 columns: 7.9 ms in place of 7.3); single CTAs, which wait for memory, take 512 (64 x 4096 x 151,936: 1.8e-7 off).
+// Gradients of logits of more than 4096 columns (bf16: 16,384) take the losses' parts too, which makes the logits the same, bit for bit, so that
+// probabilities add up to 1 whatever the logits are off: 20 rows x 16,384 x 2000 in fp16, a wrong token certain at logits of 65, are 2.3e-4 off, their own
+// rounding, in place of 1.0e-3; with 4096 columns in one accumulator 3.6e-4, less than fp16's half step.  It takes more registers than there are: 2 to 5 %
+// of a step (2048 x 8192 x 32,000: 2490 us, 2360 in one accumulator).  Gradients of a weight from more than 16,384 rows (bf16: 65,536) take parts of
+// 16,384, in tiles of half the width, 11 % of a step of 32,768 x 2048 x 32,000: 262,144 rows of one sign, fp16, are 2.3e-4 off in place of 1.6e-3.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -51,8 +55,9 @@ struct HeadGemm {
     int a_at;
 };
 
-template <bool PAIR>
-constexpr int kAccBlocks = PAIR ? 16 : 8;
+// Blocks that an accumulator holds.  LONG: sums that are taken in parts (stg_head_plan.h).
+template <int MODE, bool PAIR, bool LONG>
+constexpr int kAccBlocks = MODE == kStats || (MODE == kGrad && LONG) ? (PAIR ? 16 : 8) : MODE == kWeight && LONG ? kWeightRows / kGemmK : 1 << 30;
 constexpr int kGemmThreads = 64 + 32 * kGemmEpiWarps;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -129,7 +134,7 @@ __device__ __forceinline__ uint32_t rests_together(int n)
     return (uint64_t)most * kRestAlone > (uint64_t)__popc(many) * kRestLane + (uint64_t)all * kRestRow ? many : 0u;
 }
 
-template <int MODE, bool BF16, bool CAP, bool PAIR>
+template <int MODE, bool BF16, bool CAP, bool PAIR, bool LONG>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                const __grid_constant__ CUtensorMap map_out, const __grid_constant__ HeadGemm g)
 {
@@ -171,7 +176,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
     const int splits = MODE == kHidden ? g.info->splits : 1;
     const int tiles = tiles_m * tiles_n * splits;
     const int blocks = ((MODE == kWeight ? used : g.k) + kGemmK - 1) / kGemmK;
-    const int part = MODE == kStats ? kAccBlocks<PAIR> : 1 << 30;  // blocks of an accumulator
+    constexpr int kPart = kAccBlocks<MODE, PAIR, LONG>;
     const int first_tile = blockIdx.x / kCtas, step = gridDim.x / kCtas;
 
     if (warp == 0) {
@@ -221,7 +226,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                 const HeadTile tile(t, tiles_m, tiles_n, g.group, splits, blocks);
                 for (int k0 = tile.begin, k1; ok && k0 < tile.end; k0 = k1, unit++) {
                     const uint32_t acc = unit & 1u;
-                    k1 = min(tile.end - k0, part) + k0;
+                    k1 = min(tile.end - k0, kPart) + k0;
                     ok = bar_wait(acc_empty + 8 * acc, ((unit >> 1) & 1u) ^ 1u, dead);
                     if (!ok) break;
                     tc_fence_after();
@@ -283,23 +288,27 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                 }
                 unit++;
             };
+            // adds an accumulator's columns to their sums so far, of which it is the first
+            auto add_unit = [&](auto &z, uint32_t from, bool first, bool rows_here) {
+#pragma unroll
+                for (int c = 0; c < (int)(sizeof(z) / sizeof(z[0])); c++) {
+                    if (c_begin + c >= c_end || !rows_here) break;
+                    HeadCols x;
+                    tmem_load16(from + (c_begin + c) * 16, x.v);
+                    tmem_loaded();
+#pragma unroll
+                    for (int i = 0; i < 16; i++) z[c][i] = first ? x.f(i) : z[c][i] + x.f(i);
+                }
+                read_unit();
+            };
             if constexpr (MODE == kStats) {
                 const bool rows_here = m0 + quarter * 32 < used;  // of this warp
                 const int target = r >= used ? -1 : g.targets ? g.targets[r] : g.rows[r].target;
                 float z[8][16];
-                for (int k0 = 0; k0 < blocks; k0 += kAccBlocks<PAIR>) {
+                for (int k0 = 0; k0 < blocks; k0 += kPart) {
                     const uint32_t from = full_unit();
                     if (!ok) break;
-#pragma unroll
-                    for (int c = 0; c < 8; c++) {
-                        if (c_begin + c >= c_end || !rows_here) break;
-                        HeadCols x;
-                        tmem_load16(from + (c_begin + c) * 16, x.v);
-                        tmem_loaded();
-#pragma unroll
-                        for (int i = 0; i < 16; i++) z[c][i] = k0 == 0 ? x.f(i) : z[c][i] + x.f(i);
-                    }
-                    read_unit();
+                    add_unit(z, from, k0 == 0, rows_here);
                 }
                 if (!ok) break;
                 if (!rows_here) continue;
@@ -352,10 +361,22 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                     together = rests_together(mine.y);
                 }
                 const bool any_rests = MODE == kWeight && __any_sync(0xFFFFFFFFu, mine.y > 0);
+                // LONG: sums of all parts but the last; kWeight has as many columns as one box, kGrad's boxes are unrolled for them
+                float z[MODE == kGrad ? 8 : kOutChunks][16];
+                bool more = false;
+                for (int k0 = 0; LONG && k0 + kPart < blocks; k0 += kPart) {
+                    const uint32_t from = full_unit();
+                    if (!ok) break;
+                    add_unit(z, from, !more, rows_here);
+                    more = true;
+                }
+                if (LONG && !ok) break;
                 const uint32_t from = some ? full_unit() : 0u;
                 if (!ok) break;
-                for (int c0 = c_begin; c0 < c_end && rows_here; c0 += kOutChunks) {
-                    if (n0 + c0 * 16 >= g.n) break;
+#pragma unroll LONG && MODE == kGrad ? 8 / kOutChunks : 1
+                for (int box = 0; box < 8 / kOutChunks; box++) {
+                    const int c0 = c_begin + box * kOutChunks;
+                    if (c0 >= c_end || !rows_here || n0 + c0 * 16 >= g.n) break;
                     // all of a box's columns on their way before the first is waited for, and the last box's shared memory waited for last
                     HeadCols x[kOutChunks];
 #pragma unroll
@@ -368,6 +389,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                         }
                     }
                     if (some) tmem_loaded();
+                    if (LONG && more) {
+#pragma unroll
+                        for (int c = 0; c < kOutChunks; c++)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) x[c].v[i] = __float_as_uint(z[MODE == kGrad ? box * kOutChunks + c : c][i] + x[c].f(i));
+                    }
                     if (MODE == kWeight && any_rests) {  // what rounding has taken from the gradients of the rows whose target this is
                         const int own = together >> lane & 1u ? 0 : mine.y;
                         for (int k = 0; k < own; k++) {

@@ -374,14 +374,16 @@ static int head_map(StgHandle h, CUtensorMap *map, bool bf16, const void *p, int
     return head_map_of(h, map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p, size, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int MODE>
+template <int MODE, bool LONG>
 static cudaError_t head_gemm(StgHandle h, bool bf16, bool pair, cudaStream_t stream, const CUtensorMap &a, const CUtensorMap &b, const CUtensorMap &out,
                              HeadGemm g, int64_t tiles)
 {
     using Kernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, HeadGemm);
     constexpr bool C = MODE == kStats || MODE == kGrad;  // the others have no soft cap
-    static const Kernel kernels[2][2][2] = {{{k_head_gemm<MODE, false, false, false>, k_head_gemm<MODE, false, false, true>}, {k_head_gemm<MODE, false, C, false>, k_head_gemm<MODE, false, C, true>}},
-                                            {{k_head_gemm<MODE, true, false, false>, k_head_gemm<MODE, true, false, true>}, {k_head_gemm<MODE, true, C, false>, k_head_gemm<MODE, true, C, true>}}};
+    constexpr bool S = !(MODE == kWeight && LONG);       // so many rows are pairs'
+    static const Kernel kernels[2][2][2] = {
+        {{k_head_gemm<MODE, false, false, !S, LONG>, k_head_gemm<MODE, false, false, true, LONG>}, {k_head_gemm<MODE, false, C, !S, LONG>, k_head_gemm<MODE, false, C, true, LONG>}},
+        {{k_head_gemm<MODE, true, false, !S, LONG>, k_head_gemm<MODE, true, false, true, LONG>}, {k_head_gemm<MODE, true, C, !S, LONG>, k_head_gemm<MODE, true, C, true, LONG>}}};
     const Kernel fn = kernels[bf16][g.cap != 0.f][pair];
     const GemmRing ring = gemm_ring(MODE, pair, g.tile_n, g.a_rows);
     g.a_at = ring.a_at; g.stage_bytes = ring.stage_bytes; g.stages = ring.stages;
@@ -461,7 +463,7 @@ static int head_forward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
     g.targets = direct ? b->targets : nullptr; g.used_rows = b->rows;
     g.n = b->vocab; g.k = b->width;
     g.parts = ws.parts; g.hit = ws.hit; g.pieces = 2 * p.tiles_n;
-    CK(head_gemm<kStats>(h, bf16, p.pair, stream, rows, weight, rows, g, (int64_t)((b->rows + p.tile_m - 1) / p.tile_m) * p.tiles_n));
+    CK((head_gemm<kStats, false>(h, bf16, p.pair, stream, rows, weight, rows, g, (int64_t)((b->rows + p.tile_m - 1) / p.tile_m) * p.tiles_n)));
     CK(launch_behind(k_head_join, dim3((unsigned)b->rows), 128, 0, stream, ws, 2 * p.tiles_n, g.targets, b->vocab, b->loss, b->log_norms));
     h->stats.kernel_launches++;
     h->stats.calls++;
@@ -510,19 +512,22 @@ static int head_backward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
         g.first = first;
         g.n = count; g.k = b->width; g.a_rows = box_rows;
         g.out = ws.grads; g.out_stride = p.grads_stride; g.hit = ws.hit;
-        CK(head_gemm<kGrad>(h, bf16, p.pair, stream, rows_k, weight_k, grads_out, g, tiles_m * ((count + p.tile_n - 1) / p.tile_n)));
+        CK(((grad_in_parts(b->width, bf16) ? head_gemm<kGrad, true> : head_gemm<kGrad, false>)(h, bf16, p.pair, stream, rows_k, weight_k, grads_out, g, tiles_m * ((count + p.tile_n - 1) / p.tile_n))));
         g.n = b->width; g.tile_n = 256; g.group = kGroupGrads; g.cap = 0.f;
         if (b->grad_hidden) {
             g.k = count; g.a_rows = kHeadTileM;
             g.out = ws.sums; g.out_stride = b->width;
-            CK(head_gemm<kHidden>(h, bf16, p.pair, stream, grads_k, weight_mn, sums_out, g, tiles_m * tiles_w * 64));
+            CK((head_gemm<kHidden, false>(h, bf16, p.pair, stream, grads_k, weight_mn, sums_out, g, tiles_m * tiles_w * 64)));
         }
         if (b->grad_weight) {
             g.m = count;
             g.first_of = order ? ws.first : nullptr; g.order = ws.order; g.count = ws.count; g.hidden = (const uint16_t *)ws.hidden;
             g.out = b->grad_weight; g.out_stride = b->width;
             if ((rc = head_map(h, &weight_out, bf16, b->grad_weight, b->width, first + count, b->width, 32))) return rc;
-            CK(head_gemm<kWeight>(h, bf16, p.pair, stream, grads_mn, rows_mn, weight_out, g, (int64_t)((count + p.tile_m - 1) / p.tile_m) * tiles_w));
+            const bool in_parts = weight_in_parts(b->rows, bf16);
+            if (in_parts) g.tile_n = 128;
+            CK(((in_parts ? head_gemm<kWeight, true> : head_gemm<kWeight, false>)(h, bf16, p.pair, stream, grads_mn, rows_mn, weight_out, g,
+                                                                                 (int64_t)((count + p.tile_m - 1) / p.tile_m) * ((b->width + g.tile_n - 1) / g.tile_n))));
         }
     }
     if (b->grad_hidden) {
