@@ -132,3 +132,22 @@ def test_the_default_stream_by_its_handle(bs, data):
     torch.cuda.synchronize()
     assert all(torch.equal(got[k], want[k]) for k in want)
     assert math.isfinite(got["loss"].sum().item())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_stream_forked_inside_a_capture(bs, data, kind):
+    """The call's stream joins a capture on another one; its results and workspace are the graph's."""
+    want = _call(bs, data, kind, None)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        got = _call(bs, data, kind, side)
+        torch.cuda.current_stream().wait_stream(side)
+        copies = {k: x.clone() for k, x in got.items()}
+    for x in [*got.values(), *copies.values()]:
+        x.zero_()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(got[k], want[k]) and torch.equal(copies[k], want[k]) for k in want)
