@@ -575,14 +575,14 @@ STG_API int stg_beam_backtrace(StgHandle handle, const int32_t *trail_tokens, co
  * the sampling calls take, from a weight that stg_head_pack has laid out.  Every array is device memory, aligned to its elements
  * unless it says otherwise, and no output may overlap an input or another output.  Sizes are not bounded by the handle's capacities.
  *
- * Streams and captured graphs: the calls are enqueued on `stream`, the host waits for nothing and nothing of the handle is
- * written: what a call needs beside its arrays is its workspace, which the caller owns and which calls that may run at the same
- * time must not share.  Its contents mean nothing between calls. */
+ * Streams and captured graphs: the calls are enqueued on `stream`, the host waits for nothing, and of the handle only its statistics and
+ * error text are written (by one host thread at a time, as ever): what a call needs on the device beside its arrays is its workspace,
+ * which the caller owns and which calls that may run at the same time must not share.  Its contents mean nothing between calls. */
 
 /* Softmax cross entropy.  With z[v] = hidden . weight[v], or cap * tanh(z / cap) of it, in fp32: log_norms = log(sum(exp(z))),
- * loss = log_norms - z[target].  A target below 0 says that the row has no loss: both are 0, its hidden state is not read and it
- * adds nothing to any gradient.  So does a target of vocab or beyond, but both are NaN.  Where a bounded wait of a kernel gives up,
- * all losses (all of grad_hidden) are NaN. */
+ * loss = log_norms - z[target], never below 0.  A target below 0 says that the row has no loss: both are 0, what its hidden state holds
+ * reaches nothing and it adds nothing to any gradient.  So does a target of vocab or beyond, but both are NaN.  Where a bounded wait of a
+ * kernel gives up, what its CTA was to compute is NaN: some rows' losses, some rows of grad_hidden, some of grad_weight. */
 typedef struct StgHeadLoss {
     int32_t struct_size;            /* = sizeof(StgHeadLoss) */
     int32_t rows;
@@ -608,8 +608,9 @@ typedef struct StgHeadLoss {
 STG_API int stg_head_loss_workspace(StgHandle handle, const StgHeadLoss *loss, int32_t backward, uint64_t *out_bytes);
 STG_API int stg_head_loss(StgHandle handle, const StgHeadLoss *loss, void *stream);
 /* Gradients of sum(grad_loss * loss + grad_log_norms * log_norms).  The gradients of the logits are rounded to `dtype`, scaled by a power
- * of two of their largest factor so that fp16 holds them too; what that takes from the target's of each row - up to 64 rows: from
- * all - is made good.  Sums are fp32, outputs rounded once.  Deterministic. */
+ * of two of their largest factor so that fp16 holds them too (those 2^-38 of it and smaller are lost there: rows' factors should lie within
+ * some 2^16 of one another); what that takes from the target's of each row - up to 64 rows: from all - is made good.  Sums are fp32,
+ * outputs rounded once.  Deterministic. */
 STG_API int stg_head_loss_backward(StgHandle handle, const StgHeadLoss *loss, void *stream);
 
 /* A weight in 4 bits: weight[v][k] = (code[v][k] - zero[v][k / group]) * scale[v][k / group], codes 0 .. 15, two columns to a byte,

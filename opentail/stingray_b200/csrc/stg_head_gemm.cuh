@@ -6,7 +6,7 @@
 //   kWeight  gradients of the weight = gradients^T hidden, for a piece of the vocabulary, rounded once
 //
 // Persistent pairs of CTAs take tiles of 256 x tile_n (PAIR; up to 128 rows: single CTAs take tiles of 128 x tile_n).  Each CTA loads 64 columns
-// of its 128 rows of the one operand and of its half of the other at a time by TMA, into a ring of six stages; one thread of the pair
+// of its 128 rows of the one operand and of its half of the other at a time by TMA, into a ring of up to eight stages; one thread of the pair
 // issues tcgen05.mma into one of two accumulators in tensor memory, and eight warps of each CTA work on the other one meanwhile: a
 // thread has one row.  Operands lie in shared memory with their rows along K (hidden, weight, gradients) or along M or N
 // (weight and hidden states of the two gradients' products, gradients transposed): nothing is transposed in memory.

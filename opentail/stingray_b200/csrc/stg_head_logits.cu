@@ -311,8 +311,8 @@ __device__ __forceinline__ void stage_rows(const HeadLogits &p, int cols, unsign
 // Up to two rows as integers: hidden state x is X * 2^(e - 30), e the exponent above the row's largest finite one, X rounded - exact down to
 // 2^-22 of the largest, 2^-31 of it off below - and X four digits of -128 .. 127.  Column 4 r + d of `xs` (pitch bytes between columns) has
 // digit d of row r, the highest first; of a unit's 128 columns a lane's are next to each other: byte 32 t + 8 h + i is column
-// 32 h + 8 t + i, the middle two of every four exchanged.  A row with a hidden state that is not finite comes out NaN or infinite by `bad`, the
-// sum of what such hidden states are times zero, which is added to its logits.
+// 32 h + 8 t + i, the middle two of every four exchanged.  A row with a hidden state that is not finite comes out NaN: `bad` says
+// so, and the inverse that its logits are multiplied with at the end is NaN.
 template <bool ZEROS, int G>
 __device__ __forceinline__ void stage_digits(const HeadLogits &p, int cols, unsigned char *xs, int pitch, float *sums, float2 *unscale, uint32_t *most)
 {

@@ -7,10 +7,11 @@
 // thread multiplies, each group of columns into an accumulator of its own (a ring of them), and more warps add them up, scaled by the
 // entry's scale: a thread's numbers all have the same.  So the weight is not rounded, and scales meet fp32 sums.
 //
-// What bounds it is the way into tensor memory and out of it: a unit of eight tiles is 32 KB of unpacked weight, and each of its groups
-// 512 bytes of sums per row, at what measures as some 30 and 60 bytes a cycle.  256 rows x 4096 x 151,936 take 410 us with groups of 128
-// (780 TFLOP/s; the library's bf16 product of that size would be 193 at its best rate), 509 with zero points too, 704 with
-// groups of 32; 64 rows 173 and 282.
+// A unit of eight tiles is 32 KB of unpacked weight into tensor memory, and each of its groups 512 bytes of sums per row out of it, which by
+// themselves measure as some 30 and 60 bytes a cycle.  64 rows x 4096 x 151,936 take 173 us with groups of 128, bound by the way in (26 bytes a cycle), and 282
+// with groups of 32, by the way out.  256 rows take 410 (780 TFLOP/s; the library's bf16 product of that size would be 193 at its best rate), 22 bytes a
+// cycle in and 43 out with two thirds of the issue slots taken: nothing is full.  509 with zero points, which move no more but double the adding
+// warps' work and halve their number (TilesWarps); 704 with groups of 32.  Zero points with groups of 32 and more than 64 rows spill 96 bytes.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
