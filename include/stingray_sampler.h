@@ -609,8 +609,8 @@ STG_API int stg_head_loss_workspace(StgHandle handle, const StgHeadLoss *loss, i
 STG_API int stg_head_loss(StgHandle handle, const StgHeadLoss *loss, void *stream);
 /* Gradients of sum(grad_loss * loss + grad_log_norms * log_norms).  The gradients of the logits are rounded to `dtype`, scaled by a power
  * of two of their largest factor so that fp16 holds them too (those 2^-38 of it and smaller are lost there: rows' factors should lie within
- * some 2^16 of one another); what that takes from the target's of each row - up to 64 rows: from all - is made good.  Sums are fp32,
- * outputs rounded once.  Deterministic. */
+ * some 2^16 of one another); the target's of each row is not rounded - up to 64 rows: what rounding takes from any is
+ * made good.  Sums are fp32, outputs rounded once.  Deterministic. */
 STG_API int stg_head_loss_backward(StgHandle handle, const StgHeadLoss *loss, void *stream);
 
 /* A weight in 4 bits: weight[v][k] = (code[v][k] - zero[v][k / group]) * scale[v][k / group], codes 0 .. 15, two columns to a byte,

@@ -32,7 +32,7 @@ struct HeadWs {
     HeadRow *rows;      // [padded rows]
     int32_t *place;     // [rows]: its place among the used rows, -1: no loss, -2: its target lies outside the vocabulary
     void *hidden;       // [padded rows, width]: hidden states of the used rows
-    float *hit;         // [padded rows]: the target's logit; backward: what rounding takes from its gradient
+    float *hit;         // [padded rows]: the target's logit; backward, more than 64 rows: its gradient
     int32_t *first;     // backward, more than 64 rows: [vocab]: where the used rows with this target begin in `order`, -1: there are none;
     int32_t *order;     // [padded rows]: the used rows by their targets, those of one target in their order; and
     int32_t *count;     // [padded rows]: where a target's rows begin, their number

@@ -14,11 +14,12 @@
 // The tensor cores' additions lose up to a step of the running sum each, always towards zero, some 1e-7 of it on average.  For the losses a sum is
 // therefore kept for 1024 columns at most and the parts are added up in registers (8192 x 4096 x 151,936: the normalisers are 3.7e-7 off,
 // 1.7e-6 without, relative; 512 columns: 7.9 ms in place of 7.3); single CTAs, which wait for memory, take 512 (64 x 4096 x 151,936: 1.8e-7 off).
-// Gradients of logits of more than 4096 columns (bf16: 16,384) take the losses' parts too, which makes the logits the same, bit for bit, so that
-// probabilities add up to 1 whatever the logits are off: 20 rows x 16,384 x 2000 in fp16, a wrong token certain at logits of 65, are 2.3e-4 off, their own
-// rounding, in place of 1.0e-3; with 4096 columns in one accumulator 3.6e-4, less than fp16's half step.  It takes more registers than there are: 2 to 5 %
-// of a step (2048 x 8192 x 32,000: 2490 us, 2360 in one accumulator).  Gradients of a weight from more than 16,384 rows (bf16: 65,536) take parts of
-// 16,384, in tiles of half the width, 11 % of a step of 32,768 x 2048 x 32,000: 262,144 rows of one sign, fp16, are 2.3e-4 off in place of 1.6e-3.
+// The backward pass takes parts where a sum is so long that it would show beside the results' rounding (stg_head_plan.h; bf16, eight times as
+// coarse, from eight times as many terms on).  Gradients of logits take the losses' parts, which makes the logits the same, bit for bit, so that probabilities add
+// up to 1 whatever the logits are off: 20 rows x 16,384 x 2000 in fp16, a wrong token certain at logits of 65, are 2.3e-4 off, their own rounding, in place
+// of 1.0e-3.  It takes more registers than there are: 2 to 5 % of a step (2048 x 8192 x 32,000: 2490 us, 2360 in one accumulator).  Gradients
+// of a weight take tiles of half the width for it, 11 % of a step of 32,768 x 2048 x 32,000: 262,144 rows of one sign, fp16, are 2.3e-4 off in place of 1.6e-3.
+// Those of the hidden states add their parts in memory.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -55,9 +56,12 @@ struct HeadGemm {
     int a_at;
 };
 
-// Blocks that an accumulator holds.  LONG: sums that are taken in parts (stg_head_plan.h).
-template <int MODE, bool PAIR, bool LONG>
-constexpr int kAccBlocks = MODE == kStats || (MODE == kGrad && LONG) ? (PAIR ? 16 : 8) : MODE == kWeight && LONG ? kWeightRows / kGemmK : 1 << 30;
+// Blocks that an accumulator holds.  LONG: sums that are taken in parts in registers (stg_head_plan.h).
+template <int MODE, bool BF16, bool PAIR, bool LONG>
+constexpr int kAccBlocks = MODE == kStats || (MODE == kGrad && LONG) ? (PAIR ? 16 : 8)
+                         : MODE == kHidden                           ? part_of(kHiddenColumns, BF16) / kGemmK
+                         : MODE == kWeight && LONG                   ? part_of(kWeightRows, BF16) / kGemmK
+                                                                     : 1 << 30;
 constexpr int kGemmThreads = 64 + 32 * kGemmEpiWarps;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -176,7 +180,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
     const int splits = MODE == kHidden ? g.info->splits : 1;
     const int tiles = tiles_m * tiles_n * splits;
     const int blocks = ((MODE == kWeight ? used : g.k) + kGemmK - 1) / kGemmK;
-    constexpr int kPart = kAccBlocks<MODE, PAIR, LONG>;
+    constexpr int kPart = kAccBlocks<MODE, BF16, PAIR, LONG>;
     const int first_tile = blockIdx.x / kCtas, step = gridDim.x / kCtas;
 
     if (warp == 0) {
@@ -351,6 +355,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                 const bool rows_here = r0 < (MODE == kWeight ? g.m : MODE == kHidden ? slab : g.rows_pad) && (some || MODE != kHidden || g.first == 0);
                 HeadRow row = {};
                 if (MODE == kGrad && rows_here) row = g.rows[r];
+                // Beyond 64 rows the target's gradient, the largest of a row mostly, is left out of the products and added where their results are rounded, not
+                // rounded itself: in an accumulator it makes the additions of all that follows it coarser, too (1000 x 512 x 131,072 in fp16, weights with a
+                // mean of four deviations: 6.2e-4 off in place of 4.3e-4)
+                const bool apart = MODE == kGrad && g.info->low == 0;
                 row.a *= scale;
                 row.b *= scale;
                 int2 mine = make_int2(0, 0);
@@ -371,153 +379,159 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_head_gemm(const __grid_cons
                     more = true;
                 }
                 if (LONG && !ok) break;
-                const uint32_t from = some ? full_unit() : 0u;
-                if (!ok) break;
+                // kHidden: a sum's later parts are added to the first in memory, when that has got there
+                const int rounds = MODE == kHidden && some ? (tile.end - tile.begin + kPart - 1) / kPart : 1;
+                for (int round = 0; round < rounds; round++) {
+                    const uint32_t from = some ? full_unit() : 0u;
+                    if (!ok) break;
+                    if (MODE == kHidden && round > 0 && lane == 0) store_done();
 #pragma unroll LONG && MODE == kGrad ? 8 / kOutChunks : 1
-                for (int box = 0; box < 8 / kOutChunks; box++) {
-                    const int c0 = c_begin + box * kOutChunks;
-                    if (c0 >= c_end || !rows_here || n0 + c0 * 16 >= g.n) break;
-                    // all of a box's columns on their way before the first is waited for, and the last box's shared memory waited for last
-                    HeadCols x[kOutChunks];
+                    for (int box = 0; box < 8 / kOutChunks; box++) {
+                        const int c0 = c_begin + box * kOutChunks;
+                        if (c0 >= c_end || !rows_here || n0 + c0 * 16 >= g.n) break;
+                        // all of a box's columns on their way before the first is waited for, and the last box's shared memory waited for last
+                        HeadCols x[kOutChunks];
 #pragma unroll
-                    for (int c = 0; c < kOutChunks; c++) {
-                        if (some && c0 + c < c_end) {
-                            tmem_load16(from + (c0 + c) * 16, x[c].v);
-                        } else {
+                        for (int c = 0; c < kOutChunks; c++) {
+                            if (some && c0 + c < c_end) {
+                                tmem_load16(from + (c0 + c) * 16, x[c].v);
+                            } else {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) x[c].v[i] = 0u;
-                        }
-                    }
-                    if (some) tmem_loaded();
-                    if (LONG && more) {
-#pragma unroll
-                        for (int c = 0; c < kOutChunks; c++)
-#pragma unroll
-                            for (int i = 0; i < 16; i++) x[c].v[i] = __float_as_uint(z[MODE == kGrad ? box * kOutChunks + c : c][i] + x[c].f(i));
-                    }
-                    if (MODE == kWeight && any_rests) {  // what rounding has taken from the gradients of the rows whose target this is
-                        const int own = together >> lane & 1u ? 0 : mine.y;
-                        for (int k = 0; k < own; k++) {
-                            const int q = g.order[mine.x + k];
-                            const float rest = g.hit[q];
-                            const uint16_t *h = g.hidden + (int64_t)q * g.n + n0 + c0 * 16;
-#pragma unroll
-                            for (int c = 0; c < 2 * kOutChunks; c++) {
-                                if (n0 + c0 * 16 + 8 * c >= g.n) break;
-                                const uint4 e = ((const uint4 *)h)[c];
-                                const uint32_t w[4] = {e.x, e.y, e.z, e.w};
-#pragma unroll
-                                for (int i = 0; i < 8; i++)
-                                    x[c / 2].v[8 * (c & 1) + i] = __float_as_uint(fmaf(rest, half_of<BF16>(w[i / 2] >> (16 * (i & 1))), x[c / 2].f(8 * (c & 1) + i)));
+                                for (int i = 0; i < 16; i++) x[c].v[i] = 0u;
                             }
                         }
-                        __syncwarp();
-                        for (uint32_t left = together; left != 0u; left &= left - 1u) {  // by the warp: a lane has two columns
-                            const int to = __ffs(left) - 1, begin = __shfl_sync(0xFFFFFFFFu, mine.x, to), n = __shfl_sync(0xFFFFFFFFu, mine.y, to), col = n0 + c0 * 16 + 2 * lane;
-                            float2 sum = make_float2(0.f, 0.f);
-                            for (int k0 = 0; k0 < n; k0 += 32) {  // a lane looks up a row
-                                const int q = k0 + lane < n ? g.order[begin + k0 + lane] : 0;
-                                const float rest = k0 + lane < n ? g.hit[q] : 0.f;
-                                const int here = min(32, n - k0);
-#pragma unroll 8
-                                for (int k = 0; k < here; k++) {
-                                    const int row = __shfl_sync(0xFFFFFFFFu, q, k);
-                                    const float by = __shfl_sync(0xFFFFFFFFu, rest, k);
-                                    const uint32_t e = col < g.n ? *(const uint32_t *)(g.hidden + (int64_t)row * g.n + col) : 0u;
-                                    sum.x = fmaf(by, half_of<BF16>(e), sum.x);
-                                    sum.y = fmaf(by, half_of<BF16>(e >> 16), sum.y);
+                        if (some) tmem_loaded();
+                        if (LONG && more) {
+#pragma unroll
+                            for (int c = 0; c < kOutChunks; c++)
+#pragma unroll
+                                for (int i = 0; i < 16; i++) x[c].v[i] = __float_as_uint(z[MODE == kGrad ? box * kOutChunks + c : c][i] + x[c].f(i));
+                        }
+                        if (MODE == kWeight && any_rests) {  // the targets' gradients of the rows whose target this is
+                            const int own = together >> lane & 1u ? 0 : mine.y;
+                            for (int k = 0; k < own; k++) {
+                                const int q = g.order[mine.x + k];
+                                const float rest = g.hit[q];
+                                const uint16_t *h = g.hidden + (int64_t)q * g.n + n0 + c0 * 16;
+#pragma unroll
+                                for (int c = 0; c < 2 * kOutChunks; c++) {
+                                    if (n0 + c0 * 16 + 8 * c >= g.n) break;
+                                    const uint4 e = ((const uint4 *)h)[c];
+                                    const uint32_t w[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+                                    for (int i = 0; i < 8; i++)
+                                        x[c / 2].v[8 * (c & 1) + i] = __float_as_uint(fmaf(rest, half_of<BF16>(w[i / 2] >> (16 * (i & 1))), x[c / 2].f(8 * (c & 1) + i)));
                                 }
                             }
+                            __syncwarp();
+                            for (uint32_t left = together; left != 0u; left &= left - 1u) {  // by the warp: a lane has two columns
+                                const int to = __ffs(left) - 1, begin = __shfl_sync(0xFFFFFFFFu, mine.x, to), n = __shfl_sync(0xFFFFFFFFu, mine.y, to), col = n0 + c0 * 16 + 2 * lane;
+                                float2 sum = make_float2(0.f, 0.f);
+                                for (int k0 = 0; k0 < n; k0 += 32) {  // a lane looks up a row
+                                    const int q = k0 + lane < n ? g.order[begin + k0 + lane] : 0;
+                                    const float rest = k0 + lane < n ? g.hit[q] : 0.f;
+                                    const int here = min(32, n - k0);
+#pragma unroll 8
+                                    for (int k = 0; k < here; k++) {
+                                        const int row = __shfl_sync(0xFFFFFFFFu, q, k);
+                                        const float by = __shfl_sync(0xFFFFFFFFu, rest, k);
+                                        const uint32_t e = col < g.n ? *(const uint32_t *)(g.hidden + (int64_t)row * g.n + col) : 0u;
+                                        sum.x = fmaf(by, half_of<BF16>(e), sum.x);
+                                        sum.y = fmaf(by, half_of<BF16>(e >> 16), sum.y);
+                                    }
+                                }
+                                if (lane == 0) store_read();
+                                __syncwarp();
+                                shared_store2(out + lane * 8, __float_as_uint(sum.x), __float_as_uint(sum.y));
+                                __syncwarp();
+                                if (lane == to) {
+#pragma unroll
+                                    for (int i = 0; i < 16 * kOutChunks; i += 4) {
+                                        const float4 v = shared_load(out + i * 4);
+                                        uint32_t *at = x[i / 16].v + i % 16;
+                                        at[0] = __float_as_uint(__uint_as_float(at[0]) + v.x);
+                                        at[1] = __float_as_uint(__uint_as_float(at[1]) + v.y);
+                                        at[2] = __float_as_uint(__uint_as_float(at[2]) + v.z);
+                                        at[3] = __float_as_uint(__uint_as_float(at[3]) + v.w);
+                                    }
+                                }
+                                __syncwarp();
+                            }
+                        }
+                        uint32_t o[kOutChunks][MODE == kHidden ? 1 : 8];
+#pragma unroll
+                        for (int c = 0; c < kOutChunks; c++) {
+                            const int col = n0 + (c0 + c) * 16;
+                            if constexpr (MODE == kGrad) {
+                                float d[16], slope[16];
+#pragma unroll
+                                for (int i = 0; i < 16; i++) {
+                                    float logit = x[c].f(i);
+                                    if (CAP) {
+                                        const Capped capped = head_cap(logit, g.cap, by_cap);
+                                        logit = capped.z;
+                                        slope[i] = 1.f - capped.tanh * capped.tanh;
+                                    }
+                                    d[i] = row.a * exp2_fast((logit - row.norm) * kLog2e);
+                                }
+                                const unsigned at = (unsigned)(row.target - g.first - col);
+                                if (at < 16u && c0 + c < c_end) {
+                                    float hit = 0.f;
+#pragma unroll
+                                    for (int i = 0; i < 16; i++)
+                                        if (at == (unsigned)i) {
+                                            d[i] -= row.b;
+                                            hit = CAP ? d[i] * slope[i] : d[i];
+                                            if (apart) d[i] = 0.f;
+                                        }
+                                    if (apart && r < used) g.hit[r] = hit;
+                                }
+#pragma unroll
+                                for (int i = 0; i < 16 && CAP; i++) d[i] *= slope[i];
+                                if (row.low != 0) {
+#pragma unroll
+                                    for (int i = 0; i < 16; i++) d[i] -= BF16 ? __bfloat162float(__float2bfloat16_rn(d[i])) : __half2float(__float2half_rn(d[i]));
+                                }
+#pragma unroll
+                                for (int i = 0; i < 8; i++) o[c][i] = r < used ? pack2<BF16>(d[2 * i], d[2 * i + 1]) : 0u;
+                            } else if constexpr (MODE == kWeight) {
+#pragma unroll
+                                for (int i = 0; i < 8; i++) o[c][i] = pack2<BF16>(x[c].f(2 * i) * unscale, x[c].f(2 * i + 1) * unscale);
+                            }
+                        }
+                        if (!direct) {
                             if (lane == 0) store_read();
                             __syncwarp();
-                            shared_store2(out + lane * 8, __float_as_uint(sum.x), __float_as_uint(sum.y));
-                            __syncwarp();
-                            if (lane == to) {
-#pragma unroll
-                                for (int i = 0; i < 16 * kOutChunks; i += 4) {
-                                    const float4 v = shared_load(out + i * 4);
-                                    uint32_t *at = x[i / 16].v + i % 16;
-                                    at[0] = __float_as_uint(__uint_as_float(at[0]) + v.x);
-                                    at[1] = __float_as_uint(__uint_as_float(at[1]) + v.y);
-                                    at[2] = __float_as_uint(__uint_as_float(at[2]) + v.z);
-                                    at[3] = __float_as_uint(__uint_as_float(at[3]) + v.w);
-                                }
-                            }
-                            __syncwarp();
                         }
-                    }
-                    uint32_t o[kOutChunks][MODE == kHidden ? 1 : 8];
 #pragma unroll
-                    for (int c = 0; c < kOutChunks; c++) {
-                        const int col = n0 + (c0 + c) * 16;
-                        if constexpr (MODE == kGrad) {
-                            float d[16], slope[16];
+                        for (int c = 0; c < kOutChunks; c++) {
+                            const uint32_t to = out + lane * 128;  // its 16 bytes are exchanged as a 128-byte swizzle wants them
+                            if constexpr (MODE == kHidden) {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) {
-                                float logit = x[c].f(i);
-                                if (CAP) {
-                                    const Capped capped = head_cap(logit, g.cap, by_cap);
-                                    logit = capped.z;
-                                    slope[i] = 1.f - capped.tanh * capped.tanh;
+                                for (int i = 0; i < 4; i++) shared_store(to + (((4 * c + i) ^ (lane & 7)) << 4), x[c].v[4 * i], x[c].v[4 * i + 1], x[c].v[4 * i + 2], x[c].v[4 * i + 3]);
+                            } else if (direct) {
+                                if (c0 + c < c_end) {
+                                    uint4 *at = (uint4 *)((uint16_t *)g.out + (int64_t)r * g.out_stride + n0 + (c0 + c) * 16);
+                                    at[0] = make_uint4(o[c][0], o[c][1], o[c][2], o[c][3]);
+                                    at[1] = make_uint4(o[c][4], o[c][5], o[c][6], o[c][7]);
                                 }
-                                d[i] = row.a * exp2_fast((logit - row.norm) * kLog2e);
+                            } else {
+                                shared_store(to + (((2 * c) ^ (lane & 7)) << 4), o[c][0], o[c][1], o[c][2], o[c][3]);
+                                shared_store(to + (((2 * c + 1) ^ (lane & 7)) << 4), o[c][4], o[c][5], o[c][6], o[c][7]);
                             }
-                            const unsigned at = (unsigned)(row.target - g.first - col);
-                            if (at < 16u && c0 + c < c_end) {
-                                float hit = 0.f;
-#pragma unroll
-                                for (int i = 0; i < 16; i++)
-                                    if (at == (unsigned)i) {
-                                        d[i] -= row.b;
-                                        hit = CAP ? d[i] * slope[i] : d[i];
-                                    }
-                                if (r < used) g.hit[r] = hit - (BF16 ? __bfloat162float(__float2bfloat16_rn(hit)) : __half2float(__float2half_rn(hit)));
-                            }
-#pragma unroll
-                            for (int i = 0; i < 16 && CAP; i++) d[i] *= slope[i];
-                            if (row.low != 0) {
-#pragma unroll
-                                for (int i = 0; i < 16; i++) d[i] -= BF16 ? __bfloat162float(__float2bfloat16_rn(d[i])) : __half2float(__float2half_rn(d[i]));
-                            }
-#pragma unroll
-                            for (int i = 0; i < 8; i++) o[c][i] = r < used ? pack2<BF16>(d[2 * i], d[2 * i + 1]) : 0u;
-                        } else if constexpr (MODE == kWeight) {
-#pragma unroll
-                            for (int i = 0; i < 8; i++) o[c][i] = pack2<BF16>(x[c].f(2 * i) * unscale, x[c].f(2 * i + 1) * unscale);
                         }
-                    }
-                    if (!direct) {
-                        if (lane == 0) store_read();
+                        if (direct) continue;
+                        async_proxy_fence();
                         __syncwarp();
-                    }
-#pragma unroll
-                    for (int c = 0; c < kOutChunks; c++) {
-                        const uint32_t to = out + lane * 128;  // its 16 bytes are exchanged as a 128-byte swizzle wants them
-                        if constexpr (MODE == kHidden) {
-#pragma unroll
-                            for (int i = 0; i < 4; i++) shared_store(to + (((4 * c + i) ^ (lane & 7)) << 4), x[c].v[4 * i], x[c].v[4 * i + 1], x[c].v[4 * i + 2], x[c].v[4 * i + 3]);
-                        } else if (direct) {
-                            if (c0 + c < c_end) {
-                                uint4 *at = (uint4 *)((uint16_t *)g.out + (int64_t)r * g.out_stride + n0 + (c0 + c) * 16);
-                                at[0] = make_uint4(o[c][0], o[c][1], o[c][2], o[c][3]);
-                                at[1] = make_uint4(o[c][4], o[c][5], o[c][6], o[c][7]);
-                            }
-                        } else {
-                            shared_store(to + (((2 * c) ^ (lane & 7)) << 4), o[c][0], o[c][1], o[c][2], o[c][3]);
-                            shared_store(to + (((2 * c + 1) ^ (lane & 7)) << 4), o[c][4], o[c][5], o[c][6], o[c][7]);
+                        if (lane == 0) {
+                            const int x = n0 + c0 * 16, y = (MODE == kWeight ? g.first : MODE == kHidden ? tile.split * slab : 0) + r0;
+                            if (MODE == kHidden && (g.first > 0 || round > 0)) tma_store<true>(&map_out, x, y, out);
+                            else tma_store<false>(&map_out, x, y, out);
+                            store_commit();
                         }
                     }
-                    if (direct) continue;
-                    async_proxy_fence();
-                    __syncwarp();
-                    if (lane == 0) {
-                        const int x = n0 + c0 * 16, y = (MODE == kWeight ? g.first : MODE == kHidden ? tile.split * slab : 0) + r0;
-                        if (MODE == kHidden && g.first > 0) tma_store<true>(&map_out, x, y, out);
-                        else tma_store<false>(&map_out, x, y, out);
-                        store_commit();
-                    }
+                    if (some) read_unit();
                 }
-                if (some) read_unit();
             }
         }
         if (MODE != kStats && lane == 0) store_done();

@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(128) k_head_gather(const __grid_constant__ Hea
     }
 }
 
-// The used rows by their targets, for the remainders in the weight's gradient: a row's place is the number of rows with a smaller target and of those
+// The used rows by their targets, whose gradients are added to the weight's apart: a row's place is the number of rows with a smaller target and of those
 // ahead of it with its own.  Four threads to a row look through all rows, 4096 at a time in shared memory.
 constexpr int kOrderThreads = 256, kOrderRows = 4096;
 
@@ -236,8 +236,8 @@ __global__ void __launch_bounds__(128) k_head_join(const __grid_constant__ HeadW
 }
 
 // Gradients of the hidden states: the splits' sums added up and rounded, back in their rows; zeros where a row has no loss.  Where the logits'
-// gradients have no remainders of their own, the target's - the largest of a row, mostly - is multiplied here (without it a bf16 gradient is 2.4e-3
-// off in place of 1.7e-3, which is its own rounding).  A CTA has 256 columns
+// gradients have no remainders of their own, the target's - the largest of a row, mostly - is multiplied here (rounded like the others it made a bf16
+// gradient 2.4e-3 off in place of 1.7e-3, which is its own rounding).  A CTA has 256 columns
 // of a row, and eight threads share out the splits of each eight columns.
 template <bool BF16>
 __global__ void __launch_bounds__(256) k_head_spread(const __grid_constant__ HeadWs ws, int width, const uint16_t *weight, int64_t weight_stride,
@@ -512,7 +512,7 @@ static int head_backward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
         g.first = first;
         g.n = count; g.k = b->width; g.a_rows = box_rows;
         g.out = ws.grads; g.out_stride = p.grads_stride; g.hit = ws.hit;
-        CK(((grad_in_parts(b->width, bf16) ? head_gemm<kGrad, true> : head_gemm<kGrad, false>)(h, bf16, p.pair, stream, rows_k, weight_k, grads_out, g, tiles_m * ((count + p.tile_n - 1) / p.tile_n))));
+        CK(((b->width > part_of(kGradColumns, bf16) ? head_gemm<kGrad, true> : head_gemm<kGrad, false>)(h, bf16, p.pair, stream, rows_k, weight_k, grads_out, g, tiles_m * ((count + p.tile_n - 1) / p.tile_n))));
         g.n = b->width; g.tile_n = 256; g.group = kGroupGrads; g.cap = 0.f;
         if (b->grad_hidden) {
             g.k = count; g.a_rows = kHeadTileM;
@@ -524,7 +524,7 @@ static int head_backward(StgHandle h, const StgHeadLoss *b, cudaStream_t stream)
             g.first_of = order ? ws.first : nullptr; g.order = ws.order; g.count = ws.count; g.hidden = (const uint16_t *)ws.hidden;
             g.out = b->grad_weight; g.out_stride = b->width;
             if ((rc = head_map(h, &weight_out, bf16, b->grad_weight, b->width, first + count, b->width, 32))) return rc;
-            const bool in_parts = weight_in_parts(b->rows, bf16);
+            const bool in_parts = b->rows > part_of(kWeightRows, bf16);
             if (in_parts) g.tile_n = 128;
             CK(((in_parts ? head_gemm<kWeight, true> : head_gemm<kWeight, false>)(h, bf16, p.pair, stream, grads_mn, rows_mn, weight_out, g,
                                                                                  (int64_t)((count + p.tile_m - 1) / p.tile_m) * ((b->width + g.tile_n - 1) / g.tile_n))));

@@ -34,10 +34,10 @@ struct HeadPlan {
 // one of 256: 1607 us in place of 1154, 4096 x 256,000).
 constexpr int kLowRows = 64;
 
-// Beyond these a sum of kGrad or kWeight is taken in parts (stg_head_gemm.cuh); bf16, whose rounding is eight times as coarse, beyond four times as many.
-constexpr int kGradColumns = 4096, kWeightRows = 16384;
-inline bool grad_in_parts(int width, bool bf16) { return width > (bf16 ? 4 : 1) * kGradColumns; }
-inline bool weight_in_parts(int rows, bool bf16) { return rows > (bf16 ? 4 : 1) * kWeightRows; }
+// Terms of a sum that the backward pass's products keep in one accumulator (stg_head_gemm.cuh); bf16, whose rounding is eight times as coarse, eight times as
+// many.
+constexpr int kGradColumns = 1024, kHiddenColumns = 16384, kWeightRows = 16384;
+STG_HD constexpr int part_of(int terms, bool bf16) { return bf16 ? 8 * terms : terms; }
 
 inline HeadPlan head_shape(int rows, int vocab, int width, int sms, bool backward)
 {

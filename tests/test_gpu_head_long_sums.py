@@ -87,3 +87,43 @@ def test_many_rows_of_one_sign(bs, rows, width, vocab, dtype):
     assert _off(b["grad_hidden"], gh) <= 0.58 + 0.33
     again = bs.head_loss_backward(h, w, t, n, dl, want_hidden=False)
     assert torch.equal(again["grad_weight"], b["grad_weight"])
+
+
+@pytest.mark.parametrize("mean", [1.0, 4.0])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("rows,width,vocab", [(60, 72, 200_001), (100, 512, 262_144), (300, 264, 150_000), (1000, 512, 131_072), (1000, 2048, 40_000), (20, 1032, 40_000)])
+def test_weights_with_a_mean(bs, rows, width, vocab, dtype, mean):
+    """A direction that all vocabulary entries share: of the sums over the vocabulary that is most, and a row's target takes it off again, so that it is
+    the probabilities' sum that shows, and every addition."""
+    g = torch.Generator(device="cuda").manual_seed(rows + width)
+    s = 2.5 / math.sqrt(width)
+    w = ((torch.randn((vocab, width), generator=g, device="cuda") + mean) * s).to(getattr(torch, dtype))
+    h = torch.randn((rows, width), generator=g, device="cuda").to(w.dtype)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    n = bs.head_loss(h, w, t)["log_norms"]
+    one = torch.ones(rows, device="cuda")
+    b = bs.head_loss_backward(h, w, t, n, one, want_weight=False)["grad_hidden"]
+    norm = torch.stack([torch.logsumexp(h.double() @ w[v:v + 16384].double().T, 1) for v in range(0, vocab, 16384)], 1).logsumexp(1)
+    gh = -w[t.long()].double()
+    for v in range(0, vocab, 16384):
+        x = w[v:v + 16384].double()
+        gh += torch.exp(h.double() @ x.T - norm[:, None]) @ x
+    # beyond 64 rows the roundings of the other probabilities remain, as above; and a part's additions, 1024 at most (bf16: 8192), are off by 2^-22 of the
+    # sum each: U / 2 of the probabilities' products with the weight's sizes
+    sizes = sum(torch.exp(h.double() @ w[v:v + 16384].double().T - norm[:, None]) @ w[v:v + 16384].double().abs() for v in range(0, vocab, 16384))
+    assert _off(b, gh) <= 0.58 + (0.33 if rows > 64 else 0.0) + 0.5 * (sizes.norm() / gh.norm()).item()
+    assert torch.equal(bs.head_loss_backward(h, w, t, n, one, want_weight=False)["grad_hidden"], b)
+
+
+def test_small_probabilities_beside_a_large_target(bs):
+    """Probabilities of 1 / 40,000 each, weights of 1, and of 200 for the targets, the vocabulary's first: what the 40,000 add up to is 1.02, of
+    which nothing is lost beside the target's 200."""
+    w = torch.ones((40_000, 2048), dtype=torch.float16, device="cuda")
+    w[:4] = 200
+    h = torch.zeros((3000, 2048), dtype=torch.float16, device="cuda")
+    t = (torch.arange(3000, device="cuda") % 4).to(torch.int32)
+    n = bs.head_loss(h, w, t)["log_norms"]
+    b = bs.head_loss_backward(h, w, t, n, torch.ones(3000, device="cuda"), want_weight=False)["grad_hidden"]
+    want = (39_996 + 4 * 200) / 40_000 - 200
+    # half a step of fp16 at 199; the probability's rounding and the sums' additions 2^-12 of 1.02 each, the normaliser's 2^-22
+    assert ((b.double() - want).abs() <= 0.0625 + 2 * 1.02 * 2.0 ** -12 + 1e-5).all(), (b.double() - want).abs().max().item()
