@@ -68,8 +68,8 @@ def test_all_rows_have_one_target(bs, rows, width, vocab, target):
     _check(bs, h, w, t, dl)
 
 
-def test_a_weight_s_remainders_are_added_in_the_order_of_the_rows(bs):
-    """What is made good does not depend on where the rows lie: the same rows in another order are as close to the formula."""
+def test_rows_in_another_order(bs):
+    """The targets' gradients are added in the order of the rows, whatever it is: the same rows in another one are as close to the formula."""
     g, h, w, dl = _inputs(2000, 64, 50, torch.bfloat16, 4)
     t = (torch.arange(2000, device="cuda") % 3).to(torch.int32)
     one, want = _check(bs, h, w, t, dl)
